@@ -1,0 +1,529 @@
+// GQA decode attention over a paged cache: over listed pages, and over every
+// slot with its softmax weight gathered.
+#include "common.h"
+#include "layer_common.cuh"
+#include "paged.h"
+
+namespace rtxllm {
+namespace {
+
+typedef _Float16 half4 __attribute__((ext_vector_type(4)));
+typedef _Float16 half8 __attribute__((ext_vector_type(8)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+
+constexpr std::uint32_t kThreads = 256, kWaves = kThreads / 64u, kTile = 16;
+constexpr std::uint32_t kMaxSplits = 128;
+constexpr float kLift = 15.0f;  // softmax terms are kept times 2^15 (see the kernel)
+
+struct AttnArgs {
+  const float* q;
+  const std::uint32_t* pos;
+  const std::int32_t* pages;  // null: every slot
+  float* out;
+  float2* ml;      // [row][kv head][query head][split]: maximum (in log2), sum
+  float* part;     // [row][kv head][query head][split][head_dim]
+  float* scores;   // [row][kv head][query head][score_stride], in log2 (weights only)
+  std::uint32_t group, n_select, splits, score_stride;
+};
+
+__device__ __forceinline__ std::uint32_t from_lane(std::uint32_t v, std::uint32_t lane) {
+  return static_cast<std::uint32_t>(__builtin_amdgcn_ds_bpermute(static_cast<int>(4u * lane), static_cast<int>(v)));
+}
+
+// One workgroup of four waves per (split, kv head, row); a wave takes tiles of 16
+// positions of its split in turn, with a running maximum and sum for every head:
+//  * scores: S = K q^T by v_mfma_f32_16x16x32_f16. A = the K rows as stored (lane:
+//    position l % 16, 8 dims of each 32); B = q log2(e) / sqrt(D) of head n / 2,
+//    a power of two below 2 in magnitude, as an fp16 hi (n even) / lo (n odd)
+//    pair, so products are exact and the pair carries 22 bits at any size of q;
+//  * p = 2^(s - m + 15) split into an fp16 hi / lo pair as well: lifted by 2^15 (the
+//    largest p is 2^15, the sum l is lifted alike), terms down to 2^-29 of the
+//    largest keep 22 bits where fp16's subnormals would cut them;
+//  * o += V^T p by v_mfma_f32_4x4x4_16b_f16: a lane holds its own dimensions of
+//    four positions, as the V rows' coalesced loads leave them (a pair of lanes'
+//    worth of bytes each), and one column of p, fetched from the score layout by
+//    ds_bpermute. A lane's 4 results are one head's, so its rescaling is one factor.
+// T: heads in fours (1..4).
+template <int D, int T, bool WEIGHTS>
+__global__ __launch_bounds__(kThreads) void paged_attn_kernel(AttnArgs a, PagedView kv) {
+  constexpr int NT = (T + 1) / 2;            // score tiles of 8 heads
+  constexpr int J = D / 32;                  // score MFMAs of a tile
+  constexpr int VD = D == 256 ? 4 : 2;       // dims a lane holds of a V row
+  constexpr int RPL = D == 64 ? 2 : 1;       // V rows a load covers
+  constexpr int STEPS = 4 / RPL;             // 4-position steps of a tile
+  __shared__ __align__(16) float rec[kWaves][4 * T][D];
+  __shared__ float2 rml[kWaves][4 * T];
+  const std::uint32_t split = blockIdx.x, g = blockIdx.y, r = blockIdx.z;
+  const std::uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const std::uint32_t n = paged_filled(kv, a.pos[r]);
+  if (n == 0u) return;  // a padded row
+  const std::uint32_t total = a.pages != nullptr ? a.n_select * kv.page_size : n;
+  const std::uint32_t tiles = (total + kTile - 1u) / kTile;
+  const std::uint32_t per = (tiles + kWaves * a.splits - 1u) / (kWaves * a.splits) * kWaves;
+  const std::uint32_t tile0 = split * per, tile1 = tile0 + per < tiles ? tile0 + per : tiles;
+  const std::size_t gr = static_cast<std::size_t>(r) * kv.n_kv + g;
+  const std::size_t head0 = gr * a.group;  // first query head of the kv head, over all rows
+  if (tile0 >= tiles) {
+    if (threadIdx.x < a.group) a.ml[(head0 + threadIdx.x) * a.splits + split] = make_float2(-INFINITY, 0.0f);
+    return;
+  }
+  const std::uint32_t col = lane & 15u, qq = lane >> 4;
+
+  // B operands of the scores and each column's power of two
+  uint4 qb[NT][J];
+  float qscale[NT];
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+    const std::uint32_t h = 8u * nt + col / 2u;
+    const bool there = h < a.group;
+    const float* qr = a.q + (head0 + (there ? h : 0u)) * D + 8u * qq;
+    f32x4_any x[J][2];
+    float m = 0.0f;
+#pragma unroll
+    for (int j = 0; j < J; ++j) {
+      x[j][0] = *reinterpret_cast<const f32x4_any*>(qr + 32 * j);
+      x[j][1] = *reinterpret_cast<const f32x4_any*>(qr + 32 * j + 4);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) m = fmaxf(m, fmaxf(fabsf(x[j][0][i]), fabsf(x[j][1][i])));
+    }
+    m = fmaxf(m, lane_xor<16>(m));
+    m = fmaxf(m, lane_xor<32>(m));
+    int e = 0;
+    if (m > 0.0f && m <= 3.4e38f) frexpf(m, &e);
+    qscale[nt] = ldexpf(1.4426950408889634f / (D == 64 ? 8.0f : D == 128 ? 11.313708498984761f : 16.0f), e);
+#pragma unroll
+    for (int j = 0; j < J; ++j) {
+      half8 b;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        float v = there ? ldexpf(x[j][i / 4][i & 3], -e) : 0.0f;
+        asm("" : "+v"(v));  // one rounded value for hi and lo
+        const _Float16 hi = static_cast<_Float16>(v);
+        b[i] = (col & 1u) == 0u ? hi : static_cast<_Float16>(v - static_cast<float>(hi));
+      }
+      qb[nt][j] = __builtin_bit_cast(uint4, b);
+    }
+  }
+
+  const std::int32_t* const table = kv.table + static_cast<std::size_t>(r) * kv.table_stride;
+  const std::int32_t* const list = a.pages != nullptr ? a.pages + gr * a.n_select : nullptr;
+  float m[NT], l[NT];
+  f32x4 o[T][VD];
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) m[nt] = -INFINITY, l[nt] = 0.0f;
+#pragma unroll
+  for (int t = 0; t < T; ++t)
+#pragma unroll
+    for (int s = 0; s < VD; ++s) o[t][s] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+
+  for (std::uint32_t tile = tile0 + wave; tile < tile1; tile += kWaves) {
+    // the lane's position (col of the tile) and its row
+    const std::uint32_t x = tile * kTile + col;
+    std::uint32_t row = kNoRow;
+    if (x < total) {
+      std::uint32_t lp = x / kv.page_size;
+      const std::uint32_t off = x - lp * kv.page_size;
+      if (list != nullptr) lp = static_cast<std::uint32_t>(list[lp]);
+      if (lp < kv.entries && lp * kv.page_size + off < n) row = paged_row(kv, table[lp], g, off);
+    }
+    const std::uint32_t valid = static_cast<std::uint32_t>(__ballot(row != kNoRow)) & 0xFFFFu;
+    float* const sc_out = WEIGHTS ? a.scores + head0 * a.score_stride + tile * kTile + 4u * qq : nullptr;
+    if (valid == 0u) {
+      if constexpr (WEIGHTS) {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          const std::uint32_t h = 8u * nt + col / 2u;
+          if ((col & 1u) == 0u && h < a.group)
+            *reinterpret_cast<float4*>(sc_out + static_cast<std::size_t>(h) * a.score_stride) =
+                make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+        }
+      }
+      continue;
+    }
+    if (row == kNoRow) row = 0u;  // any row of the cache: its scores and values are dropped
+    uint4 ka[J];
+    {
+      const uint4* kr = reinterpret_cast<const uint4*>(kv.k + static_cast<std::size_t>(row) * D) + qq;
+#pragma unroll
+      for (int j = 0; j < J; ++j) ka[j] = kr[4 * j];
+    }
+    std::uint32_t vw[16 / RPL][VD / 2];
+#pragma unroll
+    for (int j = 0; j < 16 / RPL; ++j) {
+      if constexpr (D == 64) {
+        const std::uint32_t r0 = __builtin_amdgcn_readlane(row, 8 * (j / 4) + (j & 3)),
+                            r1 = __builtin_amdgcn_readlane(row, 8 * (j / 4) + 4 + (j & 3));
+        const std::uint32_t rr = lane < 32u ? r0 : r1;
+        vw[j][0] = reinterpret_cast<const std::uint32_t*>(kv.v + static_cast<std::size_t>(rr) * D)[lane & 31u];
+      } else {
+        const std::uint32_t rr = __builtin_amdgcn_readlane(row, j);
+        const std::uint16_t* vr = kv.v + static_cast<std::size_t>(rr) * D;
+        if constexpr (D == 128) {
+          vw[j][0] = reinterpret_cast<const std::uint32_t*>(vr)[lane];
+        } else {
+          const uint2 t = reinterpret_cast<const uint2*>(vr)[lane];
+          vw[j][0] = t.x, vw[j][1] = t.y;
+        }
+      }
+    }
+    if (valid != 0xFFFFu) {  // 0 times what lies behind the context must stay 0
+#pragma unroll
+      for (int j = 0; j < 16 / RPL; ++j) {
+        const std::uint32_t at = D == 64 ? 8u * (j / 4) + (lane < 32u ? 0u : 4u) + (j & 3) : j;
+#pragma unroll
+        for (int s = 0; s < VD / 2; ++s) vw[j][s] = (valid >> at & 1u) != 0u ? vw[j][s] : 0u;
+      }
+    }
+    std::uint32_t p01[NT], p23[NT];
+    float alpha[NT];
+    bool moved = false;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      f32x4 sc = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int j = 0; j < J; ++j)
+        sc = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8, ka[j]),
+                                                    __builtin_bit_cast(half8, qb[nt][j]), sc, 0, 0, 0);
+      // column n: head n / 2; positions 4 qq + i
+      float s4[4], top = -INFINITY;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float t = (sc[i] + lane_xor<1>(sc[i])) * qscale[nt];
+        s4[i] = (valid >> (4u * qq + i) & 1u) != 0u ? t : -INFINITY;
+        top = fmaxf(top, s4[i]);
+      }
+      if constexpr (WEIGHTS) {
+        const std::uint32_t h = 8u * nt + col / 2u;
+        if ((col & 1u) == 0u && h < a.group)
+          *reinterpret_cast<float4*>(sc_out + static_cast<std::size_t>(h) * a.score_stride) =
+              make_float4(s4[0], s4[1], s4[2], s4[3]);
+      }
+      top = fmaxf(top, lane_xor<16>(top));
+      top = fmaxf(top, lane_xor<32>(top));
+      const float mn = fmaxf(m[nt], top);
+      const float base = mn == -INFINITY ? 0.0f : mn;
+      alpha[nt] = __builtin_amdgcn_exp2f(m[nt] - base);
+      moved = moved || mn != m[nt];
+      m[nt] = mn;
+      float sum = 0.0f;
+      half4 ph;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        float p = __builtin_amdgcn_exp2f(s4[i] - base + kLift);
+        asm("" : "+v"(p));
+        sum += p;
+        const _Float16 hi = static_cast<_Float16>(p);
+        ph[i] = (col & 1u) == 0u ? hi : static_cast<_Float16>(p - static_cast<float>(hi));
+      }
+      l[nt] = l[nt] * alpha[nt] + sum;
+      const uint2 pk = __builtin_bit_cast(uint2, ph);
+      p01[nt] = pk.x, p23[nt] = pk.y;
+    }
+    if (__ballot(moved) != 0ull) {
+#pragma unroll
+      for (int t = 0; t < T; ++t) {
+        const float f = __uint_as_float(from_lane(__float_as_uint(alpha[t / 2]), 8u * (t & 1) + 2u * (lane & 3u)));
+#pragma unroll
+        for (int s = 0; s < VD; ++s) o[t][s] *= f;
+      }
+    }
+#pragma unroll
+    for (int st = 0; st < STEPS; ++st) {
+      half4 va[VD];
+#pragma unroll
+      for (int s = 0; s < VD; ++s) {
+        const std::uint32_t sel = (s & 1) != 0 ? 0x07060302u : 0x05040100u;  // the high / low halves of two words
+        uint2 w;
+        w.x = __builtin_amdgcn_perm(vw[4 * st + 1][s / 2], vw[4 * st][s / 2], sel);
+        w.y = __builtin_amdgcn_perm(vw[4 * st + 3][s / 2], vw[4 * st + 2][s / 2], sel);
+        va[s] = __builtin_bit_cast(half4, w);
+      }
+      const std::uint32_t src = 16u * (RPL == 2 ? 2u * st + (lane >> 5) : st) + 2u * (lane & 3u);
+#pragma unroll
+      for (int t = 0; t < T; ++t) {
+#pragma unroll
+        for (int part = 0; part < 2; ++part) {
+          uint2 w;
+          w.x = from_lane(p01[t / 2], src + 8u * (t & 1) + part);
+          w.y = from_lane(p23[t / 2], src + 8u * (t & 1) + part);
+          const half4 pb = __builtin_bit_cast(half4, w);
+#pragma unroll
+          for (int s = 0; s < VD; ++s) o[t][s] = __builtin_amdgcn_mfma_f32_4x4x4f16(va[s], pb, o[t][s], 0, 0, 0);
+        }
+      }
+    }
+  }
+
+  // the waves' records, merged: o = sum e^(m_w - M) o_w, L alike
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+    l[nt] += lane_xor<16>(l[nt]);
+    l[nt] += lane_xor<32>(l[nt]);
+    const std::uint32_t h = 8u * nt + col / 2u;
+    // a NaN among the scores makes the row NaN, also where no number gave a maximum
+    if (qq == 0u && (col & 1u) == 0u && h < 4u * T)
+      rml[wave][h] = make_float2(l[nt] != l[nt] ? INFINITY : m[nt], l[nt]);
+  }
+#pragma unroll
+  for (int t = 0; t < T; ++t) {
+    if constexpr (D == 64) {
+#pragma unroll
+      for (int s = 0; s < VD; ++s)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[t][s][i] += lane_xor<32>(o[t][s][i]);
+    }
+    if (D != 64 || lane < 32u) {
+      float* dst = &rec[wave][4 * t + (lane & 3u)][VD * (lane & ~3u)];
+#pragma unroll
+      for (int i = 0; i < 4; i += 4 / VD) {
+        if constexpr (VD == 2)
+          *reinterpret_cast<f32x4*>(dst + 2 * i) = f32x4{o[t][0][i], o[t][1][i], o[t][0][i + 1], o[t][1][i + 1]};
+        else
+          *reinterpret_cast<f32x4*>(dst + 4 * i) = f32x4{o[t][0][i], o[t][1][i], o[t][VD - 2][i], o[t][VD - 1][i]};
+      }
+    }
+  }
+  __syncthreads();
+  const std::uint32_t items = a.group * (D / 4u);
+  for (std::uint32_t it = threadIdx.x; it < items; it += kThreads) {
+    const std::uint32_t h = it / (D / 4u), d = 4u * (it % (D / 4u));
+    float M = -INFINITY;
+#pragma unroll
+    for (std::uint32_t w = 0; w < kWaves; ++w) M = fmaxf(M, rml[w][h].x);
+    const float base = M == -INFINITY ? 0.0f : M;
+    float L = 0.0f;
+    f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (std::uint32_t w = 0; w < kWaves; ++w) {
+      const float f = __builtin_amdgcn_exp2f(rml[w][h].x - base);
+      L += f * rml[w][h].y;
+      v += f * *reinterpret_cast<const f32x4*>(&rec[w][h][d]);
+    }
+    if (!WEIGHTS && a.splits == 1u) {
+      const float inv = L == 0.0f ? 0.0f : 1.0f / L;
+      *reinterpret_cast<f32x4_any*>(a.out + (head0 + h) * D + d) = f32x4_any(v * inv);
+    } else {
+      const std::size_t at = (head0 + h) * a.splits + split;
+      *reinterpret_cast<f32x4*>(a.part + at * D + d) = v;
+      if (d == 0u) a.ml[at] = make_float2(M, L);
+    }
+  }
+}
+
+// Maximum and sum of one head over its splits' records, by one wave.
+__device__ __forceinline__ float2 head_ml(const float2* __restrict__ ml, std::uint32_t splits, std::uint32_t lane) {
+  const float2 none = make_float2(-INFINITY, 0.0f);
+  const float2 x = lane < splits ? ml[lane] : none, y = lane + 64u < splits ? ml[lane + 64u] : none;
+  const float M = wave_max(fmaxf(x.x, y.x)), base = M == -INFINITY ? 0.0f : M;
+  return make_float2(M, wave_sum(x.y * __builtin_amdgcn_exp2f(x.x - base) + y.y * __builtin_amdgcn_exp2f(y.x - base)));
+}
+
+// One workgroup a query head (of all rows): its splits' records merged, D / 4
+// lanes a record.
+template <int D>
+__device__ __forceinline__ void merge_head(const AttnArgs& a, std::size_t head) {
+  constexpr std::uint32_t kLanes = D / 4u, kSub = kThreads / kLanes;
+  __shared__ __align__(16) float sums[kSub][D];
+  const std::uint32_t d = 4u * (threadIdx.x % kLanes), sub = threadIdx.x / kLanes;
+  const float2* const ml = a.ml + head * a.splits;
+  const float2 t = head_ml(ml, a.splits, threadIdx.x & 63u);
+  const float base = t.x == -INFINITY ? 0.0f : t.x;
+  f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
+  for (std::uint32_t c = sub; c < a.splits; c += kSub) {
+    const float mc = ml[c].x;
+    if (mc == -INFINITY) continue;  // (an empty split writes no sums)
+    v += __builtin_amdgcn_exp2f(mc - base) * *reinterpret_cast<const f32x4*>(a.part + (head * a.splits + c) * D + d);
+  }
+  *reinterpret_cast<f32x4*>(&sums[sub][d]) = v;
+  __syncthreads();
+  if (sub != 0u) return;
+#pragma unroll
+  for (std::uint32_t k = 1; k < kSub; ++k) v += *reinterpret_cast<const f32x4*>(&sums[k][d]);
+  const float inv = t.y == 0.0f ? 0.0f : 1.0f / t.y;
+  *reinterpret_cast<f32x4_any*>(a.out + head * D + d) = f32x4_any(v * inv);
+}
+
+template <int D>
+__global__ __launch_bounds__(kThreads) void merge_kernel(AttnArgs a, PagedView kv) {
+  const std::uint32_t r = blockIdx.y;
+  if (paged_filled(kv, a.pos[r]) == 0u) return;
+  merge_head<D>(a, static_cast<std::size_t>(r) * gridDim.x + blockIdx.x);
+}
+
+// The first `group` workgroups of (kv head, row) merge a head each; the others
+// add the softmax weights of 1024 slots each.
+template <int D>
+__global__ __launch_bounds__(kThreads) void merge_weights_kernel(AttnArgs a, PagedView kv, const float* weight,
+                                                                 float* weight_out) {
+  __shared__ float base_s[kMaxQueryGroup], inv_s[kMaxQueryGroup];
+  const std::uint32_t g = blockIdx.y, r = blockIdx.z, n = paged_filled(kv, a.pos[r]);
+  if (n == 0u) return;
+  const std::size_t gr = static_cast<std::size_t>(r) * kv.n_kv + g, head0 = gr * a.group;
+  if (blockIdx.x < a.group) {
+    merge_head<D>(a, head0 + blockIdx.x);
+    return;
+  }
+  const std::uint32_t i0 = (blockIdx.x - a.group) * 4u * kThreads + 4u * threadIdx.x;
+  if (i0 - 4u * threadIdx.x >= n) return;
+  const std::uint32_t lane = threadIdx.x & 63u;
+  for (std::uint32_t h = threadIdx.x >> 6; h < a.group; h += kWaves) {
+    const float2 t = head_ml(a.ml + (head0 + h) * a.splits, a.splits, lane);
+    if (lane == 0u) {
+      base_s[h] = (t.x == -INFINITY ? 0.0f : t.x) - kLift;
+      inv_s[h] = t.y == 0.0f ? 0.0f : 1.0f / t.y;
+    }
+  }
+  __syncthreads();
+  if (i0 >= n) return;
+  f32x4 w = {0.0f, 0.0f, 0.0f, 0.0f};
+  for (std::uint32_t h = 0; h < a.group; ++h) {
+    const f32x4 s = *reinterpret_cast<const f32x4*>(a.scores + (head0 + h) * a.score_stride + i0);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] += __builtin_amdgcn_exp2f(s[i] - base_s[h]) * inv_s[h];
+  }
+  const std::size_t at = gr * kv.capacity + i0;
+  if (i0 + 4u <= n) {
+    *reinterpret_cast<f32x4_any*>(weight_out + at) =
+        *reinterpret_cast<const f32x4_any*>(weight + at) + f32x4_any(w);
+  } else {
+    for (std::uint32_t i = 0; i < n - i0; ++i) weight_out[at + i] = weight[at + i] + w[i];
+  }
+}
+
+// Splits of each (row, kv head): enough workgroups to fill the chip, at most one
+// per 64 positions.
+std::uint32_t attn_splits(std::uint64_t items, std::uint64_t positions) {
+  const std::uint64_t want = (1024u + items - 1u) / items, most = (positions + 63u) / 64u;
+  const std::uint64_t s = want < most ? want : most;
+  return static_cast<std::uint32_t>(s < kMaxSplits ? s : kMaxSplits);
+}
+
+struct AttnSpace {
+  std::uint32_t splits = 0, score_stride = 0;
+  std::size_t ml = 0, part = 0, scores = 0;  // byte offsets past the start
+  std::size_t bytes = 0;                     // 0: refused
+};
+
+AttnSpace attn_space(const rtxllm_paged_kv* c, std::uint32_t n_heads, std::uint64_t positions, std::uint32_t count,
+                     bool weights) {
+  AttnSpace s;
+  if (!paged_cache_ok(c, count) || count == 0u || count > 65535u || c->n_kv_heads > 65535u ||
+      paged_group(c, n_heads) == 0u || positions == 0u || positions > (1ull << 31))
+    return s;
+  s.splits = attn_splits(static_cast<std::uint64_t>(count) * c->n_kv_heads, positions);
+  const std::size_t records = static_cast<std::size_t>(count) * n_heads * s.splits;
+  s.part = round_256(8u * records);
+  s.scores = s.part + round_256(4u * records * c->head_dim);
+  s.bytes = s.scores;
+  if (weights) {
+    s.score_stride = (c->capacity + kTile - 1u) / kTile * kTile;
+    s.bytes += round_256(4u * static_cast<std::size_t>(count) * n_heads * s.score_stride);
+  }
+  return s;
+}
+
+template <int D, bool WEIGHTS>
+void launch_partial(const AttnArgs& a, const PagedView& view, std::uint32_t count, hipStream_t stream) {
+  const dim3 grid(a.splits, view.n_kv, count);
+  if (a.group <= 4u)
+    hipLaunchKernelGGL((paged_attn_kernel<D, 1, WEIGHTS>), grid, dim3(kThreads), 0, stream, a, view);
+  else if (a.group <= 8u)
+    hipLaunchKernelGGL((paged_attn_kernel<D, 2, WEIGHTS>), grid, dim3(kThreads), 0, stream, a, view);
+  else
+    hipLaunchKernelGGL((paged_attn_kernel<D, 4, WEIGHTS>), grid, dim3(kThreads), 0, stream, a, view);
+}
+
+template <int D>
+hipError_t launch_pages(const AttnArgs& a, const PagedView& view, std::uint32_t count, hipStream_t stream) {
+  launch_partial<D, false>(a, view, count, stream);
+  const hipError_t rc = hipGetLastError();
+  if (rc != hipSuccess || a.splits == 1u) return rc;
+  hipLaunchKernelGGL(merge_kernel<D>, dim3(a.group * view.n_kv, count), dim3(kThreads), 0, stream, a, view);
+  return hipGetLastError();
+}
+
+template <int D>
+hipError_t launch_weights(const AttnArgs& a, const PagedView& view, std::uint32_t count, const float* weight,
+                          float* weight_out, hipStream_t stream) {
+  launch_partial<D, true>(a, view, count, stream);
+  const hipError_t rc = hipGetLastError();
+  if (rc != hipSuccess) return rc;
+  const std::uint32_t chunks = (view.capacity + 4u * kThreads - 1u) / (4u * kThreads);
+  hipLaunchKernelGGL(merge_weights_kernel<D>, dim3(a.group + chunks, view.n_kv, count), dim3(kThreads), 0, stream, a,
+                     view, weight, weight_out);
+  return hipGetLastError();
+}
+
+AttnArgs attn_args(const float* q, const std::uint32_t* pos, float* out, void* workspace, const AttnSpace& s,
+                   std::uint32_t group) {
+  auto* base = static_cast<std::uint8_t*>(workspace);
+  AttnArgs a{};
+  a.q = q;
+  a.pos = pos;
+  a.out = out;
+  a.ml = reinterpret_cast<float2*>(base);
+  a.part = reinterpret_cast<float*>(base + s.part);
+  a.scores = reinterpret_cast<float*>(base + s.scores);
+  a.group = group;
+  a.splits = s.splits;
+  a.score_stride = s.score_stride;
+  return a;
+}
+
+bool attn_pointers_ok(const float* q, const std::uint32_t* pos, const float* out, const void* workspace) {
+  return q != nullptr && pos != nullptr && out != nullptr && workspace != nullptr && aligned_to(q, 4u) &&
+         aligned_to(pos, 4u) && aligned_to(out, 4u) && aligned_to(workspace, 256u);
+}
+
+}  // namespace
+}  // namespace rtxllm
+
+using namespace rtxllm;
+
+extern "C" size_t rtxllm_attn_pages_workspace(const rtxllm_paged_kv* cache, uint32_t n_heads, uint32_t n_select,
+                                              uint32_t count) {
+  if (cache == nullptr || n_select == 0u || n_select > 65536u) return 0u;
+  return attn_space(cache, n_heads, static_cast<std::uint64_t>(n_select) * cache->page_size, count, false).bytes;
+}
+
+extern "C" hipError_t rtxllm_attn_decode_pages_gqa_f16(const rtxllm_paged_kv* cache, const float* q, uint32_t n_heads,
+                                                       const int32_t* pages, uint32_t n_select, const uint32_t* pos,
+                                                       uint32_t count, float* out, void* workspace,
+                                                       size_t workspace_bytes, hipStream_t stream) {
+  if (cache == nullptr || pages == nullptr || !aligned_to(pages, 4u) || n_select == 0u || n_select > 65536u ||
+      !attn_pointers_ok(q, pos, out, workspace))
+    return hipErrorInvalidValue;
+  const AttnSpace s = attn_space(cache, n_heads, static_cast<std::uint64_t>(n_select) * cache->page_size, count, false);
+  if (s.bytes == 0u || workspace_bytes < s.bytes) return hipErrorInvalidValue;
+  AttnArgs a = attn_args(q, pos, out, workspace, s, paged_group(cache, n_heads));
+  a.pages = pages;
+  a.n_select = n_select;
+  const PagedView view = paged_view(cache);
+  return cache->head_dim == 64u    ? launch_pages<64>(a, view, count, stream)
+         : cache->head_dim == 128u ? launch_pages<128>(a, view, count, stream)
+                                   : launch_pages<256>(a, view, count, stream);
+}
+
+extern "C" size_t rtxllm_attn_weights_workspace(const rtxllm_paged_kv* cache, uint32_t n_heads, uint32_t count) {
+  if (cache == nullptr) return 0u;
+  return attn_space(cache, n_heads, cache->capacity, count, true).bytes;
+}
+
+extern "C" hipError_t rtxllm_attn_decode_weights_gqa_f16(const rtxllm_paged_kv* cache, const float* q,
+                                                         uint32_t n_heads, const uint32_t* last, uint32_t count,
+                                                         float* out, const float* weight, float* weight_out,
+                                                         void* workspace, size_t workspace_bytes, hipStream_t stream) {
+  if (cache == nullptr || weight == nullptr || weight_out == nullptr || !aligned_to(weight, 4u) ||
+      !aligned_to(weight_out, 4u) || !attn_pointers_ok(q, last, out, workspace) ||
+      (cache->table_stride == 0u && count > 1u))
+    return hipErrorInvalidValue;
+  const AttnSpace s = attn_space(cache, n_heads, cache->capacity, count, true);
+  if (s.bytes == 0u || workspace_bytes < s.bytes) return hipErrorInvalidValue;
+  const std::size_t n = 4u * static_cast<std::size_t>(count) * cache->n_kv_heads * cache->capacity;
+  if (weight_out != weight && overlap(weight_out, n, weight, n)) return hipErrorInvalidValue;
+  const AttnArgs a = attn_args(q, last, out, workspace, s, paged_group(cache, n_heads));
+  const PagedView view = paged_view(cache);
+  return cache->head_dim == 64u    ? launch_weights<64>(a, view, count, weight, weight_out, stream)
+         : cache->head_dim == 128u ? launch_weights<128>(a, view, count, weight, weight_out, stream)
+                                   : launch_weights<256>(a, view, count, weight, weight_out, stream);
+}

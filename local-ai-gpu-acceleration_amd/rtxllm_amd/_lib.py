@@ -68,6 +68,13 @@ _LAUNCH_SIGS: dict[str, list] = {
     "rtxllm_embed_gather_q5k": [_P, _U, _U, _P, _U, _P, _S],
     "rtxllm_attn_decode_gqa_f16": [_P, _P, _P, _P, _U, _U, _U, _U, _U, _P, _U, _P, _P, c_size_t, _S],
     "rtxllm_argmax": [_P, _U, _U, _P, _S],
+    "rtxllm_qk_norm_rope_append_f16": [_P, _P, c_size_t, _P, c_size_t, _P, c_size_t, _P, _P, _U, _U, c_int, c_float,
+                                       c_float, _P, _P, _U, _P, _P, _P, _S],
+    "rtxllm_kv_page_bounds_f16": [_P, _P, _P, _U, _U, _P, _S],
+    "rtxllm_attn_select_pages": [_P, _P, _P, _U, _P, _U, _U, _U, _U, _P, _P, c_size_t, _S],
+    "rtxllm_attn_decode_pages_gqa_f16": [_P, _P, _U, _P, _U, _P, _U, _P, _P, c_size_t, _S],
+    "rtxllm_attn_decode_weights_gqa_f16": [_P, _P, _U, _P, _U, _P, _P, _P, _P, c_size_t, _S],
+    "rtxllm_kv_evict_f16": [_P, _P, _P, _U, _U, _U, _U, _P, _P, _P, _P, _P, _P, c_size_t, _S],
     "rtxllm_iq2s_units_pack": [_P, _U, _U, _P, _S],
     "rtxllm_iq3s_units_pack": [_P, _U, _U, _P, _S],
 }
@@ -98,6 +105,12 @@ class PackOptions(ctypes.Structure):
                 ("names", ctypes.c_char_p), ("layer", c_int), ("limit", c_uint64)]
 
 
+class PagedKVStruct(ctypes.Structure):
+    """rtxllm_paged_kv (include/rtxllm/paged_kv.h)."""
+    _fields_ = [("k", c_void_p), ("v", c_void_p), ("block_table", c_void_p)] + [
+        (n, c_uint32) for n in ("table_stride", "n_pages", "n_kv_heads", "head_dim", "page_size", "capacity")]
+
+
 _C = ctypes.c_char_p
 # name -> (restype, argtypes) for host helpers.
 _HOST_SIGS: dict[str, tuple] = {
@@ -113,6 +126,10 @@ _HOST_SIGS: dict[str, tuple] = {
     "rtxllm_x16_bytes": (c_size_t, [c_uint32]),
     "rtxllm_matvec_batch_workspace": (c_size_t, [c_int, c_uint32, c_uint32]),
     "rtxllm_attn_decode_workspace": (c_size_t, [c_uint32, c_uint32, c_uint32, c_uint32]),
+    "rtxllm_attn_select_workspace": (c_size_t, [_P, c_uint32]),
+    "rtxllm_attn_pages_workspace": (c_size_t, [_P, c_uint32, c_uint32, c_uint32]),
+    "rtxllm_attn_weights_workspace": (c_size_t, [_P, c_uint32, c_uint32]),
+    "rtxllm_kv_evict_workspace": (c_size_t, [_P, c_uint32, c_uint32]),
     "rtxllm_llama_destroy": (None, [_P]),
     "rtxllm_llama_weights_changed": (None, [_P]),
     "rtxllm_llama_region": (_P, [_P, ctypes.c_char_p, _U, _P]),
@@ -182,4 +199,4 @@ def check(name: str, code: int) -> None:
 
 
 __all__ = ["lib", "probe_lib", "check", "HipError", "exported_names", "LIB_PATH", "PROBE_LIB_PATH", "PackOptions",
-           "c_uint16"]
+           "PagedKVStruct", "c_uint16"]

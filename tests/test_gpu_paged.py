@@ -1,0 +1,386 @@
+"""The paged-cache operators (include/rtxllm/paged_kv.h) against float64 (paged_ref.py):
+append with norm and rotation, page bounds, page selection, attention over listed
+pages, attention that gathers weights, eviction. What lies behind a context is NaN or
+infinite throughout, tables are shuffled and may have holes."""
+
+from __future__ import annotations
+
+import numpy as np
+import paged_ref as ref
+import pytest
+
+torch = pytest.importorskip("torch")
+
+from rtxllm_amd import paged  # noqa: E402
+
+pytestmark = pytest.mark.gpu
+
+DEV = "cuda:0"
+
+
+def u32(values) -> torch.Tensor:
+    return torch.from_numpy(np.asarray(values, np.uint32).view(np.int32).copy()).to(DEV)
+
+
+def dev(a) -> torch.Tensor:
+    return torch.from_numpy(np.ascontiguousarray(a)).to(DEV)
+
+
+class Setup:
+    """A cache of len(lens) sequences; slots behind each length hold NaN and inf."""
+
+    def __init__(self, seed, lens, kv, dim, page, entries=None, hole=False, one=False, spare=3, stride=None):
+        rng = self.rng = np.random.default_rng(seed)
+        self.kv, self.dim, self.page, self.lens, self.one = kv, dim, page, lens, one
+        self.entries = entries or max(1, max(-(-n // page) for n in lens))
+        self.capacity = self.entries * page
+        self.n_pages = len(lens) * self.entries + spare
+        shape = (self.n_pages, kv, page, dim)
+        self.k = (0.9 * rng.standard_normal(shape) + 0.5 * rng.standard_normal((self.n_pages, kv, 1, dim))).astype(np.float16)
+        self.v = rng.standard_normal(shape).astype(np.float16)
+        self.table = rng.permutation(self.n_pages)[:len(lens) * self.entries].astype(np.int32).reshape(len(lens), -1)
+        self.seen = [[ref.at(self.table[i], self.n_pages, page, s) for s in range(n)] for i, n in enumerate(lens)]
+        poison = np.ones((self.n_pages, page), bool)
+        for row in self.seen:
+            for p, o in row:
+                poison[p, o] = False
+        for a, bad in ((self.k, np.nan), (self.v, np.inf)):
+            a[np.broadcast_to(poison[:, None, :, None], shape)] = bad
+            a[::2][np.broadcast_to(poison[::2, None, :, None], a[::2].shape)] = -np.inf
+        if hole:  # a page in the middle of the longest sequence is not there
+            i = int(np.argmax(lens))
+            t = max(0, -(-lens[i] // page) // 2)
+            self.table[i, t] = -1 if hole is True else hole
+            self.seen[i] = [ref.at(self.table[i], self.n_pages, page, s) for s in range(lens[i])]
+        self.kd, self.vd = dev(self.k), dev(self.v)
+        wide = np.full((len(lens), stride or self.entries), -7, np.int32)  # rows further apart than they are long
+        wide[:, :self.entries] = self.table
+        td = dev(wide)[:, :self.entries]
+        self.cache = paged.PagedKV(self.kd, self.vd, td[0].contiguous() if one else td)
+
+    def rows(self, i, g, slots):
+        """(keys, values, the slots that are there)."""
+        there = [s for s in slots if self.seen[i][s] is not None]
+        pick = [self.seen[i][s] for s in there]
+        p, o = np.array([x for x, _ in pick], int), np.array([x for _, x in pick], int)
+        return self.k[p, g, o], self.v[p, g, o], there
+
+    def last(self):
+        return [n - 1 if n else ref.NONE for n in self.lens]
+
+
+def close(got, want, tol, what):
+    bad = ~(np.abs(got.astype(np.float64) - want) <= tol)
+    assert not bad.any(), (what, np.argwhere(bad)[:4].tolist(), got[bad][:4], want[bad][:4], np.broadcast_to(tol, want.shape)[bad][:4])
+
+
+# ---- append --------------------------------------------------------------------
+
+# (query heads, kv heads, head_dim, page, rotary, pairing)
+APPEND = [(32, 8, 128, 64, 128, "halves"), (3, 1, 64, 5, 8, "adjacent"), (10, 2, 256, 24, 256, "halves"),
+          (7, 7, 128, 16, 64, "adjacent"), (16, 1, 256, 48, 72, "halves"), (1, 1, 64, 1, 64, "adjacent")]
+
+
+@pytest.mark.parametrize("shape", APPEND, ids=str)
+@pytest.mark.parametrize("mode", ["batch", "one-row", "prompt", "stacked-slots"])
+def test_append(shape, mode):
+    heads, kv, dim, page, rotary, pairing = shape
+    one = mode == "prompt"
+    count = {"batch": 5, "one-row": 1, "prompt": 37, "stacked-slots": 4}[mode]
+    s = Setup(heads + dim, [41] if one else [41] * count, kv, dim, page, one=one, hole=True, stride=60)
+    rng = s.rng
+    slot = np.arange(2, 2 + count) if one else rng.integers(0, 41, count)
+    pos = slot.astype(np.uint32)
+    if mode == "batch":
+        pos[3] = ref.NONE
+        pos[4] = s.capacity + 9  # no such slot: q alone
+    if mode == "stacked-slots":
+        pos = np.array([0, 131071, 4095, 2 ** 31 + 12345], np.uint32)
+        wide = rng.standard_normal((count, (heads + 2 * kv) * dim + 3)).astype(np.float32) * np.float32(20.0)
+        wide[0] *= np.float32(1e-6)
+        src = dev(wide)[:, 1:]
+        qd, kd, vd = src[:, :-2].split([heads * dim, kv * dim, kv * dim], 1)
+        x = wide[:, 1:-2]
+        q, k, v = (a.reshape(count, -1, dim) for a in np.split(x, [heads * dim, (heads + kv) * dim], 1))
+        qd, kd, vd = (t.unflatten(1, (-1, dim)) for t in (qd, kd, vd))
+    else:
+        q, k, v = (rng.standard_normal((count, h, dim)).astype(np.float32) for h in (heads, kv, kv))
+        qd, kd, vd = dev(q), dev(k), dev(v)
+    qw = (1.0 + 0.1 * rng.standard_normal(dim)).astype(np.float32)
+    kw = None if mode == "one-row" else (1.0 + 0.1 * rng.standard_normal(dim)).astype(np.float32)
+    nseq = len(s.lens)
+    slot_pos = rng.integers(0, 99, (nseq, kv, s.capacity)).astype(np.uint32)
+    weight = rng.random((nseq, kv, s.capacity)).astype(np.float32)
+    spd, wd = u32(slot_pos), dev(weight)
+    out = torch.full((count, heads, dim), 7.0, device=DEV)
+    use_slot = mode == "stacked-slots"
+    paged.qk_norm_rope_append(s.cache, qd, kd, vd, dev(qw), None if kw is None else dev(kw), u32(pos), theta=500000.0,
+                              eps=1e-6, rotary_dim=rotary, pairing=pairing, slot=u32(slot) if use_slot else None,
+                              q_out=out, slot_pos=spd, slot_weight=wd)
+    got, gk, gv = out.cpu().numpy(), s.kd.cpu().numpy(), s.vd.cpu().numpy()
+    k_want, v_want = s.k.copy(), s.v.copy()
+    # fp32: 8 products and 5 steps of the sum of squares, halved by the root, the mean, eps,
+    # root, quotient and two products; the angle's fraction and its sine; product and sum
+    eps32 = 24 * 2.0 ** -24
+    touched = np.zeros(s.k.shape, bool)
+    for r in range(count):
+        if pos[r] == ref.NONE:
+            assert np.all(got[r] == 7.0)
+            continue
+        for h in range(heads):
+            want, size = ref.norm_rope(q[r, h], qw, pos[r], 500000.0, 1e-6, rotary, pairing == "halves")
+            close(got[r, h], want, eps32 * size, (r, h))
+        sl = int(slot[r]) if use_slot else int(pos[r])
+        i = 0 if one else r
+        if sl >= s.capacity:
+            continue
+        slot_pos[i, :, sl], weight[i, :, sl] = pos[r], 0.0
+        place = ref.at(s.table[i], s.n_pages, page, sl)
+        if place is None:
+            continue
+        p, o = place
+        for g in range(kv):
+            want, size = ref.norm_rope(k[r, g], kw, pos[r], 500000.0, 1e-6, rotary, pairing == "halves")
+            close(gk[p, g, o], want, 2.0 ** -11 * np.abs(want) + 2 * eps32 * size + 2.0 ** -25, ("k", r, g))
+            v_want[p, g, o] = v[r, g].astype(np.float16)
+            touched[p, g, o] = True
+    np.testing.assert_array_equal(gk.view(np.uint16)[~touched], k_want.view(np.uint16)[~touched])
+    np.testing.assert_array_equal(gv.view(np.uint16), v_want.view(np.uint16))
+    np.testing.assert_array_equal(spd.cpu().numpy().view(np.uint32), slot_pos)
+    np.testing.assert_array_equal(wd.cpu().numpy(), weight)
+
+
+def test_append_in_place_and_extremes():
+    """q in place gives the bits of q apart; a zero head stays 0, one with a NaN is NaN,
+    a value beyond fp16 is stored as an infinity."""
+    s = Setup(3, [9, 9, 9], 2, 128, 4)
+    q, k, v = (s.rng.standard_normal((3, h, 128)).astype(np.float32) for h in (6, 2, 2))
+    q[0, 1], q[1, 2, 5], k[2, 0], v[2, 1, 3] = 0.0, np.nan, 0.0, 1e6
+    pos = u32([8, 3, 0])
+    qd = dev(q)
+    args = (dev(k), dev(v), None, None, pos)
+    apart = paged.qk_norm_rope_append(s.cache, qd, *args, theta=1e4).cpu().numpy()
+    paged.qk_norm_rope_append(s.cache, qd, *args, theta=1e4, q_out=qd)
+    np.testing.assert_array_equal(qd.cpu().numpy(), apart)
+    assert np.all(apart[0, 1] == 0.0) and np.isnan(apart[1, 2]).all() and not np.isnan(apart[1, 1]).any()
+    p = int(s.table[2, 0])
+    assert np.all(s.kd[p, 0, 0].cpu().numpy() == 0.0) and np.isinf(s.vd[p, 1, 0, 3].item())
+
+
+# ---- bounds and selection --------------------------------------------------------
+
+POOL = [(4, 128, 64), (2, 64, 16), (1, 256, 24), (3, 128, 7), (8, 64, 1)]
+
+
+@pytest.mark.parametrize("kv,dim,page", POOL)
+def test_page_bounds(kv, dim, page):
+    lens = [page * 9 + 1, 0, 1, page * 4, page * 6 + page // 2 + 1]
+    s = Setup(dim + page, lens, kv, dim, page, hole=True, stride=31)
+    p, o = s.seen[0][0]
+    s.k[p, 0, o, 3], s.k[p, 0, o, 5] = np.inf, -np.inf
+    s.k[p, :, :min(page, lens[0]), 7] = np.nan
+    s.kd.copy_(dev(s.k))
+    for first in (None, [0] * 5, [page + 1, 5, 0, page * 4, 0]):
+        span = 1 if first is None else 7
+        want = s.rng.standard_normal((s.n_pages, kv, 2, dim)).astype(np.float16)
+        bd = dev(want)
+        paged.page_bounds(s.cache, u32(s.last()), bd, None if first is None else u32(first), span)
+        for i, n in enumerate(lens):
+            f = n - 1 if first is None else first[i]
+            for t in range(f // page, min(f // page + span, -(-n // page))) if n and f < n else ():
+                page_at = int(s.table[i, t])
+                if page_at >= 0:
+                    for g in range(kv):
+                        want[page_at, g] = ref.bounds_of(s.k[page_at, g, :min(page, n - t * page)])
+        np.testing.assert_array_equal(bd.cpu().numpy(), want)
+
+
+@pytest.mark.parametrize("group", [1, 3, 8, 16])
+@pytest.mark.parametrize("kv,dim,page", POOL)
+@pytest.mark.parametrize("first,last,select", [(1, 1, 5), (0, 0, 1), (2, 3, 5), (0, 1, 64), (1, 2, 1000)])
+def test_select_pages(group, kv, dim, page, first, last, select):
+    lens = [page * 70 + 1, 0, 1, page * 4, page * 20]
+    s = Setup(dim + page + group, lens, kv, dim, page, hole=s_hole(select))
+    bounds = np.sort(s.rng.standard_normal((s.n_pages, kv, 2, dim)).astype(np.float16), axis=2)[:, :, ::-1]
+    for a, b in ((3, 9), (9, 30), (11, 12)):  # equal scores: the lower page
+        bounds[s.table[0, a]] = bounds[s.table[0, b]]
+    q = s.rng.standard_normal((5, group * kv, dim)).astype(np.float32)
+    q[4, 0, 1] = np.nan
+    pages = torch.full((5, kv, select), -9, dtype=torch.int32, device=DEV)
+    paged.select_pages(s.cache, dev(bounds), dev(q), u32(s.last()), select, first, last, pages=pages)
+    got = pages.cpu().numpy()
+    assert np.all(got[1] == -9)  # a padded row
+    for i, n in enumerate(lens):
+        for g in range(kv if n else 0):
+            want = ref.select(q[i, g * group:(g + 1) * group], bounds[:, g], s.table[i], s.n_pages, -(-n // page), first,
+                              last, select)
+            assert got[i, g].tolist() == want + [-1] * (select - len(want)), (i, g)
+
+
+def s_hole(select):
+    return select != 64
+
+
+def test_select_many_pages_with_ties():
+    """5000 pages of few distinct scores: ties across the whole radix, lowest first."""
+    s = Setup(1, [5000], 2, 64, 1)
+    levels = s.rng.standard_normal((6, 2, 2, 64)).astype(np.float16)
+    bounds = levels[s.rng.integers(0, 6, s.n_pages)]
+    q = s.rng.standard_normal((1, 4, 64)).astype(np.float32)
+    for select in (1, 700, 2049, 4999, 5000, 6000):
+        got = paged.select_pages(s.cache, dev(bounds), dev(q), u32([4999]), select, 3, 2).cpu().numpy() if select >= 5 else \
+            paged.select_pages(s.cache, dev(bounds), dev(q), u32([4999]), select, 0, 1).cpu().numpy()
+        for g in range(2):
+            f, l = (3, 2) if select >= 5 else (0, 1)
+            want = ref.select(q[0, 2 * g:2 * g + 2], bounds[:, g], s.table[0], s.n_pages, 5000, f, l, select)
+            assert got[0, g].tolist() == want + [-1] * (select - len(want))
+
+
+# ---- attention over listed pages ---------------------------------------------------
+
+ATTN = [(4, 8, 128, 64), (1, 2, 64, 16), (8, 1, 256, 24), (16, 2, 128, 7), (5, 3, 64, 1), (3, 1, 256, 40), (12, 1, 64, 128),
+        (16, 1, 256, 16)]
+
+
+def check_attention(s, got, q, i, g, group, slots, weight=None):
+    keys, values, there = s.rows(i, g, slots)
+    total = np.zeros(len(slots))
+    tol_w = np.zeros(len(slots))
+    index = {}
+    for j, sl in enumerate(slots):
+        index.setdefault(sl, []).append(j)
+    for h in range(g * group, (g + 1) * group):
+        p, o, tol, ptol = ref.attend(q[i, h], keys, values)
+        close(got[i, h], o, tol, (i, h))
+        for t, sl in enumerate(there):
+            total[index[sl][0]] += p[t]
+            tol_w[index[sl][0]] += ptol[t]
+    return total, tol_w
+
+
+@pytest.mark.parametrize("group,kv,dim,page", ATTN)
+@pytest.mark.parametrize("select", [1, 6, 33])
+def test_attn_pages(group, kv, dim, page, select):
+    lens = [page * 40 + page // 2 + 1, 0, 1, page * 3, page + 1]
+    s = Setup(group + dim + page, lens, kv, dim, page, hole=10 ** 6)
+    q = s.rng.standard_normal((5, group * kv, dim)).astype(np.float32)
+    q[0] *= np.float32(3.0)
+    q[3] *= np.float32(1e-7)
+    pages = np.full((5, kv, select), -1, np.int32)
+    for i, n in enumerate(lens):
+        used = -(-n // page)
+        for g in range(kv if n else 0):
+            some = s.rng.permutation(used)[:select]  # any order, and entries that name nothing between
+            pages[i, g, s.rng.permutation(select)[:len(some)]] = some
+            pages[i, g][(pages[i, g] < 0) & (s.rng.random(select) < 0.5)] = s.entries + 3
+    out = torch.full((5, group * kv, dim), 7.0, device=DEV)
+    paged.attn_pages(s.cache, dev(q), dev(pages), u32(s.last()), out=out)
+    got = out.cpu().numpy()
+    assert np.all(got[1] == 7.0)
+    for i, n in enumerate(lens):
+        for g in range(kv if n else 0):
+            listed = [t for t in pages[i, g] if 0 <= t < s.entries]
+            check_attention(s, got, q, i, g, group, [x for t in listed for x in range(t * page, min(n, t * page + page))])
+
+
+def test_attn_pages_empty_twice_and_extremes():
+    s = Setup(5, [64, 64, 64, 64, 64], 1, 128, 16)
+    q = s.rng.standard_normal((5, 2, 128)).astype(np.float32)
+    q[3, 0] *= np.float32(1e30)  # one position takes all
+    q[4, 1, 9] = np.nan
+    pages = np.array([[-1, -1, -1], [2, 2, 0], [3, -1, 99], [0, 1, 2], [0, 1, 2]], np.int32)[:, None]
+    got = paged.attn_pages(s.cache, dev(q), dev(pages), u32([63] * 5)).cpu().numpy()
+    assert np.all(got[0] == 0.0)  # nothing listed
+    check_attention(s, got, q, 1, 0, 2, [*range(32, 48), *range(32, 48), *range(16)])
+    check_attention(s, got, q, 2, 0, 2, range(48, 64))
+    keys, values, _ = s.rows(3, 0, range(48))
+    np.testing.assert_allclose(got[3, 0], values[np.argmax(keys.astype(np.float64) @ q[3, 0])], rtol=1e-6)
+    assert np.isnan(got[4, 1]).all() and np.isfinite(got[4, 0]).all()
+    # a sequence whose table names no page at all
+    s.cache.block_table[1] = -1
+    assert np.all(paged.attn_pages(s.cache, dev(q), dev(pages), u32([63] * 5)).cpu().numpy()[1] == 0.0)
+
+
+# ---- attention that gathers weights, eviction ----------------------------------------
+
+
+@pytest.mark.parametrize("group,kv,dim,page", ATTN)
+@pytest.mark.parametrize("place", ["apart", "in-place"])
+def test_attn_weights(group, kv, dim, page, place):
+    lens = [page * 17 + page // 3 + 1, 0, 1, page * 3, page + 1, 2]
+    s = Setup(group + dim + page, lens, kv, dim, page, entries=19, hole=True)
+    q = s.rng.standard_normal((6, group * kv, dim)).astype(np.float32)
+    weight = s.rng.random((6, kv, s.capacity)).astype(np.float32)
+    wd = dev(weight)
+    wo = None if place == "in-place" else torch.full_like(wd, 7.0)
+    out = torch.full((6, group * kv, dim), 7.0, device=DEV)
+    paged.attn_weights(s.cache, dev(q), u32(s.last()), wd, wo, out)
+    got, gw = out.cpu().numpy(), (wd if wo is None else wo).cpu().numpy()
+    behind = weight if wo is None else np.full_like(weight, 7.0)
+    for i, n in enumerate(lens):
+        np.testing.assert_array_equal(gw[i, :, n:], behind[i, :, n:])
+        for g in range(kv if n else 0):
+            total, tol = check_attention(s, got, q, i, g, group, list(range(n)))
+            want = weight[i, g, :n] + total
+            close(gw[i, g, :n], want, tol + (group + 1) * 2.0 ** -24 * want, ("weight", i, g))
+    assert np.all(got[1] == 7.0)
+
+
+def test_attn_weights_long():
+    """Many splits, several rounds of tiles a wave, a chunk boundary of the gathering."""
+    s = Setup(2, [9000, 2049], 1, 128, 64)
+    q = s.rng.standard_normal((2, 4, 128)).astype(np.float32)
+    weight = np.zeros((2, 1, s.capacity), np.float32)
+    wd = dev(weight)
+    got = paged.attn_weights(s.cache, dev(q), u32(s.last()), wd).cpu().numpy()
+    for i, n in enumerate(s.lens):
+        total, tol = check_attention(s, got, q, i, 0, 4, list(range(n)))
+        close(wd.cpu().numpy()[i, 0, :n], total, tol + 5 * 2.0 ** -24 * total, i)
+        assert abs(float(wd[i, 0].sum()) - 4.0) < 1e-4
+
+
+@pytest.mark.parametrize("kv,dim,page", POOL)
+@pytest.mark.parametrize("keep,first,recent", [(1, 0, 0), (30, 2, 9), (30, 30, 0), (64, 0, 64), (100, 3, 20)])
+@pytest.mark.parametrize("place", ["apart", "in-place"])
+def test_evict(kv, dim, page, keep, first, recent, place):
+    lens = [130, 0, 1, keep, keep + 1, 97, 111]
+    entries = -(-(130 + keep) // page)
+    s = Setup(dim + page + keep, lens, kv, dim, page, entries=entries)
+    rng, n_rows = s.rng, len(lens)
+    weight = (rng.integers(0, 9, (n_rows, kv, s.capacity)) / 8).astype(np.float32)  # many ties
+    weight[0, :, ::7], weight[0, :, 3], weight[5, :, 5] = np.nan, np.inf, -0.0
+    slot_pos = np.stack([[rng.permutation(s.capacity) for _ in range(kv)] for _ in range(n_rows)]).astype(np.uint32)
+    pos = [int(slot_pos[i, :, :n].max()) if n else 0 for i, n in enumerate(lens)]
+    pos[6] = ref.NONE
+    length = np.array([ref.NONE if i == 0 else n for i, n in enumerate(lens)], np.uint32)  # more than capacity: capacity
+    lens[0] = s.capacity
+    s.seen[0] = [ref.at(s.table[0], s.n_pages, page, sl) for sl in range(s.capacity)]
+    pos[0] = int(slot_pos[0].max())
+    wd, sd, ld = dev(weight), u32(slot_pos), u32(length)
+    outs = dict(weight_out=None, slot_pos_out=None, length_out=None) if place == "in-place" else dict(
+        weight_out=torch.full_like(wd, 7.0), slot_pos_out=torch.full_like(sd, 5), length_out=torch.full_like(ld, 3))
+    paged.evict(s.cache, ld, u32(pos), keep, wd, sd, first, recent, **outs)
+    gw = (outs["weight_out"] if outs["weight_out"] is not None else wd).cpu().numpy()
+    gp = (outs["slot_pos_out"] if outs["slot_pos_out"] is not None else sd).cpu().numpy().view(np.uint32)
+    gl = (outs["length_out"] if outs["length_out"] is not None else ld).cpu().numpy().view(np.uint32)
+    k_want, v_want = s.k.copy(), s.v.copy()
+    w_want, p_want = (weight.copy(), slot_pos.copy()) if place == "in-place" else (np.full_like(weight, 7.0),
+                                                                                 np.full_like(slot_pos, 5))
+    l_want = length.copy() if place == "in-place" else np.full_like(length, 3)
+    for i, n in enumerate(lens):
+        if pos[i] == ref.NONE:
+            continue
+        l_want[i] = min(n, keep)
+        for g in range(kv):
+            src = ref.evict(n, pos[i], keep, first, recent, weight[i, g], slot_pos[i, g])
+            src = list(range(n)) if src is None else src
+            w_want[i, g, :len(src)], p_want[i, g, :len(src)] = weight[i, g, src], slot_pos[i, g, src]
+            for to, of in enumerate(src):
+                if to != of:
+                    (p, o), (p2, o2) = s.seen[i][to], s.seen[i][of]
+                    k_want[p, g, o], v_want[p, g, o] = s.k[p2, g, o2], s.v[p2, g, o2]
+    np.testing.assert_array_equal(gl, l_want)
+    np.testing.assert_array_equal(gp, p_want)
+    np.testing.assert_array_equal(gw, w_want)
+    np.testing.assert_array_equal(s.kd.cpu().numpy().view(np.uint16), k_want.view(np.uint16))
+    np.testing.assert_array_equal(s.vd.cpu().numpy().view(np.uint16), v_want.view(np.uint16))
