@@ -12,6 +12,8 @@ namespace {
 constexpr std::uint32_t kThreads = 256;
 constexpr std::uint32_t kSelThreads = 1024, kSelWaves = kSelThreads / 64u;
 
+typedef std::uint32_t u32x4_any __attribute__((ext_vector_type(4), aligned(4)));
+
 __device__ __forceinline__ double lane_xor_d(double v, int mask) { return __shfl_xor(v, mask, 64); }
 
 // A score as an unsigned key of the same order: 1 for NaN, so that 0 is left for
@@ -79,112 +81,251 @@ struct Choice {
   std::uint32_t ties;
 };
 
+constexpr std::uint32_t kAllTies = 0xFFFFFFFFu;
+constexpr int kDigit = 11;  // bits of a pass
+constexpr std::uint32_t kBins = 1u << kDigit;
+static_assert(kBins == 2u * kSelThreads, "two bins a thread");
+
 struct SelectShared {
-  std::uint32_t hist[4096];
-  std::uint32_t wave[kSelWaves], bin, above, count;
+  std::uint32_t hist[2][kBins];
+  std::uint32_t wave[3][kSelWaves];
+  std::uint32_t bin, above, count;
 };
 
-// Radix selection from the top, 12 bits a pass: the workgroup counts the keys
-// that share the digits found so far by their next digit, and takes the digit in
-// which the k-th largest lies. It ends early once all keys of that digit are
-// wanted. key(i) is read anew in every pass (its array stays in the L2).
-template <class K, class Key>
-__device__ Choice<K> radix_choice(SelectShared& sh, std::uint32_t n, std::uint32_t k, Key key) {
+// Inclusive sum over the lanes below and the lane itself, by DPP.
+__device__ __forceinline__ std::uint32_t wave_scan(std::uint32_t v) {
+  auto add = [&](auto ctrl, auto rows) {
+    v += static_cast<std::uint32_t>(
+        __builtin_amdgcn_update_dpp(0, static_cast<int>(v), decltype(ctrl)::value, decltype(rows)::value, 0xF, false));
+  };
+  constexpr std::integral_constant<int, 0xF> all{};
+  add(std::integral_constant<int, 0x111>{}, all);  // row_shr:1, 2, 4, 8
+  add(std::integral_constant<int, 0x112>{}, all);
+  add(std::integral_constant<int, 0x114>{}, all);
+  add(std::integral_constant<int, 0x118>{}, all);
+  // a row's last lane into the next row (rows 1, 3), then of row 1 into rows 2 and 3
+  add(std::integral_constant<int, 0x142>{}, std::integral_constant<int, 0xA>{});
+  add(std::integral_constant<int, 0x143>{}, std::integral_constant<int, 0xC>{});
+  return v;
+}
+
+// Sum of the waves' words before this wave, and of all.
+__device__ __forceinline__ uint2 waves_before(const std::uint32_t* words, std::uint32_t wave) {
+  uint2 s = make_uint2(0u, 0u);
+#pragma unroll
+  for (std::uint32_t w = 0; w < kSelWaves; w += 4u) {
+    const uint4 x = *reinterpret_cast<const uint4*>(words + w);
+    s.x += (w < wave ? x.x : 0u) + (w + 1u < wave ? x.y : 0u) + (w + 2u < wave ? x.z : 0u) + (w + 3u < wave ? x.w : 0u);
+    s.y += (x.x + x.y) + (x.z + x.w);
+  }
+  return s;
+}
+
+// The keys of a workgroup: a wave's part contiguous, four keys a lane and round, so
+// that loads are wide and ranks follow from ballots. Up to `room` keys are read
+// once and stay in the LDS, each thread's own where it alone reads them; of more,
+// every pass reads all again (from the L2). The loops are rolled: each runs a few
+// rounds once, and unrolled code with the keys in registers took longer to fetch
+// (32 keys a thread: 92 us for 32768 keys). load(i, x): keys i..i + 3, i % 4 == 0.
+template <class K, class Load>
+struct Keys {
+  struct alignas(16) Four {
+    K k[4];
+  };
+  const Load& load;
+  Four* held;
+  std::uint32_t n, rounds, first;  // rounds of a wave, first key of its own
+  bool in_lds;
+
+  __device__ __forceinline__ Keys(const Load& l, void* lds, std::uint32_t count, std::uint32_t room)
+      : load(l), held(static_cast<Four*>(lds) + threadIdx.x), n(count), in_lds(count <= room) {
+    rounds = (n + 4u * kSelThreads - 1u) / (4u * kSelThreads);
+    first = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) * 256u * rounds;
+    if (in_lds)
+      for (std::uint32_t j = 0; j < rounds && first + 256u * j < n; ++j) load(place(j), held[kSelThreads * j].k);
+  }
+  __device__ __forceinline__ std::uint32_t place(std::uint32_t j) const {
+    return first + 256u * j + 4u * (threadIdx.x & 63u);
+  }
+  // body(four keys, index of the first) for each round of the wave
+  template <class Body>
+  __device__ __forceinline__ void each(Body body) const {
+    for (std::uint32_t j = 0; j < rounds && first + 256u * j < n; ++j) {
+      Four f;
+      if (in_lds)
+        f = held[kSelThreads * j];
+      else
+        load(place(j), f.k);
+      body(f.k, place(j));
+    }
+  }
+};
+
+// Radix selection from the top, 11 bits a pass: the workgroup counts the keys that
+// share the digits found so far by their next digit, and takes the digit in which
+// the k-th largest lies. It ends early once all keys of that digit are wanted,
+// after two or three passes where keys are spread. Lanes that all count the same
+// digit (equal keys) add once, as one address takes one addition at a time.
+template <class K, class Load>
+__device__ Choice<K> radix_choice(SelectShared& sh, const Keys<K, Load>& keys, std::uint32_t k) {
   constexpr int kBits = static_cast<int>(8u * sizeof(K));
-  const std::uint32_t tid = threadIdx.x, lane = tid & 63u, wave = tid >> 6;
-  if (k >= n) return Choice<K>{0, 0xFFFFFFFFu};
+  const std::uint32_t tid = threadIdx.x, lane = tid & 63u, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  if (k >= keys.n) return Choice<K>{0, kAllTies};
+  reinterpret_cast<uint2*>(sh.hist[0])[tid] = make_uint2(0u, 0u);
+  __syncthreads();
   K prefix = 0;
   int shift = kBits;
-  for (;;) {
-    const int bits = shift < 12 ? shift : 12;
-    const int next = shift - bits;
-    for (std::uint32_t i = tid; i < 4096u; i += kSelThreads) sh.hist[i] = 0u;
-    __syncthreads();
-    for (std::uint32_t i = tid; i < n; i += kSelThreads) {
-      const K x = key(i);
-      if (shift == kBits || (x >> shift) == prefix) atomicAdd(&sh.hist[static_cast<std::uint32_t>(x >> next) & ((1u << bits) - 1u)], 1u);
-    }
-    __syncthreads();
-    // thread t holds the four digits 4 (1023 - t) .. + 3: sums from the largest digit down
-    const uint4 d = reinterpret_cast<const uint4*>(sh.hist)[kSelThreads - 1u - tid];
-    const std::uint32_t mine = d.x + d.y + d.z + d.w;
-    std::uint32_t sum = mine;
+  for (std::uint32_t turn = 0;; turn ^= 1u) {
+    const int bits = shift < kDigit ? shift : kDigit, next = shift - bits;
+    std::uint32_t* const hist = sh.hist[turn];
+    keys.each([&](const K (&x)[4], std::uint32_t i) {
 #pragma unroll
-    for (int m = 1; m < 64; m *= 2) {
-      const std::uint32_t o = __shfl_up(sum, m, 64);
-      sum += lane >= static_cast<std::uint32_t>(m) ? o : 0u;
-    }
-    if (lane == 63u) sh.wave[wave] = sum;
+      for (int e = 0; e < 4; ++e) {
+        const bool match = i + e < keys.n && (shift == kBits || (x[e] >> shift) == prefix);
+        const std::uint32_t digit = static_cast<std::uint32_t>(x[e] >> next) & ((1u << bits) - 1u);
+        const unsigned long long who = __ballot(match);
+        if (who == 0ull) continue;
+        const std::uint32_t one = __builtin_amdgcn_readlane(digit, static_cast<int>(__builtin_ctzll(who)));
+        if (__ballot(match && digit == one) == who) {
+          if (lane == 0u) atomicAdd(&hist[one], static_cast<std::uint32_t>(__popcll(who)));
+        } else if (match) {
+          atomicAdd(&hist[digit], 1u);
+        }
+      }
+    });
     __syncthreads();
-    std::uint32_t before = sum - mine;
-    for (std::uint32_t w = 0; w < wave; ++w) before += sh.wave[w];
-    if (before < k && k <= before + mine) {
-      const std::uint32_t c[4] = {d.w, d.z, d.y, d.x};
-      std::uint32_t j = 0;
-      while (before + c[j] < k) before += c[j++];
-      sh.bin = 4u * (kSelThreads - 1u - tid) + 3u - j;
-      sh.above = before;
-      sh.count = c[j];
+    // thread t: bins 2047 - 2 t and 2046 - 2 t, sums from the largest digit down
+    const uint2 c = reinterpret_cast<const uint2*>(hist)[kSelThreads - 1u - tid];
+    reinterpret_cast<uint2*>(sh.hist[turn ^ 1u])[tid] = make_uint2(0u, 0u);
+    const std::uint32_t sum = wave_scan(c.x + c.y);
+    if (lane == 63u) sh.wave[0][wave] = sum;
+    __syncthreads();
+    const std::uint32_t before = waves_before(sh.wave[0], wave).x + sum - (c.x + c.y);
+    if (before < k && k <= before + c.x + c.y) {
+      const bool upper = k <= before + c.y;
+      sh.bin = 2u * (kSelThreads - 1u - tid) + (upper ? 1u : 0u);
+      sh.above = upper ? before : before + c.y;
+      sh.count = upper ? c.y : c.x;
     }
     __syncthreads();
     prefix = (prefix << bits) | static_cast<K>(sh.bin);
     k -= sh.above;
-    const std::uint32_t count = sh.count;
     shift = next;
-    __syncthreads();
-    if (count == k) return Choice<K>{static_cast<K>(prefix << shift), 0xFFFFFFFFu};
+    if (sh.count == k) return Choice<K>{static_cast<K>(prefix << shift), kAllTies};
     if (shift == 0) return Choice<K>{prefix, k};
   }
 }
 
-// Walks keys 0..n-1 in order, 1024 at a time: body(i, chosen, rank), rank the
-// number of chosen keys before i. Every thread calls body for its own i < n.
-template <class K, class Key, class Body>
-__device__ void for_chosen(SelectShared& sh, std::uint32_t n, const Choice<K>& ch, Key key, Body body) {
-  const std::uint32_t tid = threadIdx.x, lane = tid & 63u, wave = tid >> 6;
-  std::uint32_t base_over = 0, base_tie = 0;
-  for (std::uint32_t i0 = 0; i0 < n; i0 += kSelThreads) {
-    const std::uint32_t i = i0 + tid;
-    const K x = i < n ? key(i) : 0;
-    const bool all = ch.ties == 0xFFFFFFFFu;
-    const bool over = i < n && (all ? x >= ch.least : x > ch.least), tie = i < n && !all && x == ch.least;
-    const unsigned long long bo = __ballot(over), bt = __ballot(tie), below = (1ull << lane) - 1ull;
-    if (lane == 0u) sh.wave[wave] = static_cast<std::uint32_t>(__popcll(bo)) << 16 | static_cast<std::uint32_t>(__popcll(bt));
+// Walks the keys in two classes: kind(i, chosen) is 0 (neither), 1 or 2, put(kind, i,
+// rank) gets a place of a class with the number of those of the class before it.
+// Returns the sizes of both.
+template <class K, class Load, class Kind, class Put>
+__device__ uint2 for_chosen(SelectShared& sh, const Keys<K, Load>& keys, const Choice<K>& ch, Kind kind, Put put) {
+  const std::uint32_t tid = threadIdx.x, lane = tid & 63u, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const unsigned long long below = (1ull << lane) - 1ull;
+  const bool all = ch.ties == kAllTies;
+  std::uint32_t ties_before = 0;
+  if (!all) {
+    std::uint32_t mine = 0;
+    keys.each([&](const K (&x)[4], std::uint32_t i) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) mine += static_cast<std::uint32_t>(__popcll(__ballot(i + e < keys.n && x[e] == ch.least)));
+    });
+    if (lane == 0u) sh.wave[0][wave] = mine;
     __syncthreads();
-    std::uint32_t no = 0, nt = 0, total_o = 0, total_t = 0;
-    for (std::uint32_t w = 0; w < kSelWaves; ++w) {
-      const std::uint32_t v = sh.wave[w];
-      no += w < wave ? v >> 16 : 0u, nt += w < wave ? v & 0xFFFFu : 0u;
-      total_o += v >> 16, total_t += v & 0xFFFFu;
-    }
-    no += base_over + static_cast<std::uint32_t>(__popcll(bo & below));
-    nt += base_tie + static_cast<std::uint32_t>(__popcll(bt & below));
-    if (i < n) body(i, over || (tie && nt < ch.ties), no + (nt < ch.ties ? nt : ch.ties));
-    base_over += total_o, base_tie += total_t;
-    __syncthreads();
+    ties_before = waves_before(sh.wave[0], wave).x;
   }
+  // the classes of a round's four places, 2 bits each; `ties`: equal keys before the round
+  auto classes = [&](const K (&x)[4], std::uint32_t i, std::uint32_t& ties) {
+    std::uint32_t c = 0u;
+    unsigned long long tie[4];
+    std::uint32_t at = ties;
+    if (!all) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        tie[e] = __ballot(i + e < keys.n && x[e] == ch.least);
+        at += static_cast<std::uint32_t>(__popcll(tie[e] & below));
+        ties += static_cast<std::uint32_t>(__popcll(tie[e]));
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      bool chosen = x[e] >= ch.least;
+      if (!all && x[e] == ch.least) chosen = at++ < ch.ties;
+      c |= i + e < keys.n ? static_cast<std::uint32_t>(kind(i + e, chosen)) << (2 * e) : 0u;
+    }
+    return c;
+  };
+  std::uint32_t n1 = 0, n2 = 0, ties = ties_before;
+  keys.each([&](const K (&x)[4], std::uint32_t i) {
+    const std::uint32_t c = classes(x, i, ties);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      n1 += static_cast<std::uint32_t>(__popcll(__ballot((c >> (2 * e) & 3u) == 1u)));
+      n2 += static_cast<std::uint32_t>(__popcll(__ballot((c >> (2 * e) & 3u) == 2u)));
+    }
+  });
+  if (lane == 0u) sh.wave[1][wave] = n1, sh.wave[2][wave] = n2;
+  __syncthreads();
+  const uint2 w1 = waves_before(sh.wave[1], wave), w2 = waves_before(sh.wave[2], wave);
+  std::uint32_t at1 = w1.x, at2 = w2.x;
+  ties = ties_before;
+  keys.each([&](const K (&x)[4], std::uint32_t i) {
+    const std::uint32_t c = classes(x, i, ties);
+    std::uint32_t r1 = at1, r2 = at2;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const unsigned long long b1 = __ballot((c >> (2 * e) & 3u) == 1u), b2 = __ballot((c >> (2 * e) & 3u) == 2u);
+      r1 += static_cast<std::uint32_t>(__popcll(b1 & below)), at1 += static_cast<std::uint32_t>(__popcll(b1));
+      r2 += static_cast<std::uint32_t>(__popcll(b2 & below)), at2 += static_cast<std::uint32_t>(__popcll(b2));
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const std::uint32_t k = c >> (2 * e) & 3u;
+      if (k == 1u) put(1, i + e, r1++);
+      if (k == 2u) put(2, i + e, r2++);
+    }
+  });
+  return make_uint2(w1.y, w2.y);
 }
 
+// LDS bytes for n keys of `width` bytes, up to 128 KB, in whole rounds of a workgroup.
+std::size_t held_bytes(std::uint32_t n, std::size_t width) {
+  const std::size_t round = 4u * kSelThreads * width, rounds = (n * width + round - 1u) / round;
+  return round * rounds < (128u << 10) ? round * rounds : 128u << 10;
+}
+
+typedef unsigned long long u64x4 __attribute__((ext_vector_type(4), aligned(8)));
+
 __global__ __launch_bounds__(kSelThreads) void page_choice_kernel(PagedView kv, const std::uint32_t* __restrict__ pos,
-                                                                  const unsigned long long* __restrict__ keys,
-                                                                  std::uint32_t n_select,
+                                                                  const unsigned long long* __restrict__ row_keys,
+                                                                  std::uint32_t room, std::uint32_t n_select,
                                                                   std::int32_t* __restrict__ pages) {
   __shared__ __align__(16) SelectShared sh;
-  __shared__ std::uint32_t listed;
+  extern __shared__ __align__(16) std::uint8_t lds[];
   const std::uint32_t g = blockIdx.x, r = blockIdx.y;
   const std::uint32_t used = (paged_filled(kv, pos[r]) + kv.page_size - 1u) / kv.page_size;
   if (used == 0u) return;  // a padded row
-  const unsigned long long* const row = keys + (static_cast<std::size_t>(r) * kv.n_kv + g) * kv.entries;
+  const unsigned long long* const row = row_keys + (static_cast<std::size_t>(r) * kv.n_kv + g) * kv.entries;
   std::int32_t* const out = pages + (static_cast<std::size_t>(r) * kv.n_kv + g) * n_select;
-  auto key = [&](std::uint32_t i) { return row[i]; };
-  Choice<unsigned long long> ch = radix_choice<unsigned long long>(sh, used, n_select, key);
-  if (ch.least == 0ull) ch = Choice<unsigned long long>{1ull, 0xFFFFFFFFu};  // every candidate, and no page that is not there
-  if (threadIdx.x == 0u) listed = 0u;
-  __syncthreads();
-  for_chosen(sh, used, ch, key, [&](std::uint32_t i, bool chosen, std::uint32_t rank) {
-    if (chosen && rank < n_select) out[rank] = static_cast<std::int32_t>(i);
-    if (i + 1u == used) listed = rank + (chosen ? 1u : 0u);
-  });
+  auto load = [&](std::uint32_t i, unsigned long long (&x)[4]) {
+    if (i + 4u <= used) {
+      const u64x4 v = *reinterpret_cast<const u64x4*>(row + i);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[e] = v[e];
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[e] = i + e < used ? row[i + e] : 0ull;
+    }
+  };
+  const Keys<unsigned long long, decltype(load)> keys(load, lds, used, room);
+  Choice<unsigned long long> ch = radix_choice(sh, keys, n_select);
+  if (ch.least == 0ull) ch = Choice<unsigned long long>{1ull, kAllTies};  // every candidate, and no page that is not there
+  const std::uint32_t listed = for_chosen(
+      sh, keys, ch, [](std::uint32_t, bool chosen) { return chosen ? 1 : 0; },
+      [&](int, std::uint32_t i, std::uint32_t rank) {
+        if (rank < n_select) out[rank] = static_cast<std::int32_t>(i);
+      }).x;
   for (std::uint32_t i = listed + threadIdx.x; i < n_select; i += kSelThreads) out[i] = -1;
 }
 
@@ -207,12 +348,12 @@ struct EvictArgs {
   float* weight_out;
   std::uint32_t* slot_pos_out;
   std::uint32_t* moves;
-  std::uint32_t keep, n_first, n_recent, most;
+  std::uint32_t keep, n_first, n_recent, most, room;
 };
 
 __global__ __launch_bounds__(kSelThreads) void evict_choice_kernel(PagedView kv, EvictArgs a) {
   __shared__ __align__(16) SelectShared sh;
-  __shared__ std::uint32_t below;
+  extern __shared__ __align__(16) std::uint8_t lds[];
   const std::uint32_t g = blockIdx.x, r = blockIdx.y, tid = threadIdx.x;
   const std::size_t gr = static_cast<std::size_t>(r) * kv.n_kv + g;
   std::uint32_t* const moves = a.moves + gr * (1u + 2u * static_cast<std::size_t>(a.most));
@@ -233,30 +374,39 @@ __global__ __launch_bounds__(kSelThreads) void evict_choice_kernel(PagedView kv,
     if (tid == 0u) moves[0] = 0u;
     return;
   }
-  auto key = [&](std::uint32_t i) { return weight_key(w[i], p[i], newest, a.n_first, a.n_recent); };
-  const Choice<std::uint32_t> ch = radix_choice<std::uint32_t>(sh, n, a.keep, key);
-  if (tid == 0u) below = 0u;
-  __syncthreads();
+  auto load = [&](std::uint32_t i, std::uint32_t (&x)[4]) {
+    f32x4_any wv = {0.0f, 0.0f, 0.0f, 0.0f};
+    u32x4_any pv = {0u, 0u, 0u, 0u};
+    if (i + 4u <= n) {
+      wv = *reinterpret_cast<const f32x4_any*>(w + i);
+      pv = *reinterpret_cast<const u32x4_any*>(p + i);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (i + e < n) wv[e] = w[i + e], pv[e] = p[i + e];
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) x[e] = weight_key(wv[e], pv[e], newest, a.n_first, a.n_recent);
+  };
+  const Keys<std::uint32_t, decltype(load)> keys(load, lds, n, a.room);
+  const Choice<std::uint32_t> ch = radix_choice(sh, keys, a.keep);
   std::uint32_t* const to = moves + 1u;
   std::uint32_t* const from = to + a.most;
-  for_chosen(sh, n, ch, key, [&](std::uint32_t i, bool chosen, std::uint32_t rank) {
-    if (i < a.keep && !chosen && i - rank < a.most) to[i - rank] = i;
-    if (i + 1u == a.keep) below = rank + (chosen ? 1u : 0u);
-  });
-  __syncthreads();
-  const std::uint32_t kept_below = below, n_moves = a.keep - kept_below < a.most ? a.keep - kept_below : a.most;
-  for_chosen(sh, n, ch, key, [&](std::uint32_t i, bool chosen, std::uint32_t rank) {
-    if (i >= a.keep && chosen && rank - kept_below < a.most) from[rank - kept_below] = i;
-  });
+  const std::uint32_t holes = for_chosen(
+      sh, keys, ch,
+      [&](std::uint32_t i, bool chosen) { return i < a.keep ? (chosen ? 0 : 1) : (chosen ? 2 : 0); },
+      [&](int kind, std::uint32_t i, std::uint32_t m) {
+        if (m < a.most) (kind == 1 ? to : from)[m] = i;
+      }).x;
+  const std::uint32_t n_moves = holes < a.most ? holes : a.most;
   if (tid == 0u) moves[0] = n_moves;
-  __threadfence_block();
-  __syncthreads();
   // every slot that is written lies below keep, every moved one at or behind it: in
   // place, no read meets a write of another thread
   if (wo != w)
     for (std::uint32_t i = tid; i < stay; i += kSelThreads) wo[i] = w[i];
   if (po != p)
     for (std::uint32_t i = tid; i < stay; i += kSelThreads) po[i] = p[i];
+  __threadfence_block();
   __syncthreads();
   for (std::uint32_t m = tid; m < n_moves; m += kSelThreads) {
     wo[to[m]] = w[from[m]];
@@ -329,7 +479,9 @@ extern "C" hipError_t rtxllm_attn_select_pages(const rtxllm_paged_kv* cache, con
     hipLaunchKernelGGL(page_score_kernel<32>, grid, dim3(kThreads), 0, stream, view, bounds, q, group, pos, n_first, n_last, keys);
   hipError_t rc = hipGetLastError();
   if (rc != hipSuccess) return rc;
-  hipLaunchKernelGGL(page_choice_kernel, dim3(view.n_kv, count), dim3(kSelThreads), 0, stream, view, pos, keys, n_select, pages);
+  const std::size_t held = held_bytes(view.entries, 8u);
+  hipLaunchKernelGGL(page_choice_kernel, dim3(view.n_kv, count), dim3(kSelThreads), held, stream, view, pos, keys,
+                     static_cast<std::uint32_t>(held / 8u), n_select, pages);
   return hipGetLastError();
 }
 
@@ -364,9 +516,10 @@ extern "C" hipError_t rtxllm_kv_evict_f16(const rtxllm_paged_kv* cache, const ui
     return hipErrorInvalidValue;
   const PagedView view = paged_view(cache);
   const std::uint32_t most = most_moves(cache, keep), per = kThreads / (cache->head_dim / 8u);
+  const std::size_t held = held_bytes(view.capacity, 4u);
   const EvictArgs a{length, pos, weight, slot_pos, weight_out, slot_pos_out, static_cast<std::uint32_t*>(workspace),
-                    keep,   n_first, n_recent, most};
-  hipLaunchKernelGGL(evict_choice_kernel, dim3(view.n_kv, count), dim3(kSelThreads), 0, stream, view, a);
+                    keep,   n_first, n_recent, most, static_cast<std::uint32_t>(held / 4u)};
+  hipLaunchKernelGGL(evict_choice_kernel, dim3(view.n_kv, count), dim3(kSelThreads), held, stream, view, a);
   hipError_t rc = hipGetLastError();
   if (rc != hipSuccess) return rc;
   const dim3 grid(most > 0u ? (most + per - 1u) / per : 1u, view.n_kv, count);

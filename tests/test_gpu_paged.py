@@ -221,18 +221,19 @@ def s_hole(select):
     return select != 64
 
 
-def test_select_many_pages_with_ties():
-    """5000 pages of few distinct scores: ties across the whole radix, lowest first."""
-    s = Setup(1, [5000], 2, 64, 1)
+@pytest.mark.parametrize("n", [5000, 16384, 16385, 33000])
+def test_select_many_pages_with_ties(n):
+    """Thousands of pages of few distinct scores: ties across the whole radix, lowest
+    first; more pages than a workgroup holds at once."""
+    s = Setup(1, [n], 2, 64, 1)
     levels = s.rng.standard_normal((6, 2, 2, 64)).astype(np.float16)
     bounds = levels[s.rng.integers(0, 6, s.n_pages)]
     q = s.rng.standard_normal((1, 4, 64)).astype(np.float32)
-    for select in (1, 700, 2049, 4999, 5000, 6000):
-        got = paged.select_pages(s.cache, dev(bounds), dev(q), u32([4999]), select, 3, 2).cpu().numpy() if select >= 5 else \
-            paged.select_pages(s.cache, dev(bounds), dev(q), u32([4999]), select, 0, 1).cpu().numpy()
+    for select in (1, 700, 2049, n - 1, n, n + 1000):
+        f, l = (3, 2) if select >= 5 else (0, 1)
+        got = paged.select_pages(s.cache, dev(bounds), dev(q), u32([n - 1]), select, f, l).cpu().numpy()
         for g in range(2):
-            f, l = (3, 2) if select >= 5 else (0, 1)
-            want = ref.select(q[0, 2 * g:2 * g + 2], bounds[:, g], s.table[0], s.n_pages, 5000, f, l, select)
+            want = ref.select(q[0, 2 * g:2 * g + 2], bounds[:, g], s.table[0], s.n_pages, n, f, l, select)
             assert got[0, g].tolist() == want + [-1] * (select - len(want))
 
 
@@ -384,3 +385,29 @@ def test_evict(kv, dim, page, keep, first, recent, place):
     np.testing.assert_array_equal(gw, w_want)
     np.testing.assert_array_equal(s.kd.cpu().numpy().view(np.uint16), k_want.view(np.uint16))
     np.testing.assert_array_equal(s.vd.cpu().numpy().view(np.uint16), v_want.view(np.uint16))
+
+
+@pytest.mark.parametrize("n,keep", [(32768, 100), (32769, 32768), (70001, 40000)])
+@pytest.mark.parametrize("levels", [1, 5, 0])
+def test_evict_long(n, keep, levels):
+    """More slots than a workgroup holds at once; equal weights, few distinct ones, all distinct."""
+    s = Setup(n, [n], 2, 64, 7)
+    weight = s.rng.standard_normal((1, 2, s.capacity)).astype(np.float32)
+    if levels:
+        weight = np.floor(weight % 1 * levels)
+    slot_pos = np.stack([[s.rng.permutation(s.capacity) for _ in range(2)]]).astype(np.uint32)
+    wd, sd, ld = dev(weight), u32(slot_pos), u32([n])
+    newest = int(slot_pos[0, :, :n].max())
+    paged.evict(s.cache, ld, u32([newest]), keep, wd, sd, 3, 50)
+    assert ld.cpu().tolist() == [keep]
+    kd, vd = s.kd.cpu().numpy(), s.vd.cpu().numpy()
+    place = np.array(s.seen[0])
+    for g in range(2):
+        src = np.array(ref.evict(n, newest, keep, 3, 50, weight[0, g], slot_pos[0, g]))
+        np.testing.assert_array_equal(wd.cpu().numpy()[0, g], np.concatenate([weight[0, g, src], weight[0, g, keep:]]))
+        np.testing.assert_array_equal(sd.cpu().numpy()[0, g, :keep].view(np.uint32), slot_pos[0, g, src])
+        to, of = place[:keep], place[src]
+        for got, was in ((kd, s.k), (vd, s.v)):
+            np.testing.assert_array_equal(got[to[:, 0], g, to[:, 1]], was[of[:, 0], g, of[:, 1]])
+            rest = place[keep:]
+            np.testing.assert_array_equal(got[rest[:, 0], g, rest[:, 1]], was[rest[:, 0], g, rest[:, 1]])
