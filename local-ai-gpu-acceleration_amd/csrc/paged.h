@@ -25,7 +25,15 @@ struct PagedView {
   std::uint16_t* v;
   const std::int32_t* table;
   std::uint32_t table_stride, n_pages, n_kv, page_size, capacity, entries;
+  std::uint32_t page_mul, page_shift;  // page_of
 };
+
+// x / page_size for x < 2^31, as the high word of a product: with s = ceil(log2 d) and M =
+// ceil(2^(31 + s) / d), M d exceeds 2^(31 + s) by less than d <= 2^s, so x M / 2^(31 + s) lies
+// less than 1 / d above x / d.
+RTXLLM_HD std::uint32_t page_of(const PagedView& c, std::uint32_t x) {
+  return static_cast<std::uint32_t>(static_cast<std::uint64_t>(2u * x) * c.page_mul >> 32) >> c.page_shift;
+}
 
 // Number of the cache row (head_dim values of one position of one kv head) of
 // place `in_page` of physical page `page`, or kNoRow for a page that is not
@@ -39,7 +47,8 @@ RTXLLM_HD std::uint32_t paged_row(const PagedView& c, std::int32_t page, std::ui
 RTXLLM_HD std::uint32_t paged_slot_row(const PagedView& c, const std::int32_t* table, std::uint32_t head,
                                        std::uint32_t slot) {
   if (slot >= c.capacity) return kNoRow;
-  return paged_row(c, table[slot / c.page_size], head, slot % c.page_size);
+  const std::uint32_t page = page_of(c, slot);
+  return paged_row(c, table[page], head, slot - page * c.page_size);
 }
 
 // Filled positions of a row whose newest is `last`: 0 for a padded row, at most
@@ -64,8 +73,11 @@ inline bool paged_cache_ok(const rtxllm_paged_kv* c, std::uint32_t count) {
 }
 
 inline PagedView paged_view(const rtxllm_paged_kv* c) {
-  return PagedView{c->k,          c->v,         c->block_table, c->table_stride,          c->n_pages,
-                   c->n_kv_heads, c->page_size, c->capacity,    c->capacity / c->page_size};
+  std::uint32_t shift = 0;
+  while ((std::uint64_t{1} << shift) < c->page_size) ++shift;
+  const std::uint64_t mul = ((std::uint64_t{1} << (31u + shift)) + c->page_size - 1u) / c->page_size;
+  return PagedView{c->k,          c->v,        c->block_table,              c->table_stride, c->n_pages, c->n_kv_heads,
+                   c->page_size,  c->capacity, c->capacity / c->page_size, static_cast<std::uint32_t>(mul), shift};
 }
 
 // Query heads per kv head, or 0 if the heads do not fit the cache.

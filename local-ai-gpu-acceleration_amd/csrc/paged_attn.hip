@@ -12,18 +12,18 @@ typedef _Float16 half8 __attribute__((ext_vector_type(8)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 
 constexpr std::uint32_t kThreads = 256, kWaves = kThreads / 64u, kTile = 16;
-constexpr std::uint32_t kMaxSplits = 128;
+constexpr std::uint32_t kMaxSplits = 256;
 constexpr float kLift = 15.0f;  // softmax terms are kept times 2^15 (see the kernel)
 
 struct AttnArgs {
   const float* q;
   const std::uint32_t* pos;
-  const std::int32_t* pages;  // null: every slot
+  const std::int32_t* pages;
   float* out;
   float2* ml;      // [row][kv head][query head][split]: maximum (in log2), sum
   float* part;     // [row][kv head][query head][split][head_dim]
   float* scores;   // [row][kv head][query head][score_stride], in log2 (weights only)
-  std::uint32_t group, n_select, splits, score_stride;
+  std::uint32_t group, n_select, per, splits, score_stride;  // per: tiles of a split
 };
 
 __device__ __forceinline__ std::uint32_t from_lane(std::uint32_t v, std::uint32_t lane) {
@@ -40,10 +40,14 @@ __device__ __forceinline__ std::uint32_t from_lane(std::uint32_t v, std::uint32_
 //    largest p is 2^15, the sum l is lifted alike), terms down to 2^-29 of the
 //    largest keep 22 bits where fp16's subnormals would cut them;
 //  * o += V^T p by v_mfma_f32_4x4x4_16b_f16: a lane holds its own dimensions of
-//    four positions, as the V rows' coalesced loads leave them (a pair of lanes'
-//    worth of bytes each), and one column of p, fetched from the score layout by
-//    ds_bpermute. A lane's 4 results are one head's, so its rescaling is one factor.
-// T: heads in fours (1..4).
+//    four positions, as the V rows' coalesced loads leave them, and one column of p,
+//    fetched from the score layout by ds_bpermute. A lane's 4 results are one head's,
+//    so its rescaling is one factor.
+// T: heads in fours (1..4). WEIGHTS: every slot, the scores kept for merge_weights_kernel.
+// Bound by the reads of K and V: 4096 listed positions of eight sequences (134 MB)
+// 26.8 us, 5.0 TB/s (a 1 GiB copy: 5.2); without loads running ahead 33.9, with two sets of
+// registers in flight, at half the waves, 31.4. Workgroups next to each other take the
+// kv heads of one place, which lie next to each other in a page.
 template <int D, int T, bool WEIGHTS>
 __global__ __launch_bounds__(kThreads) void paged_attn_kernel(AttnArgs a, PagedView kv) {
   constexpr int NT = (T + 1) / 2;            // score tiles of 8 heads
@@ -53,21 +57,35 @@ __global__ __launch_bounds__(kThreads) void paged_attn_kernel(AttnArgs a, PagedV
   constexpr int STEPS = 4 / RPL;             // 4-position steps of a tile
   __shared__ __align__(16) float rec[kWaves][4 * T][D];
   __shared__ float2 rml[kWaves][4 * T];
-  const std::uint32_t split = blockIdx.x, g = blockIdx.y, r = blockIdx.z;
+  const std::uint32_t split = blockIdx.x / kv.n_kv, g = blockIdx.x % kv.n_kv, r = blockIdx.y;
   const std::uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const std::uint32_t n = paged_filled(kv, a.pos[r]);
-  if (n == 0u) return;  // a padded row
-  const std::uint32_t total = a.pages != nullptr ? a.n_select * kv.page_size : n;
-  const std::uint32_t tiles = (total + kTile - 1u) / kTile;
-  const std::uint32_t per = (tiles + kWaves * a.splits - 1u) / (kWaves * a.splits) * kWaves;
-  const std::uint32_t tile0 = split * per, tile1 = tile0 + per < tiles ? tile0 + per : tiles;
+  const std::uint32_t col = lane & 15u, qq = lane >> 4;
   const std::size_t gr = static_cast<std::size_t>(r) * kv.n_kv + g;
   const std::size_t head0 = gr * a.group;  // first query head of the kv head, over all rows
-  if (tile0 >= tiles) {
-    if (threadIdx.x < a.group) a.ml[(head0 + threadIdx.x) * a.splits + split] = make_float2(-INFINITY, 0.0f);
-    return;
-  }
-  const std::uint32_t col = lane & 15u, qq = lane >> 4;
+  const std::int32_t* const table = kv.table + static_cast<std::size_t>(r) * kv.table_stride;
+  // (WEIGHTS: every slot; else the listed pages)
+  const std::int32_t* const list = WEIGHTS ? nullptr : a.pages + gr * a.n_select;
+  const std::uint32_t room = WEIGHTS ? kv.capacity : a.n_select * kv.page_size;
+
+  // From a tile to the cache row of the lane's position (place col of it) in two
+  // dependent reads, each with a register of its own, so that they run ahead: the
+  // list's entry three tiles, the table's two. Indices past the end read the last entry.
+  auto place_of = [&](std::uint32_t tile) {
+    const std::uint32_t x = tile * kTile + col;
+    return x < room ? x : room - 1u;
+  };
+  std::int32_t entry = 0, entry_next = 0, page = 0;
+  auto load_entry = [&](std::uint32_t tile) {
+    const std::uint32_t e = page_of(kv, place_of(tile));
+    return WEIGHTS ? static_cast<std::int32_t>(e) : list[e];
+  };
+  auto load_page = [&](std::int32_t e) {
+    const auto lp = static_cast<std::uint32_t>(e);
+    return table[lp < kv.entries ? lp : kv.entries - 1u];
+  };
+  const std::uint32_t tile0 = split * a.per + wave;
+  entry = load_entry(tile0);
+  entry_next = load_entry(tile0 + kWaves);
 
   // B operands of the scores and each column's power of two
   uint4 qb[NT][J];
@@ -83,9 +101,11 @@ __global__ __launch_bounds__(kThreads) void paged_attn_kernel(AttnArgs a, PagedV
     for (int j = 0; j < J; ++j) {
       x[j][0] = *reinterpret_cast<const f32x4_any*>(qr + 32 * j);
       x[j][1] = *reinterpret_cast<const f32x4_any*>(qr + 32 * j + 4);
+    }
+#pragma unroll
+    for (int j = 0; j < J; ++j)
 #pragma unroll
       for (int i = 0; i < 4; ++i) m = fmaxf(m, fmaxf(fabsf(x[j][0][i]), fabsf(x[j][1][i])));
-    }
     m = fmaxf(m, lane_xor<16>(m));
     m = fmaxf(m, lane_xor<32>(m));
     int e = 0;
@@ -105,8 +125,13 @@ __global__ __launch_bounds__(kThreads) void paged_attn_kernel(AttnArgs a, PagedV
     }
   }
 
-  const std::int32_t* const table = kv.table + static_cast<std::size_t>(r) * kv.table_stride;
-  const std::int32_t* const list = a.pages != nullptr ? a.pages + gr * a.n_select : nullptr;
+  const std::uint32_t n = paged_filled(kv, a.pos[r]);
+  if (n == 0u) return;  // a padded row
+  const std::uint32_t total = WEIGHTS ? n : room;
+  const std::uint32_t tiles = (total + kTile - 1u) / kTile;
+  if (split * a.per >= tiles) return;  // behind the context: no record of it is read
+  const std::uint32_t tile1 = split * a.per + a.per < tiles ? split * a.per + a.per : tiles;
+
   float m[NT], l[NT];
   f32x4 o[T][VD];
 #pragma unroll
@@ -116,38 +141,25 @@ __global__ __launch_bounds__(kThreads) void paged_attn_kernel(AttnArgs a, PagedV
 #pragma unroll
     for (int s = 0; s < VD; ++s) o[t][s] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 
-  for (std::uint32_t tile = tile0 + wave; tile < tile1; tile += kWaves) {
-    // the lane's position (col of the tile) and its row
-    const std::uint32_t x = tile * kTile + col;
-    std::uint32_t row = kNoRow;
-    if (x < total) {
-      std::uint32_t lp = x / kv.page_size;
-      const std::uint32_t off = x - lp * kv.page_size;
-      if (list != nullptr) lp = static_cast<std::uint32_t>(list[lp]);
-      if (lp < kv.entries && lp * kv.page_size + off < n) row = paged_row(kv, table[lp], g, off);
-    }
-    const std::uint32_t valid = static_cast<std::uint32_t>(__ballot(row != kNoRow)) & 0xFFFFu;
-    float* const sc_out = WEIGHTS ? a.scores + head0 * a.score_stride + tile * kTile + 4u * qq : nullptr;
-    if (valid == 0u) {
-      if constexpr (WEIGHTS) {
+  // A tile's keys and values and which of its positions count. One that does not reads
+  // row 0 of the cache; its score and value are dropped.
+  uint4 ka[J];
+  std::uint32_t vw[16 / RPL][VD / 2], valid = 0u, row = 0u;
+  auto settle = [&](std::uint32_t tile) {  // from `entry` and `page`, those of the tile
+    const std::uint32_t x = place_of(tile), off = x - page_of(kv, x) * kv.page_size;
+    const auto lp = static_cast<std::uint32_t>(entry);
+    const std::uint32_t at = paged_row(kv, page, g, off);
+    const bool there = tile < tile1 && tile * kTile + col < room && lp < kv.entries && at != kNoRow &&
+                       lp * kv.page_size + off < n;
+    valid = static_cast<std::uint32_t>(__ballot(there)) & 0xFFFFu;
+    row = there ? at : 0u;
+  };
+  auto load_k = [&]() {
+    const uint4* kr = reinterpret_cast<const uint4*>(kv.k + static_cast<std::size_t>(row) * D) + qq;
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-          const std::uint32_t h = 8u * nt + col / 2u;
-          if ((col & 1u) == 0u && h < a.group)
-            *reinterpret_cast<float4*>(sc_out + static_cast<std::size_t>(h) * a.score_stride) =
-                make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
-        }
-      }
-      continue;
-    }
-    if (row == kNoRow) row = 0u;  // any row of the cache: its scores and values are dropped
-    uint4 ka[J];
-    {
-      const uint4* kr = reinterpret_cast<const uint4*>(kv.k + static_cast<std::size_t>(row) * D) + qq;
-#pragma unroll
-      for (int j = 0; j < J; ++j) ka[j] = kr[4 * j];
-    }
-    std::uint32_t vw[16 / RPL][VD / 2];
+    for (int j = 0; j < J; ++j) ka[j] = kr[4 * j];
+  };
+  auto load_v = [&]() {
 #pragma unroll
     for (int j = 0; j < 16 / RPL; ++j) {
       if constexpr (D == 64) {
@@ -166,30 +178,47 @@ __global__ __launch_bounds__(kThreads) void paged_attn_kernel(AttnArgs a, PagedV
         }
       }
     }
-    if (valid != 0xFFFFu) {  // 0 times what lies behind the context must stay 0
-#pragma unroll
-      for (int j = 0; j < 16 / RPL; ++j) {
-        const std::uint32_t at = D == 64 ? 8u * (j / 4) + (lane < 32u ? 0u : 4u) + (j & 3) : j;
-#pragma unroll
-        for (int s = 0; s < VD / 2; ++s) vw[j][s] = (valid >> at & 1u) != 0u ? vw[j][s] : 0u;
-      }
-    }
+  };
+  // Loads run ahead of use without a second set of registers: the next tile's keys are
+  // read once this tile's scores have used theirs, its values after this tile's sums.
+  // No branch skips a load, so each wait is for the loads it needs alone (behind the
+  // last tile row 0 is read, from the L2).
+  page = load_page(entry);
+  settle(tile0);
+  load_k();
+  entry = entry_next;
+  page = load_page(entry);
+  entry_next = load_entry(tile0 + 2u * kWaves);
+  load_v();
+  for (std::uint32_t tile = tile0; tile < tile1; tile += kWaves) {
+    const std::uint32_t now = valid;
+    float* const sc_out = WEIGHTS ? a.scores + head0 * a.score_stride + tile * kTile + 4u * qq : nullptr;
     std::uint32_t p01[NT], p23[NT];
     float alpha[NT];
     bool moved = false;
+    f32x4 sc_all[NT];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-      f32x4 sc = {0.0f, 0.0f, 0.0f, 0.0f};
+      sc_all[nt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
       for (int j = 0; j < J; ++j)
-        sc = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8, ka[j]),
-                                                    __builtin_bit_cast(half8, qb[nt][j]), sc, 0, 0, 0);
+        sc_all[nt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8, ka[j]),
+                                                            __builtin_bit_cast(half8, qb[nt][j]), sc_all[nt], 0, 0, 0);
+    }
+    settle(tile + kWaves);
+    load_k();
+    entry = entry_next;
+    page = load_page(entry);
+    entry_next = load_entry(tile + 3u * kWaves);
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      const f32x4 sc = sc_all[nt];
       // column n: head n / 2; positions 4 qq + i
       float s4[4], top = -INFINITY;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const float t = (sc[i] + lane_xor<1>(sc[i])) * qscale[nt];
-        s4[i] = (valid >> (4u * qq + i) & 1u) != 0u ? t : -INFINITY;
+        s4[i] = (now >> (4u * qq + i) & 1u) != 0u ? t : -INFINITY;
         top = fmaxf(top, s4[i]);
       }
       if constexpr (WEIGHTS) {
@@ -227,6 +256,14 @@ __global__ __launch_bounds__(kThreads) void paged_attn_kernel(AttnArgs a, PagedV
         for (int s = 0; s < VD; ++s) o[t][s] *= f;
       }
     }
+    if (now != 0xFFFFu) {  // 0 times what lies behind the context must stay 0
+#pragma unroll
+      for (int j = 0; j < 16 / RPL; ++j) {
+        const std::uint32_t at = D == 64 ? 8u * (j / 4) + (lane < 32u ? 0u : 4u) + (j & 3) : j;
+#pragma unroll
+        for (int s = 0; s < VD / 2; ++s) vw[j][s] = (now >> at & 1u) != 0u ? vw[j][s] : 0u;
+      }
+    }
 #pragma unroll
     for (int st = 0; st < STEPS; ++st) {
       half4 va[VD];
@@ -252,6 +289,7 @@ __global__ __launch_bounds__(kThreads) void paged_attn_kernel(AttnArgs a, PagedV
         }
       }
     }
+    load_v();
   }
 
   // the waves' records, merged: o = sum e^(m_w - M) o_w, L alike
@@ -312,28 +350,33 @@ __global__ __launch_bounds__(kThreads) void paged_attn_kernel(AttnArgs a, PagedV
 
 // Maximum and sum of one head over its splits' records, by one wave.
 __device__ __forceinline__ float2 head_ml(const float2* __restrict__ ml, std::uint32_t splits, std::uint32_t lane) {
-  const float2 none = make_float2(-INFINITY, 0.0f);
-  const float2 x = lane < splits ? ml[lane] : none, y = lane + 64u < splits ? ml[lane + 64u] : none;
-  const float M = wave_max(fmaxf(x.x, y.x)), base = M == -INFINITY ? 0.0f : M;
-  return make_float2(M, wave_sum(x.y * __builtin_amdgcn_exp2f(x.x - base) + y.y * __builtin_amdgcn_exp2f(y.x - base)));
+  float2 x[kMaxSplits / 64u];
+  float m = -INFINITY;
+#pragma unroll
+  for (std::uint32_t i = 0; i < kMaxSplits / 64u; ++i) {
+    x[i] = lane + 64u * i < splits ? ml[lane + 64u * i] : make_float2(-INFINITY, 0.0f);
+    m = fmaxf(m, x[i].x);
+  }
+  const float M = wave_max(m), base = M == -INFINITY ? 0.0f : M;
+  float l = 0.0f;
+#pragma unroll
+  for (std::uint32_t i = 0; i < kMaxSplits / 64u; ++i) l += x[i].y * __builtin_amdgcn_exp2f(x[i].x - base);
+  return make_float2(M, wave_sum(l));
 }
 
 // One workgroup a query head (of all rows): its splits' records merged, D / 4
 // lanes a record.
 template <int D>
-__device__ __forceinline__ void merge_head(const AttnArgs& a, std::size_t head) {
+__device__ __forceinline__ void merge_head(const AttnArgs& a, std::size_t head, std::uint32_t splits) {
   constexpr std::uint32_t kLanes = D / 4u, kSub = kThreads / kLanes;
   __shared__ __align__(16) float sums[kSub][D];
   const std::uint32_t d = 4u * (threadIdx.x % kLanes), sub = threadIdx.x / kLanes;
   const float2* const ml = a.ml + head * a.splits;
-  const float2 t = head_ml(ml, a.splits, threadIdx.x & 63u);
+  const float2 t = head_ml(ml, splits, threadIdx.x & 63u);
   const float base = t.x == -INFINITY ? 0.0f : t.x;
   f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
-  for (std::uint32_t c = sub; c < a.splits; c += kSub) {
-    const float mc = ml[c].x;
-    if (mc == -INFINITY) continue;  // (an empty split writes no sums)
-    v += __builtin_amdgcn_exp2f(mc - base) * *reinterpret_cast<const f32x4*>(a.part + (head * a.splits + c) * D + d);
-  }
+  for (std::uint32_t c = sub; c < splits; c += kSub)
+    v += __builtin_amdgcn_exp2f(ml[c].x - base) * *reinterpret_cast<const f32x4*>(a.part + (head * a.splits + c) * D + d);
   *reinterpret_cast<f32x4*>(&sums[sub][d]) = v;
   __syncthreads();
   if (sub != 0u) return;
@@ -347,7 +390,7 @@ template <int D>
 __global__ __launch_bounds__(kThreads) void merge_kernel(AttnArgs a, PagedView kv) {
   const std::uint32_t r = blockIdx.y;
   if (paged_filled(kv, a.pos[r]) == 0u) return;
-  merge_head<D>(a, static_cast<std::size_t>(r) * gridDim.x + blockIdx.x);
+  merge_head<D>(a, static_cast<std::size_t>(r) * gridDim.x + blockIdx.x, a.splits);
 }
 
 // The first `group` workgroups of (kv head, row) merge a head each; the others
@@ -359,15 +402,16 @@ __global__ __launch_bounds__(kThreads) void merge_weights_kernel(AttnArgs a, Pag
   const std::uint32_t g = blockIdx.y, r = blockIdx.z, n = paged_filled(kv, a.pos[r]);
   if (n == 0u) return;
   const std::size_t gr = static_cast<std::size_t>(r) * kv.n_kv + g, head0 = gr * a.group;
+  const std::uint32_t splits = (n + a.per * kTile - 1u) / (a.per * kTile);  // those with a record
   if (blockIdx.x < a.group) {
-    merge_head<D>(a, head0 + blockIdx.x);
+    merge_head<D>(a, head0 + blockIdx.x, splits);
     return;
   }
   const std::uint32_t i0 = (blockIdx.x - a.group) * 4u * kThreads + 4u * threadIdx.x;
   if (i0 - 4u * threadIdx.x >= n) return;
   const std::uint32_t lane = threadIdx.x & 63u;
   for (std::uint32_t h = threadIdx.x >> 6; h < a.group; h += kWaves) {
-    const float2 t = head_ml(a.ml + (head0 + h) * a.splits, a.splits, lane);
+    const float2 t = head_ml(a.ml + (head0 + h) * a.splits, splits, lane);
     if (lane == 0u) {
       base_s[h] = (t.x == -INFINITY ? 0.0f : t.x) - kLift;
       inv_s[h] = t.y == 0.0f ? 0.0f : 1.0f / t.y;
@@ -390,16 +434,23 @@ __global__ __launch_bounds__(kThreads) void merge_weights_kernel(AttnArgs a, Pag
   }
 }
 
-// Splits of each (row, kv head): enough workgroups to fill the chip, at most one
-// per 64 positions.
-std::uint32_t attn_splits(std::uint64_t items, std::uint64_t positions) {
-  const std::uint64_t want = (1024u + items - 1u) / items, most = (positions + 63u) / 64u;
-  const std::uint64_t s = want < most ? want : most;
-  return static_cast<std::uint32_t>(s < kMaxSplits ? s : kMaxSplits);
+// Tiles of a split (one workgroup), of at most `positions`. Of one size for every row,
+// so that a longer context is more workgroups; the largest of 4 to 64 that leaves a
+// workgroup for each CU, as a wave's prologue and the merge cost what two or three
+// tiles do. us of 32 heads over 8 kv heads of 128, per = 4 / 8 / 16 / 32 / 64: 1024
+// listed positions of one sequence 8.9 / 9.6 / 11.1 / 14.4 / 16.9, 4001 slots of one 12.0
+// / 10.5 / 11.5 / 14.6 / 21.4, 4096 listed of eight 41.9 / 35.7 / 33.4 / 31.2 / 31.1, up to
+// 16384 slots of eight 84.2 / 84.1 / 75.4 / 75.8 / 74.9.
+std::uint32_t attn_per(std::uint64_t items, std::uint64_t positions) {
+  const std::uint64_t tiles = (positions + kTile - 1u) / kTile;
+  std::uint64_t per = 64u;
+  while (per > kWaves && items * ((tiles + per - 1u) / per) < 256u) per /= 2u;
+  while ((tiles + per - 1u) / per > kMaxSplits) per *= 2u;
+  return static_cast<std::uint32_t>(per);
 }
 
 struct AttnSpace {
-  std::uint32_t splits = 0, score_stride = 0;
+  std::uint32_t per = 0, splits = 0, score_stride = 0;
   std::size_t ml = 0, part = 0, scores = 0;  // byte offsets past the start
   std::size_t bytes = 0;                     // 0: refused
 };
@@ -408,9 +459,10 @@ AttnSpace attn_space(const rtxllm_paged_kv* c, std::uint32_t n_heads, std::uint6
                      bool weights) {
   AttnSpace s;
   if (!paged_cache_ok(c, count) || count == 0u || count > 65535u || c->n_kv_heads > 65535u ||
-      paged_group(c, n_heads) == 0u || positions == 0u || positions > (1ull << 31))
+      paged_group(c, n_heads) == 0u || positions == 0u || positions > (1ull << 30))
     return s;
-  s.splits = attn_splits(static_cast<std::uint64_t>(count) * c->n_kv_heads, positions);
+  s.per = attn_per(static_cast<std::uint64_t>(count) * c->n_kv_heads, positions);
+  s.splits = static_cast<std::uint32_t>((positions + kTile * s.per - 1u) / (kTile * s.per));
   const std::size_t records = static_cast<std::size_t>(count) * n_heads * s.splits;
   s.part = round_256(8u * records);
   s.scores = s.part + round_256(4u * records * c->head_dim);
@@ -424,7 +476,7 @@ AttnSpace attn_space(const rtxllm_paged_kv* c, std::uint32_t n_heads, std::uint6
 
 template <int D, bool WEIGHTS>
 void launch_partial(const AttnArgs& a, const PagedView& view, std::uint32_t count, hipStream_t stream) {
-  const dim3 grid(a.splits, view.n_kv, count);
+  const dim3 grid(a.splits * view.n_kv, count);
   if (a.group <= 4u)
     hipLaunchKernelGGL((paged_attn_kernel<D, 1, WEIGHTS>), grid, dim3(kThreads), 0, stream, a, view);
   else if (a.group <= 8u)
@@ -465,6 +517,7 @@ AttnArgs attn_args(const float* q, const std::uint32_t* pos, float* out, void* w
   a.part = reinterpret_cast<float*>(base + s.part);
   a.scores = reinterpret_cast<float*>(base + s.scores);
   a.group = group;
+  a.per = s.per;
   a.splits = s.splits;
   a.score_stride = s.score_stride;
   return a;

@@ -10,11 +10,16 @@ namespace rtxllm {
 namespace {
 
 constexpr std::uint32_t kThreads = 256;
-constexpr std::uint32_t kSelThreads = 1024, kSelWaves = kSelThreads / 64u;
 
 typedef std::uint32_t u32x4_any __attribute__((ext_vector_type(4), aligned(4)));
 
-__device__ __forceinline__ double lane_xor_d(double v, int mask) { return __shfl_xor(v, mask, 64); }
+// lane_xor of a 64-bit value.
+template <int M>
+__device__ __forceinline__ double lane_xor_d(double v) {
+  const uint2 u = __builtin_bit_cast(uint2, v);
+  return __builtin_bit_cast(double, make_uint2(__float_as_uint(lane_xor<M>(__uint_as_float(u.x))),
+                                               __float_as_uint(lane_xor<M>(__uint_as_float(u.y)))));
+}
 
 // A score as an unsigned key of the same order: 1 for NaN, so that 0 is left for
 // "no candidate".
@@ -24,53 +29,88 @@ __device__ __forceinline__ unsigned long long score_key(double s) {
   return (b >> 63) != 0ull ? ~b : b | (1ull << 63);
 }
 
-// Scores of 64 / L pages a wave, L = head_dim / 8 lanes a page, 8 dimensions a
-// lane. With c = (hi + lo) / 2 and w = |hi - lo| / 2, max(q hi, q lo) = q c + |q| w;
-// here both are doubled, which changes no order. Products of fp32 and fp16 values are
-// exact in 64 bits, and the sums' 2^-53 keep two pages apart whose scores differ at all.
-template <int L>
+// Keys of the pages of one (row, kv head): a wave scores kSteps times 64 / L pages, L =
+// head_dim / 8 lanes a page, 8 dimensions a lane. With c = (hi + lo) / 2 and w = |hi - lo| /
+// 2, max(q hi, q lo) = q c + |q| w; here both are doubled, which changes no order.
+// Products of fp32 and fp16 values are exact in 64 bits, and the sums' 2^-53 keep two
+// pages apart whose scores differ at all. Four heads at a time: two halving exchanges
+// leave each lane one head's part, so that four heads take one head's further steps.
+// What bounds it is the chain of reads (table and q, then bounds): the position is
+// needed last, a wave's table entries are one load, and the next step's bounds are
+// read before this step's sums.
+template <int L, int kSteps>
 __global__ __launch_bounds__(kThreads) void page_score_kernel(PagedView kv, const std::uint16_t* __restrict__ bounds,
                                                               const float* __restrict__ q, std::uint32_t group,
                                                               const std::uint32_t* __restrict__ pos,
                                                               std::uint32_t n_first, std::uint32_t n_last,
                                                               unsigned long long* __restrict__ keys) {
-  constexpr std::uint32_t D = 8u * L, kPages = 64u / L;
+  constexpr std::uint32_t D = 8u * L, kPages = 64u / L, kOwn = kPages * kSteps;
+  static_assert(kOwn <= 64u, "a lane a page of the wave");
   typedef _Float16 half8 __attribute__((ext_vector_type(8)));
   const std::uint32_t g = blockIdx.y, r = blockIdx.z, lane = threadIdx.x & 63u, t = lane % L;
-  const std::uint32_t used = (paged_filled(kv, pos[r]) + kv.page_size - 1u) / kv.page_size;
-  const std::uint32_t p = (blockIdx.x * (kThreads / 64u) + (threadIdx.x >> 6)) * kPages + lane / L;
-  if (__builtin_amdgcn_readfirstlane(p) >= used) return;
-  const std::uint32_t pc = p < used ? p : used - 1u;
-  const std::int32_t page = kv.table[static_cast<std::size_t>(r) * kv.table_stride + pc];
-  const bool there = static_cast<std::uint32_t>(page) < kv.n_pages;
-  const half8* b = reinterpret_cast<const half8*>(
-                       bounds + (static_cast<std::size_t>(there ? page : 0) * kv.n_kv + g) * 2u * D) + t;
-  const half8 hi = b[0], lo = b[L];
-  double c[8], w[8];
+  const std::size_t gr = static_cast<std::size_t>(r) * kv.n_kv + g;
+  const std::uint32_t p0 = __builtin_amdgcn_readfirstlane(blockIdx.x * (kThreads / 64u) + (threadIdx.x >> 6)) * kOwn;
+  if (p0 >= kv.entries) return;
+  const std::uint32_t mine = p0 + lane % kOwn;
+  const std::int32_t entry =
+      kv.table[static_cast<std::size_t>(r) * kv.table_stride + (mine < kv.entries ? mine : kv.entries - 1u)];
+  const std::uint32_t filled = paged_filled(kv, pos[r]), used = (filled + kv.page_size - 1u) / kv.page_size;
+  const float* const qr = q + gr * group * D + 8u * t;
+  double qd[4][8];
+  auto load_q = [&](std::uint32_t h0) {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const double x = static_cast<double>(static_cast<float>(hi[i])), y = static_cast<double>(static_cast<float>(lo[i]));
-    c[i] = x + y;
-    w[i] = x - y;
-  }
-  const float* qr = q + (static_cast<std::size_t>(r) * kv.n_kv + g) * group * D + 8u * t;
-  double best = 0.0;
-  for (std::uint32_t h = 0; h < group; ++h) {
-    const f32x4_any qa = *reinterpret_cast<const f32x4_any*>(qr + h * D), qb = *reinterpret_cast<const f32x4_any*>(qr + h * D + 4u);
-    double s = 0.0;
+    for (int k = 0; k < 4; ++k) {
+      const std::uint32_t h = h0 + k < group ? h0 + k : group - 1u;  // a head twice changes no maximum
+      const f32x4_any a = *reinterpret_cast<const f32x4_any*>(qr + h * D), b = *reinterpret_cast<const f32x4_any*>(qr + h * D + 4u);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) qd[k][i] = static_cast<double>(i < 4 ? a[i & 3] : b[i & 3]);
+    }
+  };
+  half8 hi[2], lo[2];
+  bool there[2];
+  auto load_bounds = [&](int s) {
+    const std::int32_t page = __shfl(entry, static_cast<int>(kPages * s + lane / L), 64);
+    there[s & 1] = static_cast<std::uint32_t>(page) < kv.n_pages;
+    const half8* b = reinterpret_cast<const half8*>(
+                         bounds + (static_cast<std::size_t>(there[s & 1] ? page : 0) * kv.n_kv + g) * 2u * D) + t;
+    hi[s & 1] = b[0], lo[s & 1] = b[L];
+  };
+  if (p0 >= used) return;
+  load_bounds(0);
+  load_q(0u);
+  const bool odd = (lane & 1u) != 0u, odd2 = (lane & 2u) != 0u;
+#pragma unroll
+  for (int s = 0; s < kSteps; ++s) {
+    if (p0 + kPages * s >= used) break;
+    if (s + 1 < kSteps) load_bounds(s + 1);
+    double c[8], w[8], best = __builtin_nan("");
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const double x = static_cast<double>(i < 4 ? qa[i & 3] : qb[i & 3]);
-      s = fma(x, c[i], s);
-      s = fma(fabs(x), fabs(w[i]), s);
+      const double x = static_cast<double>(static_cast<float>(hi[s & 1][i])), y = static_cast<double>(static_cast<float>(lo[s & 1][i]));
+      c[i] = x + y;
+      w[i] = fabs(x - y);
     }
+    for (std::uint32_t h0 = 0; h0 < group; h0 += 4u) {
+      if (group > 4u) load_q(h0);
+      double sum[4] = {0.0, 0.0, 0.0, 0.0};
 #pragma unroll
-    for (int m = 1; m < L; m *= 2) s += lane_xor_d(s, m);
-    best = h == 0u || s > best || best != best ? s : best;  // a head's NaN gives way to a number
+      for (int i = 0; i < 8; ++i)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) sum[k] = fma(fabs(qd[k][i]), w[i], fma(qd[k][i], c[i], sum[k]));
+      const double x0 = odd ? sum[2] : sum[0], x1 = odd ? sum[3] : sum[1];
+      const double y0 = odd ? sum[0] : sum[2], y1 = odd ? sum[1] : sum[3];
+      const double v0 = x0 + lane_xor_d<1>(y0), v1 = x1 + lane_xor_d<1>(y1);
+      double v = (odd2 ? v1 : v0) + lane_xor_d<2>(odd2 ? v0 : v1);
+      v += lane_xor_d<4>(v);
+      if constexpr (L > 8) v += lane_xor_d<8>(v);
+      if constexpr (L > 16) v += lane_xor_d<16>(v);
+      v = fmax(v, lane_xor_d<1>(v));  // fmax: a head's NaN gives way to a number
+      best = fmax(best, fmax(v, lane_xor_d<2>(v)));
+    }
+    const std::uint32_t p = p0 + kPages * s + lane / L;
+    const bool forced = p < n_first || p + n_last >= used;
+    if (t == 0u && p < used) keys[gr * kv.entries + p] = !there[s & 1] ? 0ull : forced ? ~0ull : score_key(best);
   }
-  if (t != 0u || p >= used) return;
-  const bool forced = p < n_first || p + n_last >= used;
-  keys[(static_cast<std::size_t>(r) * kv.n_kv + g) * kv.entries + p] = !there ? 0ull : forced ? ~0ull : score_key(best);
 }
 
 // The best k of n keys: those >= `least`, of those equal to it only the first
@@ -84,11 +124,11 @@ struct Choice {
 constexpr std::uint32_t kAllTies = 0xFFFFFFFFu;
 constexpr int kDigit = 11;  // bits of a pass
 constexpr std::uint32_t kBins = 1u << kDigit;
-static_assert(kBins == 2u * kSelThreads, "two bins a thread");
 
+template <std::uint32_t T>  // threads
 struct SelectShared {
   std::uint32_t hist[2][kBins];
-  std::uint32_t wave[3][kSelWaves];
+  std::uint32_t wave[3][T / 64u];
   std::uint32_t bin, above, count;
 };
 
@@ -109,12 +149,19 @@ __device__ __forceinline__ std::uint32_t wave_scan(std::uint32_t v) {
   return v;
 }
 
+// Lanes of a mask below this one.
+__device__ __forceinline__ std::uint32_t lanes_below(unsigned long long mask) {
+  return __builtin_amdgcn_mbcnt_hi(static_cast<std::uint32_t>(mask >> 32),
+                                   __builtin_amdgcn_mbcnt_lo(static_cast<std::uint32_t>(mask), 0u));
+}
+
 // Sum of the waves' words before this wave, and of all.
-__device__ __forceinline__ uint2 waves_before(const std::uint32_t* words, std::uint32_t wave) {
+template <std::uint32_t T>
+__device__ __forceinline__ uint2 waves_before(const std::uint32_t (&words)[T / 64u], std::uint32_t wave) {
   uint2 s = make_uint2(0u, 0u);
 #pragma unroll
-  for (std::uint32_t w = 0; w < kSelWaves; w += 4u) {
-    const uint4 x = *reinterpret_cast<const uint4*>(words + w);
+  for (std::uint32_t w = 0; w < T / 64u; w += 4u) {
+    const uint4 x = *reinterpret_cast<const uint4*>(&words[w]);
     s.x += (w < wave ? x.x : 0u) + (w + 1u < wave ? x.y : 0u) + (w + 2u < wave ? x.z : 0u) + (w + 3u < wave ? x.w : 0u);
     s.y += (x.x + x.y) + (x.z + x.w);
   }
@@ -122,27 +169,38 @@ __device__ __forceinline__ uint2 waves_before(const std::uint32_t* words, std::u
 }
 
 // The keys of a workgroup: a wave's part contiguous, four keys a lane and round, so
-// that loads are wide and ranks follow from ballots. Up to `room` keys are read
-// once and stay in the LDS, each thread's own where it alone reads them; of more,
-// every pass reads all again (from the L2). The loops are rolled: each runs a few
-// rounds once, and unrolled code with the keys in registers took longer to fetch
-// (32 keys a thread: 92 us for 32768 keys). load(i, x): keys i..i + 3, i % 4 == 0.
-template <class K, class Load>
+// that loads are wide and ranks follow from ballots; 0 behind the last key. Up to
+// `room` keys are read once and stay in the LDS, each thread's own where it alone
+// reads them; of more, every pass reads all again (from the L2). The loops over them are
+// rolled: each runs a few rounds once, and unrolled code with the keys in registers
+// took longer to fetch (32 keys a thread: 92 us for 32768 keys). src.raw(i) loads what
+// keys i..i + 3 (i % 4 == 0) are made of, src.keys(i, raw, x) makes them.
+template <class K, class Source, std::uint32_t T>
 struct Keys {
   struct alignas(16) Four {
     K k[4];
   };
-  const Load& load;
+  const Source& src;
   Four* held;
-  std::uint32_t n, rounds, first;  // rounds of a wave, first key of its own
+  std::uint32_t n, rounds, first;  // rounds of this wave, its first key
   bool in_lds;
 
-  __device__ __forceinline__ Keys(const Load& l, void* lds, std::uint32_t count, std::uint32_t room)
-      : load(l), held(static_cast<Four*>(lds) + threadIdx.x), n(count), in_lds(count <= room) {
-    rounds = (n + 4u * kSelThreads - 1u) / (4u * kSelThreads);
-    first = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) * 256u * rounds;
-    if (in_lds)
-      for (std::uint32_t j = 0; j < rounds && first + 256u * j < n; ++j) load(place(j), held[kSelThreads * j].k);
+  __device__ __forceinline__ Keys(const Source& s, void* lds, std::uint32_t count, std::uint32_t room)
+      : src(s), held(static_cast<Four*>(lds) + threadIdx.x), n(count), in_lds(count <= room) {
+    const std::uint32_t most = (n + 4u * T - 1u) / (4u * T);
+    first = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) * 256u * most;
+    const std::uint32_t own = first < n ? (n - first + 255u) / 256u : 0u;
+    rounds = own < most ? own : most;
+    if (!in_lds) return;
+    std::uint32_t j = 0;
+    for (; j + 4u <= rounds; j += 4u) {  // four rounds' loads in flight
+      decltype(src.raw(0u)) v[4];
+#pragma unroll
+      for (std::uint32_t u = 0; u < 4u; ++u) v[u] = src.raw(place(j + u));
+#pragma unroll
+      for (std::uint32_t u = 0; u < 4u; ++u) src.keys(place(j + u), v[u], held[T * (j + u)].k);
+    }
+    for (; j < rounds; ++j) src.keys(place(j), src.raw(place(j)), held[T * j].k);
   }
   __device__ __forceinline__ std::uint32_t place(std::uint32_t j) const {
     return first + 256u * j + 4u * (threadIdx.x & 63u);
@@ -150,12 +208,12 @@ struct Keys {
   // body(four keys, index of the first) for each round of the wave
   template <class Body>
   __device__ __forceinline__ void each(Body body) const {
-    for (std::uint32_t j = 0; j < rounds && first + 256u * j < n; ++j) {
+    for (std::uint32_t j = 0; j < rounds; ++j) {
       Four f;
       if (in_lds)
-        f = held[kSelThreads * j];
+        f = held[T * j];
       else
-        load(place(j), f.k);
+        src.keys(place(j), src.raw(place(j)), f.k);
       body(f.k, place(j));
     }
   }
@@ -165,47 +223,63 @@ struct Keys {
 // share the digits found so far by their next digit, and takes the digit in which
 // the k-th largest lies. It ends early once all keys of that digit are wanted,
 // after two or three passes where keys are spread. Lanes that all count the same
-// digit (equal keys) add once, as one address takes one addition at a time.
-template <class K, class Load>
-__device__ Choice<K> radix_choice(SelectShared& sh, const Keys<K, Load>& keys, std::uint32_t k) {
+// digit (equal keys) add once, as one address takes one addition at a time. k is at
+// most the number of keys: the zeros behind the last one are never among the best,
+// since of equal keys the first count.
+template <class K, class Source, std::uint32_t T>
+__device__ Choice<K> radix_choice(SelectShared<T>& sh, const Keys<K, Source, T>& keys, std::uint32_t k) {
   constexpr int kBits = static_cast<int>(8u * sizeof(K));
   const std::uint32_t tid = threadIdx.x, lane = tid & 63u, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  if (k >= keys.n) return Choice<K>{0, kAllTies};
-  reinterpret_cast<uint2*>(sh.hist[0])[tid] = make_uint2(0u, 0u);
+  constexpr std::uint32_t kOwn = kBins / T;  // bins of a thread
+  static_assert(kOwn % 2u == 0u, "pairs of bins");
+  auto clear = [&](std::uint32_t* h) {
+#pragma unroll
+    for (std::uint32_t i = 0; i < kOwn; i += 2u) *reinterpret_cast<uint2*>(h + i * T + 2u * tid) = make_uint2(0u, 0u);
+  };
+  clear(sh.hist[0]);
   __syncthreads();
   K prefix = 0;
   int shift = kBits;
   for (std::uint32_t turn = 0;; turn ^= 1u) {
     const int bits = shift < kDigit ? shift : kDigit, next = shift - bits;
     std::uint32_t* const hist = sh.hist[turn];
-    keys.each([&](const K (&x)[4], std::uint32_t i) {
+    keys.each([&](const K (&x)[4], std::uint32_t) {
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const bool match = i + e < keys.n && (shift == kBits || (x[e] >> shift) == prefix);
+        if (shift != kBits && (x[e] >> shift) != prefix) continue;
         const std::uint32_t digit = static_cast<std::uint32_t>(x[e] >> next) & ((1u << bits) - 1u);
-        const unsigned long long who = __ballot(match);
-        if (who == 0ull) continue;
-        const std::uint32_t one = __builtin_amdgcn_readlane(digit, static_cast<int>(__builtin_ctzll(who)));
-        if (__ballot(match && digit == one) == who) {
-          if (lane == 0u) atomicAdd(&hist[one], static_cast<std::uint32_t>(__popcll(who)));
-        } else if (match) {
+        const unsigned long long who = __ballot(true);
+        if (__ballot(digit == __builtin_amdgcn_readfirstlane(digit)) != who)
           atomicAdd(&hist[digit], 1u);
-        }
+        else if (lanes_below(who) == 0u)
+          atomicAdd(&hist[digit], static_cast<std::uint32_t>(__popcll(who)));
       }
     });
     __syncthreads();
-    // thread t: bins 2047 - 2 t and 2046 - 2 t, sums from the largest digit down
-    const uint2 c = reinterpret_cast<const uint2*>(hist)[kSelThreads - 1u - tid];
-    reinterpret_cast<uint2*>(sh.hist[turn ^ 1u])[tid] = make_uint2(0u, 0u);
-    const std::uint32_t sum = wave_scan(c.x + c.y);
+    // thread t: the kOwn bins below kBins - kOwn t, sums from the largest digit down
+    const std::uint32_t low = kBins - kOwn * (tid + 1u);
+    std::uint32_t c[kOwn], own = 0u;
+#pragma unroll
+    for (std::uint32_t i = 0; i < kOwn; i += 2u) {
+      const uint2 v = *reinterpret_cast<const uint2*>(hist + low + i);
+      c[i] = v.x, c[i + 1u] = v.y;
+      own += v.x + v.y;
+    }
+    clear(sh.hist[turn ^ 1u]);
+    const std::uint32_t sum = wave_scan(own);
     if (lane == 63u) sh.wave[0][wave] = sum;
     __syncthreads();
-    const std::uint32_t before = waves_before(sh.wave[0], wave).x + sum - (c.x + c.y);
-    if (before < k && k <= before + c.x + c.y) {
-      const bool upper = k <= before + c.y;
-      sh.bin = 2u * (kSelThreads - 1u - tid) + (upper ? 1u : 0u);
-      sh.above = upper ? before : before + c.y;
-      sh.count = upper ? c.y : c.x;
+    std::uint32_t before = waves_before<T>(sh.wave[0], wave).x + sum - own;
+    if (before < k && k <= before + own) {
+#pragma unroll
+      for (int i = static_cast<int>(kOwn) - 1; i >= 0; --i) {
+        if (before < k && k <= before + c[i]) {
+          sh.bin = low + static_cast<std::uint32_t>(i);
+          sh.above = before;
+          sh.count = c[i];
+        }
+        before += c[i];
+      }
     }
     __syncthreads();
     prefix = (prefix << bits) | static_cast<K>(sh.bin);
@@ -216,117 +290,137 @@ __device__ Choice<K> radix_choice(SelectShared& sh, const Keys<K, Load>& keys, s
   }
 }
 
-// Walks the keys in two classes: kind(i, chosen) is 0 (neither), 1 or 2, put(kind, i,
-// rank) gets a place of a class with the number of those of the class before it.
-// Returns the sizes of both.
-template <class K, class Load, class Kind, class Put>
-__device__ uint2 for_chosen(SelectShared& sh, const Keys<K, Load>& keys, const Choice<K>& ch, Kind kind, Put put) {
+// Walks the choice: freed(i, rank) for each key below `split` that is not chosen, kept(i,
+// rank) for each chosen one at or behind it, rank counting those of the same kind before
+// it. Returns the number of both.
+template <class K, class Source, std::uint32_t T, class Freed, class Kept>
+__device__ uint2 for_choice(SelectShared<T>& sh, const Keys<K, Source, T>& keys, const Choice<K>& ch, std::uint32_t split,
+                            Freed freed, Kept kept) {
   const std::uint32_t tid = threadIdx.x, lane = tid & 63u, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const unsigned long long below = (1ull << lane) - 1ull;
   const bool all = ch.ties == kAllTies;
   std::uint32_t ties_before = 0;
   if (!all) {
     std::uint32_t mine = 0;
-    keys.each([&](const K (&x)[4], std::uint32_t i) {
+    keys.each([&](const K (&x)[4], std::uint32_t) {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) mine += static_cast<std::uint32_t>(__popcll(__ballot(i + e < keys.n && x[e] == ch.least)));
+      for (int e = 0; e < 4; ++e) mine += static_cast<std::uint32_t>(__popcll(__ballot(x[e] == ch.least)));
     });
     if (lane == 0u) sh.wave[0][wave] = mine;
     __syncthreads();
-    ties_before = waves_before(sh.wave[0], wave).x;
+    ties_before = waves_before<T>(sh.wave[0], wave).x;
   }
-  // the classes of a round's four places, 2 bits each; `ties`: equal keys before the round
-  auto classes = [&](const K (&x)[4], std::uint32_t i, std::uint32_t& ties) {
-    std::uint32_t c = 0u;
-    unsigned long long tie[4];
+  // the lanes of a round's four places that are of either kind; `ties`: equal keys before the round
+  auto kinds = [&](const K (&x)[4], std::uint32_t i, std::uint32_t& ties, unsigned long long (&f)[4],
+                   unsigned long long (&k)[4]) {
     std::uint32_t at = ties;
     if (!all) {
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        tie[e] = __ballot(i + e < keys.n && x[e] == ch.least);
-        at += static_cast<std::uint32_t>(__popcll(tie[e] & below));
-        ties += static_cast<std::uint32_t>(__popcll(tie[e]));
+        const unsigned long long b = __ballot(x[e] == ch.least);
+        at += lanes_below(b);
+        ties += static_cast<std::uint32_t>(__popcll(b));
       }
     }
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       bool chosen = x[e] >= ch.least;
       if (!all && x[e] == ch.least) chosen = at++ < ch.ties;
-      c |= i + e < keys.n ? static_cast<std::uint32_t>(kind(i + e, chosen)) << (2 * e) : 0u;
+      const unsigned long long c = __ballot(chosen), low = __ballot(i + e < split);
+      f[e] = low & ~c;
+      k[e] = c & ~low;
     }
-    return c;
   };
-  std::uint32_t n1 = 0, n2 = 0, ties = ties_before;
+  std::uint32_t nf = 0, nk = 0, ties = ties_before;
   keys.each([&](const K (&x)[4], std::uint32_t i) {
-    const std::uint32_t c = classes(x, i, ties);
+    unsigned long long f[4], k[4];
+    kinds(x, i, ties, f, k);
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      n1 += static_cast<std::uint32_t>(__popcll(__ballot((c >> (2 * e) & 3u) == 1u)));
-      n2 += static_cast<std::uint32_t>(__popcll(__ballot((c >> (2 * e) & 3u) == 2u)));
+      nf += static_cast<std::uint32_t>(__popcll(f[e]));
+      nk += static_cast<std::uint32_t>(__popcll(k[e]));
     }
   });
-  if (lane == 0u) sh.wave[1][wave] = n1, sh.wave[2][wave] = n2;
+  if (lane == 0u) sh.wave[1][wave] = nf, sh.wave[2][wave] = nk;
   __syncthreads();
-  const uint2 w1 = waves_before(sh.wave[1], wave), w2 = waves_before(sh.wave[2], wave);
-  std::uint32_t at1 = w1.x, at2 = w2.x;
+  const uint2 wf = waves_before<T>(sh.wave[1], wave), wk = waves_before<T>(sh.wave[2], wave);
+  std::uint32_t at_f = wf.x, at_k = wk.x;
   ties = ties_before;
+  auto put = [&](const unsigned long long (&m)[4], std::uint32_t i, std::uint32_t& at, auto& to) {
+    if (((m[0] | m[1]) | (m[2] | m[3])) == 0ull) return;
+    std::uint32_t rank = at;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      rank += lanes_below(m[e]);
+      at += static_cast<std::uint32_t>(__popcll(m[e]));
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if ((m[e] >> lane & 1ull) != 0ull) to(i + e, rank++);
+  };
   keys.each([&](const K (&x)[4], std::uint32_t i) {
-    const std::uint32_t c = classes(x, i, ties);
-    std::uint32_t r1 = at1, r2 = at2;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const unsigned long long b1 = __ballot((c >> (2 * e) & 3u) == 1u), b2 = __ballot((c >> (2 * e) & 3u) == 2u);
-      r1 += static_cast<std::uint32_t>(__popcll(b1 & below)), at1 += static_cast<std::uint32_t>(__popcll(b1));
-      r2 += static_cast<std::uint32_t>(__popcll(b2 & below)), at2 += static_cast<std::uint32_t>(__popcll(b2));
-    }
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const std::uint32_t k = c >> (2 * e) & 3u;
-      if (k == 1u) put(1, i + e, r1++);
-      if (k == 2u) put(2, i + e, r2++);
-    }
+    unsigned long long f[4], k[4];
+    kinds(x, i, ties, f, k);
+    put(f, i, at_f, freed);
+    put(k, i, at_k, kept);
   });
-  return make_uint2(w1.y, w2.y);
+  return make_uint2(wf.y, wk.y);
 }
+
+// Threads of a choice over at most n keys.
+std::uint32_t choice_threads(std::uint32_t n) { return n <= 2048u ? 256u : 1024u; }
 
 // LDS bytes for n keys of `width` bytes, up to 128 KB, in whole rounds of a workgroup.
 std::size_t held_bytes(std::uint32_t n, std::size_t width) {
-  const std::size_t round = 4u * kSelThreads * width, rounds = (n * width + round - 1u) / round;
+  const std::size_t round = 4u * choice_threads(n) * width, rounds = (n * width + round - 1u) / round;
   return round * rounds < (128u << 10) ? round * rounds : 128u << 10;
 }
 
 typedef unsigned long long u64x4 __attribute__((ext_vector_type(4), aligned(8)));
 
-__global__ __launch_bounds__(kSelThreads) void page_choice_kernel(PagedView kv, const std::uint32_t* __restrict__ pos,
-                                                                  const unsigned long long* __restrict__ row_keys,
-                                                                  std::uint32_t room, std::uint32_t n_select,
-                                                                  std::int32_t* __restrict__ pages) {
-  __shared__ __align__(16) SelectShared sh;
+struct KeyRow {
+  const unsigned long long* row;
+  std::uint32_t n;
+  __device__ __forceinline__ u64x4 raw(std::uint32_t i) const {
+    u64x4 v = {0ull, 0ull, 0ull, 0ull};
+    if (i + 4u <= n) {
+      v = *reinterpret_cast<const u64x4*>(row + i);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (i + e < n) v[e] = row[i + e];
+    }
+    return v;
+  }
+  __device__ __forceinline__ void keys(std::uint32_t, const u64x4& v, unsigned long long (&x)[4]) const {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) x[e] = v[e];
+  }
+};
+
+template <std::uint32_t T>
+__global__ __launch_bounds__(T) void page_choice_kernel(PagedView kv, const std::uint32_t* __restrict__ pos,
+                                                        const unsigned long long* __restrict__ row_keys,
+                                                        std::uint32_t room, std::uint32_t n_select,
+                                                        std::int32_t* __restrict__ pages) {
+  __shared__ __align__(16) SelectShared<T> sh;
   extern __shared__ __align__(16) std::uint8_t lds[];
   const std::uint32_t g = blockIdx.x, r = blockIdx.y;
   const std::uint32_t used = (paged_filled(kv, pos[r]) + kv.page_size - 1u) / kv.page_size;
   if (used == 0u) return;  // a padded row
-  const unsigned long long* const row = row_keys + (static_cast<std::size_t>(r) * kv.n_kv + g) * kv.entries;
-  std::int32_t* const out = pages + (static_cast<std::size_t>(r) * kv.n_kv + g) * n_select;
-  auto load = [&](std::uint32_t i, unsigned long long (&x)[4]) {
-    if (i + 4u <= used) {
-      const u64x4 v = *reinterpret_cast<const u64x4*>(row + i);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) x[e] = v[e];
-    } else {
-#pragma unroll
-      for (int e = 0; e < 4; ++e) x[e] = i + e < used ? row[i + e] : 0ull;
-    }
-  };
-  const Keys<unsigned long long, decltype(load)> keys(load, lds, used, room);
-  Choice<unsigned long long> ch = radix_choice(sh, keys, n_select);
-  if (ch.least == 0ull) ch = Choice<unsigned long long>{1ull, kAllTies};  // every candidate, and no page that is not there
-  const std::uint32_t listed = for_chosen(
-      sh, keys, ch, [](std::uint32_t, bool chosen) { return chosen ? 1 : 0; },
-      [&](int, std::uint32_t i, std::uint32_t rank) {
+  const std::size_t gr = static_cast<std::size_t>(r) * kv.n_kv + g;
+  const KeyRow src{row_keys + gr * kv.entries, used};
+  const Keys<unsigned long long, KeyRow, T> keys(src, lds, used, room);
+  std::int32_t* const out = pages + gr * n_select;
+  // 1 and more: every page that is there
+  Choice<unsigned long long> ch{1ull, kAllTies};
+  if (n_select < used) ch = radix_choice(sh, keys, n_select);
+  if (ch.least == 0ull) ch = Choice<unsigned long long>{1ull, kAllTies};
+  const std::uint32_t listed = for_choice(
+      sh, keys, ch, 0u, [](std::uint32_t, std::uint32_t) {},
+      [&](std::uint32_t i, std::uint32_t rank) {
         if (rank < n_select) out[rank] = static_cast<std::int32_t>(i);
-      }).x;
-  for (std::uint32_t i = listed + threadIdx.x; i < n_select; i += kSelThreads) out[i] = -1;
+      }).y;
+  for (std::uint32_t i = listed + threadIdx.x; i < n_select; i += T) out[i] = -1;
 }
 
 // A weight as an unsigned key of the same order, 0 for NaN; protected slots above
@@ -351,8 +445,67 @@ struct EvictArgs {
   std::uint32_t keep, n_first, n_recent, most, room;
 };
 
-__global__ __launch_bounds__(kSelThreads) void evict_choice_kernel(PagedView kv, EvictArgs a) {
-  __shared__ __align__(16) SelectShared sh;
+struct SlotKeys {
+  const float* w;
+  const std::uint32_t* p;
+  float* wo;  // null, or where the slots below `stay` are copied as they are read
+  std::uint32_t* po;
+  std::uint32_t n, stay, newest, n_first, n_recent;
+  struct Raw {
+    f32x4_any w;
+    u32x4_any p;
+  };
+  __device__ __forceinline__ Raw raw(std::uint32_t i) const {
+    Raw v{{0.0f, 0.0f, 0.0f, 0.0f}, {0u, 0u, 0u, 0u}};
+    if (i + 4u <= n) {
+      v.w = *reinterpret_cast<const f32x4_any*>(w + i);
+      v.p = *reinterpret_cast<const u32x4_any*>(p + i);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (i + e < n) v.w[e] = w[i + e], v.p[e] = p[i + e];
+    }
+    return v;
+  }
+  __device__ __forceinline__ void keys(std::uint32_t i, const Raw& v, std::uint32_t (&x)[4]) const {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) x[e] = i + e < n ? weight_key(v.w[e], v.p[e], newest, n_first, n_recent) : 0u;
+  }
+  // slots below `stay`, unless they lie there already
+  __device__ __forceinline__ void copy(std::uint32_t threads) const {
+    for (std::uint32_t i = 4u * threadIdx.x; i < stay; i += 4u * threads) {
+      const Raw v = raw(i);
+      if (i + 4u <= stay) {
+        if (wo != w) *reinterpret_cast<f32x4_any*>(wo + i) = v.w;
+        if (po != p) *reinterpret_cast<u32x4_any*>(po + i) = v.p;
+      } else {
+        for (std::uint32_t e = 0; i + e < stay; ++e) wo[i + e] = v.w[e], po[i + e] = v.p[e];
+      }
+    }
+  }
+};
+
+// One move: the row's key and value by L = head_dim / 8 lanes, 16 bytes each of
+// both, its weight and position by the first two of them. Every slot that is written
+// lies below keep, every moved one at or behind it: no read meets a write.
+template <int L>
+__device__ __forceinline__ void move_row(const PagedView& kv, const EvictArgs& a, std::uint32_t r, std::uint32_t g,
+                                         std::uint32_t to_slot, std::uint32_t from_slot, std::uint32_t t) {
+  const std::int32_t* const table = kv.table + static_cast<std::size_t>(r) * kv.table_stride;
+  const std::size_t state = (static_cast<std::size_t>(r) * kv.n_kv + g) * kv.capacity;
+  const std::uint32_t to = paged_slot_row(kv, table, g, to_slot), from = paged_slot_row(kv, table, g, from_slot);
+  if (t == 0u) a.weight_out[state + to_slot] = a.weight[state + from_slot];
+  if (t == 1u) a.slot_pos_out[state + to_slot] = a.slot_pos[state + from_slot];
+  if (to == kNoRow || from == kNoRow) return;
+  const uint4 x = reinterpret_cast<const uint4*>(kv.k)[static_cast<std::size_t>(from) * L + t];
+  const uint4 y = reinterpret_cast<const uint4*>(kv.v)[static_cast<std::size_t>(from) * L + t];
+  reinterpret_cast<uint4*>(kv.k)[static_cast<std::size_t>(to) * L + t] = x;
+  reinterpret_cast<uint4*>(kv.v)[static_cast<std::size_t>(to) * L + t] = y;
+}
+
+template <std::uint32_t T>
+__global__ __launch_bounds__(T) void evict_choice_kernel(PagedView kv, EvictArgs a) {
+  __shared__ __align__(16) SelectShared<T> sh;
   extern __shared__ __align__(16) std::uint8_t lds[];
   const std::uint32_t g = blockIdx.x, r = blockIdx.y, tid = threadIdx.x;
   const std::size_t gr = static_cast<std::size_t>(r) * kv.n_kv + g;
@@ -364,80 +517,69 @@ __global__ __launch_bounds__(kSelThreads) void evict_choice_kernel(PagedView kv,
     if (tid == 0u) moves[0] = 0u;
     return;
   }
-  const float* const w = a.weight + gr * kv.capacity;
-  const std::uint32_t* const p = a.slot_pos + gr * kv.capacity;
-  float* const wo = a.weight_out + gr * kv.capacity;
-  std::uint32_t* const po = a.slot_pos_out + gr * kv.capacity;
-  const std::uint32_t stay = n < a.keep ? n : a.keep;
+  const SlotKeys src{a.weight + gr * kv.capacity, a.slot_pos + gr * kv.capacity, a.weight_out + gr * kv.capacity,
+                     a.slot_pos_out + gr * kv.capacity, n, n < a.keep ? n : a.keep, newest, a.n_first, a.n_recent};
+  if (src.wo != src.w || src.po != src.p) src.copy(T);
   if (n <= a.keep) {
-    for (std::uint32_t i = tid; i < stay; i += kSelThreads) wo[i] = w[i], po[i] = p[i];
     if (tid == 0u) moves[0] = 0u;
     return;
   }
-  auto load = [&](std::uint32_t i, std::uint32_t (&x)[4]) {
-    f32x4_any wv = {0.0f, 0.0f, 0.0f, 0.0f};
-    u32x4_any pv = {0u, 0u, 0u, 0u};
-    if (i + 4u <= n) {
-      wv = *reinterpret_cast<const f32x4_any*>(w + i);
-      pv = *reinterpret_cast<const u32x4_any*>(p + i);
-    } else {
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (i + e < n) wv[e] = w[i + e], pv[e] = p[i + e];
-    }
-#pragma unroll
-    for (int e = 0; e < 4; ++e) x[e] = weight_key(wv[e], pv[e], newest, a.n_first, a.n_recent);
-  };
-  const Keys<std::uint32_t, decltype(load)> keys(load, lds, n, a.room);
+  const Keys<std::uint32_t, SlotKeys, T> keys(src, lds, n, a.room);
   const Choice<std::uint32_t> ch = radix_choice(sh, keys, a.keep);
   std::uint32_t* const to = moves + 1u;
   std::uint32_t* const from = to + a.most;
-  const std::uint32_t holes = for_chosen(
-      sh, keys, ch,
-      [&](std::uint32_t i, bool chosen) { return i < a.keep ? (chosen ? 0 : 1) : (chosen ? 2 : 0); },
-      [&](int kind, std::uint32_t i, std::uint32_t m) {
-        if (m < a.most) (kind == 1 ? to : from)[m] = i;
+  const std::uint32_t freed = for_choice(
+      sh, keys, ch, a.keep,
+      [&](std::uint32_t i, std::uint32_t m) {
+        if (m < a.most) to[m] = i;
+      },
+      [&](std::uint32_t i, std::uint32_t m) {
+        if (m < a.most) from[m] = i;
       }).x;
-  const std::uint32_t n_moves = holes < a.most ? holes : a.most;
-  if (tid == 0u) moves[0] = n_moves;
-  // every slot that is written lies below keep, every moved one at or behind it: in
-  // place, no read meets a write of another thread
-  if (wo != w)
-    for (std::uint32_t i = tid; i < stay; i += kSelThreads) wo[i] = w[i];
-  if (po != p)
-    for (std::uint32_t i = tid; i < stay; i += kSelThreads) po[i] = p[i];
-  __threadfence_block();
-  __syncthreads();
-  for (std::uint32_t m = tid; m < n_moves; m += kSelThreads) {
-    wo[to[m]] = w[from[m]];
-    po[to[m]] = p[from[m]];
-  }
+  if (tid == 0u) moves[0] = freed < a.most ? freed : a.most;
 }
 
-// L = head_dim / 8 lanes a row: 16 bytes a lane of its key and of its value.
 template <int L>
-__global__ __launch_bounds__(kThreads) void evict_move_kernel(PagedView kv, const std::uint32_t* moves_all,
-                                                              std::uint32_t most, std::uint32_t keep,
-                                                              const std::uint32_t* pos, const std::uint32_t* length,
-                                                              std::uint32_t* length_out) {
+__global__ __launch_bounds__(kThreads) void evict_move_kernel(PagedView kv, EvictArgs a, std::uint32_t* length_out) {
   const std::uint32_t g = blockIdx.y, r = blockIdx.z;
-  if (blockIdx.x == 0u && g == 0u && threadIdx.x == 0u && pos[r] != RTXLLM_NO_POSITION) {
-    std::uint32_t n = length[r];
+  if (blockIdx.x == 0u && g == 0u && threadIdx.x == 0u && a.pos[r] != RTXLLM_NO_POSITION) {
+    std::uint32_t n = a.length[r];
     n = n < kv.capacity ? n : kv.capacity;
-    length_out[r] = n < keep ? n : keep;
+    length_out[r] = n < a.keep ? n : a.keep;
   }
   const std::uint32_t* const moves =
-      moves_all + (static_cast<std::size_t>(r) * kv.n_kv + g) * (1u + 2u * static_cast<std::size_t>(most));
-  const std::uint32_t m = blockIdx.x * (kThreads / L) + threadIdx.x / L, t = threadIdx.x % L;
-  if (m >= moves[0]) return;
-  const std::int32_t* const table = kv.table + static_cast<std::size_t>(r) * kv.table_stride;
-  const std::uint32_t to = paged_slot_row(kv, table, g, moves[1u + m]);
-  const std::uint32_t from = paged_slot_row(kv, table, g, moves[1u + most + m]);
-  if (to == kNoRow || from == kNoRow) return;
-  const uint4 x = reinterpret_cast<const uint4*>(kv.k)[static_cast<std::size_t>(from) * L + t];
-  const uint4 y = reinterpret_cast<const uint4*>(kv.v)[static_cast<std::size_t>(from) * L + t];
-  reinterpret_cast<uint4*>(kv.k)[static_cast<std::size_t>(to) * L + t] = x;
-  reinterpret_cast<uint4*>(kv.v)[static_cast<std::size_t>(to) * L + t] = y;
+      a.moves + (static_cast<std::size_t>(r) * kv.n_kv + g) * (1u + 2u * static_cast<std::size_t>(a.most));
+  const std::uint32_t m = blockIdx.x * (kThreads / L) + threadIdx.x / L;
+  if (m >= a.most) return;
+  const std::uint32_t to = moves[1u + m], from = moves[1u + a.most + m];  // read with the count: used below it
+  if (m < moves[0]) move_row<L>(kv, a, r, g, to, from, threadIdx.x % L);
+}
+
+template <int L>
+hipError_t launch_select(const PagedView& view, const std::uint16_t* bounds, const float* q, std::uint32_t group,
+                         const std::uint32_t* pos, std::uint32_t count, std::uint32_t n_first, std::uint32_t n_last,
+                         std::uint32_t n_select, unsigned long long* keys, std::int32_t* pages, hipStream_t stream) {
+  const dim3 choices(view.n_kv, count);
+  auto score = [&](auto steps) {
+    constexpr int kSteps = decltype(steps)::value;
+    constexpr std::uint32_t kPer = kSteps * kThreads / L;  // pages of a workgroup
+    hipLaunchKernelGGL((page_score_kernel<L, kSteps>), dim3((view.entries + kPer - 1u) / kPer, view.n_kv, count),
+                       dim3(kThreads), 0, stream, view, bounds, q, group, pos, n_first, n_last, keys);
+  };
+  const std::uint64_t waves = static_cast<std::uint64_t>(count) * view.n_kv * ((view.entries + 64u / L - 1u) / (64u / L));
+  if (waves > 4096u)
+    score(std::integral_constant<int, 4>{});
+  else
+    score(std::integral_constant<int, 1>{});
+  const hipError_t rc = hipGetLastError();
+  if (rc != hipSuccess) return rc;
+  const std::size_t held = held_bytes(view.entries, 8u);
+  const auto room = static_cast<std::uint32_t>(held / 8u);
+  if (choice_threads(view.entries) == 256u)
+    hipLaunchKernelGGL(page_choice_kernel<256>, choices, dim3(256), held, stream, view, pos, keys, room, n_select, pages);
+  else
+    hipLaunchKernelGGL(page_choice_kernel<1024>, choices, dim3(1024), held, stream, view, pos, keys, room, n_select, pages);
+  return hipGetLastError();
 }
 
 std::uint32_t most_moves(const rtxllm_paged_kv* c, std::uint32_t keep) {
@@ -469,20 +611,9 @@ extern "C" hipError_t rtxllm_attn_select_pages(const rtxllm_paged_kv* cache, con
   if (group == 0u) return hipErrorInvalidValue;
   const PagedView view = paged_view(cache);
   auto* keys = static_cast<unsigned long long*>(workspace);
-  const std::uint32_t per = (kThreads / 64u) * (512u / cache->head_dim);
-  const dim3 grid((view.entries + per - 1u) / per, view.n_kv, count);
-  if (cache->head_dim == 64u)
-    hipLaunchKernelGGL(page_score_kernel<8>, grid, dim3(kThreads), 0, stream, view, bounds, q, group, pos, n_first, n_last, keys);
-  else if (cache->head_dim == 128u)
-    hipLaunchKernelGGL(page_score_kernel<16>, grid, dim3(kThreads), 0, stream, view, bounds, q, group, pos, n_first, n_last, keys);
-  else
-    hipLaunchKernelGGL(page_score_kernel<32>, grid, dim3(kThreads), 0, stream, view, bounds, q, group, pos, n_first, n_last, keys);
-  hipError_t rc = hipGetLastError();
-  if (rc != hipSuccess) return rc;
-  const std::size_t held = held_bytes(view.entries, 8u);
-  hipLaunchKernelGGL(page_choice_kernel, dim3(view.n_kv, count), dim3(kSelThreads), held, stream, view, pos, keys,
-                     static_cast<std::uint32_t>(held / 8u), n_select, pages);
-  return hipGetLastError();
+  return cache->head_dim == 64u    ? launch_select<8>(view, bounds, q, group, pos, count, n_first, n_last, n_select, keys, pages, stream)
+         : cache->head_dim == 128u ? launch_select<16>(view, bounds, q, group, pos, count, n_first, n_last, n_select, keys, pages, stream)
+                                   : launch_select<32>(view, bounds, q, group, pos, count, n_first, n_last, n_select, keys, pages, stream);
 }
 
 extern "C" size_t rtxllm_kv_evict_workspace(const rtxllm_paged_kv* cache, uint32_t keep, uint32_t count) {
@@ -519,15 +650,18 @@ extern "C" hipError_t rtxllm_kv_evict_f16(const rtxllm_paged_kv* cache, const ui
   const std::size_t held = held_bytes(view.capacity, 4u);
   const EvictArgs a{length, pos, weight, slot_pos, weight_out, slot_pos_out, static_cast<std::uint32_t*>(workspace),
                     keep,   n_first, n_recent, most, static_cast<std::uint32_t>(held / 4u)};
-  hipLaunchKernelGGL(evict_choice_kernel, dim3(view.n_kv, count), dim3(kSelThreads), held, stream, view, a);
+  if (choice_threads(view.capacity) == 256u)
+    hipLaunchKernelGGL(evict_choice_kernel<256>, dim3(view.n_kv, count), dim3(256), held, stream, view, a);
+  else
+    hipLaunchKernelGGL(evict_choice_kernel<1024>, dim3(view.n_kv, count), dim3(1024), held, stream, view, a);
   hipError_t rc = hipGetLastError();
   if (rc != hipSuccess) return rc;
   const dim3 grid(most > 0u ? (most + per - 1u) / per : 1u, view.n_kv, count);
   if (cache->head_dim == 64u)
-    hipLaunchKernelGGL(evict_move_kernel<8>, grid, dim3(kThreads), 0, stream, view, a.moves, most, keep, pos, length, length_out);
+    hipLaunchKernelGGL(evict_move_kernel<8>, grid, dim3(kThreads), 0, stream, view, a, length_out);
   else if (cache->head_dim == 128u)
-    hipLaunchKernelGGL(evict_move_kernel<16>, grid, dim3(kThreads), 0, stream, view, a.moves, most, keep, pos, length, length_out);
+    hipLaunchKernelGGL(evict_move_kernel<16>, grid, dim3(kThreads), 0, stream, view, a, length_out);
   else
-    hipLaunchKernelGGL(evict_move_kernel<32>, grid, dim3(kThreads), 0, stream, view, a.moves, most, keep, pos, length, length_out);
+    hipLaunchKernelGGL(evict_move_kernel<32>, grid, dim3(kThreads), 0, stream, view, a, length_out);
   return hipGetLastError();
 }

@@ -128,7 +128,8 @@ def test_row_addresses(tmp_path):
     src = tmp_path / "t.cpp"
     src.write_text('#include "paged.h"\n#include <cstdio>\nusing namespace rtxllm;\nint main() {\n'
                    "  const std::int32_t table[4] = {2, -1, 7, 6};\n"
-                   "  const PagedView c{nullptr, nullptr, table, 4, 7, 3, 5, 20, 4};\n"
+                   "  const rtxllm_paged_kv d{reinterpret_cast<std::uint16_t*>(16), reinterpret_cast<std::uint16_t*>(16), table, 4, 7, 3, 64, 5, 20};\n"
+                   "  const PagedView c = paged_view(&d);\n"
                    "  for (std::uint32_t s = 0; s < 22; ++s) std::printf(\"%u \", paged_slot_row(c, table, 2, s));\n"
                    "  std::printf(\"%u %u %u %u\", paged_filled(c, 0xFFFFFFFFu), paged_filled(c, 0), paged_filled(c, 19),\n"
                    "              paged_filled(c, 4000000000u));\n}\n")
