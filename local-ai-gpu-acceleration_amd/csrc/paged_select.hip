@@ -132,7 +132,8 @@ struct SelectShared {
   std::uint32_t bin, above, count;
 };
 
-// Inclusive sum over the lanes below and the lane itself, by DPP.
+// Inclusive sum over the lanes below and the lane itself (of its row of 16), by DPP.
+template <int LANES = 64>
 __device__ __forceinline__ std::uint32_t wave_scan(std::uint32_t v) {
   auto add = [&](auto ctrl, auto rows) {
     v += static_cast<std::uint32_t>(
@@ -143,6 +144,7 @@ __device__ __forceinline__ std::uint32_t wave_scan(std::uint32_t v) {
   add(std::integral_constant<int, 0x112>{}, all);
   add(std::integral_constant<int, 0x114>{}, all);
   add(std::integral_constant<int, 0x118>{}, all);
+  if constexpr (LANES == 16) return v;
   // a row's last lane into the next row (rows 1, 3), then of row 1 into rows 2 and 3
   add(std::integral_constant<int, 0x142>{}, std::integral_constant<int, 0xA>{});
   add(std::integral_constant<int, 0x143>{}, std::integral_constant<int, 0xC>{});
@@ -155,17 +157,14 @@ __device__ __forceinline__ std::uint32_t lanes_below(unsigned long long mask) {
                                    __builtin_amdgcn_mbcnt_lo(static_cast<std::uint32_t>(mask), 0u));
 }
 
-// Sum of the waves' words before this wave, and of all.
+// Sum of the waves' words before this wave, and of all: a lane a wave (at most 16, one
+// row of lanes), every wave for itself.
 template <std::uint32_t T>
 __device__ __forceinline__ uint2 waves_before(const std::uint32_t (&words)[T / 64u], std::uint32_t wave) {
-  uint2 s = make_uint2(0u, 0u);
-#pragma unroll
-  for (std::uint32_t w = 0; w < T / 64u; w += 4u) {
-    const uint4 x = *reinterpret_cast<const uint4*>(&words[w]);
-    s.x += (w < wave ? x.x : 0u) + (w + 1u < wave ? x.y : 0u) + (w + 2u < wave ? x.z : 0u) + (w + 3u < wave ? x.w : 0u);
-    s.y += (x.x + x.y) + (x.z + x.w);
-  }
-  return s;
+  constexpr std::uint32_t kWaves = T / 64u;
+  const std::uint32_t lane = threadIdx.x & 63u;
+  const std::uint32_t own = lane < kWaves ? words[lane] : 0u, sum = wave_scan<16>(own);
+  return make_uint2(__builtin_amdgcn_readlane(sum - own, wave), __builtin_amdgcn_readlane(sum, kWaves - 1u));
 }
 
 // The keys of a workgroup: a wave's part contiguous, four keys a lane and round, so
@@ -174,7 +173,8 @@ __device__ __forceinline__ uint2 waves_before(const std::uint32_t (&words)[T / 6
 // reads them; of more, every pass reads all again (from the L2). The loops over them are
 // rolled: each runs a few rounds once, and unrolled code with the keys in registers
 // took longer to fetch (32 keys a thread: 92 us for 32768 keys). src.raw(i) loads what
-// keys i..i + 3 (i % 4 == 0) are made of, src.keys(i, raw, x) makes them.
+// keys i..i + 3 (i % 4 == 0) are made of, src.keys(i, raw, x) makes them, src.seen(i, raw)
+// is called for each once, where they go into the LDS.
 template <class K, class Source, std::uint32_t T>
 struct Keys {
   struct alignas(16) Four {
@@ -198,9 +198,16 @@ struct Keys {
 #pragma unroll
       for (std::uint32_t u = 0; u < 4u; ++u) v[u] = src.raw(place(j + u));
 #pragma unroll
-      for (std::uint32_t u = 0; u < 4u; ++u) src.keys(place(j + u), v[u], held[T * (j + u)].k);
+      for (std::uint32_t u = 0; u < 4u; ++u) {
+        src.seen(place(j + u), v[u]);
+        src.keys(place(j + u), v[u], held[T * (j + u)].k);
+      }
     }
-    for (; j < rounds; ++j) src.keys(place(j), src.raw(place(j)), held[T * j].k);
+    for (; j < rounds; ++j) {
+      const auto v = src.raw(place(j));
+      src.seen(place(j), v);
+      src.keys(place(j), v, held[T * j].k);
+    }
   }
   __device__ __forceinline__ std::uint32_t place(std::uint32_t j) const {
     return first + 256u * j + 4u * (threadIdx.x & 63u);
@@ -222,21 +229,15 @@ struct Keys {
 // Radix selection from the top, 11 bits a pass: the workgroup counts the keys that
 // share the digits found so far by their next digit, and takes the digit in which
 // the k-th largest lies. It ends early once all keys of that digit are wanted,
-// after two or three passes where keys are spread. Lanes that all count the same
-// digit (equal keys) add once, as one address takes one addition at a time. k is at
+// after two or three passes where keys are spread. 256 keys of one digit are one
+// addition, as an address takes one at a time (equal weights, protected slots). k is at
 // most the number of keys: the zeros behind the last one are never among the best,
 // since of equal keys the first count.
 template <class K, class Source, std::uint32_t T>
 __device__ Choice<K> radix_choice(SelectShared<T>& sh, const Keys<K, Source, T>& keys, std::uint32_t k) {
   constexpr int kBits = static_cast<int>(8u * sizeof(K));
   const std::uint32_t tid = threadIdx.x, lane = tid & 63u, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  constexpr std::uint32_t kOwn = kBins / T;  // bins of a thread
-  static_assert(kOwn % 2u == 0u, "pairs of bins");
-  auto clear = [&](std::uint32_t* h) {
-#pragma unroll
-    for (std::uint32_t i = 0; i < kOwn; i += 2u) *reinterpret_cast<uint2*>(h + i * T + 2u * tid) = make_uint2(0u, 0u);
-  };
-  clear(sh.hist[0]);
+  for (std::uint32_t i = 4u * tid; i < kBins; i += 4u * T) *reinterpret_cast<uint4*>(&sh.hist[0][i]) = make_uint4(0u, 0u, 0u, 0u);
   __syncthreads();
   K prefix = 0;
   int shift = kBits;
@@ -244,42 +245,48 @@ __device__ Choice<K> radix_choice(SelectShared<T>& sh, const Keys<K, Source, T>&
     const int bits = shift < kDigit ? shift : kDigit, next = shift - bits;
     std::uint32_t* const hist = sh.hist[turn];
     keys.each([&](const K (&x)[4], std::uint32_t) {
+      std::uint32_t digit[4], others = 0u;  // kBins: of other digits above
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        if (shift != kBits && (x[e] >> shift) != prefix) continue;
-        const std::uint32_t digit = static_cast<std::uint32_t>(x[e] >> next) & ((1u << bits) - 1u);
-        const unsigned long long who = __ballot(true);
-        if (__ballot(digit == __builtin_amdgcn_readfirstlane(digit)) != who)
-          atomicAdd(&hist[digit], 1u);
-        else if (lanes_below(who) == 0u)
-          atomicAdd(&hist[digit], static_cast<std::uint32_t>(__popcll(who)));
+        const bool match = shift == kBits || (x[e] >> shift) == prefix;
+        digit[e] = match ? static_cast<std::uint32_t>(x[e] >> next) & ((1u << bits) - 1u) : kBins;
       }
+      const std::uint32_t one = __builtin_amdgcn_readfirstlane(digit[0]);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) others |= digit[e] ^ one;
+      if (__ballot(others != 0u) == 0ull) {
+        if (lane == 0u && one != kBins) atomicAdd(&hist[one], 256u);
+        return;
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (digit[e] != kBins) atomicAdd(&hist[digit[e]], 1u);
     });
     __syncthreads();
-    // thread t: the kOwn bins below kBins - kOwn t, sums from the largest digit down
-    const std::uint32_t low = kBins - kOwn * (tid + 1u);
-    std::uint32_t c[kOwn], own = 0u;
+    if (wave == 0u) {
+      // lane l sums the 32 bins below 2048 - 32 l; in the lane whose sums pass k, the bins
+      // again, one a lane, from the largest digit down
+      constexpr std::uint32_t kOwn = kBins / 64u;
+      const uint4* own = reinterpret_cast<const uint4*>(hist + kBins - kOwn * (lane + 1u));
+      std::uint32_t mine = 0;
 #pragma unroll
-    for (std::uint32_t i = 0; i < kOwn; i += 2u) {
-      const uint2 v = *reinterpret_cast<const uint2*>(hist + low + i);
-      c[i] = v.x, c[i + 1u] = v.y;
-      own += v.x + v.y;
-    }
-    clear(sh.hist[turn ^ 1u]);
-    const std::uint32_t sum = wave_scan(own);
-    if (lane == 63u) sh.wave[0][wave] = sum;
-    __syncthreads();
-    std::uint32_t before = waves_before<T>(sh.wave[0], wave).x + sum - own;
-    if (before < k && k <= before + own) {
-#pragma unroll
-      for (int i = static_cast<int>(kOwn) - 1; i >= 0; --i) {
-        if (before < k && k <= before + c[i]) {
-          sh.bin = low + static_cast<std::uint32_t>(i);
-          sh.above = before;
-          sh.count = c[i];
-        }
-        before += c[i];
+      for (std::uint32_t i = 0; i < kOwn / 4u; ++i) {
+        const uint4 v = own[(i + lane) % (kOwn / 4u)];  // turned by the lane: no two of eight in one bank
+        mine += (v.x + v.y) + (v.z + v.w);
       }
+      const std::uint32_t upto = wave_scan(mine);
+      const auto l = static_cast<std::uint32_t>(__builtin_ctzll(__ballot(upto >= k)));
+      const std::uint32_t before = __builtin_amdgcn_readlane(upto - mine, l);
+      const std::uint32_t bin = kBins - kOwn * l - 1u - (lane & (kOwn - 1u));
+      const std::uint32_t c = lane < kOwn ? hist[bin] : 0u, sum = before + wave_scan(c);
+      if (lane == static_cast<std::uint32_t>(__builtin_ctzll(__ballot(sum >= k)))) {
+        sh.bin = bin;
+        sh.above = sum - c;
+        sh.count = c;
+      }
+    } else {
+      for (std::uint32_t i = 4u * (tid - 64u); i < kBins; i += 4u * (T - 64u))
+        *reinterpret_cast<uint4*>(&sh.hist[turn ^ 1u][i]) = make_uint4(0u, 0u, 0u, 0u);
     }
     __syncthreads();
     prefix = (prefix << bits) | static_cast<K>(sh.bin);
@@ -309,59 +316,54 @@ __device__ uint2 for_choice(SelectShared<T>& sh, const Keys<K, Source, T>& keys,
     __syncthreads();
     ties_before = waves_before<T>(sh.wave[0], wave).x;
   }
-  // the lanes of a round's four places that are of either kind; `ties`: equal keys before the round
-  auto kinds = [&](const K (&x)[4], std::uint32_t i, std::uint32_t& ties, unsigned long long (&f)[4],
-                   unsigned long long (&k)[4]) {
-    std::uint32_t at = ties;
-    if (!all) {
+  // a lane's four places of either kind, a bit each; `ties`: equal keys before the round
+  struct Kinds {
+    std::uint32_t freed, kept;
+  };
+  auto kinds = [&](const K (&x)[4], std::uint32_t i, std::uint32_t& ties) {
+    std::uint32_t chosen = 0u;
+    if (all) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) chosen |= x[e] >= ch.least ? 1u << e : 0u;
+    } else {
+      std::uint32_t at = ties;
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const unsigned long long b = __ballot(x[e] == ch.least);
         at += lanes_below(b);
         ties += static_cast<std::uint32_t>(__popcll(b));
       }
-    }
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      bool chosen = x[e] >= ch.least;
-      if (!all && x[e] == ch.least) chosen = at++ < ch.ties;
-      const unsigned long long c = __ballot(chosen), low = __ballot(i + e < split);
-      f[e] = low & ~c;
-      k[e] = c & ~low;
+      for (int e = 0; e < 4; ++e) chosen |= x[e] > ch.least || (x[e] == ch.least && at++ < ch.ties) ? 1u << e : 0u;
     }
+    const std::uint32_t low = i >= split ? 0u : split - i >= 4u ? 15u : (1u << (split - i)) - 1u;
+    return Kinds{low & ~chosen, chosen & ~low};
   };
-  std::uint32_t nf = 0, nk = 0, ties = ties_before;
+  std::uint32_t nf = 0, nk = 0, ties = ties_before;  // of the lane
   keys.each([&](const K (&x)[4], std::uint32_t i) {
-    unsigned long long f[4], k[4];
-    kinds(x, i, ties, f, k);
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      nf += static_cast<std::uint32_t>(__popcll(f[e]));
-      nk += static_cast<std::uint32_t>(__popcll(k[e]));
-    }
+    const Kinds s = kinds(x, i, ties);
+    nf += static_cast<std::uint32_t>(__popc(s.freed));
+    nk += static_cast<std::uint32_t>(__popc(s.kept));
   });
-  if (lane == 0u) sh.wave[1][wave] = nf, sh.wave[2][wave] = nk;
+  const std::uint32_t sum_f = wave_scan(nf), sum_k = wave_scan(nk);
+  if (lane == 63u) sh.wave[1][wave] = sum_f, sh.wave[2][wave] = sum_k;
   __syncthreads();
   const uint2 wf = waves_before<T>(sh.wave[1], wave), wk = waves_before<T>(sh.wave[2], wave);
   std::uint32_t at_f = wf.x, at_k = wk.x;
   ties = ties_before;
-  auto put = [&](const unsigned long long (&m)[4], std::uint32_t i, std::uint32_t& at, auto& to) {
-    if (((m[0] | m[1]) | (m[2] | m[3])) == 0ull) return;
-    std::uint32_t rank = at;
+  auto put = [&](std::uint32_t bits, std::uint32_t i, std::uint32_t& at, auto& to) {
+    if (__ballot(bits != 0u) == 0ull) return;
+    const std::uint32_t own = static_cast<std::uint32_t>(__popc(bits)), upto = wave_scan(own);
+    std::uint32_t rank = at + upto - own;
+    at += __builtin_amdgcn_readlane(upto, 63);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      rank += lanes_below(m[e]);
-      at += static_cast<std::uint32_t>(__popcll(m[e]));
-    }
-#pragma unroll
-    for (int e = 0; e < 4; ++e)
-      if ((m[e] >> lane & 1ull) != 0ull) to(i + e, rank++);
+    for (std::uint32_t e = 0; e < 4u; ++e)
+      if ((bits >> e & 1u) != 0u) to(i + e, rank++);
   };
   keys.each([&](const K (&x)[4], std::uint32_t i) {
-    unsigned long long f[4], k[4];
-    kinds(x, i, ties, f, k);
-    put(f, i, at_f, freed);
-    put(k, i, at_k, kept);
+    const Kinds s = kinds(x, i, ties);
+    put(s.freed, i, at_f, freed);
+    put(s.kept, i, at_k, kept);
   });
   return make_uint2(wf.y, wk.y);
 }
@@ -391,6 +393,7 @@ struct KeyRow {
     }
     return v;
   }
+  __device__ __forceinline__ void seen(std::uint32_t, const u64x4&) const {}
   __device__ __forceinline__ void keys(std::uint32_t, const u64x4& v, unsigned long long (&x)[4]) const {
 #pragma unroll
     for (int e = 0; e < 4; ++e) x[e] = v[e];
@@ -448,7 +451,7 @@ struct EvictArgs {
 struct SlotKeys {
   const float* w;
   const std::uint32_t* p;
-  float* wo;  // null, or where the slots below `stay` are copied as they are read
+  float* wo;
   std::uint32_t* po;
   std::uint32_t n, stay, newest, n_first, n_recent;
   struct Raw {
@@ -471,16 +474,15 @@ struct SlotKeys {
 #pragma unroll
     for (int e = 0; e < 4; ++e) x[e] = i + e < n ? weight_key(v.w[e], v.p[e], newest, n_first, n_recent) : 0u;
   }
-  // slots below `stay`, unless they lie there already
-  __device__ __forceinline__ void copy(std::uint32_t threads) const {
-    for (std::uint32_t i = 4u * threadIdx.x; i < stay; i += 4u * threads) {
-      const Raw v = raw(i);
-      if (i + 4u <= stay) {
-        if (wo != w) *reinterpret_cast<f32x4_any*>(wo + i) = v.w;
-        if (po != p) *reinterpret_cast<u32x4_any*>(po + i) = v.p;
-      } else {
-        for (std::uint32_t e = 0; i + e < stay; ++e) wo[i + e] = v.w[e], po[i + e] = v.p[e];
-      }
+  // copies the slots below `stay`, unless they lie there already
+  __device__ __forceinline__ void seen(std::uint32_t i, const Raw& v) const {
+    if (i + 4u <= stay) {
+      if (wo != w) *reinterpret_cast<f32x4_any*>(wo + i) = v.w;
+      if (po != p) *reinterpret_cast<u32x4_any*>(po + i) = v.p;
+    } else {
+#pragma unroll
+      for (std::uint32_t e = 0; e < 4u; ++e)
+        if (i + e < stay) wo[i + e] = v.w[e], po[i + e] = v.p[e];
     }
   }
 };
@@ -503,8 +505,10 @@ __device__ __forceinline__ void move_row(const PagedView& kv, const EvictArgs& a
   reinterpret_cast<uint4*>(kv.v)[static_cast<std::size_t>(to) * L + t] = y;
 }
 
-template <std::uint32_t T>
-__global__ __launch_bounds__(T) void evict_choice_kernel(PagedView kv, EvictArgs a) {
+// L: 0, or the moves follow in the same workgroup, L lanes a row (and the length, of
+// which then no other workgroup's copy is overwritten).
+template <std::uint32_t T, int L>
+__global__ __launch_bounds__(T) void evict_choice_kernel(PagedView kv, EvictArgs a, std::uint32_t* length_out) {
   __shared__ __align__(16) SelectShared<T> sh;
   extern __shared__ __align__(16) std::uint8_t lds[];
   const std::uint32_t g = blockIdx.x, r = blockIdx.y, tid = threadIdx.x;
@@ -513,13 +517,15 @@ __global__ __launch_bounds__(T) void evict_choice_kernel(PagedView kv, EvictArgs
   const std::uint32_t newest = a.pos[r];
   std::uint32_t n = a.length[r];
   n = n < kv.capacity ? n : kv.capacity;
-  if (newest == RTXLLM_NO_POSITION || n == 0u) {
+  if (newest == RTXLLM_NO_POSITION) {
     if (tid == 0u) moves[0] = 0u;
     return;
   }
+  if (L != 0 && g == 0u && tid == 0u) length_out[r] = n < a.keep ? n : a.keep;
   const SlotKeys src{a.weight + gr * kv.capacity, a.slot_pos + gr * kv.capacity, a.weight_out + gr * kv.capacity,
                      a.slot_pos_out + gr * kv.capacity, n, n < a.keep ? n : a.keep, newest, a.n_first, a.n_recent};
-  if (src.wo != src.w || src.po != src.p) src.copy(T);
+  if (n <= a.keep || n > a.room)
+    for (std::uint32_t i = 4u * tid; i < src.stay; i += 4u * T) src.seen(i, src.raw(i));
   if (n <= a.keep) {
     if (tid == 0u) moves[0] = 0u;
     return;
@@ -536,7 +542,14 @@ __global__ __launch_bounds__(T) void evict_choice_kernel(PagedView kv, EvictArgs
       [&](std::uint32_t i, std::uint32_t m) {
         if (m < a.most) from[m] = i;
       }).x;
-  if (tid == 0u) moves[0] = freed < a.most ? freed : a.most;
+  const std::uint32_t n_moves = freed < a.most ? freed : a.most;
+  if constexpr (L == 0) {
+    if (tid == 0u) moves[0] = n_moves;
+  } else {
+    __threadfence_block();
+    __syncthreads();
+    for (std::uint32_t m = tid / L; m < n_moves; m += T / L) move_row<L>(kv, a, r, g, to[m], from[m], tid % L);
+  }
 }
 
 template <int L>
@@ -581,6 +594,9 @@ hipError_t launch_select(const PagedView& view, const std::uint16_t* bounds, con
     hipLaunchKernelGGL(page_choice_kernel<1024>, choices, dim3(1024), held, stream, view, pos, keys, room, n_select, pages);
   return hipGetLastError();
 }
+
+// Moves that the choosing workgroup makes itself, at most.
+constexpr std::uint32_t kMoveHere = 256;
 
 std::uint32_t most_moves(const rtxllm_paged_kv* c, std::uint32_t keep) {
   const std::uint32_t behind = c->capacity - keep;
@@ -650,10 +666,24 @@ extern "C" hipError_t rtxllm_kv_evict_f16(const rtxllm_paged_kv* cache, const ui
   const std::size_t held = held_bytes(view.capacity, 4u);
   const EvictArgs a{length, pos, weight, slot_pos, weight_out, slot_pos_out, static_cast<std::uint32_t*>(workspace),
                     keep,   n_first, n_recent, most, static_cast<std::uint32_t>(held / 4u)};
-  if (choice_threads(view.capacity) == 256u)
-    hipLaunchKernelGGL(evict_choice_kernel<256>, dim3(view.n_kv, count), dim3(256), held, stream, view, a);
-  else
-    hipLaunchKernelGGL(evict_choice_kernel<1024>, dim3(view.n_kv, count), dim3(1024), held, stream, view, a);
+  auto choose = [&](auto lanes) {
+    constexpr int L = decltype(lanes)::value;
+    if (choice_threads(view.capacity) == 256u)
+      hipLaunchKernelGGL((evict_choice_kernel<256, L>), dim3(view.n_kv, count), dim3(256), held, stream, view, a, length_out);
+    else
+      hipLaunchKernelGGL((evict_choice_kernel<1024, L>), dim3(view.n_kv, count), dim3(1024), held, stream, view, a, length_out);
+  };
+  // In place, a kv head's workgroup may read the length after another has written it.
+  if (most <= kMoveHere && length_out != length) {
+    if (cache->head_dim == 64u)
+      choose(std::integral_constant<int, 8>{});
+    else if (cache->head_dim == 128u)
+      choose(std::integral_constant<int, 16>{});
+    else
+      choose(std::integral_constant<int, 32>{});
+    return hipGetLastError();
+  }
+  choose(std::integral_constant<int, 0>{});
   hipError_t rc = hipGetLastError();
   if (rc != hipSuccess) return rc;
   const dim3 grid(most > 0u ? (most + per - 1u) / per : 1u, view.n_kv, count);
