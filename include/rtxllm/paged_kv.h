@@ -24,8 +24,8 @@
 extern "C" {
 #endif
 
-/* The position of a padded row: nothing is read for the row and nothing of it is
- * written. */
+/* The position of a padded row: its inputs do not count, whatever they hold (they
+ * must be allocated), and no output of it is written. */
 #define RTXLLM_NO_POSITION 0xFFFFFFFFu
 
 /* A layer's cache as a call's rows see it. Row r of a call reads the block table
@@ -42,7 +42,7 @@ typedef struct {
   uint32_t n_kv_heads;
   uint32_t head_dim;  /* 64, 128 or 256 */
   uint32_t page_size; /* positions of a page, any >= 1 */
-  uint32_t capacity;  /* positions of a sequence, % page_size == 0, <= 2^30 */
+  uint32_t capacity;  /* positions of a sequence, % page_size == 0, <= 2^24 */
 } rtxllm_paged_kv;
 
 /* New tokens of count rows. Per row r and head, with x the head's head_dim fp32
@@ -79,7 +79,8 @@ hipError_t rtxllm_qk_norm_rope_append_f16(const rtxllm_paged_kv* cache, const fl
  * (first null: the newest page, last[r]'s), at most `span` of them (1..2^20) from the
  * first on; last[r] >= capacity counts as capacity - 1; last[r] RTXLLM_NO_POSITION
  * or first[r] > last[r]: none. Rows that share pages compute the same values
- * where they fill them alike. count <= 65535. */
+ * where they fill them alike. bounds 16-byte aligned; count <= 65535; span *
+ * n_kv_heads <= 2^24 (a larger span than a sequence has pages counts as that). */
 hipError_t rtxllm_kv_page_bounds_f16(const rtxllm_paged_kv* cache, const uint32_t* first, const uint32_t* last,
                                      uint32_t count, uint32_t span, uint16_t* bounds, hipStream_t stream);
 
@@ -90,8 +91,8 @@ hipError_t rtxllm_kv_page_bounds_f16(const rtxllm_paged_kv* cache, const uint32_
  * behind the last. score = max over the kv head's query heads h of sum_d
  * max(q_hd largest_d, q_hd smallest_d): no key of the page has a larger product
  * with any of them. Scores are sums in 64 bits, so that the choice does not hang
- * on the order of a sum; the lower page wins between equal scores; a NaN score
- * ranks below every number. A page with no entry in the table is never listed.
+ * on the order of a sum; the lower page wins between equal scores; a head whose
+ * product is NaN does not count, and a page where none does ranks last. A page with no entry in the table is never listed.
  * n_heads / n_kv_heads 1..16, n_first + n_last <= n_select <= 65536, count <= 65535.
  * workspace: rtxllm_attn_select_workspace() bytes, 256-byte aligned. */
 size_t rtxllm_attn_select_workspace(const rtxllm_paged_kv* cache, uint32_t count);
@@ -105,7 +106,11 @@ hipError_t rtxllm_attn_select_pages(const rtxllm_paged_kv* cache, const uint16_t
  * order; an entry outside the table (-1) is passed over, a page listed twice
  * counts twice. Scores q k / sqrt(head_dim), softmax with the maximum subtracted,
  * sums in fp32; out fp32 [count][n_heads][head_dim]; a row that attends nothing
- * is 0. n_heads / n_kv_heads 1..16; count <= 65535; n_select 1..65536. */
+ * is 0. What a position that is not attended holds, NaN and infinities included, has
+ * no effect; a NaN or an infinity among the attended keys or values makes NaN of what
+ * it enters. q and the softmax terms enter the products as pairs of fp16 of 22 bits, at
+ * any size of q. n_heads / n_kv_heads 1..16; count <= 65535; n_select 1..65536, n_select
+ * * page_size <= 2^30. workspace: rtxllm_attn_pages_workspace() bytes, 256-byte aligned. */
 size_t rtxllm_attn_pages_workspace(const rtxllm_paged_kv* cache, uint32_t n_heads, uint32_t n_select,
                                    uint32_t count);
 hipError_t rtxllm_attn_decode_pages_gqa_f16(const rtxllm_paged_kv* cache, const float* q, uint32_t n_heads,

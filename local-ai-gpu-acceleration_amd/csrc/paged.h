@@ -61,7 +61,7 @@ RTXLLM_HD std::uint32_t paged_filled(const PagedView& c, std::uint32_t last) {
 inline bool paged_cache_ok(const rtxllm_paged_kv* c, std::uint32_t count) {
   if (c == nullptr || c->k == nullptr || c->v == nullptr || c->block_table == nullptr || c->n_pages == 0u ||
       c->n_kv_heads == 0u || c->n_kv_heads > 4096u || c->page_size == 0u || c->capacity == 0u ||
-      c->capacity > (1u << 30) || c->capacity % c->page_size != 0u || c->n_pages > 0x7FFFFFFFu)
+      c->capacity > (1u << 24) || c->capacity % c->page_size != 0u || c->n_pages > 0x7FFFFFFFu)
     return false;
   if (c->head_dim != 64u && c->head_dim != 128u && c->head_dim != 256u) return false;
   if (c->table_stride != 0u && count > 1u && c->table_stride < c->capacity / c->page_size) return false;

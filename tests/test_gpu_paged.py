@@ -411,3 +411,287 @@ def test_evict_long(n, keep, levels):
             np.testing.assert_array_equal(got[to[:, 0], g, to[:, 1]], was[of[:, 0], g, of[:, 1]])
             rest = place[keep:]
             np.testing.assert_array_equal(got[rest[:, 0], g, rest[:, 1]], was[rest[:, 0], g, rest[:, 1]])
+
+
+# ---- used together, captured, on streams, far offsets ---------------------------------
+
+
+def heads(rng, count, n, dim):
+    return rng.standard_normal((count, n, dim)).astype(np.float32)
+
+
+class Decoder:
+    """A layer's decode loop over fixed buffers: append, gather weights, evict; and the
+    float64 form of the same, which carries the cache of the GPU's fp16 values along."""
+
+    def __init__(self, seed, lens, group, kv, dim, page, keep, room):
+        self.s = s = Setup(seed, lens, kv, dim, page, entries=-(-room // page))
+        self.group, self.keep, self.count = group, keep, len(lens)
+        rng = s.rng
+        self.slot_pos = np.zeros((self.count, kv, s.capacity), np.uint32)
+        self.slot_pos[:] = np.arange(s.capacity)
+        self.weight = rng.random((self.count, kv, s.capacity)).astype(np.float32)
+        self.length = np.array(lens, np.uint32)
+        self.pos = np.array([n - 1 if n else ref.NONE for n in lens], np.uint32)
+        self.qw, self.kw = ((1 + 0.1 * rng.standard_normal(dim)).astype(np.float32) for _ in range(2))
+        self.d = {n: u32(getattr(self, n)) for n in ("slot_pos", "length", "pos")}
+        self.d.update(weight=dev(self.weight), qw=dev(self.qw), kw=dev(self.kw), slot=u32(self.length))
+        for n, h in (("q", group * kv), ("k", kv), ("v", kv)):
+            self.d[n] = torch.zeros(self.count, h, dim, device=DEV)
+        self.out, self.q_out = torch.full_like(self.d["q"], 7.0), torch.full_like(self.d["q"], 7.0)
+        self.work = paged.attn_weights_workspace(s.cache, group * kv, self.count)
+        self.work2 = paged.evict_workspace(s.cache, keep, self.count)
+
+    def feed(self):
+        """The next token's projections, positions and slots into the fixed buffers."""
+        s = self.s
+        self.live = self.pos != ref.NONE
+        self.pos[self.live] += 1
+        self.x = {n: heads(s.rng, self.count, h, s.dim) for n, h in (("q", self.group * s.kv), ("k", s.kv), ("v", s.kv))}
+        for n, a in self.x.items():
+            self.d[n].copy_(dev(a))
+        self.d["pos"].copy_(u32(self.pos))
+        slot = self.length.copy()
+        slot[~self.live] = ref.NONE
+        self.slot = slot
+        self.d["slot"].copy_(u32(slot))
+        length = np.where(self.live, self.length + 1, 0).astype(np.uint32)
+        self.d["length"].copy_(u32(length))
+
+    def step(self):
+        d, c = self.d, self.s.cache
+        paged.qk_norm_rope_append(c, d["q"], d["k"], d["v"], d["qw"], d["kw"], d["pos"], theta=1e4, slot=d["slot"],
+                                  q_out=self.q_out, slot_pos=d["slot_pos"], slot_weight=d["weight"])
+        paged.attn_weights(c, self.q_out, d["slot"], d["weight"], out=self.out, workspace=self.work)
+        paged.evict(c, d["length"], d["pos"], self.keep, d["weight"], d["slot_pos"], 2, 4, workspace=self.work2)
+
+    def check(self):
+        s = self.s
+        gk, gv = s.kd.cpu().numpy(), s.vd.cpu().numpy()
+        gq, go, gw = self.q_out.cpu().numpy(), self.out.cpu().numpy(), self.d["weight"].cpu().numpy()
+        gp, gl = (self.d[n].cpu().numpy().view(np.uint32) for n in ("slot_pos", "length"))
+        for i in range(self.count):
+            if not self.live[i]:
+                assert np.all(go[i] == 7.0) and np.all(gq[i] == 7.0)
+                continue
+            n = int(self.length[i]) + 1
+            assert gl[i] == min(n, self.keep)
+            s.seen[i] = [ref.at(s.table[i], s.n_pages, s.page, t) for t in range(s.capacity)]
+            p, o = s.seen[i][n - 1]
+            for g in range(s.kv):
+                want, size = ref.norm_rope(self.x["k"][i, g], self.kw, self.pos[i], 1e4, 1e-6, s.dim, True)
+                got = want.astype(np.float16)
+                s.v[p, g, o] = self.x["v"][i, g].astype(np.float16)
+                self.slot_pos[i, g, n - 1], self.weight[i, g, n - 1] = self.pos[i], 0.0
+                # the new key as the GPU stored it, wherever the eviction left it
+                where = [t for t in range(min(n, self.keep)) if gp[i, g, t] == self.pos[i]]
+                assert len(where) == 1  # the newest position is protected
+                pw, ow = s.seen[i][where[0]]
+                stored = gk[pw, g, ow]
+                close(stored, want, 2.0 ** -11 * np.abs(want) + 48 * 2.0 ** -24 * size + 2.0 ** -25, ("k", i, g))
+                s.k[p, g, o] = stored
+                total, tol = check_attention(s, go, gq, i, g, self.group, list(range(n)))
+                w = self.weight[i, g, :n] + total
+                # the eviction by the GPU's own sums, which the attention's bound ties to w
+                kept = ref.evict(n, int(self.pos[i]), self.keep, 2, 4, w, self.slot_pos[i, g])
+                src = list(range(n)) if kept is None else kept
+                by_pos = {int(q): t for t, q in enumerate(self.slot_pos[i, g, :n])}
+                mine = [by_pos[int(q)] for q in gp[i, g, :len(src)]]
+                if mine != src:  # only where two weights lie within the bound of one another
+                    gap = np.abs(np.sort(w[sorted(set(src) ^ set(mine))]))
+                    assert np.ptp(gap) <= 2 * tol.max() + 1e-6, (i, g)
+                close(gw[i, g, :len(src)], w[mine], tol[mine] + 20 * 2.0 ** -24 * w[mine], ("weight", i, g))
+                keys, values = (np.stack([a[s.seen[i][t][0], g, s.seen[i][t][1]] for t in mine]) for a in (s.k, s.v))
+                for t in range(len(src)):
+                    pt, ot = s.seen[i][t]
+                    np.testing.assert_array_equal(gk[pt, g, ot], keys[t])
+                    np.testing.assert_array_equal(gv[pt, g, ot], values[t])
+                self.slot_pos[i, g], self.weight[i, g] = gp[i, g], gw[i, g]
+            self.length[i] = gl[i]
+        s.k, s.v = gk.copy(), gv.copy()
+
+
+@pytest.mark.parametrize("captured", [False, True], ids=["eager", "graph"])
+def test_decode_with_eviction(captured):
+    """Ten steps of three live sequences and a padded one, into and past their budget, eager
+    or one graph replayed on another stream with eager work between the replays."""
+    d = Decoder(11, [37, 20, 0, 41], 3, 2, 64, 7, 40, 48)
+    step = d.step
+    if captured:
+        d.feed()
+        before = [t.clone() for t in (*d.d.values(), d.s.kd, d.s.vd, d.out, d.q_out)]
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            d.step()
+        for t, b in zip((*d.d.values(), d.s.kd, d.s.vd, d.out, d.q_out), before):
+            torch.testing.assert_close(t, b, rtol=0, atol=0, equal_nan=True)  # (a capture runs nothing)
+        d.pos[d.live] -= 1
+
+        def step():
+            side.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(side):
+                graph.replay()
+            torch.cuda.current_stream().wait_stream(side)
+
+    for _ in range(10):
+        d.feed()
+        step()
+        d.check()
+
+
+def test_decode_over_selected_pages():
+    """Append, the newest page's bounds, selection and attention, step by step: the bounds
+    stay those of the filled positions and the listed pages are the float64 choice."""
+    s = Setup(12, [61, 5, 100], 2, 128, 8, entries=16)
+    group, select = 4, 5
+    bounds = torch.zeros(s.n_pages, s.kv, 2, s.dim, dtype=torch.float16, device=DEV)
+    paged.page_bounds(s.cache, u32(s.last()), bounds, u32([0, 0, 0]), s.entries)
+    pos = np.array(s.last(), np.uint32)
+    for _ in range(9):
+        pos += 1
+        q, k, v = (heads(s.rng, 3, n, s.dim) for n in (group * s.kv, s.kv, s.kv))
+        turned = paged.qk_norm_rope_append(s.cache, dev(q), dev(k), dev(v), None, None, u32(pos), theta=1e6,
+                                           pairing="adjacent", rotary_dim=64)
+        paged.page_bounds(s.cache, u32(pos), bounds)
+        pages = paged.select_pages(s.cache, bounds, turned, u32(pos), select, 1, 2)
+        out = paged.attn_pages(s.cache, turned, pages, u32(pos)).cpu().numpy()
+        s.k, s.v = s.kd.cpu().numpy(), s.vd.cpu().numpy()
+        gb, gp, gq = bounds.cpu().numpy(), pages.cpu().numpy(), turned.cpu().numpy()
+        for i in range(3):
+            n = int(pos[i]) + 1
+            s.seen[i] = [ref.at(s.table[i], s.n_pages, s.page, t) for t in range(n)]
+            for g in range(s.kv):
+                for t in range(-(-n // s.page)):
+                    at = s.table[i, t]
+                    np.testing.assert_array_equal(gb[at, g], ref.bounds_of(s.k[at, g, :min(s.page, n - t * s.page)]))
+                want = ref.select(gq[i, g * group:(g + 1) * group], gb[:, g], s.table[i], s.n_pages, -(-n // s.page), 1, 2,
+                                  select)
+                assert gp[i, g].tolist() == want + [-1] * (select - len(want))
+                check_attention(s, out, gq, i, g, group,
+                                [x for t in want for x in range(t * s.page, min(n, t * s.page + s.page))])
+
+
+def test_all_pages_agree_with_dense_attention():
+    """Every page listed, over the cache that rtxllm_attn_decode_gqa_f16 reads: both within
+    their error of one another (each within 1e-5 of the largest value of a row)."""
+    from rtxllm_amd import ops
+    from rtxllm_amd._lib import lib
+
+    s = Setup(13, [300, 512, 1], 8, 128, 64, entries=8)
+    q = dev(heads(s.rng, 3, 32, 128))
+    pos = u32(s.last())
+    pages = torch.arange(8, dtype=torch.int32, device=DEV).expand(3, 8, 8).contiguous()
+    got = paged.attn_pages(s.cache, q, pages, pos)
+    out = torch.empty_like(q)
+    table = dev(s.table)
+    need = int(lib().rtxllm_attn_decode_workspace(32, 8, 512, 3))
+    ws = torch.empty(need, dtype=torch.uint8, device=DEV)
+    assert lib().rtxllm_attn_decode_gqa_f16(ops.ptr(q), ops.ptr(s.kd), ops.ptr(s.vd), ops.ptr(table), 8, 32, 8, 64, 512,
+                                            ops.ptr(pos), 3, ops.ptr(out), ops.ptr(ws), need, ops.stream()) == 0
+    for r in range(3):
+        assert float((got[r] - out[r]).abs().max()) <= 2e-5 * float(out[r].abs().max())
+
+
+def test_offsets_past_32_bits():
+    """Pages whose rows lie more than 2^32 values into the cache (9 GB of keys)."""
+    kv, dim, page = 8, 128, 64
+    n_pages = (1 << 32) // (kv * dim * page) + 40
+    k = torch.empty(n_pages, kv, page, dim, dtype=torch.float16, device=DEV)
+    v = torch.empty_like(k)
+    far = n_pages - 1 - torch.randperm(12, generator=torch.Generator().manual_seed(3))
+    small = Setup(14, [12 * page - 5], kv, dim, page)
+    table = far.to(torch.int32).reshape(1, 12)
+    for t in range(12):
+        k[far[t]], v[far[t]] = small.kd[small.table[0, t]], small.vd[small.table[0, t]]
+    cache = paged.PagedKV(k, v, table.to(DEV))
+    rng = small.rng
+    q, kn, vn = (dev(heads(rng, 1, n, dim)) for n in (4 * kv, kv, kv))
+    pos, slot_pos = u32(small.last()), u32(rng.permutation(12 * page)).expand(1, kv, 12 * page).contiguous()
+    weight = dev(rng.random((1, kv, 12 * page)).astype(np.float32))
+    answers = []
+    for c, kk, vv, tab in ((cache, k, v, far), (small.cache, small.kd, small.vd, torch.from_numpy(small.table[0]).long())):
+        w, sp = weight.clone(), slot_pos.clone()
+        turned = paged.qk_norm_rope_append(c, q, kn, vn, None, None, pos, theta=1e4)
+        bounds = torch.zeros(kk.shape[0], kv, 2, dim, dtype=torch.float16, device=DEV)
+        paged.page_bounds(c, pos, bounds, torch.zeros_like(pos), 12)
+        pages = paged.select_pages(c, bounds, turned, pos, 5)
+        some = paged.attn_pages(c, turned, pages, pos)
+        out = paged.attn_weights(c, turned, pos, w)
+        paged.evict(c, pos + 1, u32([12 * page]), 600, w, sp, 3, 9)
+        answers.append([turned, bounds[tab.to(DEV)], pages, some, out, w, sp, kk[tab.to(DEV)], vv[tab.to(DEV)]])
+    for a, b in zip(*answers):
+        assert torch.equal(a.view(torch.int16) if a.dtype == torch.float16 else a,
+                           b.view(torch.int16) if b.dtype == torch.float16 else b)
+
+
+def test_two_streams_and_repeats_give_the_same_bits():
+    """Two calls at once on streams of their own, each with its workspace, repeatedly: the
+    bits of a call alone."""
+    s = Setup(15, [3000, 900], 4, 128, 64)
+    q = [dev(heads(s.rng, 2, 20, 128)) for _ in range(2)]
+    pos = u32(s.last())
+    bounds = torch.zeros(s.n_pages, 4, 2, 128, dtype=torch.float16, device=DEV)
+    paged.page_bounds(s.cache, pos, bounds, torch.zeros_like(pos), s.entries)
+    weight = torch.zeros(2, 4, s.capacity, device=DEV)
+
+    def run(x):
+        pages = paged.select_pages(s.cache, bounds, x, pos, 9)
+        w = torch.empty_like(weight).fill_(-1.0)
+        return pages, paged.attn_pages(s.cache, x, pages, pos), paged.attn_weights(s.cache, x, pos, weight, w), w
+
+    alone = [run(x) for x in q]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for _ in range(5):
+        got = []
+        for x, st in zip(q, streams):
+            with torch.cuda.stream(st):
+                got.append(run(x))
+        torch.cuda.synchronize()
+        for a, b in zip(alone, got):
+            assert all(torch.equal(m, n) for m, n in zip(a, b))
+
+
+def test_wrapper_refusals():
+    s = Setup(16, [20, 20], 2, 64, 8)
+    c, pos = s.cache, u32([3, 4])
+    q, k = torch.zeros(2, 4, 64, device=DEV), torch.zeros(2, 2, 64, device=DEV)
+    bounds = torch.zeros(s.n_pages, 2, 2, 64, dtype=torch.float16, device=DEV)
+    state = torch.zeros(2, 2, s.capacity, device=DEV)
+    pages = torch.zeros(2, 2, 3, dtype=torch.int32, device=DEV)
+    from rtxllm_amd import HipError
+
+    bad = [
+        lambda: paged.PagedKV(s.kd.float(), s.vd, c.block_table),
+        lambda: paged.PagedKV(s.kd, s.vd[:1], c.block_table),
+        lambda: paged.PagedKV(s.kd, s.vd, c.block_table.long()),
+        lambda: paged.PagedKV(s.kd.cpu(), s.vd.cpu(), c.block_table.cpu()),
+        lambda: paged.PagedKV(s.kd, s.vd, c.block_table[:1].expand(2, -1)),
+        lambda: paged.qk_norm_rope_append(c, q, k, k, None, None, u32([1, 2, 3]), theta=1e4),
+        lambda: paged.qk_norm_rope_append(c, q, k[:, :1], k, None, None, pos, theta=1e4),
+        lambda: paged.qk_norm_rope_append(c, q.transpose(1, 2), k, k, None, None, pos, theta=1e4),
+        lambda: paged.qk_norm_rope_append(c, q, k, k, None, None, pos, theta=1e4, pairing="both"),
+        lambda: paged.qk_norm_rope_append(c, q, k, k, q[0, 0, :32], None, pos, theta=1e4),
+        lambda: paged.qk_norm_rope_append(c, q, k, k, None, None, pos.long(), theta=1e4),
+        lambda: paged.qk_norm_rope_append(c, q, k, k, None, None, pos, theta=1e4, slot_weight=state[:1]),
+        lambda: paged.page_bounds(c, pos, bounds[:2]),
+        lambda: paged.select_pages(c, bounds, q[:, :3], pos, 3),
+        lambda: paged.select_pages(c, bounds, q, pos, 3, workspace=torch.zeros(8, dtype=torch.uint8, device=DEV)),
+        lambda: paged.attn_pages(c, q, pages[:, :1], pos),
+        lambda: paged.attn_pages(c, q, pages, pos, out=torch.zeros(2, 4, 64)),
+        lambda: paged.attn_weights(c, q, pos, state[..., :-1]),
+        lambda: paged.evict(c, pos, pos, 0, state, state.int()),
+        lambda: paged.evict(c, pos, pos, 4, state, state),
+    ]
+    for i, call in enumerate(bad):
+        with pytest.raises(ValueError):
+            call()
+            pytest.fail(f"call {i} was not refused")
+    for call in (lambda: paged.qk_norm_rope_append(c, q, k, k, None, None, pos, theta=1e4, rotary_dim=12),
+                 lambda: paged.select_pages(c, bounds, q, pos, 3, 2, 2),
+                 lambda: paged.evict(c, pos, pos, 4, state, state.int(), 3, 2),
+                 lambda: paged.page_bounds(c, pos, bounds, span=0)):
+        with pytest.raises(HipError):
+            call()

@@ -50,7 +50,7 @@ CALLS = {
 BAD_CACHE = [dict(k=None), dict(v=None), dict(block_table=None), dict(k=BASE + 8), dict(v=BASE + 2),
              dict(block_table=BASE + 2), dict(n_pages=0), dict(n_pages=1 << 31), dict(n_kv_heads=0),
              dict(n_kv_heads=4097), dict(head_dim=96), dict(head_dim=0), dict(page_size=0), dict(capacity=0),
-             dict(capacity=120), dict(capacity=1 << 31), dict(table_stride=7), dict(n_pages=(1 << 31) - 1, page_size=128)]
+             dict(capacity=120), dict(capacity=(1 << 24) + 16), dict(table_stride=7), dict(n_pages=(1 << 31) - 1, page_size=128)]
 
 BAD = {
     "rtxllm_qk_norm_rope_append_f16": [
@@ -62,7 +62,7 @@ BAD = {
         dict(q_out=ptr(0), q_stride=600), dict(q_out=ptr(0) + 512), dict(q_out=ptr(1)), dict(q_out=ptr(2) - 512)],
     "rtxllm_kv_page_bounds_f16": [dict(last=None), dict(bounds=None), dict(bounds=ptr(1) + 8), dict(last=ptr(0) + 2),
                                   dict(first=ptr(5) + 1), dict(count=0), dict(count=65536), dict(span=0),
-                                  dict(span=(1 << 20) + 1)],
+                                  dict(span=(1 << 20) + 1), dict(last=ptr(0) + 1)],
     "rtxllm_attn_select_pages": [
         dict(bounds=None), dict(q=None), dict(pos=None), dict(pages=None), dict(workspace=None), dict(bounds=ptr(0) + 8),
         dict(q=ptr(1) + 1), dict(workspace=ptr(4) + 16), dict(workspace_bytes=0), dict(n_heads=3), dict(n_heads=0),
@@ -130,6 +130,11 @@ def test_row_addresses(tmp_path):
                    "  const std::int32_t table[4] = {2, -1, 7, 6};\n"
                    "  const rtxllm_paged_kv d{reinterpret_cast<std::uint16_t*>(16), reinterpret_cast<std::uint16_t*>(16), table, 4, 7, 3, 64, 5, 20};\n"
                    "  const PagedView c = paged_view(&d);\n"
+                   "  for (std::uint32_t p : {1u, 2u, 3u, 5u, 7u, 24u, 64u, 100u, 4095u, 65537u, (1u << 24) - 1u}) {\n"
+                   "    rtxllm_paged_kv e = d;\n    e.page_size = p, e.capacity = p;\n    const PagedView v = paged_view(&e);\n"
+                   "    for (std::uint64_t x = 0; x < (1ull << 31); x += 1 + x / 97)\n"
+                   "      for (std::uint64_t y : {x, x / p * p, x / p * p + p - 1})\n"
+                   "        if (y < (1ull << 31) && page_of(v, static_cast<std::uint32_t>(y)) != y / p) return 1;\n  }\n"
                    "  for (std::uint32_t s = 0; s < 22; ++s) std::printf(\"%u \", paged_slot_row(c, table, 2, s));\n"
                    "  std::printf(\"%u %u %u %u\", paged_filled(c, 0xFFFFFFFFu), paged_filled(c, 0), paged_filled(c, 19),\n"
                    "              paged_filled(c, 4000000000u));\n}\n")
