@@ -39,8 +39,11 @@ __device__ __forceinline__ float group_sum(float v) {
 // a row), so a rotation needs no exchange, and in place is safe. The row's
 // (cos, sin) go through LDS, one thread a pair: revolutions pos theta^(-2i/R) /
 // 2 pi in 64 bits, of which the nearest whole number is dropped; the rest, at
-// most half a turn, is exact enough in fp32 for sincospif's last bit.
-template <int L>
+// most half a turn, is exact enough in fp32 for sincospif's last bit. ROW: a workgroup
+// takes every head of its row in turn, else 2048 / head_dim of them. Bound by bytes from
+// some hundred rows on: 4001 rows of 32 + 2 x 8 heads of 128 37.1 us, 4.9 TB/s (a 1 GiB
+// copy: 5.2); one row 2.8 us, a launch.
+template <int L, bool ROW>
 __global__ __launch_bounds__(kThreads) void append_kernel(AppendArgs a, PagedView kv) {
   constexpr std::uint32_t D = 8u * L, kUnits = kThreads / L;
   __shared__ float2 cs[128];
@@ -56,91 +59,98 @@ __global__ __launch_bounds__(kThreads) void append_kernel(AppendArgs a, PagedVie
   }
   __syncthreads();
   const std::uint32_t units = a.n_heads + 2u * kv.n_kv;
-  const std::uint32_t u = blockIdx.y * kUnits + threadIdx.x / L, t = threadIdx.x % L;
-  const std::uint32_t h = u < units ? u : units - 1u;  // past the last: computed, not stored
-  const bool is_q = h < a.n_heads, is_v = h >= a.n_heads + kv.n_kv;
-  const float* src = is_q   ? a.q + r * a.q_stride + h * D
-                     : is_v ? a.v + r * a.v_stride + (h - a.n_heads - kv.n_kv) * D
-                            : a.k + r * a.k_stride + (h - a.n_heads) * D;
-  const bool rot = 8u * t < a.rotary && !is_v;
-  const bool split = a.halves != 0u && 8u * t < a.rotary;
-  const std::uint32_t ia = split ? 4u * t : 8u * t, ib = split ? ia + half : ia + 4u;
-  f32x4_any xa = *reinterpret_cast<const f32x4_any*>(src + ia), xb = *reinterpret_cast<const f32x4_any*>(src + ib);
-  float ss = 0.0f;
+  const std::uint32_t t = threadIdx.x % L;
+  const std::uint32_t slot = a.slot != nullptr ? a.slot[r] : pos;
+  auto head = [&](std::uint32_t u) {
+    const std::uint32_t h = u < units ? u : units - 1u;  // past the last: computed, not stored
+    const bool is_q = h < a.n_heads, is_v = h >= a.n_heads + kv.n_kv;
+    const float* src = is_q   ? a.q + r * a.q_stride + h * D
+                       : is_v ? a.v + r * a.v_stride + (h - a.n_heads - kv.n_kv) * D
+                              : a.k + r * a.k_stride + (h - a.n_heads) * D;
+    const bool rot = 8u * t < a.rotary && !is_v;
+    const bool split = a.halves != 0u && 8u * t < a.rotary;
+    const std::uint32_t ia = split ? 4u * t : 8u * t, ib = split ? ia + half : ia + 4u;
+    f32x4_any xa = *reinterpret_cast<const f32x4_any*>(src + ia), xb = *reinterpret_cast<const f32x4_any*>(src + ib);
+    float ss = 0.0f;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) ss = fmaf(xa[i], xa[i], ss);
+    for (int i = 0; i < 4; ++i) ss = fmaf(xa[i], xa[i], ss);
 #pragma unroll
-  for (int i = 0; i < 4; ++i) ss = fmaf(xb[i], xb[i], ss);
-  ss = group_sum<L>(ss);
-  if (!is_v) {
-    const float inv = 1.0f / sqrtf(ss / static_cast<float>(D) + a.eps);
-    const float* w = is_q ? a.qw : a.kw;
-    f32x4_any wa = {1.0f, 1.0f, 1.0f, 1.0f}, wb = wa;
-    if (w != nullptr) {
-      wa = *reinterpret_cast<const f32x4_any*>(w + ia);
-      wb = *reinterpret_cast<const f32x4_any*>(w + ib);
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      xa[i] = xa[i] * inv * wa[i];
-      xb[i] = xb[i] * inv * wb[i];
-    }
-  }
-  if (rot) {
-    if (split) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float2 t2 = cs[ia + i];
-        const float x = xa[i], y = xb[i];
-        xa[i] = x * t2.x - y * t2.y;
-        xb[i] = x * t2.y + y * t2.x;
+    for (int i = 0; i < 4; ++i) ss = fmaf(xb[i], xb[i], ss);
+    ss = group_sum<L>(ss);
+    if (!is_v) {
+      const float inv = 1.0f / sqrtf(ss / static_cast<float>(D) + a.eps);
+      const float* w = is_q ? a.qw : a.kw;
+      f32x4_any wa = {1.0f, 1.0f, 1.0f, 1.0f}, wb = wa;
+      if (w != nullptr) {
+        wa = *reinterpret_cast<const f32x4_any*>(w + ia);
+        wb = *reinterpret_cast<const f32x4_any*>(w + ib);
       }
-    } else {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const float2 t2 = cs[4u * t + i];
-        const float x = i < 2 ? xa[2 * i] : xb[2 * i - 4], y = i < 2 ? xa[2 * i + 1] : xb[2 * i - 3];
-        const float e = x * t2.x - y * t2.y, o = x * t2.y + y * t2.x;
-        if (i < 2) {
-          xa[2 * i] = e, xa[2 * i + 1] = o;
-        } else {
-          xb[2 * i - 4] = e, xb[2 * i - 3] = o;
+        xa[i] = xa[i] * inv * wa[i];
+        xb[i] = xb[i] * inv * wb[i];
+      }
+    }
+    if (rot) {
+      if (split) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float2 t2 = cs[ia + i];
+          const float x = xa[i], y = xb[i];
+          xa[i] = x * t2.x - y * t2.y;
+          xb[i] = x * t2.y + y * t2.x;
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float2 t2 = cs[4u * t + i];
+          const float x = i < 2 ? xa[2 * i] : xb[2 * i - 4], y = i < 2 ? xa[2 * i + 1] : xb[2 * i - 3];
+          const float e = x * t2.x - y * t2.y, o = x * t2.y + y * t2.x;
+          if (i < 2) {
+            xa[2 * i] = e, xa[2 * i + 1] = o;
+          } else {
+            xb[2 * i - 4] = e, xb[2 * i - 3] = o;
+          }
         }
       }
     }
-  }
-  if (u >= units) return;
-  if (is_q) {
-    float* dst = a.q_out + (static_cast<std::size_t>(r) * a.n_heads + h) * D;
-    *reinterpret_cast<f32x4_any*>(dst + ia) = xa;
-    *reinterpret_cast<f32x4_any*>(dst + ib) = xb;
-    return;
-  }
-  const std::uint32_t g = is_v ? h - a.n_heads - kv.n_kv : h - a.n_heads;
-  const std::uint32_t slot = a.slot != nullptr ? a.slot[r] : pos;
-  if (slot >= kv.capacity) return;
-  const std::uint32_t row = paged_slot_row(kv, kv.table + static_cast<std::size_t>(r) * kv.table_stride, g, slot);
-  if (row != kNoRow) {
-    std::uint16_t* dst = (is_v ? kv.v : kv.k) + static_cast<std::size_t>(row) * D;
-    auto pack = [](const f32x4_any& x) {
-      return make_uint2(f2h(x[0]) | static_cast<std::uint32_t>(f2h(x[1])) << 16,
-                        f2h(x[2]) | static_cast<std::uint32_t>(f2h(x[3])) << 16);
-    };
-    *reinterpret_cast<uint2*>(dst + ia) = pack(xa);
-    *reinterpret_cast<uint2*>(dst + ib) = pack(xb);
-  }
-  if (!is_v && t == 0u) {
-    const std::size_t i = (static_cast<std::size_t>(kv.table_stride != 0u ? r : 0u) * kv.n_kv + g) * kv.capacity + slot;
-    if (a.slot_pos != nullptr) a.slot_pos[i] = pos;
-    if (a.slot_weight != nullptr) a.slot_weight[i] = 0.0f;
-  }
+    if (u >= units) return;
+    if (is_q) {
+      float* dst = a.q_out + (static_cast<std::size_t>(r) * a.n_heads + h) * D;
+      *reinterpret_cast<f32x4_any*>(dst + ia) = xa;
+      *reinterpret_cast<f32x4_any*>(dst + ib) = xb;
+      return;
+    }
+    const std::uint32_t g = is_v ? h - a.n_heads - kv.n_kv : h - a.n_heads;
+    if (slot >= kv.capacity) return;
+    const std::uint32_t row = paged_slot_row(kv, kv.table + static_cast<std::size_t>(r) * kv.table_stride, g, slot);
+    if (row != kNoRow) {
+      std::uint16_t* dst = (is_v ? kv.v : kv.k) + static_cast<std::size_t>(row) * D;
+      auto pack = [](const f32x4_any& x) {
+        return make_uint2(f2h(x[0]) | static_cast<std::uint32_t>(f2h(x[1])) << 16,
+                          f2h(x[2]) | static_cast<std::uint32_t>(f2h(x[3])) << 16);
+      };
+      *reinterpret_cast<uint2*>(dst + ia) = pack(xa);
+      *reinterpret_cast<uint2*>(dst + ib) = pack(xb);
+    }
+    if (!is_v && t == 0u) {
+      const std::size_t i = (static_cast<std::size_t>(kv.table_stride != 0u ? r : 0u) * kv.n_kv + g) * kv.capacity + slot;
+      if (a.slot_pos != nullptr) a.slot_pos[i] = pos;
+      if (a.slot_weight != nullptr) a.slot_weight[i] = 0.0f;
+    }
+  };
+  if constexpr (ROW)
+    for (std::uint32_t u0 = 0; u0 < units; u0 += kUnits) head(u0 + threadIdx.x / L);
+  else
+    head(blockIdx.y * kUnits + threadIdx.x / L);
 }
 
 typedef _Float16 half8 __attribute__((ext_vector_type(8)));
 
 // One wave a (page, kv head): L = head_dim / 8 lanes a key, 64 / L keys at a
 // time. Repeating a filled key changes neither extreme, so the last step reads
-// its last key again instead of masking.
+// its last key again instead of masking. Bound by bytes: 1024 pages of 64 keys of 8
+// heads of 128 28.4 us, 4.9 TB/s.
 template <int L>
 __global__ __launch_bounds__(kThreads) void page_bounds_kernel(PagedView kv, const std::uint32_t* first,
                                                                const std::uint32_t* last, std::uint32_t span,
@@ -240,13 +250,24 @@ extern "C" hipError_t rtxllm_qk_norm_rope_append_f16(const rtxllm_paged_kv* cach
                      eps,  n_heads, rotary_dim, pairing == RTXLLM_PAIR_HALVES ? 1u : 0u};
   const PagedView view = paged_view(cache);
   const std::uint32_t units = n_heads + 2u * cache->n_kv_heads, per = kThreads / static_cast<std::uint32_t>(d / 8u);
-  const dim3 grid(count, (units + per - 1u) / per);
-  if (d == 64u)
-    hipLaunchKernelGGL(append_kernel<8>, grid, dim3(kThreads), 0, stream, a, view);
-  else if (d == 128u)
-    hipLaunchKernelGGL(append_kernel<16>, grid, dim3(kThreads), 0, stream, a, view);
+  auto launch = [&](auto row) {
+    constexpr bool kRow = decltype(row)::value;
+    const dim3 grid(count, kRow ? 1u : (units + per - 1u) / per);
+    if (d == 64u)
+      hipLaunchKernelGGL((append_kernel<8, kRow>), grid, dim3(kThreads), 0, stream, a, view);
+    else if (d == 128u)
+      hipLaunchKernelGGL((append_kernel<16, kRow>), grid, dim3(kThreads), 0, stream, a, view);
+    else
+      hipLaunchKernelGGL((append_kernel<32, kRow>), grid, dim3(kThreads), 0, stream, a, view);
+  };
+  // One workgroup a row saves the row's angles and the others' starts where rows alone
+  // fill the chip (us of one / several a row: 32 + 2 x 8 heads of 128 at 512 rows 7.4 /
+  // 7.1, 1024 10.4 / 10.6, 4001 37.1 / 39.4; 16 + 2 x 2 of 256 at 4001 32.2 / 35.5; rows that
+  // one workgroup holds at once, 8 + 2 x 1 of 64 at 4001, 8.6 / 7.8).
+  if (count >= 1024u && units > per)
+    launch(std::true_type{});
   else
-    hipLaunchKernelGGL(append_kernel<32>, grid, dim3(kThreads), 0, stream, a, view);
+    launch(std::false_type{});
   return hipGetLastError();
 }
 
