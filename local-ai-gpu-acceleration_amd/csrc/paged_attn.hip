@@ -9,6 +9,8 @@ namespace {
 
 typedef _Float16 half4 __attribute__((ext_vector_type(4)));
 typedef _Float16 half8 __attribute__((ext_vector_type(8)));
+typedef std::uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef std::uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 
 constexpr std::uint32_t kThreads = 256, kWaves = kThreads / 64u, kTile = 16;
@@ -45,8 +47,9 @@ __device__ __forceinline__ std::uint32_t from_lane(std::uint32_t v, std::uint32_
 //    so its rescaling is one factor.
 // T: heads in fours (1..4). WEIGHTS: every slot, the scores kept for merge_weights_kernel.
 // Bound by the reads of K and V: 4096 listed positions of eight sequences (134 MB)
-// 26.8 us, 5.0 TB/s (a 1 GiB copy: 5.2); without loads running ahead 33.9, with two sets of
-// registers in flight, at half the waves, 31.4. Workgroups next to each other take the
+// 25.2 us, 5.3 TB/s (a 1 GiB copy: 5.2); without loads running ahead 33.9, with two sets of
+// registers in flight, at half the waves, 31.4; with loads that stay in the caches, which a
+// step's other reads need more, 26.8. Workgroups next to each other take the
 // kv heads of one place, which lie next to each other in a page.
 template <int D, int T, bool WEIGHTS>
 __global__ __launch_bounds__(kThreads) void paged_attn_kernel(AttnArgs a, PagedView kv) {
@@ -57,6 +60,7 @@ __global__ __launch_bounds__(kThreads) void paged_attn_kernel(AttnArgs a, PagedV
   constexpr int STEPS = 4 / RPL;             // 4-position steps of a tile
   __shared__ __align__(16) float rec[kWaves][4 * T][D];
   __shared__ float2 rml[kWaves][4 * T];
+  extern __shared__ __align__(16) float held[];
   const std::uint32_t split = blockIdx.x / kv.n_kv, g = blockIdx.x % kv.n_kv, r = blockIdx.y;
   const std::uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const std::uint32_t col = lane & 15u, qq = lane >> 4;
@@ -143,7 +147,7 @@ __global__ __launch_bounds__(kThreads) void paged_attn_kernel(AttnArgs a, PagedV
 
   // A tile's keys and values and which of its positions count. One that does not reads
   // row 0 of the cache; its score and value are dropped.
-  uint4 ka[J];
+  u32x4 ka[J];
   std::uint32_t vw[16 / RPL][VD / 2], valid = 0u, row = 0u;
   auto settle = [&](std::uint32_t tile) {  // from `entry` and `page`, those of the tile
     const std::uint32_t x = place_of(tile), off = x - page_of(kv, x) * kv.page_size;
@@ -155,9 +159,9 @@ __global__ __launch_bounds__(kThreads) void paged_attn_kernel(AttnArgs a, PagedV
     row = there ? at : 0u;
   };
   auto load_k = [&]() {
-    const uint4* kr = reinterpret_cast<const uint4*>(kv.k + static_cast<std::size_t>(row) * D) + qq;
+    const u32x4* kr = reinterpret_cast<const u32x4*>(kv.k + static_cast<std::size_t>(row) * D) + qq;
 #pragma unroll
-    for (int j = 0; j < J; ++j) ka[j] = kr[4 * j];
+    for (int j = 0; j < J; ++j) ka[j] = __builtin_nontemporal_load(kr + 4 * j);
   };
   auto load_v = [&]() {
 #pragma unroll
@@ -166,14 +170,14 @@ __global__ __launch_bounds__(kThreads) void paged_attn_kernel(AttnArgs a, PagedV
         const std::uint32_t r0 = __builtin_amdgcn_readlane(row, 8 * (j / 4) + (j & 3)),
                             r1 = __builtin_amdgcn_readlane(row, 8 * (j / 4) + 4 + (j & 3));
         const std::uint32_t rr = lane < 32u ? r0 : r1;
-        vw[j][0] = reinterpret_cast<const std::uint32_t*>(kv.v + static_cast<std::size_t>(rr) * D)[lane & 31u];
+        vw[j][0] = __builtin_nontemporal_load(reinterpret_cast<const std::uint32_t*>(kv.v + static_cast<std::size_t>(rr) * D) + (lane & 31u));
       } else {
         const std::uint32_t rr = __builtin_amdgcn_readlane(row, j);
         const std::uint16_t* vr = kv.v + static_cast<std::size_t>(rr) * D;
         if constexpr (D == 128) {
-          vw[j][0] = reinterpret_cast<const std::uint32_t*>(vr)[lane];
+          vw[j][0] = __builtin_nontemporal_load(reinterpret_cast<const std::uint32_t*>(vr) + lane);
         } else {
-          const uint2 t = reinterpret_cast<const uint2*>(vr)[lane];
+          const u32x2 t = __builtin_nontemporal_load(reinterpret_cast<const u32x2*>(vr) + lane);
           vw[j][0] = t.x, vw[j][1] = t.y;
         }
       }
@@ -192,7 +196,6 @@ __global__ __launch_bounds__(kThreads) void paged_attn_kernel(AttnArgs a, PagedV
   load_v();
   for (std::uint32_t tile = tile0; tile < tile1; tile += kWaves) {
     const std::uint32_t now = valid;
-    float* const sc_out = WEIGHTS ? a.scores + head0 * a.score_stride + tile * kTile + 4u * qq : nullptr;
     std::uint32_t p01[NT], p23[NT];
     float alpha[NT];
     bool moved = false;
@@ -224,8 +227,7 @@ __global__ __launch_bounds__(kThreads) void paged_attn_kernel(AttnArgs a, PagedV
       if constexpr (WEIGHTS) {
         const std::uint32_t h = 8u * nt + col / 2u;
         if ((col & 1u) == 0u && h < a.group)
-          *reinterpret_cast<float4*>(sc_out + static_cast<std::size_t>(h) * a.score_stride) =
-              make_float4(s4[0], s4[1], s4[2], s4[3]);
+          *reinterpret_cast<f32x4*>(&held[(h * a.per + (tile - split * a.per)) * kTile + 4u * qq]) = f32x4{s4[0], s4[1], s4[2], s4[3]};
       }
       top = fmaxf(top, lane_xor<16>(top));
       top = fmaxf(top, lane_xor<32>(top));
@@ -322,6 +324,13 @@ __global__ __launch_bounds__(kThreads) void paged_attn_kernel(AttnArgs a, PagedV
     }
   }
   __syncthreads();
+  if constexpr (WEIGHTS) {  // at once and in whole lines: tile by tile from the loop 68 us instead of 61
+    const std::uint32_t own = (tile1 - split * a.per) * (kTile / 4u);
+    for (std::uint32_t h = 0; h < a.group; ++h)
+      for (std::uint32_t i = threadIdx.x; i < own; i += kThreads)
+        *reinterpret_cast<f32x4*>(a.scores + (head0 + h) * a.score_stride + split * a.per * kTile + 4u * i) =
+            *reinterpret_cast<const f32x4*>(&held[h * a.per * kTile + 4u * i]);
+  }
   const std::uint32_t items = a.group * (D / 4u);
   for (std::uint32_t it = threadIdx.x; it < items; it += kThreads) {
     const std::uint32_t h = it / (D / 4u), d = 4u * (it % (D / 4u));
@@ -477,12 +486,14 @@ AttnSpace attn_space(const rtxllm_paged_kv* c, std::uint32_t n_heads, std::uint6
 template <int D, bool WEIGHTS>
 void launch_partial(const AttnArgs& a, const PagedView& view, std::uint32_t count, hipStream_t stream) {
   const dim3 grid(a.splits * view.n_kv, count);
+  // a split's scores: at most 16 heads of 64 tiles
+  const std::size_t lds = WEIGHTS ? 4u * a.group * a.per * kTile : 0u;
   if (a.group <= 4u)
-    hipLaunchKernelGGL((paged_attn_kernel<D, 1, WEIGHTS>), grid, dim3(kThreads), 0, stream, a, view);
+    hipLaunchKernelGGL((paged_attn_kernel<D, 1, WEIGHTS>), grid, dim3(kThreads), lds, stream, a, view);
   else if (a.group <= 8u)
-    hipLaunchKernelGGL((paged_attn_kernel<D, 2, WEIGHTS>), grid, dim3(kThreads), 0, stream, a, view);
+    hipLaunchKernelGGL((paged_attn_kernel<D, 2, WEIGHTS>), grid, dim3(kThreads), lds, stream, a, view);
   else
-    hipLaunchKernelGGL((paged_attn_kernel<D, 4, WEIGHTS>), grid, dim3(kThreads), 0, stream, a, view);
+    hipLaunchKernelGGL((paged_attn_kernel<D, 4, WEIGHTS>), grid, dim3(kThreads), lds, stream, a, view);
 }
 
 template <int D>

@@ -695,3 +695,46 @@ def test_wrapper_refusals():
                  lambda: paged.page_bounds(c, pos, bounds, span=0)):
         with pytest.raises(HipError):
             call()
+
+
+@pytest.mark.parametrize("heads,kv,dim,page,rotary,pairing", [(32, 8, 128, 64, 128, "halves"), (40, 2, 64, 24, 16, "adjacent"),
+                                                              (8, 1, 64, 16, 64, "halves")])
+def test_append_long_prompt(heads, kv, dim, page, rotary, pairing):
+    """1100 rows of one sequence (the kernel of long prompts where a row has more heads than a
+    workgroup holds), some of them padded, against float64."""
+    count = 1100
+    s = Setup(17, [count], kv, dim, page, one=True)
+    q, k, v = (s.rng.standard_normal((count, h, dim)).astype(np.float32) for h in (heads, kv, kv))
+    w = (1.0 + 0.1 * s.rng.standard_normal(dim)).astype(np.float32)
+    pos = s.rng.permutation(count).astype(np.uint32)  # any order
+    pad = s.rng.random(count) < 0.05
+    given = np.where(pad, ref.NONE, pos).astype(np.uint32)
+    out = torch.full((count, heads, dim), 7.0, device=DEV)
+    paged.qk_norm_rope_append(s.cache, dev(q), dev(k), dev(v), dev(w), dev(w), u32(given), theta=1e5, rotary_dim=rotary,
+                              pairing=pairing, q_out=out)
+    gk, gv, got = s.kd.cpu().numpy(), s.vd.cpu().numpy(), out.cpu().numpy()
+    i = np.arange(rotary // 2)
+    a, b = (i, i + rotary // 2) if pairing == "halves" else (2 * i, 2 * i + 1)
+    angle = pos[:, None].astype(np.float64) * 1e5 ** (-2.0 * i / rotary)
+
+    def form(x):
+        y = x.astype(np.float64)
+        y = y / np.sqrt((y * y).mean(-1, keepdims=True) + 1e-6) * w.astype(np.float64)
+        z, size = y.copy(), np.abs(y)
+        c, sn = np.cos(angle)[:, None], np.sin(angle)[:, None]
+        z[..., a], z[..., b] = y[..., a] * c - y[..., b] * sn, y[..., a] * sn + y[..., b] * c
+        size[..., a] = size[..., b] = np.abs(y[..., a]) + np.abs(y[..., b])
+        return z, size
+
+    want, size = form(q)
+    live = ~pad
+    close(got[live], want[live], 24 * 2.0 ** -24 * size[live], "q")
+    assert np.all(got[pad] == 7.0)
+    want, size = form(k)
+    place = np.array(s.seen[0])[pos]
+    k_want, v_want = s.k.copy(), s.v.copy()
+    p, o = place[live, 0], place[live, 1]
+    close(gk[p, :, o], want[live], 2.0 ** -11 * np.abs(want[live]) + 48 * 2.0 ** -24 * size[live] + 2.0 ** -25, "k")
+    k_want[p, :, o], v_want[p, :, o] = gk[p, :, o], v[live].astype(np.float16)
+    np.testing.assert_array_equal(gk.view(np.uint16), k_want.view(np.uint16))
+    np.testing.assert_array_equal(gv.view(np.uint16), v_want.view(np.uint16))
