@@ -167,6 +167,24 @@ __device__ __forceinline__ uint2 waves_before(const std::uint32_t (&words)[T / 6
   return make_uint2(__builtin_amdgcn_readlane(sum - own, wave), __builtin_amdgcn_readlane(sum, kWaves - 1u));
 }
 
+// Counts four keys a lane by a digit, those that match.
+template <class Digit>
+__device__ __forceinline__ void count_digits(std::uint32_t* hist, Digit digit_of) {
+  std::uint32_t digit[4], others = 0u;  // kBins: no match
+#pragma unroll
+  for (int e = 0; e < 4; ++e) digit[e] = digit_of(e);
+  const std::uint32_t one = __builtin_amdgcn_readfirstlane(digit[0]);
+#pragma unroll
+  for (int e = 0; e < 4; ++e) others |= digit[e] ^ one;
+  if (__ballot(others != 0u) == 0ull) {
+    if ((threadIdx.x & 63u) == 0u && one != kBins) atomicAdd(&hist[one], 256u);
+    return;
+  }
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    if (digit[e] != kBins) atomicAdd(&hist[digit[e]], 1u);
+}
+
 // The keys of a workgroup: a wave's part contiguous, four keys a lane and round, so
 // that loads are wide and ranks follow from ballots; 0 behind the last key. Up to
 // `room` keys are read once and stay in the LDS, each thread's own where it alone
@@ -185,29 +203,33 @@ struct Keys {
   std::uint32_t n, rounds, first;  // rounds of this wave, its first key
   bool in_lds;
 
-  __device__ __forceinline__ Keys(const Source& s, void* lds, std::uint32_t count, std::uint32_t room)
+  // `hist` gets the counts of the keys' first digit where they are read into the LDS.
+  __device__ __forceinline__ Keys(const Source& s, void* lds, std::uint32_t* hist, std::uint32_t count, std::uint32_t room)
       : src(s), held(static_cast<Four*>(lds) + threadIdx.x), n(count), in_lds(count <= room) {
     const std::uint32_t most = (n + 4u * T - 1u) / (4u * T);
     first = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) * 256u * most;
     const std::uint32_t own = first < n ? (n - first + 255u) / 256u : 0u;
     rounds = own < most ? own : most;
+    for (std::uint32_t i = 4u * threadIdx.x; i < kBins; i += 4u * T)
+      *reinterpret_cast<uint4*>(hist + i) = make_uint4(0u, 0u, 0u, 0u);
+    __syncthreads();
     if (!in_lds) return;
+    auto take = [&](std::uint32_t at, std::uint32_t round, const decltype(src.raw(0u))& v) {
+      Four f;
+      src.seen(at, v);
+      src.keys(at, v, f.k);
+      held[T * round] = f;
+      count_digits(hist, [&](int e) { return static_cast<std::uint32_t>(f.k[e] >> (8 * sizeof(K) - kDigit)); });
+    };
     std::uint32_t j = 0;
     for (; j + 4u <= rounds; j += 4u) {  // four rounds' loads in flight
       decltype(src.raw(0u)) v[4];
 #pragma unroll
       for (std::uint32_t u = 0; u < 4u; ++u) v[u] = src.raw(place(j + u));
 #pragma unroll
-      for (std::uint32_t u = 0; u < 4u; ++u) {
-        src.seen(place(j + u), v[u]);
-        src.keys(place(j + u), v[u], held[T * (j + u)].k);
-      }
+      for (std::uint32_t u = 0; u < 4u; ++u) take(place(j + u), j + u, v[u]);
     }
-    for (; j < rounds; ++j) {
-      const auto v = src.raw(place(j));
-      src.seen(place(j), v);
-      src.keys(place(j), v, held[T * j].k);
-    }
+    for (; j < rounds; ++j) take(place(j), j, src.raw(place(j)));
   }
   __device__ __forceinline__ std::uint32_t place(std::uint32_t j) const {
     return first + 256u * j + 4u * (threadIdx.x & 63u);
@@ -237,31 +259,18 @@ template <class K, class Source, std::uint32_t T>
 __device__ Choice<K> radix_choice(SelectShared<T>& sh, const Keys<K, Source, T>& keys, std::uint32_t k) {
   constexpr int kBits = static_cast<int>(8u * sizeof(K));
   const std::uint32_t tid = threadIdx.x, lane = tid & 63u, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  for (std::uint32_t i = 4u * tid; i < kBins; i += 4u * T) *reinterpret_cast<uint4*>(&sh.hist[0][i]) = make_uint4(0u, 0u, 0u, 0u);
-  __syncthreads();
   K prefix = 0;
   int shift = kBits;
   for (std::uint32_t turn = 0;; turn ^= 1u) {
     const int bits = shift < kDigit ? shift : kDigit, next = shift - bits;
     std::uint32_t* const hist = sh.hist[turn];
-    keys.each([&](const K (&x)[4], std::uint32_t) {
-      std::uint32_t digit[4], others = 0u;  // kBins: of other digits above
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const bool match = shift == kBits || (x[e] >> shift) == prefix;
-        digit[e] = match ? static_cast<std::uint32_t>(x[e] >> next) & ((1u << bits) - 1u) : kBins;
-      }
-      const std::uint32_t one = __builtin_amdgcn_readfirstlane(digit[0]);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) others |= digit[e] ^ one;
-      if (__ballot(others != 0u) == 0ull) {
-        if (lane == 0u && one != kBins) atomicAdd(&hist[one], 256u);
-        return;
-      }
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (digit[e] != kBins) atomicAdd(&hist[digit[e]], 1u);
-    });
+    if (shift < kBits || !keys.in_lds)
+      keys.each([&](const K (&x)[4], std::uint32_t) {
+        count_digits(hist, [&](int e) {
+          const bool match = shift == kBits || (x[e] >> shift) == prefix;
+          return match ? static_cast<std::uint32_t>(x[e] >> next) & ((1u << bits) - 1u) : kBins;
+        });
+      });
     __syncthreads();
     if (wave == 0u) {
       // lane l sums the 32 bins below 2048 - 32 l; in the lane whose sums pass k, the bins
@@ -412,7 +421,7 @@ __global__ __launch_bounds__(T) void page_choice_kernel(PagedView kv, const std:
   if (used == 0u) return;  // a padded row
   const std::size_t gr = static_cast<std::size_t>(r) * kv.n_kv + g;
   const KeyRow src{row_keys + gr * kv.entries, used};
-  const Keys<unsigned long long, KeyRow, T> keys(src, lds, used, room);
+  const Keys<unsigned long long, KeyRow, T> keys(src, lds, sh.hist[0], used, room);
   std::int32_t* const out = pages + gr * n_select;
   // 1 and more: every page that is there
   Choice<unsigned long long> ch{1ull, kAllTies};
@@ -530,7 +539,7 @@ __global__ __launch_bounds__(T) void evict_choice_kernel(PagedView kv, EvictArgs
     if (tid == 0u) moves[0] = 0u;
     return;
   }
-  const Keys<std::uint32_t, SlotKeys, T> keys(src, lds, n, a.room);
+  const Keys<std::uint32_t, SlotKeys, T> keys(src, lds, sh.hist[0], n, a.room);
   const Choice<std::uint32_t> ch = radix_choice(sh, keys, a.keep);
   std::uint32_t* const to = moves + 1u;
   std::uint32_t* const from = to + a.most;
