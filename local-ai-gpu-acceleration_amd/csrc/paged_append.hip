@@ -264,9 +264,9 @@ extern "C" hipError_t rtxllm_qk_norm_rope_append_f16(const rtxllm_paged_kv* cach
       hipLaunchKernelGGL((append_kernel<32, kRow>), grid, dim3(kThreads), 0, stream, a, view);
   };
   // One workgroup a row saves the row's angles and the others' starts where rows alone
-  // fill the chip (us of one / several a row: 32 + 2 x 8 heads of 128 at 512 rows 7.4 /
-  // 7.1, 1024 10.4 / 10.6, 4001 37.1 / 39.4; 16 + 2 x 2 of 256 at 4001 32.2 / 35.5; rows that
-  // one workgroup holds at once, 8 + 2 x 1 of 64 at 4001, 8.6 / 7.8).
+  // fill the chip (us of one / several a row: 32 + 2 x 8 heads of 128 at 512 rows 7.6 /
+  // 6.8, 1024 11.7 / 11.9, 4001 32.5 / 34.2; 16 + 2 x 2 of 256 at 4001 27.8 / 30.7; rows that
+  // one workgroup holds at once, 8 + 2 x 1 of 64 at 4001, 8.8 / 7.9).
   if (count >= 1024u && units > per)
     launch(std::true_type{});
   else

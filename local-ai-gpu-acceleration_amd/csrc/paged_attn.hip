@@ -14,7 +14,7 @@ typedef std::uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 
 constexpr std::uint32_t kThreads = 256, kWaves = kThreads / 64u, kTile = 16;
-constexpr std::uint32_t kMaxSplits = 256;
+constexpr std::uint32_t kMaxPer = 64;  // tiles of a split, at most: what its scores take in the LDS
 constexpr float kLift = 15.0f;  // softmax terms are kept times 2^15 (see the kernel)
 
 struct AttnArgs {
@@ -359,33 +359,57 @@ __global__ __launch_bounds__(kThreads) void paged_attn_kernel(AttnArgs a, PagedV
 
 // Maximum and sum of one head over its splits' records, by one wave.
 __device__ __forceinline__ float2 head_ml(const float2* __restrict__ ml, std::uint32_t splits, std::uint32_t lane) {
-  float2 x[kMaxSplits / 64u];
-  float m = -INFINITY;
+  float M = -INFINITY, l = 0.0f;
+  for (std::uint32_t c0 = 0; c0 < splits; c0 += 256u) {  // (one round up to 262144 positions)
+    float2 x[4];
+    float m = M;
 #pragma unroll
-  for (std::uint32_t i = 0; i < kMaxSplits / 64u; ++i) {
-    x[i] = lane + 64u * i < splits ? ml[lane + 64u * i] : make_float2(-INFINITY, 0.0f);
-    m = fmaxf(m, x[i].x);
+    for (std::uint32_t i = 0; i < 4u; ++i) {
+      const std::uint32_t c = c0 + lane + 64u * i;
+      x[i] = c < splits ? ml[c] : make_float2(-INFINITY, 0.0f);
+    }
+#pragma unroll
+    for (std::uint32_t i = 0; i < 4u; ++i) m = fmaxf(m, x[i].x);
+    m = wave_max(m);
+    const float base = m == -INFINITY ? 0.0f : m;
+    l *= __builtin_amdgcn_exp2f(M - base);
+#pragma unroll
+    for (std::uint32_t i = 0; i < 4u; ++i) l += x[i].y * __builtin_amdgcn_exp2f(x[i].x - base);
+    M = m;
   }
-  const float M = wave_max(m), base = M == -INFINITY ? 0.0f : M;
-  float l = 0.0f;
-#pragma unroll
-  for (std::uint32_t i = 0; i < kMaxSplits / 64u; ++i) l += x[i].y * __builtin_amdgcn_exp2f(x[i].x - base);
   return make_float2(M, wave_sum(l));
 }
 
 // One workgroup a query head (of all rows): its splits' records merged, D / 4
-// lanes a record.
+// lanes a record, eight records of a lane in flight.
 template <int D>
 __device__ __forceinline__ void merge_head(const AttnArgs& a, std::size_t head, std::uint32_t splits) {
   constexpr std::uint32_t kLanes = D / 4u, kSub = kThreads / kLanes;
   __shared__ __align__(16) float sums[kSub][D];
   const std::uint32_t d = 4u * (threadIdx.x % kLanes), sub = threadIdx.x / kLanes;
   const float2* const ml = a.ml + head * a.splits;
-  const float2 t = head_ml(ml, splits, threadIdx.x & 63u);
-  const float base = t.x == -INFINITY ? 0.0f : t.x;
+  const float* const part = a.part + head * a.splits * D + d;
   f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
-  for (std::uint32_t c = sub; c < splits; c += kSub)
-    v += __builtin_amdgcn_exp2f(ml[c].x - base) * *reinterpret_cast<const f32x4*>(a.part + (head * a.splits + c) * D + d);
+  float M = -INFINITY;
+  for (std::uint32_t c0 = sub; c0 < splits; c0 += 8u * kSub) {
+    f32x4 x[8];
+    float m[8], top = M;
+#pragma unroll
+    for (std::uint32_t j = 0; j < 8u; ++j) {
+      const std::uint32_t c = c0 + kSub * j < splits ? c0 + kSub * j : c0;  // past the last: read again, weighted 0
+      x[j] = *reinterpret_cast<const f32x4*>(part + static_cast<std::size_t>(c) * D);
+      m[j] = ml[c].x;
+    }
+#pragma unroll
+    for (std::uint32_t j = 0; j < 8u; ++j) top = fmaxf(top, m[j]);
+    const float base = top == -INFINITY ? 0.0f : top;
+    v *= __builtin_amdgcn_exp2f(M - base);
+#pragma unroll
+    for (std::uint32_t j = 0; j < 8u; ++j) v += (c0 + kSub * j < splits ? __builtin_amdgcn_exp2f(m[j] - base) : 0.0f) * x[j];
+    M = top;
+  }
+  const float2 t = head_ml(ml, splits, threadIdx.x & 63u);
+  v *= __builtin_amdgcn_exp2f(M - (t.x == -INFINITY ? 0.0f : t.x));
   *reinterpret_cast<f32x4*>(&sums[sub][d]) = v;
   __syncthreads();
   if (sub != 0u) return;
@@ -446,16 +470,20 @@ __global__ __launch_bounds__(kThreads) void merge_weights_kernel(AttnArgs a, Pag
 // Tiles of a split (one workgroup), of at most `positions`. Of one size for every row,
 // so that a longer context is more workgroups; the largest of 4 to 64 that leaves a
 // workgroup for each CU, as a wave's prologue and the merge cost what two or three
-// tiles do. us of 32 heads over 8 kv heads of 128, per = 4 / 8 / 16 / 32 / 64: 1024
-// listed positions of one sequence 8.9 / 9.6 / 11.1 / 14.4 / 16.9, 4001 slots of one 12.0
-// / 10.5 / 11.5 / 14.6 / 21.4, 4096 listed of eight 41.9 / 35.7 / 33.4 / 31.2 / 31.1, up to
-// 16384 slots of eight 84.2 / 84.1 / 75.4 / 75.8 / 74.9.
-std::uint32_t attn_per(std::uint64_t items, std::uint64_t positions) {
+// tiles do; over whole contexts, whose lengths differ, more than 16 only where the longest
+// still makes 16 of them. us at 4 / 8 / 16 / 32 / 64 tiles, 32 heads over 8 kv heads of 128
+// - whole: 1024 slots of one sequence 7.9 / 8.8 / 10.7 / 14.5 / 22.1, 4001 of one 10.9 / 10.0 /
+//   11.8 / 15.9 / 23.9, 65536 of one 88 / 68 / 58 / 53 / 51, up to 4096 of eight 31.1 / 25.9 / 23.3 /
+//   26.0 / 27.2, up to 16384 of eight 100 / 78 / 71 / 70 / 66;
+// - listed: 4096 positions of eight 39.6 / 32.0 / 29.1 / 27.9 / 24.7.
+std::uint32_t attn_per(std::uint64_t items, std::uint64_t positions, bool whole) {
   const std::uint64_t tiles = (positions + kTile - 1u) / kTile;
-  std::uint64_t per = 64u;
-  while (per > kWaves && items * ((tiles + per - 1u) / per) < 256u) per /= 2u;
-  while ((tiles + per - 1u) / per > kMaxSplits) per *= 2u;
-  return static_cast<std::uint32_t>(per);
+  std::uint32_t per = kMaxPer;
+  for (; per > kWaves; per /= 2u) {
+    const std::uint64_t splits = (tiles + per - 1u) / per;
+    if (items * splits >= 256u && (!whole || per <= 16u || splits >= 16u)) break;
+  }
+  return per;
 }
 
 struct AttnSpace {
@@ -470,8 +498,9 @@ AttnSpace attn_space(const rtxllm_paged_kv* c, std::uint32_t n_heads, std::uint6
   if (!paged_cache_ok(c, count) || count == 0u || count > 65535u || c->n_kv_heads > 65535u ||
       paged_group(c, n_heads) == 0u || positions == 0u || positions > (1ull << 30))
     return s;
-  s.per = attn_per(static_cast<std::uint64_t>(count) * c->n_kv_heads, positions);
+  s.per = attn_per(static_cast<std::uint64_t>(count) * c->n_kv_heads, positions, weights);
   s.splits = static_cast<std::uint32_t>((positions + kTile * s.per - 1u) / (kTile * s.per));
+  if (static_cast<std::uint64_t>(s.splits) * c->n_kv_heads > (1u << 23)) return s;  // the launch's thread count
   const std::size_t records = static_cast<std::size_t>(count) * n_heads * s.splits;
   s.part = round_256(8u * records);
   s.scores = s.part + round_256(4u * records * c->head_dim);
@@ -486,7 +515,8 @@ AttnSpace attn_space(const rtxllm_paged_kv* c, std::uint32_t n_heads, std::uint6
 template <int D, bool WEIGHTS>
 void launch_partial(const AttnArgs& a, const PagedView& view, std::uint32_t count, hipStream_t stream) {
   const dim3 grid(a.splits * view.n_kv, count);
-  // a split's scores: at most 16 heads of 64 tiles
+  // a split's scores: 64 KB at most (16 heads of 64 tiles), beside at most 66 KB of records
+  static_assert(4u * kMaxQueryGroup * kMaxPer * kTile <= 65536u, "fits the LDS");
   const std::size_t lds = WEIGHTS ? 4u * a.group * a.per * kTile : 0u;
   if (a.group <= 4u)
     hipLaunchKernelGGL((paged_attn_kernel<D, 1, WEIGHTS>), grid, dim3(kThreads), lds, stream, a, view);

@@ -377,12 +377,9 @@ __device__ uint2 for_choice(SelectShared<T>& sh, const Keys<K, Source, T>& keys,
   return make_uint2(wf.y, wk.y);
 }
 
-// Threads of a choice over at most n keys.
-std::uint32_t choice_threads(std::uint32_t n) { return n <= 2048u ? 256u : 1024u; }
-
 // LDS bytes for n keys of `width` bytes, up to 128 KB, in whole rounds of a workgroup.
-std::size_t held_bytes(std::uint32_t n, std::size_t width) {
-  const std::size_t round = 4u * choice_threads(n) * width, rounds = (n * width + round - 1u) / round;
+std::size_t held_bytes(std::uint32_t n, std::size_t width, std::uint32_t threads) {
+  const std::size_t round = 4u * threads * width, rounds = (n * width + round - 1u) / round;
   return round * rounds < (128u << 10) ? round * rounds : 128u << 10;
 }
 
@@ -589,23 +586,30 @@ hipError_t launch_select(const PagedView& view, const std::uint16_t* bounds, con
                        dim3(kThreads), 0, stream, view, bounds, q, group, pos, n_first, n_last, keys);
   };
   const std::uint64_t waves = static_cast<std::uint64_t>(count) * view.n_kv * ((view.entries + 64u / L - 1u) / (64u / L));
+  // four steps a wave from where single steps fill the chip more than once (us of four / one:
+  // 504 waves 9.5 / 7.8, 4096 12.0 / 11.5, 8000 12.0 / 12.0, 16384 15.5 / 16.4)
   if (waves > 4096u)
     score(std::integral_constant<int, 4>{});
   else
     score(std::integral_constant<int, 1>{});
   const hipError_t rc = hipGetLastError();
   if (rc != hipSuccess) return rc;
-  const std::size_t held = held_bytes(view.entries, 8u);
+  // four waves up to 1024 pages, whose barriers cost less (us of both launches, four / 16
+  // waves: 250 pages of 8 heads 7.9 / 8.3, 1024 8.6 / 8.9, 2047 11.8 / 11.0, 4094 18.7 / 16.3)
+  const std::uint32_t threads = view.entries <= 1024u ? 256u : 1024u;
+  const std::size_t held = held_bytes(view.entries, 8u, threads);
   const auto room = static_cast<std::uint32_t>(held / 8u);
-  if (choice_threads(view.entries) == 256u)
+  if (threads == 256u)
     hipLaunchKernelGGL(page_choice_kernel<256>, choices, dim3(256), held, stream, view, pos, keys, room, n_select, pages);
   else
     hipLaunchKernelGGL(page_choice_kernel<1024>, choices, dim3(1024), held, stream, view, pos, keys, room, n_select, pages);
   return hipGetLastError();
 }
 
-// Moves that the choosing workgroup makes itself, at most.
-constexpr std::uint32_t kMoveHere = 256;
+// Moves that the choosing workgroup makes itself, at most (us of here / in a launch of
+// their own: 64 of 2112 slots 9.3 / 10.6, 96 of 4096 10.6 / 11.1, 256 of 2304 13.5 / 12.4, 512 of
+// 2560 18.3 / 14.4).
+constexpr std::uint32_t kMoveHere = 128;
 
 std::uint32_t most_moves(const rtxllm_paged_kv* c, std::uint32_t keep) {
   const std::uint32_t behind = c->capacity - keep;
@@ -672,12 +676,15 @@ extern "C" hipError_t rtxllm_kv_evict_f16(const rtxllm_paged_kv* cache, const ui
     return hipErrorInvalidValue;
   const PagedView view = paged_view(cache);
   const std::uint32_t most = most_moves(cache, keep), per = kThreads / (cache->head_dim / 8u);
-  const std::size_t held = held_bytes(view.capacity, 4u);
+  // 16 waves, but where short sequences give each CU several workgroups (us of four / 16
+  // waves: 1024 slots of 8 x 8 8.8 / 8.4, of 64 x 8 16.2 / 20.5, 2112 of 8 x 8 14.9 / 9.4)
+  const bool small = view.capacity <= 1024u && static_cast<std::uint64_t>(count) * view.n_kv > 256u;
+  const std::size_t held = held_bytes(view.capacity, 4u, small ? 256u : 1024u);
   const EvictArgs a{length, pos, weight, slot_pos, weight_out, slot_pos_out, static_cast<std::uint32_t*>(workspace),
                     keep,   n_first, n_recent, most, static_cast<std::uint32_t>(held / 4u)};
   auto choose = [&](auto lanes) {
     constexpr int L = decltype(lanes)::value;
-    if (choice_threads(view.capacity) == 256u)
+    if (small)
       hipLaunchKernelGGL((evict_choice_kernel<256, L>), dim3(view.n_kv, count), dim3(256), held, stream, view, a, length_out);
     else
       hipLaunchKernelGGL((evict_choice_kernel<1024, L>), dim3(view.n_kv, count), dim3(1024), held, stream, view, a, length_out);

@@ -738,3 +738,34 @@ def test_append_long_prompt(heads, kv, dim, page, rotary, pairing):
     k_want[p, :, o], v_want[p, :, o] = gk[p, :, o], v[live].astype(np.float16)
     np.testing.assert_array_equal(gk.view(np.uint16), k_want.view(np.uint16))
     np.testing.assert_array_equal(gv.view(np.uint16), v_want.view(np.uint16))
+
+
+@pytest.mark.parametrize("group,dim,n", [(16, 64, 300001), (5, 256, 270000)])
+def test_attention_of_very_long_contexts(group, dim, n):
+    """More splits than one round of the merge holds; and the scores that a split keeps in
+    the LDS stay of one size. float64 on the GPU, the bounds of paged_ref.attend."""
+    page = 128
+    entries = -(-n // page) + 1
+    g = torch.Generator(device=DEV).manual_seed(n)
+    k, v = (torch.randn(entries, 1, page, dim, generator=g, device=DEV).half() for _ in range(2))
+    table = torch.randperm(entries, generator=g, device=DEV).int().reshape(1, -1)
+    cache = paged.PagedKV(k, v, table)
+    q = torch.randn(1, group, dim, generator=g, device=DEV)
+    weight = torch.zeros(1, 1, cache.capacity, device=DEV)
+    pos = u32([n - 1])
+    out = paged.attn_weights(cache, q, pos, weight)[0].double()
+    pages = torch.arange(entries, dtype=torch.int32, device=DEV).reshape(1, 1, -1).contiguous()
+    listed = paged.attn_pages(cache, q, pages, pos)[0].double()
+    keys, values = (x[table[0].long(), 0].reshape(-1, dim)[:n].double() for x in (k, v))
+    total = torch.zeros(n, dtype=torch.float64, device=DEV)
+    for h in range(group):
+        s = keys @ q[0, h].double() / dim ** 0.5
+        p = torch.softmax(s, 0)
+        delta = (2.0 ** -23 * q[0, h].abs().max() * keys.abs().sum(1).max() +
+                 (dim + 8) * 2.0 ** -24 * (keys.abs() @ q[0, h].abs().double()).max()) / dim ** 0.5
+        bound = 2.0 * (delta + 2.0 ** -21 * (1.0 + s.abs().max())) + (n / 4 + 40) * 2.0 ** -24
+        for got in (out[h], listed[h]):
+            assert bool(((got - p @ values).abs() <= bound * (p @ values.abs())).all())
+        total += p
+    assert bool(((weight[0, 0, :n].double() - total).abs() <= bound * total).all())
+    assert float(weight[0, 0, n:].abs().max()) == 0.0

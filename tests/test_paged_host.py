@@ -146,3 +146,18 @@ def test_row_addresses(tmp_path):
     none = 0xFFFFFFFF
     want = [(2 * 3 + 2) * 5 + i for i in range(5)] + [none] * 10 + [(6 * 3 + 2) * 5 + i for i in range(5)] + [none] * 2
     assert got == want + [0, 1, 20, 20]
+
+
+def test_attention_sizes(rlib):
+    """A split's scores have one size in the LDS at any capacity (no launch asks for more LDS
+    than there is), and sizes beyond a launch's threads are refused."""
+    for capacity in (1 << 18, 1 << 20, 1 << 24):
+        c = cache(capacity=capacity, table_stride=1 << 20, page_size=256)
+        need = rlib.rtxllm_attn_weights_workspace(ctypes.addressof(c), 32, 1)
+        splits = capacity // (64 * 16)
+        assert need == 8 * 32 * splits + 4 * 32 * splits * 128 + 4 * 32 * capacity
+    c = cache(n_kv_heads=4096, n_pages=1024, page_size=256, capacity=1 << 24, table_stride=1 << 16)
+    assert rlib.rtxllm_attn_weights_workspace(ctypes.addressof(c), 4096, 1) == 0
+    assert rlib.rtxllm_attn_pages_workspace(ctypes.addressof(c), 4096, 65536, 1) == 0
+    c = cache(page_size=16384 * 2, capacity=1 << 16, n_pages=2)
+    assert rlib.rtxllm_attn_pages_workspace(ctypes.addressof(c), 4, 65536, 1) == 0  # 2^31 positions
