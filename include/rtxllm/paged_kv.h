@@ -54,7 +54,7 @@ typedef struct {
  * taken in 64 bits (rtxllm_rope_theta rounds it to fp32: up to pos 2^-24 of a
  * radian apart). q' goes to q_out [count][n_heads][head_dim] (fp32, in place
  * allowed when q_stride is n_heads * head_dim), k' and v, each rounded to fp16
- * once, into slot slot[r] of the row's sequence (slot null: pos[r]).
+ * once (beyond its range to an infinity), into slot slot[r] of the row's sequence (slot null: pos[r]).
  * q, k and v rows lie q_stride, k_stride and v_stride floats apart (one stacked
  * projection's output: the same stride three times); any 4-byte alignment.
  * rotary_dim % 8 == 0, 8..head_dim. pos[r] RTXLLM_NO_POSITION: a padded row. A slot >=

@@ -769,3 +769,82 @@ def test_attention_of_very_long_contexts(group, dim, n):
         total += p
     assert bool(((weight[0, 0, :n].double() - total).abs() <= bound * total).all())
     assert float(weight[0, 0, n:].abs().max()) == 0.0
+
+
+def test_queries_of_one_sequence():
+    """Rows that share one block table: a prompt's last positions, each over its own past."""
+    s = Setup(18, [150], 2, 64, 16, one=True)
+    count, group = 9, 3
+    pos = np.array([149, 0, 15, 16, ref.NONE, 77, 148, 31, 2 ** 31], np.uint32)  # (past the capacity: all of it)
+    q = heads(s.rng, count, group * s.kv, s.dim)
+    bounds = torch.zeros(s.n_pages, s.kv, 2, s.dim, dtype=torch.float16, device=DEV)
+    paged.page_bounds(s.cache, u32([149]), bounds, u32([0]), 10)
+    pages = torch.full((count, s.kv, 4), -9, dtype=torch.int32, device=DEV)
+    paged.select_pages(s.cache, bounds, dev(q), u32(pos), 4, 1, 1, pages=pages)
+    out = torch.full((count, group * s.kv, s.dim), 7.0, device=DEV)
+    paged.attn_pages(s.cache, dev(q), pages, u32(pos), out=out)
+    got, gp, gb = out.cpu().numpy(), pages.cpu().numpy(), bounds.cpu().numpy()
+    assert np.all(got[4] == 7.0) and np.all(gp[4] == -9)
+    s.seen = [s.seen[0] + [ref.at(s.table[0], s.n_pages, s.page, t) for t in range(150, s.capacity)]] * count
+    for i in (0, 1, 2, 3, 5, 6, 7):
+        n = int(pos[i]) + 1
+        for g in range(s.kv):
+            want = ref.select(q[i, g * group:(g + 1) * group], gb[:, g], s.table[0], s.n_pages, -(-n // s.page), 1, 1, 4)
+            assert gp[i, g].tolist() == want + [-1] * (4 - len(want))
+            check_attention(s, got, q, i, g, group, [x for t in want for x in range(t * 16, min(n, t * 16 + 16))])
+    assert gp[8].max() == 9  # 160 slots are 10 pages
+
+
+def off(a, floats=1):
+    """a on the GPU, its data `floats` values past a 16-byte boundary."""
+    t = torch.from_numpy(np.ascontiguousarray(a))
+    big = torch.zeros(t.numel() + 8, dtype=t.dtype, device=DEV)
+    view = big[floats:floats + t.numel()].view(t.shape)
+    view.copy_(t)
+    return view
+
+
+def test_unaligned_buffers():
+    """Queries, results, weights, positions and lists at any 4-byte alignment, odd capacity."""
+    s = Setup(19, [63, 40], 3, 64, 7, entries=11)  # capacity 77
+    q = heads(s.rng, 2, 6, 64)
+    weight = s.rng.random((2, 3, 77)).astype(np.float32)
+    slot_pos = np.stack([[s.rng.permutation(77) for _ in range(3)] for _ in range(2)]).astype(np.int32)
+    bounds = torch.zeros(s.n_pages, 3, 2, 64, dtype=torch.float16, device=DEV)
+    pos = u32(s.last())
+    paged.page_bounds(s.cache, pos, bounds, torch.zeros_like(pos), 11)
+    answers = []
+    for place in (dev, off):
+        lists, out, out2 = place(np.full((2, 3, 5), -9, np.int32)), place(np.zeros_like(q)), place(np.zeros_like(q))
+        w, sp, ln = place(weight), place(slot_pos), place(np.array([63, 40], np.int32))
+        k, v = s.kd.clone(), s.vd.clone()
+        cache = paged.PagedKV(k, v, s.cache.block_table)
+        at = place(np.array([n - 1 for n in s.lens], np.int32))
+        paged.select_pages(cache, bounds, place(q), at, 5, 1, 1, pages=lists)
+        paged.attn_pages(cache, place(q), lists, at, out=out)
+        paged.attn_weights(cache, place(q), at, w, out=out2)
+        paged.evict(cache, ln, place(np.array([76, 76], np.int32)), 33, w, sp, 2, 5)
+        answers.append([lists, out, out2, w, sp, ln, k.view(torch.int16), v.view(torch.int16)])
+    for a, b in zip(*answers):
+        assert torch.equal(a, b)
+
+
+def test_smallest_cache():
+    """One page of one slot, one head: every operator."""
+    s = Setup(20, [1], 1, 64, 1, spare=0)
+    assert s.capacity == 1 and s.n_pages == 1
+    q, k, v = (heads(s.rng, 1, 1, 64) for _ in range(3))
+    pos = u32([0])
+    turned = paged.qk_norm_rope_append(s.cache, dev(q), dev(k), dev(v), None, None, pos, theta=1e4)
+    bounds = paged.page_bounds(s.cache, pos, torch.zeros(1, 1, 2, 64, dtype=torch.float16, device=DEV))
+    assert torch.equal(bounds[0, 0, 0], s.kd[0, 0, 0]) and torch.equal(bounds[0, 0, 1], s.kd[0, 0, 0])
+    pages = paged.select_pages(s.cache, bounds, turned, pos, 2)
+    assert pages.flatten().tolist() == [0, -1]
+    weight = torch.zeros(1, 1, 1, device=DEV)
+    value = s.vd[0, 0, 0].float()
+    for out in (paged.attn_pages(s.cache, turned, pages, pos), paged.attn_weights(s.cache, turned, pos, weight)):
+        assert torch.equal(out[0, 0], value)  # one term: 2^15 v / 2^15
+    assert weight.item() == 1.0
+    length, slot_pos = u32([1]), u32([[[0]]])
+    paged.evict(s.cache, length, pos, 1, weight, slot_pos)
+    assert length.item() == 1 and slot_pos.item() == 0 and weight.item() == 1.0
