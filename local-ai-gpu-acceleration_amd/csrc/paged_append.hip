@@ -2,6 +2,8 @@
 // head, its rotation and the store into the page slot in one pass over the
 // projections' output; and the bounds of a page's keys, which the selection of
 // pages reads.
+#include <type_traits>
+
 #include "common.h"
 #include "layer_common.cuh"
 #include "paged.h"

@@ -12,6 +12,7 @@ typedef _Float16 half8 __attribute__((ext_vector_type(8)));
 typedef std::uint32_t u32x2 __attribute__((ext_vector_type(2)));
 typedef std::uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
 
 constexpr std::uint32_t kThreads = 256, kWaves = kThreads / 64u, kTile = 16;
 constexpr std::uint32_t kMaxPer = 64;  // tiles of a split, at most: what its scores take in the LDS
@@ -44,22 +45,31 @@ __device__ __forceinline__ std::uint32_t from_lane(std::uint32_t v, std::uint32_
 //  * o += V^T p by v_mfma_f32_4x4x4_16b_f16: a lane holds its own dimensions of
 //    four positions, as the V rows' coalesced loads leave them, and one column of p,
 //    fetched from the score layout by ds_bpermute. A lane's 4 results are one head's,
-//    so its rescaling is one factor.
-// T: heads in fours (1..4). WEIGHTS: every slot, the scores kept for merge_weights_kernel.
+//    so its rescaling is one factor;
+//  * WIDE (9 to 16 heads): a column a head, hi and lo in two MFMAs of the scores, and o by
+//    v_mfma_f32_16x16x4_4b_f16, whose A has the same layout: a quarter of the
+//    instructions and exchanges of four 4x4 columns (12 heads of 128 83 -> 63 us).
+// T: heads in fours (1, 2, 4). WEIGHTS: every slot, the scores kept for merge_weights_kernel.
 // Bound by the reads of K and V: 4096 listed positions of eight sequences (134 MB)
 // 25.2 us, 5.3 TB/s (a 1 GiB copy: 5.2); without loads running ahead 33.9, with two sets of
 // registers in flight, at half the waves, 31.4; with loads that stay in the caches, which a
 // step's other reads need more, 26.8. Workgroups next to each other take the
 // kv heads of one place, which lie next to each other in a page.
+// Waves a SIMD that the registers are held down for, where that pays: 9 to 16 heads (12
+// heads of 64 35.9 -> 33.1 us, of 128 62.9 -> 58.9, of 256 listed 51.0 -> 45.7; of 256 with
+// weights it spills, 67 -> 109, and up to 8 heads of 128 with weights lose, 68 -> 80).
 template <int D, int T, bool WEIGHTS>
-__global__ __launch_bounds__(kThreads) void paged_attn_kernel(AttnArgs a, PagedView kv) {
-  constexpr int NT = (T + 1) / 2;            // score tiles of 8 heads
+constexpr int attn_waves() { return T < 4 || (D == 256 && WEIGHTS) ? 1 : D == 64 ? 3 : 2; }
+template <int D, int T, bool WEIGHTS>
+__global__ __launch_bounds__(kThreads, (attn_waves<D, T, WEIGHTS>())) void paged_attn_kernel(AttnArgs a, PagedView kv) {
+  constexpr bool WIDE = T == 4;
+  constexpr std::uint32_t kHeads = 4u * T;   // heads a workgroup has room for
   constexpr int J = D / 32;                  // score MFMAs of a tile
   constexpr int VD = D == 256 ? 4 : 2;       // dims a lane holds of a V row
   constexpr int RPL = D == 64 ? 2 : 1;       // V rows a load covers
   constexpr int STEPS = 4 / RPL;             // 4-position steps of a tile
-  __shared__ __align__(16) float rec[kWaves][4 * T][D];
-  __shared__ float2 rml[kWaves][4 * T];
+  __shared__ __align__(16) float rec[kWaves][kHeads][D];
+  __shared__ float2 rml[kWaves][kHeads];
   extern __shared__ __align__(16) float held[];
   const std::uint32_t split = blockIdx.x / kv.n_kv, g = blockIdx.x % kv.n_kv, r = blockIdx.y;
   const std::uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -88,17 +98,18 @@ __global__ __launch_bounds__(kThreads) void paged_attn_kernel(AttnArgs a, PagedV
     return table[lp < kv.entries ? lp : kv.entries - 1u];
   };
   const std::uint32_t tile0 = split * a.per + wave;
+  // the list's first 64 entries, a lane each, for its length below
+  const std::int32_t listed = WEIGHTS ? 0 : list[lane < a.n_select ? lane : 0u];
   entry = load_entry(tile0);
   entry_next = load_entry(tile0 + kWaves);
 
-  // B operands of the scores and each column's power of two
-  uint4 qb[NT][J];
-  float qscale[NT];
-#pragma unroll
-  for (int nt = 0; nt < NT; ++nt) {
-    const std::uint32_t h = 8u * nt + col / 2u;
-    const bool there = h < a.group;
-    const float* qr = a.q + (head0 + (there ? h : 0u)) * D + 8u * qq;
+  // B operands of the scores and the column's power of two
+  const std::uint32_t h = WIDE ? col : col / 2u;  // the lane's head
+  const bool my_head = h < a.group;
+  uint4 qb[WIDE ? 2 : 1][J];
+  float qscale;
+  {
+    const float* qr = a.q + (head0 + (my_head ? h : 0u)) * D + 8u * qq;
     f32x4_any x[J][2];
     float m = 0.0f;
 #pragma unroll
@@ -106,6 +117,7 @@ __global__ __launch_bounds__(kThreads) void paged_attn_kernel(AttnArgs a, PagedV
       x[j][0] = *reinterpret_cast<const f32x4_any*>(qr + 32 * j);
       x[j][1] = *reinterpret_cast<const f32x4_any*>(qr + 32 * j + 4);
     }
+    page = load_page(entry);  // with the query in flight
 #pragma unroll
     for (int j = 0; j < J; ++j)
 #pragma unroll
@@ -114,36 +126,67 @@ __global__ __launch_bounds__(kThreads) void paged_attn_kernel(AttnArgs a, PagedV
     m = fmaxf(m, lane_xor<32>(m));
     int e = 0;
     if (m > 0.0f && m <= 3.4e38f) frexpf(m, &e);
-    qscale[nt] = ldexpf(1.4426950408889634f / (D == 64 ? 8.0f : D == 128 ? 11.313708498984761f : 16.0f), e);
+    qscale = ldexpf(1.4426950408889634f / (D == 64 ? 8.0f : D == 128 ? 11.313708498984761f : 16.0f), e);
 #pragma unroll
     for (int j = 0; j < J; ++j) {
-      half8 b;
+      half8 hi, lo;
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        float v = there ? ldexpf(x[j][i / 4][i & 3], -e) : 0.0f;
+        float v = my_head ? ldexpf(x[j][i / 4][i & 3], -e) : 0.0f;
         asm("" : "+v"(v));  // one rounded value for hi and lo
-        const _Float16 hi = static_cast<_Float16>(v);
-        b[i] = (col & 1u) == 0u ? hi : static_cast<_Float16>(v - static_cast<float>(hi));
+        hi[i] = static_cast<_Float16>(v);
+        lo[i] = static_cast<_Float16>(v - static_cast<float>(hi[i]));
       }
-      qb[nt][j] = __builtin_bit_cast(uint4, b);
+      if constexpr (WIDE) {
+        qb[0][j] = __builtin_bit_cast(uint4, hi);
+        qb[1][j] = __builtin_bit_cast(uint4, lo);
+      } else {
+        const uint4 uh = __builtin_bit_cast(uint4, hi), ul = __builtin_bit_cast(uint4, lo);
+        qb[0][j] = (col & 1u) == 0u ? uh : ul;
+      }
     }
   }
 
   const std::uint32_t n = paged_filled(kv, a.pos[r]);
   if (n == 0u) return;  // a padded row
-  const std::uint32_t total = WEIGHTS ? n : room;
+  std::uint32_t total = n;
+  if constexpr (!WEIGHTS) {  // up to the list's last entry that names a page of the table
+    total = 0u;
+    for (std::uint32_t i = 0; i < a.n_select; i += 64u) {
+      const std::uint32_t e = i + lane;
+      const std::int32_t lp = i == 0u ? listed : list[e < a.n_select ? e : 0u];
+      const unsigned long long b = __ballot(e < a.n_select && static_cast<std::uint32_t>(lp) < kv.entries);
+      if (b != 0ull) total = (i + 64u - static_cast<std::uint32_t>(__builtin_clzll(b))) * kv.page_size;
+    }
+  }
   const std::uint32_t tiles = (total + kTile - 1u) / kTile;
-  if (split * a.per >= tiles) return;  // behind the context: no record of it is read
+  if (split * a.per >= tiles) {  // nothing of the row is here
+    if constexpr (!WEIGHTS) {
+      for (std::uint32_t i = threadIdx.x; i < a.group * D; i += kThreads) {
+        if (a.splits == 1u)
+          a.out[head0 * D + i] = 0.0f;
+        else
+          a.part[((head0 + i / D) * a.splits + split) * D + i % D] = 0.0f;
+      }
+      if (a.splits > 1u && threadIdx.x < a.group)
+        a.ml[(head0 + threadIdx.x) * a.splits + split] = make_float2(-INFINITY, 0.0f);
+    }
+    return;
+  }
   const std::uint32_t tile1 = split * a.per + a.per < tiles ? split * a.per + a.per : tiles;
 
-  float m[NT], l[NT];
-  f32x4 o[T][VD];
+  float m = -INFINITY, l = 0.0f;
+  f32x4 o[WIDE ? 1 : T][VD];
+  f32x16 ow[WIDE ? VD : 1];
+  if constexpr (WIDE) {
 #pragma unroll
-  for (int nt = 0; nt < NT; ++nt) m[nt] = -INFINITY, l[nt] = 0.0f;
+    for (int s = 0; s < VD; ++s) ow[s] = f32x16{};
+  } else {
 #pragma unroll
-  for (int t = 0; t < T; ++t)
+    for (int t = 0; t < T; ++t)
 #pragma unroll
-    for (int s = 0; s < VD; ++s) o[t][s] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+      for (int s = 0; s < VD; ++s) o[t][s] = f32x4{};
+  }
 
   // A tile's keys and values and which of its positions count. One that does not reads
   // row 0 of the cache; its score and value are dropped.
@@ -187,7 +230,6 @@ __global__ __launch_bounds__(kThreads) void paged_attn_kernel(AttnArgs a, PagedV
   // read once this tile's scores have used theirs, its values after this tile's sums.
   // No branch skips a load, so each wait is for the loads it needs alone (behind the
   // last tile row 0 is read, from the L2).
-  page = load_page(entry);
   settle(tile0);
   load_k();
   entry = entry_next;
@@ -196,66 +238,58 @@ __global__ __launch_bounds__(kThreads) void paged_attn_kernel(AttnArgs a, PagedV
   load_v();
   for (std::uint32_t tile = tile0; tile < tile1; tile += kWaves) {
     const std::uint32_t now = valid;
-    std::uint32_t p01[NT], p23[NT];
-    float alpha[NT];
-    bool moved = false;
-    f32x4 sc_all[NT];
+    f32x4 sc = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-      sc_all[nt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    for (int k = 0; k < (WIDE ? 2 : 1); ++k)
 #pragma unroll
       for (int j = 0; j < J; ++j)
-        sc_all[nt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8, ka[j]),
-                                                            __builtin_bit_cast(half8, qb[nt][j]), sc_all[nt], 0, 0, 0);
-    }
+        sc = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8, ka[j]), __builtin_bit_cast(half8, qb[k][j]),
+                                                    sc, 0, 0, 0);
     settle(tile + kWaves);
     load_k();
     entry = entry_next;
     page = load_page(entry);
     entry_next = load_entry(tile + 3u * kWaves);
+    // positions 4 qq + i of the lane's head
+    float s4[4], top = -INFINITY;
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-      const f32x4 sc = sc_all[nt];
-      // column n: head n / 2; positions 4 qq + i
-      float s4[4], top = -INFINITY;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float t = (sc[i] + lane_xor<1>(sc[i])) * qscale[nt];
-        s4[i] = (now >> (4u * qq + i) & 1u) != 0u ? t : -INFINITY;
-        top = fmaxf(top, s4[i]);
-      }
-      if constexpr (WEIGHTS) {
-        const std::uint32_t h = 8u * nt + col / 2u;
-        if ((col & 1u) == 0u && h < a.group)
-          *reinterpret_cast<f32x4*>(&held[(h * a.per + (tile - split * a.per)) * kTile + 4u * qq]) = f32x4{s4[0], s4[1], s4[2], s4[3]};
-      }
-      top = fmaxf(top, lane_xor<16>(top));
-      top = fmaxf(top, lane_xor<32>(top));
-      const float mn = fmaxf(m[nt], top);
-      const float base = mn == -INFINITY ? 0.0f : mn;
-      alpha[nt] = __builtin_amdgcn_exp2f(m[nt] - base);
-      moved = moved || mn != m[nt];
-      m[nt] = mn;
-      float sum = 0.0f;
-      half4 ph;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        float p = __builtin_amdgcn_exp2f(s4[i] - base + kLift);
-        asm("" : "+v"(p));
-        sum += p;
-        const _Float16 hi = static_cast<_Float16>(p);
-        ph[i] = (col & 1u) == 0u ? hi : static_cast<_Float16>(p - static_cast<float>(hi));
-      }
-      l[nt] = l[nt] * alpha[nt] + sum;
-      const uint2 pk = __builtin_bit_cast(uint2, ph);
-      p01[nt] = pk.x, p23[nt] = pk.y;
+    for (int i = 0; i < 4; ++i) {
+      const float t = (WIDE ? sc[i] : sc[i] + lane_xor<1>(sc[i])) * qscale;
+      s4[i] = (now >> (4u * qq + i) & 1u) != 0u ? t : -INFINITY;
+      top = fmaxf(top, s4[i]);
     }
+    if constexpr (WEIGHTS) {
+      if ((WIDE || (col & 1u) == 0u) && my_head)
+        *reinterpret_cast<f32x4*>(&held[(h * a.per + (tile - split * a.per)) * kTile + 4u * qq]) = f32x4{s4[0], s4[1], s4[2], s4[3]};
+    }
+    top = fmaxf(top, lane_xor<16>(top));
+    top = fmaxf(top, lane_xor<32>(top));
+    const float mn = fmaxf(m, top), base = mn == -INFINITY ? 0.0f : mn;
+    const float alpha = __builtin_amdgcn_exp2f(m - base);
+    const bool moved = mn != m;
+    m = mn;
+    float sum = 0.0f;
+    half4 p_hi, p_lo;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      float p = __builtin_amdgcn_exp2f(s4[i] - base + kLift);
+      asm("" : "+v"(p));
+      sum += p;
+      p_hi[i] = static_cast<_Float16>(p);
+      p_lo[i] = static_cast<_Float16>(p - static_cast<float>(p_hi[i]));
+    }
+    l = l * alpha + sum;
     if (__ballot(moved) != 0ull) {
+      if constexpr (WIDE) {
 #pragma unroll
-      for (int t = 0; t < T; ++t) {
-        const float f = __uint_as_float(from_lane(__float_as_uint(alpha[t / 2]), 8u * (t & 1) + 2u * (lane & 3u)));
+        for (int s = 0; s < VD; ++s) ow[s] *= alpha;  // a lane's results are its own head's
+      } else {
 #pragma unroll
-        for (int s = 0; s < VD; ++s) o[t][s] *= f;
+        for (int t = 0; t < T; ++t) {
+          const float f = __uint_as_float(from_lane(__float_as_uint(alpha), 8u * t + 2u * (lane & 3u)));
+#pragma unroll
+          for (int s = 0; s < VD; ++s) o[t][s] *= f;
+        }
       }
     }
     if (now != 0xFFFFu) {  // 0 times what lies behind the context must stay 0
@@ -277,17 +311,26 @@ __global__ __launch_bounds__(kThreads) void paged_attn_kernel(AttnArgs a, PagedV
         w.y = __builtin_amdgcn_perm(vw[4 * st + 3][s / 2], vw[4 * st + 2][s / 2], sel);
         va[s] = __builtin_bit_cast(half4, w);
       }
-      const std::uint32_t src = 16u * (RPL == 2 ? 2u * st + (lane >> 5) : st) + 2u * (lane & 3u);
+      const std::uint32_t row16 = 16u * (RPL == 2 ? 2u * st + (lane >> 5) : st);  // where the step's p lies
+      if constexpr (WIDE) {
+        const uint2 hi = __builtin_bit_cast(uint2, p_hi), lo = __builtin_bit_cast(uint2, p_lo);
+        const half4 bh = __builtin_bit_cast(half4, make_uint2(from_lane(hi.x, row16 + col), from_lane(hi.y, row16 + col)));
+        const half4 bl = __builtin_bit_cast(half4, make_uint2(from_lane(lo.x, row16 + col), from_lane(lo.y, row16 + col)));
 #pragma unroll
-      for (int t = 0; t < T; ++t) {
+        for (int s = 0; s < VD; ++s) ow[s] = __builtin_amdgcn_mfma_f32_16x16x4f16(va[s], bh, ow[s], 0, 0, 0);
 #pragma unroll
-        for (int part = 0; part < 2; ++part) {
-          uint2 w;
-          w.x = from_lane(p01[t / 2], src + 8u * (t & 1) + part);
-          w.y = from_lane(p23[t / 2], src + 8u * (t & 1) + part);
-          const half4 pb = __builtin_bit_cast(half4, w);
+        for (int s = 0; s < VD; ++s) ow[s] = __builtin_amdgcn_mfma_f32_16x16x4f16(va[s], bl, ow[s], 0, 0, 0);
+      } else {
+        const uint2 pk = __builtin_bit_cast(uint2, (col & 1u) == 0u ? p_hi : p_lo);
 #pragma unroll
-          for (int s = 0; s < VD; ++s) o[t][s] = __builtin_amdgcn_mfma_f32_4x4x4f16(va[s], pb, o[t][s], 0, 0, 0);
+        for (int t = 0; t < T; ++t) {
+#pragma unroll
+          for (int part = 0; part < 2; ++part) {
+            const std::uint32_t src = row16 + 8u * t + 2u * (lane & 3u) + part;
+            const half4 pb = __builtin_bit_cast(half4, make_uint2(from_lane(pk.x, src), from_lane(pk.y, src)));
+#pragma unroll
+            for (int s = 0; s < VD; ++s) o[t][s] = __builtin_amdgcn_mfma_f32_4x4x4f16(va[s], pb, o[t][s], 0, 0, 0);
+          }
         }
       }
     }
@@ -295,31 +338,43 @@ __global__ __launch_bounds__(kThreads) void paged_attn_kernel(AttnArgs a, PagedV
   }
 
   // the waves' records, merged: o = sum e^(m_w - M) o_w, L alike
+  l += lane_xor<16>(l);
+  l += lane_xor<32>(l);
+  // a NaN among the scores makes the row NaN, also where no number gave a maximum
+  if (qq == 0u && (WIDE || (col & 1u) == 0u) && h < kHeads) rml[wave][h] = make_float2(l != l ? INFINITY : m, l);
+  if constexpr (WIDE) {
+    // register 4 b + i: lane 16 b + 4 qq + i of the values' loads
 #pragma unroll
-  for (int nt = 0; nt < NT; ++nt) {
-    l[nt] += lane_xor<16>(l[nt]);
-    l[nt] += lane_xor<32>(l[nt]);
-    const std::uint32_t h = 8u * nt + col / 2u;
-    // a NaN among the scores makes the row NaN, also where no number gave a maximum
-    if (qq == 0u && (col & 1u) == 0u && h < 4u * T)
-      rml[wave][h] = make_float2(l[nt] != l[nt] ? INFINITY : m[nt], l[nt]);
-  }
+    for (int b = 0; b < (D == 64 ? 2 : 4); ++b) {
+      float v[4 * VD];
 #pragma unroll
-  for (int t = 0; t < T; ++t) {
-    if constexpr (D == 64) {
+      for (int i = 0; i < 4; ++i)
 #pragma unroll
-      for (int s = 0; s < VD; ++s)
+        for (int s = 0; s < VD; ++s)
+          v[VD * i + s] = D == 64 ? ow[s][4 * b + i] + ow[s][(4 * b + i + 8) % 16] : ow[s][4 * b + i];
+      float* dst = &rec[wave][col][VD * (16 * b + 4u * qq)];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) o[t][s][i] += lane_xor<32>(o[t][s][i]);
+      for (int i = 0; i < VD; ++i)
+        *reinterpret_cast<f32x4*>(dst + 4 * i) = f32x4{v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]};
     }
-    if (D != 64 || lane < 32u) {
-      float* dst = &rec[wave][4 * t + (lane & 3u)][VD * (lane & ~3u)];
+  } else {
 #pragma unroll
-      for (int i = 0; i < 4; i += 4 / VD) {
-        if constexpr (VD == 2)
-          *reinterpret_cast<f32x4*>(dst + 2 * i) = f32x4{o[t][0][i], o[t][1][i], o[t][0][i + 1], o[t][1][i + 1]};
-        else
-          *reinterpret_cast<f32x4*>(dst + 4 * i) = f32x4{o[t][0][i], o[t][1][i], o[t][VD - 2][i], o[t][VD - 1][i]};
+    for (int t = 0; t < T; ++t) {
+      if constexpr (D == 64) {
+#pragma unroll
+        for (int s = 0; s < VD; ++s)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) o[t][s][i] += lane_xor<32>(o[t][s][i]);
+      }
+      if (D != 64 || lane < 32u) {
+        float* dst = &rec[wave][4 * t + (lane & 3u)][VD * (lane & ~3u)];
+#pragma unroll
+        for (int i = 0; i < 4; i += 4 / VD) {
+          if constexpr (VD == 2)
+            *reinterpret_cast<f32x4*>(dst + 2 * i) = f32x4{o[t][0][i], o[t][1][i], o[t][0][i + 1], o[t][1][i + 1]};
+          else
+            *reinterpret_cast<f32x4*>(dst + 4 * i) = f32x4{o[t][0][i], o[t][1][i], o[t][VD - 2][i], o[t][VD - 1][i]};
+        }
       }
     }
   }

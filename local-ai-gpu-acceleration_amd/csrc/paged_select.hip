@@ -2,6 +2,8 @@
 // worth keeping. Both rank up to some ten thousand keys per (sequence, kv head) and
 // take the best k of them, the lower index between equals: a radix selection in
 // one workgroup, exact in every bit of the keys.
+#include <type_traits>
+
 #include "common.h"
 #include "layer_common.cuh"
 #include "paged.h"
@@ -586,9 +588,10 @@ hipError_t launch_select(const PagedView& view, const std::uint16_t* bounds, con
                        dim3(kThreads), 0, stream, view, bounds, q, group, pos, n_first, n_last, keys);
   };
   const std::uint64_t waves = static_cast<std::uint64_t>(count) * view.n_kv * ((view.entries + 64u / L - 1u) / (64u / L));
-  // four steps a wave from where single steps fill the chip more than once (us of four / one:
-  // 504 waves 9.5 / 7.8, 4096 12.0 / 11.5, 8000 12.0 / 12.0, 16384 15.5 / 16.4)
-  if (waves > 4096u)
+  // four steps a wave from where single steps, whose sums grow with the heads, fill the
+  // chip more than once (us of four / one: 504 waves of 4 heads 9.5 / 7.8, 4096 12.0 / 11.5, 8000
+  // 12.0 / 12.0, 16384 15.5 / 16.4; the scores alone of 4980 waves of 12 heads 14.0 / 8.6)
+  if (waves > 8192u * ((group + 3u) / 4u))
     score(std::integral_constant<int, 4>{});
   else
     score(std::integral_constant<int, 1>{});
