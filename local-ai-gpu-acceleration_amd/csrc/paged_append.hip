@@ -150,6 +150,40 @@ __global__ __launch_bounds__(kThreads) void append_kernel(AppendArgs a, PagedVie
 }
 
 typedef _Float16 half8 __attribute__((ext_vector_type(8)));
+constexpr _Float16 kHalfMax = static_cast<_Float16>(65504.0f);
+
+// The w-th (page, kv head) of row r's pages from first[r] on: its first cache row, its
+// filled keys (0: there is none), its place among the bounds.
+struct PageUnit {
+  std::uint32_t row, keys;
+  std::size_t at;
+};
+__device__ __forceinline__ PageUnit page_unit(const PagedView& kv, const std::uint32_t* first, const std::uint32_t* last,
+                                              std::uint32_t r, std::uint32_t w, std::uint32_t span) {
+  const PageUnit none{kNoRow, 0u, 0u};
+  const std::uint32_t n = paged_filled(kv, last[r]);
+  if (n == 0u || w / kv.n_kv >= span) return none;
+  const std::uint32_t from = first != nullptr ? first[r] : n - 1u;
+  if (from >= n) return none;
+  const std::uint32_t lp = page_of(kv, from) + w / kv.n_kv, g = w % kv.n_kv;
+  if (lp >= kv.entries || lp * kv.page_size >= n) return none;
+  const std::int32_t page = kv.table[static_cast<std::size_t>(r) * kv.table_stride + lp];
+  const std::uint32_t row = paged_row(kv, page, g, 0u), rest = n - lp * kv.page_size;
+  if (row == kNoRow) return none;
+  return PageUnit{row, rest < kv.page_size ? rest : kv.page_size, static_cast<std::size_t>(page) * kv.n_kv + g};
+}
+
+template <int L>
+__device__ __forceinline__ void store_bounds(std::uint16_t* bounds, std::size_t at, std::uint32_t t, half8 hi, half8 lo) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    hi[i] = hi[i] > kHalfMax ? kHalfMax : hi[i];
+    lo[i] = lo[i] < -kHalfMax ? -kHalfMax : lo[i];
+  }
+  half8* dst = reinterpret_cast<half8*>(bounds) + at * 2u * L + t;
+  dst[0] = hi;
+  dst[L] = lo;
+}
 
 // One wave a (page, kv head): L = head_dim / 8 lanes a key, 64 / L keys at a
 // time. Repeating a filled key changes neither extreme, so the last step reads
@@ -162,27 +196,16 @@ __global__ __launch_bounds__(kThreads) void page_bounds_kernel(PagedView kv, con
   constexpr std::uint32_t D = 8u * L, kKeys = 64u / L;
   const std::uint32_t r = blockIdx.y, lane = threadIdx.x & 63u;
   const std::uint32_t w = __builtin_amdgcn_readfirstlane(blockIdx.x * (kThreads / 64u) + (threadIdx.x >> 6));
-  const std::uint32_t n = paged_filled(kv, last[r]);
-  if (n == 0u || w / kv.n_kv >= span) return;
-  const std::uint32_t from = first != nullptr ? first[r] : n - 1u;
-  if (from >= n) return;
-  const std::uint32_t lp = from / kv.page_size + w / kv.n_kv, g = w % kv.n_kv;
-  if (lp >= kv.entries || lp * kv.page_size >= n) return;
-  const std::int32_t page = kv.table[static_cast<std::size_t>(r) * kv.table_stride + lp];
-  const std::uint32_t row = paged_row(kv, page, g, 0u);
-  if (row == kNoRow) return;
-  const std::uint32_t keys = n - lp * kv.page_size < kv.page_size ? n - lp * kv.page_size : kv.page_size;
-  const half8* src = reinterpret_cast<const half8*>(kv.k + static_cast<std::size_t>(row) * D) + lane % L;
-  const _Float16 big = static_cast<_Float16>(65504.0f);
-  half8 hi, lo;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) hi[i] = -big, lo[i] = big;
-  for (std::uint32_t i0 = lane / L; i0 < keys + lane / L; i0 += 4u * kKeys) {
+  const PageUnit u = page_unit(kv, first, last, r, w, span);
+  if (u.keys == 0u) return;
+  const half8* src = reinterpret_cast<const half8*>(kv.k + static_cast<std::size_t>(u.row) * D) + lane % L;
+  half8 hi = half8{} - kHalfMax, lo = half8{} + kHalfMax;
+  for (std::uint32_t i0 = lane / L; i0 < u.keys + lane / L; i0 += 4u * kKeys) {
     half8 x[4];
 #pragma unroll
     for (std::uint32_t j = 0; j < 4u; ++j) {
       const std::uint32_t i = i0 + kKeys * j;
-      const half8* at = src + static_cast<std::size_t>(i < keys ? i : keys - 1u) * L;
+      const half8* at = src + static_cast<std::size_t>(i < u.keys ? i : u.keys - 1u) * L;
       x[j] = STREAM ? __builtin_nontemporal_load(at) : *at;
     }
 #pragma unroll
@@ -204,14 +227,37 @@ __global__ __launch_bounds__(kThreads) void page_bounds_kernel(PagedView kv, con
   if constexpr (L <= 16) fold(std::integral_constant<int, 16>{});
   fold(std::integral_constant<int, 32>{});
   if (lane >= static_cast<std::uint32_t>(L)) return;
+  store_bounds<L>(bounds, u.at, lane, hi, lo);
+}
+
+// Small pages of a prompt: each L lanes take a (page, kv head) of their own, all its
+// keys one after the other, eight in flight. No exchange between lanes, which is most of
+// the work above where a page has few keys.
+template <int L>
+__global__ __launch_bounds__(kThreads) void prompt_bounds_kernel(PagedView kv, const std::uint32_t* first,
+                                                                 const std::uint32_t* last, std::uint32_t span,
+                                                                 std::uint16_t* bounds) {
+  constexpr std::uint32_t D = 8u * L;
+  const std::uint32_t r = blockIdx.y, t = threadIdx.x % L;
+  const std::uint32_t w = blockIdx.x * (kThreads / L) + threadIdx.x / L;
+  const PageUnit u = page_unit(kv, first, last, r, w, span);
+  if (u.keys == 0u) return;
+  const half8* src = reinterpret_cast<const half8*>(kv.k + static_cast<std::size_t>(u.row) * D) + t;
+  half8 hi = half8{} - kHalfMax, lo = half8{} + kHalfMax;
+  for (std::uint32_t i0 = 0; i0 < u.keys; i0 += 8u) {
+    half8 x[8];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    hi[i] = hi[i] > big ? big : hi[i];
-    lo[i] = lo[i] < -big ? -big : lo[i];
+    for (std::uint32_t j = 0; j < 8u; ++j) {
+      const std::uint32_t i = i0 + j < u.keys ? i0 + j : u.keys - 1u;
+      x[j] = __builtin_nontemporal_load(src + static_cast<std::size_t>(i) * L);
+    }
+#pragma unroll
+    for (std::uint32_t j = 0; j < 8u; ++j) {
+      hi = __builtin_elementwise_max(hi, x[j]);
+      lo = __builtin_elementwise_min(lo, x[j]);
+    }
   }
-  half8* dst = reinterpret_cast<half8*>(bounds + (static_cast<std::size_t>(page) * kv.n_kv + g) * 2u * D) + lane;
-  dst[0] = hi;
-  dst[L] = lo;
+  store_bounds<L>(bounds, u.at, t, hi, lo);
 }
 
 }  // namespace
@@ -287,20 +333,27 @@ extern "C" hipError_t rtxllm_kv_page_bounds_f16(const rtxllm_paged_kv* cache, co
   const std::uint64_t waves = static_cast<std::uint64_t>(pages) * view.n_kv;
   if (waves > (1ull << 24)) return hipErrorInvalidValue;  // the launch's thread count
   const dim3 grid(static_cast<std::uint32_t>((waves + 3u) / 4u), count);
-  auto launch = [&](auto stream_keys) {
-    constexpr bool kStream = decltype(stream_keys)::value;
-    if (cache->head_dim == 64u)
-      hipLaunchKernelGGL((page_bounds_kernel<8, kStream>), grid, dim3(kThreads), 0, stream, view, first, last, pages, bounds);
-    else if (cache->head_dim == 128u)
-      hipLaunchKernelGGL((page_bounds_kernel<16, kStream>), grid, dim3(kThreads), 0, stream, view, first, last, pages, bounds);
-    else
-      hipLaunchKernelGGL((page_bounds_kernel<32, kStream>), grid, dim3(kThreads), 0, stream, view, first, last, pages, bounds);
-  };
   // A newest page alone is attended next: its keys stay in the caches (one sequence's 3.5
-  // us, streamed 5.1); those of many pages would only push others out.
-  if (pages > 1u)
-    launch(std::true_type{});
+  // us, streamed 5.1); those of many pages would only push others out. Pages of fewer keys
+  // than a wave reads at once go to a part of it each (60000 positions of 8 heads, us of a
+  // wave / a part a page: 8 keys of 128 38.2 / 29.0, 16 of 64 30.1 / 19.6, 16 of 128 26.6 / 27.3, 64
+  // of 128 23.3 / 22.6; 4000 positions in pages of 64 5.3 / 9.2).
+  auto launch = [&](auto lanes) {
+    constexpr int L = decltype(lanes)::value;
+    const std::uint32_t per = kThreads / L;
+    if (pages == 1u)
+      hipLaunchKernelGGL((page_bounds_kernel<L, false>), grid, dim3(kThreads), 0, stream, view, first, last, pages, bounds);
+    else if (view.page_size < 256u / L)
+      hipLaunchKernelGGL(prompt_bounds_kernel<L>, dim3(static_cast<std::uint32_t>((waves + per - 1u) / per), count),
+                         dim3(kThreads), 0, stream, view, first, last, pages, bounds);
+    else
+      hipLaunchKernelGGL((page_bounds_kernel<L, true>), grid, dim3(kThreads), 0, stream, view, first, last, pages, bounds);
+  };
+  if (cache->head_dim == 64u)
+    launch(std::integral_constant<int, 8>{});
+  else if (cache->head_dim == 128u)
+    launch(std::integral_constant<int, 16>{});
   else
-    launch(std::false_type{});
+    launch(std::integral_constant<int, 32>{});
   return hipGetLastError();
 }
