@@ -185,28 +185,29 @@ __device__ __forceinline__ void store_bounds(std::uint16_t* bounds, std::size_t 
   dst[L] = lo;
 }
 
-// One wave a (page, kv head): L = head_dim / 8 lanes a key, 64 / L keys at a
-// time. Repeating a filled key changes neither extreme, so the last step reads
+// One wave a (page, kv head), or W of a workgroup whose extremes meet in LDS: L = head_dim
+// / 8 lanes a key, 64 / L keys at a time. Repeating a filled key changes neither extreme, so the last step reads
 // its last key again instead of masking. Bound by bytes: 1024 pages of 64 keys of 8
 // heads of 128 (138 MB) 24.0 us, 5.8 TB/s, streamed past the caches (28.4 through them).
-template <int L, bool STREAM>
+template <int L, int W>
 __global__ __launch_bounds__(kThreads) void page_bounds_kernel(PagedView kv, const std::uint32_t* first,
                                                                const std::uint32_t* last, std::uint32_t span,
                                                                std::uint16_t* bounds) {
   constexpr std::uint32_t D = 8u * L, kKeys = 64u / L;
   const std::uint32_t r = blockIdx.y, lane = threadIdx.x & 63u;
-  const std::uint32_t w = __builtin_amdgcn_readfirstlane(blockIdx.x * (kThreads / 64u) + (threadIdx.x >> 6));
-  const PageUnit u = page_unit(kv, first, last, r, w, span);
-  if (u.keys == 0u) return;
+  const std::uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), part = wave % W;
+  const PageUnit u = page_unit(kv, first, last, r, blockIdx.x * (kThreads / 64u / W) + wave / W, span);
+  if (u.keys == 0u) return;  // (W > 1: the whole workgroup)
   const half8* src = reinterpret_cast<const half8*>(kv.k + static_cast<std::size_t>(u.row) * D) + lane % L;
   half8 hi = half8{} - kHalfMax, lo = half8{} + kHalfMax;
-  for (std::uint32_t i0 = lane / L; i0 < u.keys + lane / L; i0 += 4u * kKeys) {
+  for (std::uint32_t k0 = 4u * kKeys * part; k0 < u.keys; k0 += 4u * kKeys * W) {
+    const std::uint32_t i0 = k0 + lane / L;
     half8 x[4];
 #pragma unroll
     for (std::uint32_t j = 0; j < 4u; ++j) {
       const std::uint32_t i = i0 + kKeys * j;
       const half8* at = src + static_cast<std::size_t>(i < u.keys ? i : u.keys - 1u) * L;
-      x[j] = STREAM ? __builtin_nontemporal_load(at) : *at;
+      x[j] = W == 1 ? __builtin_nontemporal_load(at) : *at;
     }
 #pragma unroll
     for (std::uint32_t j = 0; j < 4u; ++j) {
@@ -226,6 +227,17 @@ __global__ __launch_bounds__(kThreads) void page_bounds_kernel(PagedView kv, con
   if constexpr (L <= 8) fold(std::integral_constant<int, 8>{});
   if constexpr (L <= 16) fold(std::integral_constant<int, 16>{});
   fold(std::integral_constant<int, 32>{});
+  if constexpr (W > 1) {
+    __shared__ half8 parts[W][2][L];
+    if (lane < static_cast<std::uint32_t>(L)) parts[wave][0][lane] = hi, parts[wave][1][lane] = lo;
+    __syncthreads();
+    if (wave != 0u || lane >= static_cast<std::uint32_t>(L)) return;
+#pragma unroll
+    for (int k = 1; k < W; ++k) {
+      hi = __builtin_elementwise_max(hi, parts[k][0][lane]);
+      lo = __builtin_elementwise_min(lo, parts[k][1][lane]);
+    }
+  }
   if (lane >= static_cast<std::uint32_t>(L)) return;
   store_bounds<L>(bounds, u.at, lane, hi, lo);
 }
@@ -333,21 +345,29 @@ extern "C" hipError_t rtxllm_kv_page_bounds_f16(const rtxllm_paged_kv* cache, co
   const std::uint64_t waves = static_cast<std::uint64_t>(pages) * view.n_kv;
   if (waves > (1ull << 24)) return hipErrorInvalidValue;  // the launch's thread count
   const dim3 grid(static_cast<std::uint32_t>((waves + 3u) / 4u), count);
-  // A newest page alone is attended next: its keys stay in the caches (one sequence's 3.5
-  // us, streamed 5.1); those of many pages would only push others out. Pages of fewer keys
-  // than a wave reads at once go to a part of it each (60000 positions of 8 heads, us of a
-  // wave / a part a page: 8 keys of 128 38.2 / 29.0, 16 of 64 30.1 / 19.6, 16 of 128 26.6 / 27.3, 64
-  // of 128 23.3 / 22.6; 4000 positions in pages of 64 5.3 / 9.2).
+  // Three ways to share the pages out, by the units (a page of a head) and by the rounds of
+  // 256 / L keys that a wave reads one at a page of them:
+  // Few units: a page's rounds go to the four waves of a workgroup (8 heads of 128, us of one wave / four:
+  // 256 keys at 8000 positions 12.5 / 5.9 and at 24000 15.0 / 10.9, 128 at 16000 9.1 / 8.7
+  // and at 32000 13.0 / 13.2, 64 at 4000 5.4 / 4.4 and at 8000 5.6 / 6.2, 32 at 2000 3.4 / 3.7; the newest page
+  // alone of 256 keys 6.2 / 3.4, of 16, one round, 2.8 / 3.1). The keys stay in the
+  // caches then: a newest page alone is attended next.
+  // Pages of less than a round: L lanes take a page each (60000 positions of 8 heads, us of
+  // a wave / L lanes: 8 keys of 128 38.2 / 29.0, 16 of 64 30.1 / 19.6, 16 of 128 26.6 / 27.3).
+  // Everything else: a wave a page, streamed past the caches, which hold nothing of it for
+  // long.
   auto launch = [&](auto lanes) {
     constexpr int L = decltype(lanes)::value;
-    const std::uint32_t per = kThreads / L;
-    if (pages == 1u)
-      hipLaunchKernelGGL((page_bounds_kernel<L, false>), grid, dim3(kThreads), 0, stream, view, first, last, pages, bounds);
-    else if (view.page_size < 256u / L)
+    const std::uint32_t per = kThreads / L, rounds = view.page_size / (256u / L);
+    const std::uint64_t units = waves * count;
+    if (rounds >= 2u && units <= 128u * rounds && units <= 1024u)
+      hipLaunchKernelGGL((page_bounds_kernel<L, 4>), dim3(static_cast<std::uint32_t>(waves), count), dim3(kThreads), 0,
+                         stream, view, first, last, pages, bounds);
+    else if (rounds == 0u)
       hipLaunchKernelGGL(prompt_bounds_kernel<L>, dim3(static_cast<std::uint32_t>((waves + per - 1u) / per), count),
                          dim3(kThreads), 0, stream, view, first, last, pages, bounds);
     else
-      hipLaunchKernelGGL((page_bounds_kernel<L, true>), grid, dim3(kThreads), 0, stream, view, first, last, pages, bounds);
+      hipLaunchKernelGGL((page_bounds_kernel<L, 1>), grid, dim3(kThreads), 0, stream, view, first, last, pages, bounds);
   };
   if (cache->head_dim == 64u)
     launch(std::integral_constant<int, 8>{});

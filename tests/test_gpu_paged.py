@@ -172,7 +172,8 @@ def test_append_in_place_and_extremes():
 POOL = [(4, 128, 64), (2, 64, 16), (1, 256, 24), (3, 128, 7), (8, 64, 1)]
 
 
-@pytest.mark.parametrize("kv,dim,page", POOL)
+# (a wave, a part of one or four waves a page, by its size and by the pages of a call)
+@pytest.mark.parametrize("kv,dim,page", POOL + [(16, 128, 64), (2, 128, 21), (1, 128, 300), (3, 64, 130)])
 def test_page_bounds(kv, dim, page):
     lens = [page * 9 + 1, 0, 1, page * 4, page * 6 + page // 2 + 1]
     s = Setup(dim + page, lens, kv, dim, page, hole=True, stride=31)
