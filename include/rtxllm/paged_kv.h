@@ -92,7 +92,8 @@ hipError_t rtxllm_kv_page_bounds_f16(const rtxllm_paged_kv* cache, const uint32_
  * max(q_hd largest_d, q_hd smallest_d): no key of the page has a larger product
  * with any of them. Scores are sums in 64 bits, so that the choice does not hang
  * on the order of a sum; the lower page wins between equal scores; a head whose
- * product is NaN does not count, and a page where none does ranks last. A page with no entry in the table is never listed.
+ * product is NaN does not count, and a page where none does ranks last. A page with
+ * no entry in the table is never listed.
  * n_heads / n_kv_heads 1..16, n_first + n_last <= n_select <= 65536, count <= 65535.
  * workspace: rtxllm_attn_select_workspace() bytes, 256-byte aligned. */
 size_t rtxllm_attn_select_workspace(const rtxllm_paged_kv* cache, uint32_t count);
@@ -109,8 +110,9 @@ hipError_t rtxllm_attn_select_pages(const rtxllm_paged_kv* cache, const uint16_t
  * is 0. What a position that is not attended holds, NaN and infinities included, has
  * no effect; a NaN or an infinity among the attended keys or values makes NaN of what
  * it enters. q and the softmax terms enter the products as pairs of fp16 of 22 bits, at
- * any size of q. n_heads / n_kv_heads 1..16; count <= 65535; n_select 1..65536, n_select
- * * page_size <= 2^30. workspace: rtxllm_attn_pages_workspace() bytes, 256-byte aligned. */
+ * any size of q. out may be q, and shares no memory with it otherwise. n_heads /
+ * n_kv_heads 1..16; count <= 65535; n_select 1..65536, n_select * page_size <= 2^30.
+ * workspace: rtxllm_attn_pages_workspace() bytes, 256-byte aligned. */
 size_t rtxllm_attn_pages_workspace(const rtxllm_paged_kv* cache, uint32_t n_heads, uint32_t n_select,
                                    uint32_t count);
 hipError_t rtxllm_attn_decode_pages_gqa_f16(const rtxllm_paged_kv* cache, const float* q, uint32_t n_heads,
@@ -133,9 +135,9 @@ hipError_t rtxllm_attn_decode_weights_gqa_f16(const rtxllm_paged_kv* cache, cons
 /* Eviction: sequence r's first length[r] slots are filled (more than capacity
  * counts as capacity); if they are more than `keep`, keep of them stay, for each
  * kv head its own: first those whose position is protected (slot_pos < n_first,
- * or slot_pos + n_recent > pos[r], pos[r] being the newest position), then those
- * with the largest weight; the lower slot between equals; a NaN weight ranks below every
- * number. The i-th kept slot at or behind `keep` moves into the i-th freed slot
+ * or slot_pos + n_recent > pos[r], pos[r] being the newest position; they are all
+ * alike), then those with the largest weight; the lower slot between equals; a NaN
+ * weight ranks below every number. The i-th kept slot at or behind `keep` moves into the i-th freed slot
  * below it (its key, value, weight and position), so that slots 0..keep - 1 are
  * filled and few rows move; order among slots means nothing to attention, the
  * keys being rotated already. K and V move in the cache; weight_out and

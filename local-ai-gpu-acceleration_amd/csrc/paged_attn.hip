@@ -619,9 +619,16 @@ AttnArgs attn_args(const float* q, const std::uint32_t* pos, float* out, void* w
   return a;
 }
 
-bool attn_pointers_ok(const float* q, const std::uint32_t* pos, const float* out, const void* workspace) {
+// out is q itself (a workgroup has read its heads before it writes them) or shares no memory with it.
+bool attn_pointers_ok(const float* q, const std::uint32_t* pos, const float* out, const void* workspace,
+                      std::uint64_t rows_bytes) {
   return q != nullptr && pos != nullptr && out != nullptr && workspace != nullptr && aligned_to(q, 4u) &&
-         aligned_to(pos, 4u) && aligned_to(out, 4u) && aligned_to(workspace, 256u);
+         aligned_to(pos, 4u) && aligned_to(out, 4u) && aligned_to(workspace, 256u) &&
+         (out == q || !overlap(out, rows_bytes, q, rows_bytes));
+}
+
+std::uint64_t rows_bytes(const rtxllm_paged_kv* cache, std::uint32_t n_heads, std::uint32_t count) {
+  return 4ull * count * n_heads * cache->head_dim;
 }
 
 }  // namespace
@@ -640,7 +647,7 @@ extern "C" hipError_t rtxllm_attn_decode_pages_gqa_f16(const rtxllm_paged_kv* ca
                                                        uint32_t count, float* out, void* workspace,
                                                        size_t workspace_bytes, hipStream_t stream) {
   if (cache == nullptr || pages == nullptr || !aligned_to(pages, 4u) || n_select == 0u || n_select > 65536u ||
-      !attn_pointers_ok(q, pos, out, workspace))
+      !attn_pointers_ok(q, pos, out, workspace, rows_bytes(cache, n_heads, count)))
     return hipErrorInvalidValue;
   const AttnSpace s = attn_space(cache, n_heads, static_cast<std::uint64_t>(n_select) * cache->page_size, count, false);
   if (s.bytes == 0u || workspace_bytes < s.bytes) return hipErrorInvalidValue;
@@ -663,7 +670,7 @@ extern "C" hipError_t rtxllm_attn_decode_weights_gqa_f16(const rtxllm_paged_kv* 
                                                          float* out, const float* weight, float* weight_out,
                                                          void* workspace, size_t workspace_bytes, hipStream_t stream) {
   if (cache == nullptr || weight == nullptr || weight_out == nullptr || !aligned_to(weight, 4u) ||
-      !aligned_to(weight_out, 4u) || !attn_pointers_ok(q, last, out, workspace) ||
+      !aligned_to(weight_out, 4u) || !attn_pointers_ok(q, last, out, workspace, rows_bytes(cache, n_heads, count)) ||
       (cache->table_stride == 0u && count > 1u))
     return hipErrorInvalidValue;
   const AttnSpace s = attn_space(cache, n_heads, cache->capacity, count, true);

@@ -435,13 +435,11 @@ __global__ __launch_bounds__(T) void page_choice_kernel(PagedView kv, const std:
 }
 
 // A weight as an unsigned key of the same order, 0 for NaN; protected slots above
-// every weight.
-__device__ __forceinline__ std::uint32_t weight_key(float w, std::uint32_t p, std::uint32_t newest,
-                                                    std::uint32_t n_first, std::uint32_t n_recent) {
-  if (p < n_first || static_cast<std::uint64_t>(p) + n_recent > newest) return 0xFFFFFFFFu;
-  if (w != w) return 0u;
+// every weight. The positions from n_first on that are not protected are `open` many.
+__device__ __forceinline__ std::uint32_t weight_key(float w, std::uint32_t p, std::uint32_t n_first, std::uint32_t open) {
   const std::uint32_t b = __float_as_uint(w + 0.0f);
-  return (b >> 31) != 0u ? ~b : b | 0x80000000u;
+  const std::uint32_t key = b ^ (static_cast<std::uint32_t>(static_cast<std::int32_t>(b) >> 31) | 0x80000000u);
+  return p - n_first >= open ? 0xFFFFFFFFu : w != w ? 0u : key;
 }
 
 // The moves of one (sequence, kv head): moves[0] of them, then their destination
@@ -461,7 +459,7 @@ struct SlotKeys {
   const std::uint32_t* p;
   float* wo;
   std::uint32_t* po;
-  std::uint32_t n, stay, newest, n_first, n_recent;
+  std::uint32_t n, stay, n_first, open;
   struct Raw {
     f32x4_any w;
     u32x4_any p;
@@ -480,10 +478,15 @@ struct SlotKeys {
   }
   __device__ __forceinline__ void keys(std::uint32_t i, const Raw& v, std::uint32_t (&x)[4]) const {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) x[e] = i + e < n ? weight_key(v.w[e], v.p[e], newest, n_first, n_recent) : 0u;
+    for (int e = 0; e < 4; ++e) x[e] = weight_key(v.w[e], v.p[e], n_first, open);
+    if (__ballot(i + 4u > n) == 0ull) return;
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (i + e >= n) x[e] = 0u;
   }
   // copies the slots below `stay`, unless they lie there already
   __device__ __forceinline__ void seen(std::uint32_t i, const Raw& v) const {
+    if (__ballot(i < stay) == 0ull) return;
     if (i + 4u <= stay) {
       if (wo != w) *reinterpret_cast<f32x4_any*>(wo + i) = v.w;
       if (po != p) *reinterpret_cast<u32x4_any*>(po + i) = v.p;
@@ -530,8 +533,10 @@ __global__ __launch_bounds__(T) void evict_choice_kernel(PagedView kv, EvictArgs
     return;
   }
   if (L != 0 && g == 0u && tid == 0u) length_out[r] = n < a.keep ? n : a.keep;
+  const std::uint32_t recent = newest >= a.n_recent ? newest - a.n_recent + 1u : 0u;  // the first such position
   const SlotKeys src{a.weight + gr * kv.capacity, a.slot_pos + gr * kv.capacity, a.weight_out + gr * kv.capacity,
-                     a.slot_pos_out + gr * kv.capacity, n, n < a.keep ? n : a.keep, newest, a.n_first, a.n_recent};
+                     a.slot_pos_out + gr * kv.capacity, n, n < a.keep ? n : a.keep, a.n_first,
+                     recent > a.n_first ? recent - a.n_first : 0u};
   if (n <= a.keep || n > a.room)
     for (std::uint32_t i = 4u * tid; i < src.stay; i += 4u * T) src.seen(i, src.raw(i));
   if (n <= a.keep) {
@@ -675,7 +680,9 @@ extern "C" hipError_t rtxllm_kv_evict_f16(const rtxllm_paged_kv* cache, const ui
   if ((weight_out != weight && overlap(weight_out, n, weight, n)) || overlap(weight_out, n, slot_pos, n) ||
       (slot_pos_out != slot_pos && overlap(slot_pos_out, n, slot_pos, n)) || overlap(slot_pos_out, n, weight, n) ||
       overlap(weight_out, n, slot_pos_out, n) || (length_out != length && overlap(length_out, 4u * count, length, 4u * count)) ||
-      overlap(length_out, 4u * count, pos, 4u * count))
+      overlap(length_out, 4u * count, pos, 4u * count) || overlap(length_out, 4u * count, weight, n) ||
+      overlap(length_out, 4u * count, slot_pos, n) || overlap(length_out, 4u * count, weight_out, n) ||
+      overlap(length_out, 4u * count, slot_pos_out, n))
     return hipErrorInvalidValue;
   const PagedView view = paged_view(cache);
   const std::uint32_t most = most_moves(cache, keep), per = kThreads / (cache->head_dim / 8u);

@@ -89,7 +89,9 @@ def evict(length, newest, keep, n_first, n_recent, weight, slot_pos):
     def rank(i):
         p, w = int(slot_pos[i]), float(weight[i])
         protected = p < n_first or p + n_recent > newest
-        return (not protected, np.isnan(w), 0.0 if np.isnan(w) else -w, i)
+        if protected:  # all alike
+            return (0, 0.0, i)
+        return (2, 0.0, i) if np.isnan(w) else (1, -w, i)
     kept = set(sorted(range(length), key=rank)[:keep])
     late = iter(sorted(i for i in kept if i >= keep))
     return [i if i in kept else next(late) for i in range(keep)]

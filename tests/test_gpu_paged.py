@@ -283,6 +283,10 @@ def test_attn_pages(group, kv, dim, page, select):
         for g in range(kv if n else 0):
             listed = [t for t in pages[i, g] if 0 <= t < s.entries]
             check_attention(s, got, q, i, g, group, [x for t in listed for x in range(t * page, min(n, t * page + page))])
+    over = dev(q)  # the queries make way for the results
+    paged.attn_pages(s.cache, over, dev(pages), u32(s.last()), out=over)
+    got[1] = q[1]
+    np.testing.assert_array_equal(over.cpu().numpy(), got)
 
 
 def test_attn_pages_empty_twice_and_extremes():
@@ -386,6 +390,22 @@ def test_evict(kv, dim, page, keep, first, recent, place):
     np.testing.assert_array_equal(gw, w_want)
     np.testing.assert_array_equal(s.kd.cpu().numpy().view(np.uint16), k_want.view(np.uint16))
     np.testing.assert_array_equal(s.vd.cpu().numpy().view(np.uint16), v_want.view(np.uint16))
+
+
+@pytest.mark.parametrize("newest", [0, 6, 80, 2**32 - 2])
+@pytest.mark.parametrize("first,recent", [(0, 0), (5, 0), (0, 7), (20, 30)])
+def test_evict_protected_positions(newest, first, recent):
+    """Newest positions below n_recent, between the slots' own, and the largest one."""
+    s = Setup(newest % 97 + first, [100], 2, 64, 8)
+    weight = s.rng.standard_normal((1, 2, s.capacity)).astype(np.float32)
+    at = [0, 1, 4, 5, 6, 7, 50, 51, 73, 74, 80, 81, 2**31, 2**32 - 10, 2**32 - 9, 2**32 - 2, 2**32 - 1]
+    slot_pos = s.rng.choice(at, (1, 2, s.capacity)).astype(np.uint32)
+    wd, sd = dev(weight), u32(slot_pos)
+    paged.evict(s.cache, u32([100]), u32([newest]), 60, wd, sd, first, recent)
+    for g in range(2):
+        src = ref.evict(100, newest, 60, first, recent, weight[0, g], slot_pos[0, g])
+        np.testing.assert_array_equal(wd.cpu().numpy()[0, g, :60], weight[0, g, src])
+        np.testing.assert_array_equal(sd.cpu().numpy()[0, g, :60].view(np.uint32), slot_pos[0, g, src])
 
 
 @pytest.mark.parametrize("n,keep", [(32768, 100), (32769, 32768), (70001, 40000)])

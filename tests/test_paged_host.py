@@ -71,16 +71,16 @@ BAD = {
     "rtxllm_attn_decode_pages_gqa_f16": [
         dict(q=None), dict(pages=None), dict(pos=None), dict(out=None), dict(workspace=None), dict(out=ptr(3) + 2),
         dict(workspace=ptr(4) + 8), dict(workspace_bytes=1024), dict(n_heads=5), dict(n_heads=34), dict(count=0),
-        dict(count=65536), dict(n_select=0), dict(n_select=65537)],
+        dict(count=65536), dict(n_select=0), dict(n_select=65537), dict(out=ptr(0) + 512), dict(out=ptr(0) - 512)],
     "rtxllm_attn_decode_weights_gqa_f16": [
         dict(q=None), dict(last=None), dict(out=None), dict(weight=None), dict(weight_out=None), dict(workspace=None),
-        dict(weight_out=ptr(3) + 4), dict(weight=ptr(3) + 1), dict(workspace_bytes=4096), dict(n_heads=7), dict(count=0)],
+        dict(weight_out=ptr(3) + 4), dict(weight=ptr(3) + 1), dict(out=ptr(0) + 512), dict(workspace_bytes=4096), dict(n_heads=7), dict(count=0)],
     "rtxllm_kv_evict_f16": [
         dict(length=None), dict(pos=None), dict(weight=None), dict(slot_pos=None), dict(weight_out=None),
         dict(slot_pos_out=None), dict(length_out=None), dict(workspace=None), dict(workspace_bytes=16),
         dict(workspace=ptr(7) + 4), dict(keep=0), dict(keep=129), dict(n_first=60), dict(n_recent=0xFFFFFFFF),
         dict(weight_out=ptr(2) + 16), dict(weight_out=ptr(3)), dict(slot_pos_out=ptr(2)), dict(slot_pos_out=ptr(4)),
-        dict(length_out=ptr(1)), dict(length_out=ptr(0) + 4), dict(pos=ptr(1) + 1), dict(count=0), dict(count=65536)],
+        dict(length_out=ptr(1)), dict(length_out=ptr(0) + 4), dict(length_out=ptr(2)), dict(length_out=ptr(5) + 8), dict(pos=ptr(1) + 1), dict(count=0), dict(count=65536)],
 }
 
 
