@@ -193,8 +193,8 @@ __device__ __forceinline__ void count_digits(std::uint32_t* hist, Digit digit_of
 // reads them; of more, every pass reads all again (from the L2). The loops over them are
 // rolled: each runs a few rounds once, and unrolled code with the keys in registers
 // took longer to fetch (32 keys a thread: 92 us for 32768 keys). src.raw(i) loads what
-// keys i..i + 3 (i % 4 == 0) are made of, src.keys(i, raw, x) makes them, src.seen(i, raw)
-// is called for each once, where they go into the LDS.
+// keys i..i + 3 (i % 4 == 0) are made of, src.keys(i, raw, x) makes them (<true>: all four
+// are there), src.seen(i, raw) is called for each once, where they go into the LDS.
 template <class K, class Source, std::uint32_t T>
 struct Keys {
   struct alignas(16) Four {
@@ -216,22 +216,24 @@ struct Keys {
       *reinterpret_cast<uint4*>(hist + i) = make_uint4(0u, 0u, 0u, 0u);
     __syncthreads();
     if (!in_lds) return;
-    auto take = [&](std::uint32_t at, std::uint32_t round, const decltype(src.raw(0u))& v) {
+    using Raw = decltype(src.template raw<true>(0u));
+    auto take = [&](auto full, std::uint32_t round, const Raw& v) {
+      const std::uint32_t at = place(round);
       Four f;
       src.seen(at, v);
-      src.keys(at, v, f.k);
+      src.template keys<decltype(full)::value>(at, v, f.k);
       held[T * round] = f;
       count_digits(hist, [&](int e) { return static_cast<std::uint32_t>(f.k[e] >> (8 * sizeof(K) - kDigit)); });
     };
     std::uint32_t j = 0;
-    for (; j + 4u <= rounds; j += 4u) {  // four rounds' loads in flight
-      decltype(src.raw(0u)) v[4];
+    for (; j + 4u <= rounds && first + 256u * (j + 4u) <= n; j += 4u) {  // four rounds' loads in flight
+      Raw v[4];
 #pragma unroll
-      for (std::uint32_t u = 0; u < 4u; ++u) v[u] = src.raw(place(j + u));
+      for (std::uint32_t u = 0; u < 4u; ++u) v[u] = src.template raw<true>(place(j + u));
 #pragma unroll
-      for (std::uint32_t u = 0; u < 4u; ++u) take(place(j + u), j + u, v[u]);
+      for (std::uint32_t u = 0; u < 4u; ++u) take(std::true_type{}, j + u, v[u]);
     }
-    for (; j < rounds; ++j) take(place(j), j, src.raw(place(j)));
+    for (; j < rounds; ++j) take(std::false_type{}, j, src.template raw<false>(place(j)));
   }
   __device__ __forceinline__ std::uint32_t place(std::uint32_t j) const {
     return first + 256u * j + 4u * (threadIdx.x & 63u);
@@ -244,7 +246,7 @@ struct Keys {
       if (in_lds)
         f = held[T * j];
       else
-        src.keys(place(j), src.raw(place(j)), f.k);
+        src.template keys<false>(place(j), src.template raw<false>(place(j)), f.k);
       body(f.k, place(j));
     }
   }
@@ -390,9 +392,10 @@ typedef unsigned long long u64x4 __attribute__((ext_vector_type(4), aligned(8)))
 struct KeyRow {
   const unsigned long long* row;
   std::uint32_t n;
+  template <bool FULL>
   __device__ __forceinline__ u64x4 raw(std::uint32_t i) const {
     u64x4 v = {0ull, 0ull, 0ull, 0ull};
-    if (i + 4u <= n) {
+    if (FULL || i + 4u <= n) {
       v = *reinterpret_cast<const u64x4*>(row + i);
     } else {
 #pragma unroll
@@ -402,6 +405,7 @@ struct KeyRow {
     return v;
   }
   __device__ __forceinline__ void seen(std::uint32_t, const u64x4&) const {}
+  template <bool>
   __device__ __forceinline__ void keys(std::uint32_t, const u64x4& v, unsigned long long (&x)[4]) const {
 #pragma unroll
     for (int e = 0; e < 4; ++e) x[e] = v[e];
@@ -464,9 +468,10 @@ struct SlotKeys {
     f32x4_any w;
     u32x4_any p;
   };
+  template <bool FULL>
   __device__ __forceinline__ Raw raw(std::uint32_t i) const {
     Raw v{{0.0f, 0.0f, 0.0f, 0.0f}, {0u, 0u, 0u, 0u}};
-    if (i + 4u <= n) {
+    if (FULL || i + 4u <= n) {
       v.w = *reinterpret_cast<const f32x4_any*>(w + i);
       v.p = *reinterpret_cast<const u32x4_any*>(p + i);
     } else {
@@ -476,10 +481,11 @@ struct SlotKeys {
     }
     return v;
   }
+  template <bool FULL>
   __device__ __forceinline__ void keys(std::uint32_t i, const Raw& v, std::uint32_t (&x)[4]) const {
 #pragma unroll
     for (int e = 0; e < 4; ++e) x[e] = weight_key(v.w[e], v.p[e], n_first, open);
-    if (__ballot(i + 4u > n) == 0ull) return;
+    if (FULL || __ballot(i + 4u > n) == 0ull) return;
 #pragma unroll
     for (int e = 0; e < 4; ++e)
       if (i + e >= n) x[e] = 0u;
@@ -538,7 +544,7 @@ __global__ __launch_bounds__(T) void evict_choice_kernel(PagedView kv, EvictArgs
                      a.slot_pos_out + gr * kv.capacity, n, n < a.keep ? n : a.keep, a.n_first,
                      recent > a.n_first ? recent - a.n_first : 0u};
   if (n <= a.keep || n > a.room)
-    for (std::uint32_t i = 4u * tid; i < src.stay; i += 4u * T) src.seen(i, src.raw(i));
+    for (std::uint32_t i = 4u * tid; i < src.stay; i += 4u * T) src.seen(i, src.raw<false>(i));
   if (n <= a.keep) {
     if (tid == 0u) moves[0] = 0u;
     return;
