@@ -310,12 +310,18 @@ __device__ Choice<K> radix_choice(SelectShared<T>& sh, const Keys<K, Source, T>&
   }
 }
 
-// Walks the choice: freed(i, rank) for each key below `split` that is not chosen, kept(i,
-// rank) for each chosen one at or behind it, rank counting those of the same kind before
-// it. Returns the number of both.
-template <class K, class Source, std::uint32_t T, class Freed, class Kept>
+// A list of indices, `most` at most (a round that would pass them, which keys that change
+// meanwhile could make, is dropped whole).
+struct Places {
+  std::uint32_t* to;
+  std::uint32_t most;
+};
+
+// Walks the choice: the keys below `split` that are not chosen go into `freed`, the chosen ones
+// at or behind it into `kept`, both in order. Returns the number of both.
+template <class K, class Source, std::uint32_t T>
 __device__ uint2 for_choice(SelectShared<T>& sh, const Keys<K, Source, T>& keys, const Choice<K>& ch, std::uint32_t split,
-                            Freed freed, Kept kept) {
+                            Places freed, Places kept) {
   const std::uint32_t tid = threadIdx.x, lane = tid & 63u, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const bool all = ch.ties == kAllTies;
   std::uint32_t ties_before = 0;
@@ -364,14 +370,15 @@ __device__ uint2 for_choice(SelectShared<T>& sh, const Keys<K, Source, T>& keys,
   const uint2 wf = waves_before<T>(sh.wave[1], wave), wk = waves_before<T>(sh.wave[2], wave);
   std::uint32_t at_f = wf.x, at_k = wk.x;
   ties = ties_before;
-  auto put = [&](std::uint32_t bits, std::uint32_t i, std::uint32_t& at, auto& to) {
+  auto put = [&](std::uint32_t bits, std::uint32_t i, std::uint32_t& at, const Places& list) {
     if (__ballot(bits != 0u) == 0ull) return;
     const std::uint32_t own = static_cast<std::uint32_t>(__popc(bits)), upto = wave_scan(own);
     std::uint32_t rank = at + upto - own;
     at += __builtin_amdgcn_readlane(upto, 63);
+    if (at > list.most) return;
 #pragma unroll
     for (std::uint32_t e = 0; e < 4u; ++e)
-      if ((bits >> e & 1u) != 0u) to(i + e, rank++);
+      if ((bits >> e & 1u) != 0u) list.to[rank++] = i + e;
   };
   keys.each([&](const K (&x)[4], std::uint32_t i) {
     const Kinds s = kinds(x, i, ties);
@@ -430,11 +437,8 @@ __global__ __launch_bounds__(T) void page_choice_kernel(PagedView kv, const std:
   Choice<unsigned long long> ch{1ull, kAllTies};
   if (n_select < used) ch = radix_choice(sh, keys, n_select);
   if (ch.least == 0ull) ch = Choice<unsigned long long>{1ull, kAllTies};
-  const std::uint32_t listed = for_choice(
-      sh, keys, ch, 0u, [](std::uint32_t, std::uint32_t) {},
-      [&](std::uint32_t i, std::uint32_t rank) {
-        if (rank < n_select) out[rank] = static_cast<std::int32_t>(i);
-      }).y;
+  const std::uint32_t listed =
+      for_choice(sh, keys, ch, 0u, Places{nullptr, 0u}, Places{reinterpret_cast<std::uint32_t*>(out), n_select}).y;
   for (std::uint32_t i = listed + threadIdx.x; i < n_select; i += T) out[i] = -1;
 }
 
@@ -510,6 +514,7 @@ struct SlotKeys {
 template <int L>
 __device__ __forceinline__ void move_row(const PagedView& kv, const EvictArgs& a, std::uint32_t r, std::uint32_t g,
                                          std::uint32_t to_slot, std::uint32_t from_slot, std::uint32_t t) {
+  if (to_slot >= kv.capacity || from_slot >= kv.capacity) return;  // (weights that changed meanwhile)
   const std::int32_t* const table = kv.table + static_cast<std::size_t>(r) * kv.table_stride;
   const std::size_t state = (static_cast<std::size_t>(r) * kv.n_kv + g) * kv.capacity;
   const std::uint32_t to = paged_slot_row(kv, table, g, to_slot), from = paged_slot_row(kv, table, g, from_slot);
@@ -553,14 +558,7 @@ __global__ __launch_bounds__(T) void evict_choice_kernel(PagedView kv, EvictArgs
   const Choice<std::uint32_t> ch = radix_choice(sh, keys, a.keep);
   std::uint32_t* const to = moves + 1u;
   std::uint32_t* const from = to + a.most;
-  const std::uint32_t freed = for_choice(
-      sh, keys, ch, a.keep,
-      [&](std::uint32_t i, std::uint32_t m) {
-        if (m < a.most) to[m] = i;
-      },
-      [&](std::uint32_t i, std::uint32_t m) {
-        if (m < a.most) from[m] = i;
-      }).x;
+  const std::uint32_t freed = for_choice(sh, keys, ch, a.keep, Places{to, a.most}, Places{from, a.most}).x;
   const std::uint32_t n_moves = freed < a.most ? freed : a.most;
   if constexpr (L == 0) {
     if (tid == 0u) moves[0] = n_moves;
