@@ -531,8 +531,12 @@ __global__ __launch_bounds__(kThreads) void merge_weights_kernel(AttnArgs a, Pag
 //   11.8 / 15.9 / 23.9, 65536 of one 88 / 68 / 58 / 53 / 51, up to 4096 of eight 31.1 / 25.9 / 23.3 /
 //   26.0 / 27.2, up to 16384 of eight 100 / 78 / 71 / 70 / 66;
 // - listed: 4096 positions of eight 39.6 / 32.0 / 29.1 / 27.9 / 24.7.
-std::uint32_t attn_per(std::uint64_t items, std::uint64_t positions, bool whole) {
+// A short list is one workgroup's, which saves the merge's launch: 128 positions 7.2 us at 4 tiles,
+// 5.4 at 8 (8 heads a kv head of 256 10.3 / 9.1), 256 positions 7.5 at 4, 7.2 at 16 (64 heads of 64 7.5 /
+// 7.1; but 5 heads a kv head of 256 10.6 / 13.4, 12 of 128 8.9 / 9.2), 512 7.9 at 4, 10.9 at 32.
+std::uint32_t attn_per(std::uint64_t items, std::uint64_t positions, bool whole, bool light) {
   const std::uint64_t tiles = (positions + kTile - 1u) / kTile;
+  if (!whole && tiles <= (light ? 16u : 8u)) return tiles <= 8u ? 8u : 16u;
   std::uint32_t per = kMaxPer;
   for (; per > kWaves; per /= 2u) {
     const std::uint64_t splits = (tiles + per - 1u) / per;
@@ -553,7 +557,8 @@ AttnSpace attn_space(const rtxllm_paged_kv* c, std::uint32_t n_heads, std::uint6
   if (!paged_cache_ok(c, count) || count == 0u || count > 65535u || c->n_kv_heads > 65535u ||
       paged_group(c, n_heads) == 0u || positions == 0u || positions > (1ull << 30))
     return s;
-  s.per = attn_per(static_cast<std::uint64_t>(count) * c->n_kv_heads, positions, weights);
+  s.per = attn_per(static_cast<std::uint64_t>(count) * c->n_kv_heads, positions, weights,
+                   c->head_dim < 256u && paged_group(c, n_heads) <= 8u);
   s.splits = static_cast<std::uint32_t>((positions + kTile * s.per - 1u) / (kTile * s.per));
   if (static_cast<std::uint64_t>(s.splits) * c->n_kv_heads > (1u << 23)) return s;  // the launch's thread count
   const std::size_t records = static_cast<std::size_t>(count) * n_heads * s.splits;
