@@ -531,6 +531,10 @@ __global__ __launch_bounds__(kThreads) void merge_weights_kernel(AttnArgs a, Pag
 //   11.8 / 15.9 / 23.9, 65536 of one 88 / 68 / 58 / 53 / 51, up to 4096 of eight 31.1 / 25.9 / 23.3 /
 //   26.0 / 27.2, up to 16384 of eight 100 / 78 / 71 / 70 / 66;
 // - listed: 4096 positions of eight 39.6 / 32.0 / 29.1 / 27.9 / 24.7.
+// 8 tiles already where 4 would make more workgroups than CUs, 16 where they make 160 (workgroups
+// at 8, us at 4 / 8: 128 8.3 / 9.0, 160 12.4 / 11.3, 192 10.1 / 9.4, 132 of 16 heads of 256 30.7 / 21.3;
+// at 16, us at 8 / 16: 156 9.9 / 11.4, 160 11.8 / 11.2, 208 12.5 / 12.0, 208 of 8 heads a kv head of 256
+// 21.8 / 19.2; at 32, us at 16 / 32: 192 of 64 15.1 / 17.0).
 // A short list is one workgroup's, which saves the merge's launch: 128 positions 7.2 us at 4 tiles,
 // 5.4 at 8 (8 heads a kv head of 256 10.3 / 9.1), 256 positions 7.5 at 4, 7.2 at 16 (64 heads of 64 7.5 /
 // 7.1; but 5 heads a kv head of 256 10.6 / 13.4, 12 of 128 8.9 / 9.2), 512 7.9 at 4, 10.9 at 32.
@@ -539,8 +543,8 @@ std::uint32_t attn_per(std::uint64_t items, std::uint64_t positions, bool whole,
   if (!whole && tiles <= (light ? 16u : 8u)) return tiles <= 8u ? 8u : 16u;
   std::uint32_t per = kMaxPer;
   for (; per > kWaves; per /= 2u) {
-    const std::uint64_t splits = (tiles + per - 1u) / per;
-    if (items * splits >= 256u && (!whole || per <= 16u || splits >= 16u)) break;
+    const std::uint64_t splits = (tiles + per - 1u) / per, enough = per == 8u ? 129u : per == 16u ? 160u : 256u;
+    if (items * splits >= enough && (!whole || per <= 16u || splits >= 16u)) break;
   }
   return per;
 }
