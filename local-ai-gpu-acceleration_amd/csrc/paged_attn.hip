@@ -33,6 +33,32 @@ __device__ __forceinline__ std::uint32_t from_lane(std::uint32_t v, std::uint32_
   return static_cast<std::uint32_t>(__builtin_amdgcn_ds_bpermute(static_cast<int>(4u * lane), static_cast<int>(v)));
 }
 
+// Tiles of a split (one workgroup), of at most `tiles`. Of one size for every row,
+// so that a longer context is more workgroups; the largest of 4 to 64 that leaves a
+// workgroup for each CU, as a wave's prologue and the merge cost what two or three
+// tiles do; over whole contexts, whose lengths differ, more than 16 only where the longest
+// still makes 16 of them. us at 4 / 8 / 16 / 32 / 64 tiles, 32 heads over 8 kv heads of 128
+// - whole: 1024 slots of one sequence 7.9 / 8.8 / 10.7 / 14.5 / 22.1, 4001 of one 10.9 / 10.0 /
+//   11.8 / 15.9 / 23.9, 65536 of one 88 / 68 / 58 / 53 / 51, up to 4096 of eight 31.1 / 25.9 / 23.3 /
+//   26.0 / 27.2, up to 16384 of eight 100 / 78 / 71 / 70 / 66;
+// - listed: 4096 positions of eight 39.6 / 32.0 / 29.1 / 27.9 / 24.7.
+// 8 tiles already where 4 would make more workgroups than CUs, 16 where they make 160 (workgroups
+// at 8, us at 4 / 8: 128 8.3 / 9.0, 160 12.4 / 11.3, 192 10.1 / 9.4, 132 of 16 heads of 256 30.7 / 21.3;
+// at 16, us at 8 / 16: 156 9.9 / 11.4, 160 11.8 / 11.2, 208 12.5 / 12.0, 208 of 8 heads a kv head of 256
+// 21.8 / 19.2; at 32, us at 16 / 32: 192 of 64 15.1 / 17.0).
+// A short list is one workgroup's, which saves the merge's launch: 128 positions 7.2 us at 4 tiles,
+// 5.4 at 8 (8 heads a kv head of 256 10.3 / 9.1), 256 positions 7.5 at 4, 7.2 at 16 (64 heads of 64 7.5 /
+// 7.1; but 5 heads a kv head of 256 10.6 / 13.4, 12 of 128 8.9 / 9.2), 512 7.9 at 4, 10.9 at 32.
+RTXLLM_HD std::uint32_t attn_per(std::uint64_t items, std::uint64_t tiles, bool whole, bool light) {
+  if (!whole && tiles <= (light ? 16u : 8u)) return tiles <= 8u ? 8u : 16u;
+  std::uint32_t per = kMaxPer;
+  for (; per > kWaves; per /= 2u) {
+    const std::uint64_t splits = (tiles + per - 1u) / per, enough = per == 8u ? 129u : per == 16u ? 160u : 256u;
+    if (items * splits >= enough && (!whole || per <= 16u || splits >= 16u)) break;
+  }
+  return per;
+}
+
 // One workgroup of four waves per (split, kv head, row); a wave takes tiles of 16
 // positions of its split in turn, with a running maximum and sum for every head:
 //  * scores: S = K q^T by v_mfma_f32_16x16x32_f16. A = the K rows as stored (lane:
@@ -97,7 +123,7 @@ __global__ __launch_bounds__(kThreads, (attn_waves<D, T, WEIGHTS>())) void paged
     const auto lp = static_cast<std::uint32_t>(e);
     return table[lp < kv.entries ? lp : kv.entries - 1u];
   };
-  const std::uint32_t tile0 = split * a.per + wave;
+  std::uint32_t per = a.per, tile0 = split * per + wave;
   // the list's first 64 entries, a lane each, for its length below
   const std::int32_t listed = WEIGHTS ? 0 : list[lane < a.n_select ? lane : 0u];
   entry = load_entry(tile0);
@@ -160,7 +186,20 @@ __global__ __launch_bounds__(kThreads, (attn_waves<D, T, WEIGHTS>())) void paged
     }
   }
   const std::uint32_t tiles = (total + kTile - 1u) / kTile;
-  if (split * a.per >= tiles) {  // nothing of the row is here
+  if constexpr (!WEIGHTS) {
+    // A list that ends early (a context shorter than what it has room for) is split anew,
+    // into at most as many parts (9997 positions of four, lists of 120 pages of 256: 37.9 -> 22.1
+    // us; one of 600, 1024 pages of 16: 15.8 -> 10.3).
+    if (a.splits > 1u && 2u * tiles <= a.per * a.splits) {
+      per = attn_per(static_cast<std::uint64_t>(gridDim.y) * kv.n_kv, tiles, false, D < 256 && !WIDE);
+      while (per * a.splits < tiles) per *= 2u;
+      tile0 = split * per + wave;
+      entry = load_entry(tile0);
+      entry_next = load_entry(tile0 + kWaves);
+      page = load_page(entry);
+    }
+  }
+  if (split * per >= tiles) {  // nothing of the row is here
     if constexpr (!WEIGHTS) {
       for (std::uint32_t i = threadIdx.x; i < a.group * D; i += kThreads) {
         if (a.splits == 1u)
@@ -173,7 +212,7 @@ __global__ __launch_bounds__(kThreads, (attn_waves<D, T, WEIGHTS>())) void paged
     }
     return;
   }
-  const std::uint32_t tile1 = split * a.per + a.per < tiles ? split * a.per + a.per : tiles;
+  const std::uint32_t tile1 = split * per + per < tiles ? split * per + per : tiles;
 
   float m = -INFINITY, l = 0.0f;
   f32x4 o[WIDE ? 1 : T][VD];
@@ -522,33 +561,6 @@ __global__ __launch_bounds__(kThreads) void merge_weights_kernel(AttnArgs a, Pag
   }
 }
 
-// Tiles of a split (one workgroup), of at most `positions`. Of one size for every row,
-// so that a longer context is more workgroups; the largest of 4 to 64 that leaves a
-// workgroup for each CU, as a wave's prologue and the merge cost what two or three
-// tiles do; over whole contexts, whose lengths differ, more than 16 only where the longest
-// still makes 16 of them. us at 4 / 8 / 16 / 32 / 64 tiles, 32 heads over 8 kv heads of 128
-// - whole: 1024 slots of one sequence 7.9 / 8.8 / 10.7 / 14.5 / 22.1, 4001 of one 10.9 / 10.0 /
-//   11.8 / 15.9 / 23.9, 65536 of one 88 / 68 / 58 / 53 / 51, up to 4096 of eight 31.1 / 25.9 / 23.3 /
-//   26.0 / 27.2, up to 16384 of eight 100 / 78 / 71 / 70 / 66;
-// - listed: 4096 positions of eight 39.6 / 32.0 / 29.1 / 27.9 / 24.7.
-// 8 tiles already where 4 would make more workgroups than CUs, 16 where they make 160 (workgroups
-// at 8, us at 4 / 8: 128 8.3 / 9.0, 160 12.4 / 11.3, 192 10.1 / 9.4, 132 of 16 heads of 256 30.7 / 21.3;
-// at 16, us at 8 / 16: 156 9.9 / 11.4, 160 11.8 / 11.2, 208 12.5 / 12.0, 208 of 8 heads a kv head of 256
-// 21.8 / 19.2; at 32, us at 16 / 32: 192 of 64 15.1 / 17.0).
-// A short list is one workgroup's, which saves the merge's launch: 128 positions 7.2 us at 4 tiles,
-// 5.4 at 8 (8 heads a kv head of 256 10.3 / 9.1), 256 positions 7.5 at 4, 7.2 at 16 (64 heads of 64 7.5 /
-// 7.1; but 5 heads a kv head of 256 10.6 / 13.4, 12 of 128 8.9 / 9.2), 512 7.9 at 4, 10.9 at 32.
-std::uint32_t attn_per(std::uint64_t items, std::uint64_t positions, bool whole, bool light) {
-  const std::uint64_t tiles = (positions + kTile - 1u) / kTile;
-  if (!whole && tiles <= (light ? 16u : 8u)) return tiles <= 8u ? 8u : 16u;
-  std::uint32_t per = kMaxPer;
-  for (; per > kWaves; per /= 2u) {
-    const std::uint64_t splits = (tiles + per - 1u) / per, enough = per == 8u ? 129u : per == 16u ? 160u : 256u;
-    if (items * splits >= enough && (!whole || per <= 16u || splits >= 16u)) break;
-  }
-  return per;
-}
-
 struct AttnSpace {
   std::uint32_t per = 0, splits = 0, score_stride = 0;
   std::size_t ml = 0, part = 0, scores = 0;  // byte offsets past the start
@@ -561,7 +573,7 @@ AttnSpace attn_space(const rtxllm_paged_kv* c, std::uint32_t n_heads, std::uint6
   if (!paged_cache_ok(c, count) || count == 0u || count > 65535u || c->n_kv_heads > 65535u ||
       paged_group(c, n_heads) == 0u || positions == 0u || positions > (1ull << 30))
     return s;
-  s.per = attn_per(static_cast<std::uint64_t>(count) * c->n_kv_heads, positions, weights,
+  s.per = attn_per(static_cast<std::uint64_t>(count) * c->n_kv_heads, (positions + kTile - 1u) / kTile, weights,
                    c->head_dim < 256u && paged_group(c, n_heads) <= 8u);
   s.splits = static_cast<std::uint32_t>((positions + kTile * s.per - 1u) / (kTile * s.per));
   if (static_cast<std::uint64_t>(s.splits) * c->n_kv_heads > (1u << 23)) return s;  // the launch's thread count

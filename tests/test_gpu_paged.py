@@ -289,6 +289,26 @@ def test_attn_pages(group, kv, dim, page, select):
     np.testing.assert_array_equal(over.cpu().numpy(), got)
 
 
+@pytest.mark.parametrize("group,kv,dim", [(4, 2, 64), (1, 8, 128), (8, 1, 256), (12, 2, 128), (2, 16, 128)])
+@pytest.mark.parametrize("select", [60, 600])
+def test_attn_pages_lists_longer_than_the_context(group, kv, dim, select):
+    """Room for far more pages than are listed: rows of few tiles, one of many whose list
+    names pages again and again to its end."""
+    page, lens = 16, [700, 0, 1, 90, 130]
+    s = Setup(group + dim + select, lens, kv, dim, page)
+    q = s.rng.standard_normal((5, group * kv, dim)).astype(np.float32)
+    pages = np.full((5, kv, select), -1, np.int32)
+    for i, n in enumerate(lens):
+        used = -(-n // page)
+        pages[i, :, :used] = s.rng.permutation(used)
+    pages[4, :, ::2] = s.rng.integers(0, 9, (kv, -(-select // 2)))
+    got = paged.attn_pages(s.cache, dev(q), dev(pages), u32(s.last())).cpu().numpy()
+    for i, n in enumerate(lens):
+        for g in range(kv if n else 0):
+            listed = [t for t in pages[i, g] if 0 <= t < s.entries]
+            check_attention(s, got, q, i, g, group, [x for t in listed for x in range(t * page, min(n, t * page + page))])
+
+
 def test_attn_pages_empty_twice_and_extremes():
     s = Setup(5, [64, 64, 64, 64, 64], 1, 128, 16)
     q = s.rng.standard_normal((5, 2, 128)).astype(np.float32)
