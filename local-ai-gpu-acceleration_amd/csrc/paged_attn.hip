@@ -33,11 +33,12 @@ __device__ __forceinline__ std::uint32_t from_lane(std::uint32_t v, std::uint32_
   return static_cast<std::uint32_t>(__builtin_amdgcn_ds_bpermute(static_cast<int>(4u * lane), static_cast<int>(v)));
 }
 
-// Tiles of a split (one workgroup), of at most `tiles`. Of one size for every row,
-// so that a longer context is more workgroups; the largest of 4 to 64 that leaves a
+// Tiles of a split (one workgroup), of at most `tiles`. Of one size for all rows but much
+// shorter ones (row_per), so that a longer context is more workgroups; the largest of 4 to 64 that leaves a
 // workgroup for each CU, as a wave's prologue and the merge cost what two or three
-// tiles do; over whole contexts, whose lengths differ, more than 16 only where the longest
-// still makes 16 of them. us at 4 / 8 / 16 / 32 / 64 tiles, 32 heads over 8 kv heads of 128
+// tiles do; over whole contexts, whose lengths differ, more than 16 only where the row
+// still makes 12 of them (eight rows of 12000, us with at least 16 / 12 / 8: 87 / 82 / 81, of 8000 63 / 64 / 69,
+// up to 16384 62 / 62 / 67). us at 4 / 8 / 16 / 32 / 64 tiles, 32 heads over 8 kv heads of 128
 // - whole: 1024 slots of one sequence 7.9 / 8.8 / 10.7 / 14.5 / 22.1, 4001 of one 10.9 / 10.0 /
 //   11.8 / 15.9 / 23.9, 65536 of one 88 / 68 / 58 / 53 / 51, up to 4096 of eight 31.1 / 25.9 / 23.3 /
 //   26.0 / 27.2, up to 16384 of eight 100 / 78 / 71 / 70 / 66;
@@ -54,9 +55,22 @@ RTXLLM_HD std::uint32_t attn_per(std::uint64_t items, std::uint64_t tiles, bool 
   std::uint32_t per = kMaxPer;
   for (; per > kWaves; per /= 2u) {
     const std::uint64_t splits = (tiles + per - 1u) / per, enough = per == 8u ? 129u : per == 16u ? 160u : 256u;
-    if (items * splits >= enough && (!whole || per <= 16u || splits >= 16u)) break;
+    if (items * splits >= enough && (!whole || per <= 16u || splits >= 12u)) break;
   }
   return per;
+}
+
+// The tiles of a split of a row that has `tiles`: a.per, but a row much shorter than what
+// there is room for (a list that ends early, a cache that is not full) is split anew, into at
+// most as many parts (us without / with: 9997 positions of four, lists of 120 pages of 256
+// 37.9 / 22.1; one of 600, lists of 1024 pages of 16 15.8 / 10.3; 2000 slots of 32768 21.9 / 9.7, of
+// eight 51.3 / 26.8, contexts up to 16384 of eight in 16384 68 / 62).
+template <bool WEIGHTS>
+__device__ __forceinline__ std::uint32_t row_per(const AttnArgs& a, std::uint32_t items, std::uint32_t tiles, bool light) {
+  if (a.splits == 1u || 2u * tiles > a.per * a.splits) return a.per;
+  std::uint32_t per = attn_per(items, tiles, WEIGHTS, light);
+  while (per * a.splits < tiles) per *= 2u;
+  return WEIGHTS && per > a.per ? a.per : per;
 }
 
 // One workgroup of four waves per (split, kv head, row); a wave takes tiles of 16
@@ -186,18 +200,12 @@ __global__ __launch_bounds__(kThreads, (attn_waves<D, T, WEIGHTS>())) void paged
     }
   }
   const std::uint32_t tiles = (total + kTile - 1u) / kTile;
-  if constexpr (!WEIGHTS) {
-    // A list that ends early (a context shorter than what it has room for) is split anew,
-    // into at most as many parts (9997 positions of four, lists of 120 pages of 256: 37.9 -> 22.1
-    // us; one of 600, 1024 pages of 16: 15.8 -> 10.3).
-    if (a.splits > 1u && 2u * tiles <= a.per * a.splits) {
-      per = attn_per(static_cast<std::uint64_t>(gridDim.y) * kv.n_kv, tiles, false, D < 256 && !WIDE);
-      while (per * a.splits < tiles) per *= 2u;
-      tile0 = split * per + wave;
-      entry = load_entry(tile0);
-      entry_next = load_entry(tile0 + kWaves);
-      page = load_page(entry);
-    }
+  per = row_per<WEIGHTS>(a, gridDim.y * kv.n_kv, tiles, D < 256 && !WIDE);
+  if (per != a.per) {
+    tile0 = split * per + wave;
+    entry = load_entry(tile0);
+    entry_next = load_entry(tile0 + kWaves);
+    page = load_page(entry);
   }
   if (split * per >= tiles) {  // nothing of the row is here
     if constexpr (!WEIGHTS) {
@@ -299,7 +307,7 @@ __global__ __launch_bounds__(kThreads, (attn_waves<D, T, WEIGHTS>())) void paged
     }
     if constexpr (WEIGHTS) {
       if ((WIDE || (col & 1u) == 0u) && my_head)
-        *reinterpret_cast<f32x4*>(&held[(h * a.per + (tile - split * a.per)) * kTile + 4u * qq]) = f32x4{s4[0], s4[1], s4[2], s4[3]};
+        *reinterpret_cast<f32x4*>(&held[(h * a.per + (tile - split * per)) * kTile + 4u * qq]) = f32x4{s4[0], s4[1], s4[2], s4[3]};
     }
     top = fmaxf(top, lane_xor<16>(top));
     top = fmaxf(top, lane_xor<32>(top));
@@ -419,10 +427,10 @@ __global__ __launch_bounds__(kThreads, (attn_waves<D, T, WEIGHTS>())) void paged
   }
   __syncthreads();
   if constexpr (WEIGHTS) {  // at once and in whole lines: tile by tile from the loop 68 us instead of 61
-    const std::uint32_t own = (tile1 - split * a.per) * (kTile / 4u);
+    const std::uint32_t own = (tile1 - split * per) * (kTile / 4u);
     for (std::uint32_t h = 0; h < a.group; ++h)
       for (std::uint32_t i = threadIdx.x; i < own; i += kThreads)
-        *reinterpret_cast<f32x4*>(a.scores + (head0 + h) * a.score_stride + split * a.per * kTile + 4u * i) =
+        *reinterpret_cast<f32x4*>(a.scores + (head0 + h) * a.score_stride + split * per * kTile + 4u * i) =
             *reinterpret_cast<const f32x4*>(&held[h * a.per * kTile + 4u * i]);
   }
   const std::uint32_t items = a.group * (D / 4u);
@@ -529,7 +537,9 @@ __global__ __launch_bounds__(kThreads) void merge_weights_kernel(AttnArgs a, Pag
   const std::uint32_t g = blockIdx.y, r = blockIdx.z, n = paged_filled(kv, a.pos[r]);
   if (n == 0u) return;
   const std::size_t gr = static_cast<std::size_t>(r) * kv.n_kv + g, head0 = gr * a.group;
-  const std::uint32_t splits = (n + a.per * kTile - 1u) / (a.per * kTile);  // those with a record
+  const std::uint32_t tiles = (n + kTile - 1u) / kTile;
+  const std::uint32_t per = row_per<true>(a, gridDim.y * gridDim.z, tiles, false);
+  const std::uint32_t splits = (tiles + per - 1u) / per;  // those with a record
   if (blockIdx.x < a.group) {
     merge_head<D>(a, head0 + blockIdx.x, splits);
     return;

@@ -352,6 +352,24 @@ def test_attn_weights(group, kv, dim, page, place):
     assert np.all(got[1] == 7.0)
 
 
+@pytest.mark.parametrize("group,kv,dim", [(4, 2, 64), (1, 3, 128), (7, 2, 128), (16, 2, 128), (3, 1, 256)])
+def test_attn_weights_in_a_large_cache(group, kv, dim):
+    """Room for 11200 slots a sequence: a full one, and shorter ones beside it."""
+    page, lens = 16, [11200, 0, 1500, 17, 2900]
+    s = Setup(group + dim, lens, kv, dim, page)
+    q = s.rng.standard_normal((5, group * kv, dim)).astype(np.float32)
+    weight = s.rng.random((5, kv, s.capacity)).astype(np.float32)
+    wd = dev(weight)
+    got = paged.attn_weights(s.cache, dev(q), u32(s.last()), wd).cpu().numpy()
+    gw = wd.cpu().numpy()
+    for i, n in enumerate(lens):
+        np.testing.assert_array_equal(gw[i, :, n:], weight[i, :, n:])
+        for g in range(kv if n else 0):
+            total, tol = check_attention(s, got, q, i, g, group, list(range(n)))
+            want = weight[i, g, :n] + total
+            close(gw[i, g, :n], want, tol + (group + 1) * 2.0 ** -24 * want, ("weight", i, g))
+
+
 def test_attn_weights_long():
     """Many splits, several rounds of tiles a wave, a chunk boundary of the gathering."""
     s = Setup(2, [9000, 2049], 1, 128, 64)
