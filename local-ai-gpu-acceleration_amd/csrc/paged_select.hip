@@ -51,9 +51,11 @@ __global__ __launch_bounds__(kThreads) void page_score_kernel(PagedView kv, cons
   typedef _Float16 half8 __attribute__((ext_vector_type(8)));
   const std::uint32_t g = blockIdx.y, r = blockIdx.z, lane = threadIdx.x & 63u, t = lane % L;
   const std::size_t gr = static_cast<std::size_t>(r) * kv.n_kv + g;
-  const std::uint32_t p0 = __builtin_amdgcn_readfirstlane(blockIdx.x * (kThreads / 64u) + (threadIdx.x >> 6)) * kOwn;
+  // step s of a wave lies s * stride pages on: where few pages are filled, waves take a step each
+  const std::uint32_t p0 = __builtin_amdgcn_readfirstlane(blockIdx.x * (kThreads / 64u) + (threadIdx.x >> 6)) * kPages;
+  const std::uint32_t stride = gridDim.x * (kThreads / 64u) * kPages;
   if (p0 >= kv.entries) return;
-  const std::uint32_t mine = p0 + lane % kOwn;
+  const std::uint32_t mine = p0 + lane % kOwn / kPages * stride + lane % kPages;
   const std::int32_t entry =
       kv.table[static_cast<std::size_t>(r) * kv.table_stride + (mine < kv.entries ? mine : kv.entries - 1u)];
   const std::uint32_t filled = paged_filled(kv, pos[r]), used = (filled + kv.page_size - 1u) / kv.page_size;
@@ -83,7 +85,7 @@ __global__ __launch_bounds__(kThreads) void page_score_kernel(PagedView kv, cons
   const bool odd = (lane & 1u) != 0u, odd2 = (lane & 2u) != 0u;
 #pragma unroll
   for (int s = 0; s < kSteps; ++s) {
-    if (p0 + kPages * s >= used) break;
+    if (p0 + stride * s >= used) break;
     if (s + 1 < kSteps) load_bounds(s + 1);
     double c[8], w[8], best = __builtin_nan("");
 #pragma unroll
@@ -109,7 +111,7 @@ __global__ __launch_bounds__(kThreads) void page_score_kernel(PagedView kv, cons
       v = fmax(v, lane_xor_d<1>(v));  // fmax: a head's NaN gives way to a number
       best = fmax(best, fmax(v, lane_xor_d<2>(v)));
     }
-    const std::uint32_t p = p0 + kPages * s + lane / L;
+    const std::uint32_t p = p0 + stride * s + lane / L;
     const bool forced = p < n_first || p + n_last >= used;
     if (t == 0u && p < used) keys[gr * kv.entries + p] = !there[s & 1] ? 0ull : forced ? ~0ull : score_key(best);
   }
