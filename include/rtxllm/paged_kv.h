@@ -80,7 +80,8 @@ hipError_t rtxllm_qk_norm_rope_append_f16(const rtxllm_paged_kv* cache, const fl
  * first on; last[r] >= capacity counts as capacity - 1; last[r] RTXLLM_NO_POSITION
  * or first[r] > last[r]: none. Rows that share pages compute the same values
  * where they fill them alike. bounds 16-byte aligned; count <= 65535; span *
- * n_kv_heads <= 2^24 (a larger span than a sequence has pages counts as that). */
+ * n_kv_heads <= 2^24 (a larger span than a sequence has pages counts as that; the
+ * launch is sized by it). */
 hipError_t rtxllm_kv_page_bounds_f16(const rtxllm_paged_kv* cache, const uint32_t* first, const uint32_t* last,
                                      uint32_t count, uint32_t span, uint16_t* bounds, hipStream_t stream);
 
