@@ -91,9 +91,13 @@ hipError_t rtxllm_kv_page_bounds_f16(const rtxllm_paged_kv* cache, const uint32_
  * n_select in all (or all there are); pages[r][kv head][n_select], ascending, -1
  * behind the last. score = max over the kv head's query heads h of sum_d
  * max(q_hd largest_d, q_hd smallest_d): no key of the page has a larger product
- * with any of them. Scores are sums in 64 bits, so that the choice does not hang
- * on the order of a sum; the lower page wins between equal scores; a head whose
- * product is NaN does not count, and a page where none does ranks last. A page with
+ * with any of them. The larger product is that with the extreme on q's side (the larger
+ * one where q_hd >= 0), the other extreme has no effect. Products are exact and
+ * summed in 64 bits, in one order for all pages: scores of like terms are equal, and others
+ * come out in order unless they lie within some 2^-45 of their terms' sizes. The lower page wins
+ * between equal scores; a head whose
+ * sum is NaN does not count (an infinite q gives one where it meets an extreme of 0), and
+ * a page where none does ranks last. A page with
  * no entry in the table is never listed.
  * n_heads / n_kv_heads 1..16, n_first + n_last <= n_select <= 65536, count <= 65535.
  * workspace: rtxllm_attn_select_workspace() bytes, 256-byte aligned. */

@@ -32,10 +32,12 @@ __device__ __forceinline__ unsigned long long score_key(double s) {
 }
 
 // Keys of the pages of one (row, kv head): a wave scores kSteps times 64 / L pages, L =
-// head_dim / 8 lanes a page, 8 dimensions a lane. With c = (hi + lo) / 2 and w = |hi - lo| /
-// 2, max(q hi, q lo) = q c + |q| w; here both are doubled, which changes no order.
-// Products of fp32 and fp16 values are exact in 64 bits, and the sums' 2^-53 keep two
-// pages apart whose scores differ at all. Four heads at a time: two halving exchanges
+// head_dim / 8 lanes a page, 8 dimensions a lane. max(q hi, q lo) is q times the larger
+// extreme where q >= 0, the smaller one where it is not: chosen by the sign, two dimensions
+// at a time as fp16 pairs, so that the other extreme enters nothing (an infinite q times a
+// zero of its page would be a NaN, and equal scores would differ by the roundings of what
+// cancels). Products of fp32 and fp16 values are exact in 64 bits; their sums take one
+// order for every page. Four heads at a time: two halving exchanges
 // leave each lane one head's part, so that four heads take one head's further steps.
 // What bounds it is the chain of reads (table and q, then bounds): the position is
 // needed last, a wave's table entries are one load, and the next step's bounds are
@@ -48,7 +50,10 @@ __global__ __launch_bounds__(kThreads) void page_score_kernel(PagedView kv, cons
                                                               unsigned long long* __restrict__ keys) {
   constexpr std::uint32_t D = 8u * L, kPages = 64u / L, kOwn = kPages * kSteps;
   static_assert(kOwn <= 64u, "a lane a page of the wave");
+  typedef _Float16 half2 __attribute__((ext_vector_type(2)));
   typedef _Float16 half8 __attribute__((ext_vector_type(8)));
+  typedef short short2_t __attribute__((ext_vector_type(2)));
+  typedef std::uint32_t u32x4 __attribute__((ext_vector_type(4)));
   const std::uint32_t g = blockIdx.y, r = blockIdx.z, lane = threadIdx.x & 63u, t = lane % L;
   const std::size_t gr = static_cast<std::size_t>(r) * kv.n_kv + g;
   // step s of a wave lies s * stride pages on: where few pages are filled, waves take a step each
@@ -61,6 +66,7 @@ __global__ __launch_bounds__(kThreads) void page_score_kernel(PagedView kv, cons
   const std::uint32_t filled = paged_filled(kv, pos[r]), used = (filled + kv.page_size - 1u) / kv.page_size;
   const float* const qr = q + gr * group * D + 8u * t;
   double qd[4][8];
+  std::uint32_t below[4][4];  // all ones in the half of a dimension whose q is below 0
   auto load_q = [&](std::uint32_t h0) {
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
@@ -68,6 +74,13 @@ __global__ __launch_bounds__(kThreads) void page_score_kernel(PagedView kv, cons
       const f32x4_any a = *reinterpret_cast<const f32x4_any*>(qr + h * D), b = *reinterpret_cast<const f32x4_any*>(qr + h * D + 4u);
 #pragma unroll
       for (int i = 0; i < 8; ++i) qd[k][i] = static_cast<double>(i < 4 ? a[i & 3] : b[i & 3]);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const f32x4_any& v = i < 2 ? a : b;
+        const short2_t top = {static_cast<short>(__float_as_uint(v[2 * i & 3]) >> 16),
+                              static_cast<short>(__float_as_uint(v[(2 * i & 3) + 1]) >> 16)};
+        below[k][i] = __builtin_bit_cast(std::uint32_t, top >> static_cast<short>(15));
+      }
     }
   };
   half8 hi[2], lo[2];
@@ -87,20 +100,21 @@ __global__ __launch_bounds__(kThreads) void page_score_kernel(PagedView kv, cons
   for (int s = 0; s < kSteps; ++s) {
     if (p0 + stride * s >= used) break;
     if (s + 1 < kSteps) load_bounds(s + 1);
-    double c[8], w[8], best = __builtin_nan("");
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const double x = static_cast<double>(static_cast<float>(hi[s & 1][i])), y = static_cast<double>(static_cast<float>(lo[s & 1][i]));
-      c[i] = x + y;
-      w[i] = fabs(x - y);
-    }
+    double best = __builtin_nan("");
+    // (a page of NaN keys alone has them in reverse order)
+    const u32x4 large = __builtin_bit_cast(u32x4, __builtin_elementwise_max(hi[s & 1], lo[s & 1]));
+    const u32x4 small = __builtin_bit_cast(u32x4, __builtin_elementwise_min(hi[s & 1], lo[s & 1]));
     for (std::uint32_t h0 = 0; h0 < group; h0 += 4u) {
       if (group > 4u) load_q(h0);
       double sum[4] = {0.0, 0.0, 0.0, 0.0};
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
+      for (int i = 0; i < 4; ++i)
 #pragma unroll
-        for (int k = 0; k < 4; ++k) sum[k] = fma(fabs(qd[k][i]), w[i], fma(qd[k][i], c[i], sum[k]));
+        for (int k = 0; k < 4; ++k) {
+          const half2 x = __builtin_bit_cast(half2, (below[k][i] & small[i]) | (~below[k][i] & large[i]));
+          sum[k] = fma(qd[k][2 * i], static_cast<double>(static_cast<float>(x[0])), sum[k]);
+          sum[k] = fma(qd[k][2 * i + 1], static_cast<double>(static_cast<float>(x[1])), sum[k]);
+        }
       const double x0 = odd ? sum[2] : sum[0], x1 = odd ? sum[3] : sum[1];
       const double y0 = odd ? sum[0] : sum[2], y1 = odd ? sum[1] : sum[3];
       const double v0 = x0 + lane_xor_d<1>(y0), v1 = x1 + lane_xor_d<1>(y1);
