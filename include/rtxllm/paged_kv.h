@@ -149,7 +149,8 @@ hipError_t rtxllm_attn_decode_weights_gqa_f16(const rtxllm_paged_kv* cache, cons
  * slot_pos_out get slots 0..min(length, keep) - 1 and are left as they were
  * behind (each may be its input); length_out[r] = min(length[r], keep) (may be
  * length). A row with pos[r] RTXLLM_NO_POSITION is a padded row. A slot in no
- * page keeps its place in the order, but no key or value moves from or to it.
+ * page has nothing to move and no room: whatever its weight and position it stays where
+ * it lies below keep and leaves where it lies behind, and the others fill what is left of keep.
  * Sequences of one call must not share pages. n_first + n_recent <= keep <=
  * capacity, keep >= 1, count <= 65535; table_stride 0 only with count 1. */
 size_t rtxllm_kv_evict_workspace(const rtxllm_paged_kv* cache, uint32_t keep, uint32_t count);

@@ -210,19 +210,20 @@ __device__ __forceinline__ void count_digits(std::uint32_t* hist, Digit digit_of
 // rolled: each runs a few rounds once, and unrolled code with the keys in registers
 // took longer to fetch (32 keys a thread: 92 us for 32768 keys). src.raw(i) loads what
 // keys i..i + 3 (i % 4 == 0) are made of, src.keys(i, raw, x) makes them (<true>: all four
-// are there), src.seen(i, raw) is called for each once, where they go into the LDS.
+// are there), src.seen(i, raw) is called for each once, where they go into the LDS;
+// src.begin() comes before all of them, behind a barrier.
 template <class K, class Source, std::uint32_t T>
 struct Keys {
   struct alignas(16) Four {
     K k[4];
   };
-  const Source& src;
+  Source& src;
   Four* held;
   std::uint32_t n, rounds, first;  // rounds of this wave, its first key
   bool in_lds;
 
   // `hist` gets the counts of the keys' first digit where they are read into the LDS.
-  __device__ __forceinline__ Keys(const Source& s, void* lds, std::uint32_t* hist, std::uint32_t count, std::uint32_t room)
+  __device__ __forceinline__ Keys(Source& s, void* lds, std::uint32_t* hist, std::uint32_t count, std::uint32_t room)
       : src(s), held(static_cast<Four*>(lds) + threadIdx.x), n(count), in_lds(count <= room) {
     const std::uint32_t most = (n + 4u * T - 1u) / (4u * T);
     first = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) * 256u * most;
@@ -231,6 +232,7 @@ struct Keys {
     for (std::uint32_t i = 4u * threadIdx.x; i < kBins; i += 4u * T)
       *reinterpret_cast<uint4*>(hist + i) = make_uint4(0u, 0u, 0u, 0u);
     __syncthreads();
+    src.begin();
     if (!in_lds) return;
     using Raw = decltype(src.template raw<true>(0u));
     auto take = [&](auto full, std::uint32_t round, const Raw& v) {
@@ -427,6 +429,7 @@ struct KeyRow {
     }
     return v;
   }
+  __device__ __forceinline__ void begin() const {}
   __device__ __forceinline__ void seen(std::uint32_t, const u64x4&) const {}
   template <bool>
   __device__ __forceinline__ void keys(std::uint32_t, const u64x4& v, unsigned long long (&x)[4]) const {
@@ -446,7 +449,7 @@ __global__ __launch_bounds__(T) void page_choice_kernel(PagedView kv, const std:
   const std::uint32_t used = (paged_filled(kv, pos[r]) + kv.page_size - 1u) / kv.page_size;
   if (used == 0u) return;  // a padded row
   const std::size_t gr = static_cast<std::size_t>(r) * kv.n_kv + g;
-  const KeyRow src{row_keys + gr * kv.entries, used};
+  KeyRow src{row_keys + gr * kv.entries, used};
   const Keys<unsigned long long, KeyRow, T> keys(src, lds, sh.hist[0], used, room);
   std::int32_t* const out = pages + gr * n_select;
   // 1 and more: every page that is there
@@ -458,12 +461,14 @@ __global__ __launch_bounds__(T) void page_choice_kernel(PagedView kv, const std:
   for (std::uint32_t i = listed + threadIdx.x; i < n_select; i += T) out[i] = -1;
 }
 
-// A weight as an unsigned key of the same order, 0 for NaN; protected slots above
-// every weight. The positions from n_first on that are not protected are `open` many.
+// A weight as an unsigned key of the same order, 1 for NaN; protected slots above every
+// weight. 0 and kStays are left for slots in no page (SlotKeys). The positions from n_first on
+// that are not protected are `open` many.
+constexpr std::uint32_t kStays = 0xFFFFFFFFu;
 __device__ __forceinline__ std::uint32_t weight_key(float w, std::uint32_t p, std::uint32_t n_first, std::uint32_t open) {
   const std::uint32_t b = __float_as_uint(w + 0.0f);
   const std::uint32_t key = b ^ (static_cast<std::uint32_t>(static_cast<std::int32_t>(b) >> 31) | 0x80000000u);
-  return p - n_first >= open ? 0xFFFFFFFFu : w != w ? 0u : key;
+  return p - n_first >= open ? kStays - 1u : w != w ? 1u : key;
 }
 
 // The moves of one (sequence, kv head): moves[0] of them, then their destination
@@ -478,12 +483,24 @@ struct EvictArgs {
   std::uint32_t keep, n_first, n_recent, most, room;
 };
 
+// A slot in no page holds no key or value that could move, and takes none: below keep it
+// stays whatever it weighs, behind it it leaves. (There are enough others: those below keep
+// alone make up the number.) Such slots are looked for once, in the table.
 struct SlotKeys {
   const float* w;
   const std::uint32_t* p;
   float* wo;
   std::uint32_t* po;
   std::uint32_t n, stay, n_first, open;
+  const PagedView& kv;
+  const std::int32_t* table;
+  const std::uint32_t* wave_holes;  // in the LDS: whether a wave has found one
+  std::uint32_t waves;
+  bool holes;
+  __device__ __forceinline__ void begin() {
+    const std::uint32_t lane = threadIdx.x & 63u;
+    holes = __ballot(lane < waves && wave_holes[lane] != 0u) != 0ull;
+  }
   struct Raw {
     f32x4_any w;
     u32x4_any p;
@@ -505,6 +522,11 @@ struct SlotKeys {
   __device__ __forceinline__ void keys(std::uint32_t i, const Raw& v, std::uint32_t (&x)[4]) const {
 #pragma unroll
     for (int e = 0; e < 4; ++e) x[e] = weight_key(v.w[e], v.p[e], n_first, open);
+    if (holes) {
+#pragma unroll
+      for (std::uint32_t e = 0; e < 4u; ++e)
+        if (i + e < n && static_cast<std::uint32_t>(table[page_of(kv, i + e)]) >= kv.n_pages) x[e] = i + e < stay ? kStays : 0u;
+    }
     if (FULL || __ballot(i + 4u > n) == 0ull) return;
 #pragma unroll
     for (int e = 0; e < 4; ++e)
@@ -552,6 +574,8 @@ __global__ __launch_bounds__(T) void evict_choice_kernel(PagedView kv, EvictArgs
   const std::uint32_t g = blockIdx.x, r = blockIdx.y, tid = threadIdx.x;
   const std::size_t gr = static_cast<std::size_t>(r) * kv.n_kv + g;
   std::uint32_t* const moves = a.moves + gr * (1u + 2u * static_cast<std::size_t>(a.most));
+  const std::int32_t* const table = kv.table + static_cast<std::size_t>(r) * kv.table_stride;
+  const std::int32_t entry = table[tid < kv.entries ? tid : 0u];  // (with the length in flight)
   const std::uint32_t newest = a.pos[r];
   std::uint32_t n = a.length[r];
   n = n < kv.capacity ? n : kv.capacity;
@@ -561,15 +585,22 @@ __global__ __launch_bounds__(T) void evict_choice_kernel(PagedView kv, EvictArgs
   }
   if (L != 0 && g == 0u && tid == 0u) length_out[r] = n < a.keep ? n : a.keep;
   const std::uint32_t recent = newest >= a.n_recent ? newest - a.n_recent + 1u : 0u;  // the first such position
-  const SlotKeys src{a.weight + gr * kv.capacity, a.slot_pos + gr * kv.capacity, a.weight_out + gr * kv.capacity,
-                     a.slot_pos_out + gr * kv.capacity, n, n < a.keep ? n : a.keep, a.n_first,
-                     recent > a.n_first ? recent - a.n_first : 0u};
+  SlotKeys src{a.weight + gr * kv.capacity, a.slot_pos + gr * kv.capacity, a.weight_out + gr * kv.capacity,
+               a.slot_pos_out + gr * kv.capacity, n, n < a.keep ? n : a.keep, a.n_first,
+               recent > a.n_first ? recent - a.n_first : 0u, kv, table, sh.wave[0], T / 64u, false};
   if (n <= a.keep || n > a.room)
     for (std::uint32_t i = 4u * tid; i < src.stay; i += 4u * T) src.seen(i, src.raw<false>(i));
   if (n <= a.keep) {
     if (tid == 0u) moves[0] = 0u;
     return;
   }
+  const std::uint32_t used = page_of(kv, n - 1u) + 1u;
+  bool hole = tid < used && static_cast<std::uint32_t>(entry) >= kv.n_pages;
+  for (std::uint32_t t = T + 4u * tid; t < used; t += 4u * T)
+#pragma unroll
+    for (std::uint32_t e = 0; e < 4u; ++e)  // past the last: read again
+      hole |= static_cast<std::uint32_t>(table[t + e < used ? t + e : used - 1u]) >= kv.n_pages;
+  if (const unsigned long long b = __ballot(hole); (tid & 63u) == 0u) sh.wave[0][tid >> 6] = b != 0ull ? 1u : 0u;
   const Keys<std::uint32_t, SlotKeys, T> keys(src, lds, sh.hist[0], n, a.room);
   const Choice<std::uint32_t> ch = radix_choice(sh, keys, a.keep);
   std::uint32_t* const to = moves + 1u;

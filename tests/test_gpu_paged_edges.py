@@ -105,3 +105,68 @@ def test_reversed_bounds_count_both_ways():
     bounds[s.table[0, 6], 0, 0], bounds[s.table[0, 6], 0, 1] = -ref.H_MAX, ref.H_MAX
     q = s.rng.standard_normal((1, 3, 64)).astype(np.float32)
     assert listed_pages(s, bounds, q, 1)[0].tolist() == [6]
+
+
+# ---- eviction from a table with holes ------------------------------------------------
+
+
+def evict_around_holes(there, length, newest, keep, n_first, n_recent, weight, slot_pos):
+    """Source slot of each slot below keep: slots in no page stay below keep and leave behind it,
+    the others fill what is left of keep by rank."""
+    def rank(i):
+        p, w = int(slot_pos[i]), float(weight[i])
+        if p < n_first or p + n_recent > newest:
+            return (0, 0.0, i)
+        return (2, 0.0, i) if np.isnan(w) else (1, -w, i)
+
+    fixed = {i for i in range(keep) if not there[i]}
+    kept = fixed | set(sorted((i for i in range(length) if there[i]), key=rank)[:keep - len(fixed)])
+    late = iter(sorted(i for i in kept if i >= keep))
+    return [i if i in kept else next(late) for i in range(keep)]
+
+
+# (slots, keep, page): moves in the choosing workgroup and apart, more table entries than one
+# round of a workgroup's loads, more slots than the LDS holds, four waves of many short sequences
+@pytest.mark.parametrize("n,keep,page,count,dim", [
+    (130, 100, 7, 3, 64), (130, 100, 7, 3, 256), (130, 100, 1, 3, 128), (600, 300, 16, 2, 64), (600, 300, 16, 2, 256),
+    (2112, 2048, 64, 2, 128), (9000, 5000, 1, 1, 64), (33000, 20000, 24, 1, 64), (200, 150, 8, 130, 64), (200, 150, 8, 130, 256)])
+@pytest.mark.parametrize("place", ["apart", "in-place"])
+@pytest.mark.parametrize("where", ["below", "behind", "both", "all-behind", "all-below"])
+def test_evict_around_holes(n, keep, page, count, dim, place, where):
+    """No key or value of a page that is not there counts: what stays is read back key by key."""
+    kv = 2
+    s = Setup(n + keep + page, [n] * count, kv, dim, page)
+    rng = s.rng
+    first_behind = -(-keep // page)
+    for row in s.table:
+        low, high = np.arange(0, keep // page), np.arange(first_behind, s.entries)
+        some = {"below": rng.permutation(low)[:max(1, len(low) // 3)], "behind": rng.permutation(high)[:max(1, len(high) // 3)],
+                "all-behind": high, "all-below": low}
+        some["both"] = np.concatenate([some["below"], some["behind"]])
+        row[some[where]] = rng.choice([-1, s.n_pages, 2 ** 31 - 1], len(some[where]))
+    s.cache.block_table.copy_(dev(s.table))
+    weight = (rng.integers(0, 50, (count, kv, s.capacity)) / 8).astype(np.float32)
+    weight[:, :, ::5] = np.nan
+    slot_pos = np.stack([[rng.permutation(s.capacity) for _ in range(kv)] for _ in range(count)]).astype(np.uint32)
+    newest = [int(p[:, :n].max()) for p in slot_pos]
+    wd, sd, ld = dev(weight), u32(slot_pos), u32([n] * count)
+    apart = place == "apart"
+    wo, so, lo = (torch.full_like(t, 7) for t in (wd, sd, ld)) if apart else (wd, sd, ld)
+    paged.evict(s.cache, ld, u32(newest), keep, wd, sd, 3, 20, wo if apart else None, so if apart else None,
+                lo if apart else None)
+    gw, gp, gk, gv = wo.cpu().numpy(), so.cpu().numpy().view(np.uint32), s.kd.cpu().numpy(), s.vd.cpu().numpy()
+    assert lo.cpu().tolist() == [keep] * count
+    k_want, v_want = s.k.copy(), s.v.copy()
+    for i in range(count):
+        place_of = np.array([ref.at(s.table[i], s.n_pages, page, t) or (-1, -1) for t in range(n)])
+        there = place_of[:, 0] >= 0
+        for g in range(kv):
+            src = np.array(evict_around_holes(there, n, newest[i], keep, 3, 20, weight[i, g], slot_pos[i, g]))
+            np.testing.assert_array_equal(gw[i, g, :keep], weight[i, g, src])
+            np.testing.assert_array_equal(gp[i, g, :keep], slot_pos[i, g, src])
+            to = np.flatnonzero(src != np.arange(keep))
+            assert there[to].all() and there[src[to]].all()
+            (p, o), (p2, o2) = place_of[to].T, place_of[src[to]].T
+            k_want[p, g, o], v_want[p, g, o] = s.k[p2, g, o2], s.v[p2, g, o2]
+    np.testing.assert_array_equal(gk.view(np.uint16), k_want.view(np.uint16))
+    np.testing.assert_array_equal(gv.view(np.uint16), v_want.view(np.uint16))
