@@ -16,7 +16,7 @@ typedef float f32x16 __attribute__((ext_vector_type(16)));
 
 constexpr std::uint32_t kThreads = 256, kWaves = kThreads / 64u, kTile = 16;
 constexpr std::uint32_t kMaxPer = 64;  // tiles of a split, at most: what its scores take in the LDS
-constexpr float kLift = 15.0f;  // softmax terms are kept times 2^15 (see the kernel)
+constexpr int kLift = 15;  // queries and softmax terms are brought to 2^15 (see the kernel)
 
 struct AttnArgs {
   const float* q;
@@ -76,12 +76,14 @@ __device__ __forceinline__ std::uint32_t row_per(const AttnArgs& a, std::uint32_
 // One workgroup of four waves per (split, kv head, row); a wave takes tiles of 16
 // positions of its split in turn, with a running maximum and sum for every head:
 //  * scores: S = K q^T by v_mfma_f32_16x16x32_f16. A = the K rows as stored (lane:
-//    position l % 16, 8 dims of each 32); B = q log2(e) / sqrt(D) of head n / 2,
-//    a power of two below 2 in magnitude, as an fp16 hi (n even) / lo (n odd)
-//    pair, so products are exact and the pair carries 22 bits at any size of q;
-//  * p = 2^(s - m + 15) split into an fp16 hi / lo pair as well: lifted by 2^15 (the
-//    largest p is 2^15, the sum l is lifted alike), terms down to 2^-29 of the
-//    largest keep 22 bits where fp16's subnormals would cut them;
+//    position l % 16, 8 dims of each 32); B = q of head n / 2 as an fp16 hi (n even) / lo
+//    (n odd) pair, brought by a power of two to 2^14..2^15 in its largest element, so that
+//    the subnormals come late: products are exact, an element is off by 2^-22 of itself or,
+//    where lo is subnormal, by 2^-25 of 2^14, 2^-39 of the largest;
+//  * p = 2^(s - m + 15) split into an fp16 hi / lo pair alike (the largest p is 2^15, the
+//    sum l is lifted as well): terms down to 2^-18 of the largest keep 22 bits, smaller
+//    ones are off by 2^-40 of the largest at most, which 2^16 positions add up to one
+//    rounding of fp32;
 //  * o += V^T p by v_mfma_f32_4x4x4_16b_f16: a lane holds its own dimensions of
 //    four positions, as the V rows' coalesced loads leave them, and one column of p,
 //    fetched from the score layout by ds_bpermute. A lane's 4 results are one head's,
@@ -166,13 +168,13 @@ __global__ __launch_bounds__(kThreads, (attn_waves<D, T, WEIGHTS>())) void paged
     m = fmaxf(m, lane_xor<32>(m));
     int e = 0;
     if (m > 0.0f && m <= 3.4e38f) frexpf(m, &e);
-    qscale = ldexpf(1.4426950408889634f / (D == 64 ? 8.0f : D == 128 ? 11.313708498984761f : 16.0f), e);
+    qscale = ldexpf(1.4426950408889634f / (D == 64 ? 8.0f : D == 128 ? 11.313708498984761f : 16.0f), e - kLift);
 #pragma unroll
     for (int j = 0; j < J; ++j) {
       half8 hi, lo;
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        float v = my_head ? ldexpf(x[j][i / 4][i & 3], -e) : 0.0f;
+        float v = my_head ? ldexpf(x[j][i / 4][i & 3], kLift - e) : 0.0f;
         asm("" : "+v"(v));  // one rounded value for hi and lo
         hi[i] = static_cast<_Float16>(v);
         lo[i] = static_cast<_Float16>(v - static_cast<float>(hi[i]));

@@ -170,3 +170,46 @@ def test_evict_around_holes(n, keep, page, count, dim, place, where):
             k_want[p, g, o], v_want[p, g, o] = s.k[p2, g, o2], s.v[p2, g, o2]
     np.testing.assert_array_equal(gk.view(np.uint16), k_want.view(np.uint16))
     np.testing.assert_array_equal(gv.view(np.uint16), v_want.view(np.uint16))
+
+
+# ---- attention: queries of very different sizes in one head ---------------------------
+
+
+@pytest.mark.parametrize("group", [1, 4, 8, 12, 16])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("large", [1e4, 1e5, 1e7])
+def test_attention_beside_a_large_query(group, dim, large):
+    """One element of a query is some powers of ten above the others, where the keys are 0. Each
+    element enters as an fp16 pair: off by 2^-22 of itself or 2^-39 of the head's largest.
+    The rest of the bound is that of paged_ref.attend."""
+    s = Setup(group + dim, [150, 70], 2, dim, 16)
+    rng = s.rng
+    at = rng.integers(0, dim)
+    s.k[..., at] = 0.0
+    s.kd.copy_(dev(s.k))
+    q = rng.standard_normal((2, 2 * group, dim)).astype(np.float32)
+    q[..., at] = large
+    weight = torch.zeros(2, 2, s.capacity, device=DEV)
+    pages = torch.arange(s.entries, dtype=torch.int32, device=DEV).expand(2, 2, -1).contiguous()
+    listed = paged.attn_pages(s.cache, dev(q), pages, u32(s.last())).cpu().numpy()
+    dense = paged.attn_weights(s.cache, dev(q), u32(s.last()), weight).cpu().numpy()
+    gathered = weight.cpu().numpy()
+    for i, n in enumerate(s.lens):
+        for g in range(2):
+            keys, values, _ = s.rows(i, g, range(n))
+            keys, values = keys.astype(np.float64), values.astype(np.float64)
+            total, slack = np.zeros(n), np.zeros(n)
+            for h in range(g * group, (g + 1) * group):
+                x = q[i, h].astype(np.float64)
+                score = keys @ x / np.sqrt(dim)
+                p = np.exp(score - score.max())
+                p /= p.sum()
+                size = np.abs(keys) @ np.abs(x)
+                delta = ((2.0 ** -22 + (dim + 8) * 2.0 ** -24) * size +
+                         2.0 ** -39 * np.abs(x).max() * np.abs(keys).sum(1)).max() / np.sqrt(dim)
+                bound = 2.0 * (delta + 2.0 ** -21 * (1.0 + np.abs(score).max())) + (n / 4 + 40) * 2.0 ** -24
+                for got in (listed, dense):
+                    assert (np.abs(got[i, h] - p @ values) <= bound * (p @ np.abs(values)) + 1e-37).all(), (i, h)
+                total += p
+                slack += p * bound + 2.0 ** -40
+            assert (np.abs(gathered[i, g, :n] - total) <= slack + (group + 1) * 2.0 ** -24 * total).all(), (i, g)
