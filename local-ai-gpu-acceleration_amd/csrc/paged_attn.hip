@@ -552,8 +552,8 @@ __global__ __launch_bounds__(kThreads) void merge_weights_kernel(AttnArgs a, Pag
   for (std::uint32_t h = threadIdx.x >> 6; h < a.group; h += kWaves) {
     const float2 t = head_ml(a.ml + (head0 + h) * a.splits, splits, lane);
     if (lane == 0u) {
-      base_s[h] = (t.x == -INFINITY ? 0.0f : t.x) - kLift;
-      inv_s[h] = t.y == 0.0f ? 0.0f : 1.0f / t.y;
+      base_s[h] = t.x == -INFINITY ? 0.0f : t.x;
+      inv_s[h] = t.y == 0.0f ? 0.0f : static_cast<float>(1 << kLift) / t.y;  // (a large base would swallow the lift)
     }
   }
   __syncthreads();

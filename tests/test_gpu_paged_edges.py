@@ -213,3 +213,34 @@ def test_attention_beside_a_large_query(group, dim, large):
                 total += p
                 slack += p * bound + 2.0 ** -40
             assert (np.abs(gathered[i, g, :n] - total) <= slack + (group + 1) * 2.0 ** -24 * total).all(), (i, g)
+
+
+@pytest.mark.parametrize("group", [1, 5, 12])
+@pytest.mark.parametrize("large", [1e3, 1e7, 1e20])
+def test_gathered_weights_of_large_scores(group, large):
+    """Scores of thousands and more: what is gathered is the softmax itself, 1 for each head in all.
+    Two positions of each head lie a few units apart, all others far below; products and sums
+    are exact (one nonzero dimension, keys of few bits)."""
+    s = Setup(group + 2, [200], 1, 64, 16)
+    p, o = np.array(s.seen[0]).T
+    s.k[:] = 0.0
+    s.k[p, 0, o, 3] = s.rng.integers(0, 64, 200) / np.float16(64.0)
+    s.k[p[[7, 150]], 0, o[[7, 150]], 3] = 2.0
+    s.k[p[7], 0, o[7], 4] = 1.0
+    s.kd.copy_(dev(s.k))
+    q = np.zeros((1, group, 64), np.float32)
+    q[0, :, 3] = large
+    q[0, :, 4] = np.arange(group) / 2.0
+    weight = torch.zeros(1, 1, s.capacity, device=DEV)
+    paged.attn_weights(s.cache, dev(q), u32([199]), weight)
+    got = weight.cpu().numpy()[0, 0]
+    # the scores round to fp32 at 2 large / 8 (log2(e) in), where they lie apart by half a unit a head
+    score = 2.0 * large / 8.0 * 1.4427
+    want = np.zeros(s.capacity)
+    apart = q[0, :, 4].astype(np.float64) / 8.0
+    want[7], want[150] = (1.0 / (1.0 + np.exp(-apart))).sum(), (1.0 / (1.0 + np.exp(apart))).sum()
+    slack = group * min(1.0, 2.0 * score * 2.0 ** -22) + 1e-6
+    assert abs(got.sum() - group) <= group * 16 * 2.0 ** -24
+    assert (np.abs(got - want) <= slack).all()
+
+
