@@ -167,7 +167,7 @@ __global__ __launch_bounds__(kThreads, (attn_waves<D, T, WEIGHTS>())) void paged
     m = fmaxf(m, lane_xor<16>(m));
     m = fmaxf(m, lane_xor<32>(m));
     int e = 0;
-    if (m > 0.0f && m <= 3.4e38f) frexpf(m, &e);
+    if (m > 0.0f && m < INFINITY) frexpf(m, &e);
     qscale = ldexpf(1.4426950408889634f / (D == 64 ? 8.0f : D == 128 ? 11.313708498984761f : 16.0f), e - kLift);
 #pragma unroll
     for (int j = 0; j < J; ++j) {

@@ -244,3 +244,24 @@ def test_gathered_weights_of_large_scores(group, large):
     assert (np.abs(got - want) <= slack).all()
 
 
+@pytest.mark.parametrize("group", [1, 12])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_attention_with_the_largest_queries(group, dim):
+    """Finite queries up to the largest fp32 number, over keys so small that the scores are finite:
+    the position with the largest score takes all (the others lie 10^28 and more below)."""
+    s = Setup(group + dim + 1, [90], 1, dim, 16)
+    rng = s.rng
+    s.k[:] = 0.0
+    p, o = np.array(s.seen[0]).T
+    steps = rng.permutation(90)
+    s.k[p, 0, o, 7] = steps * np.float16(2.0 ** -24)  # exact subnormals
+    s.kd.copy_(dev(s.k))
+    q = np.zeros((1, group, dim), np.float32)
+    q[..., 7] = np.where(np.arange(group) % 2, -1.0, 1.0) * np.finfo(np.float32).max
+    weight = torch.zeros(1, 1, s.capacity, device=DEV)
+    pages = torch.arange(s.entries, dtype=torch.int32, device=DEV).reshape(1, 1, -1)
+    for got in (paged.attn_pages(s.cache, dev(q), pages, u32([89])), paged.attn_weights(s.cache, dev(q), u32([89]), weight)):
+        for h, row in enumerate(got.cpu().numpy()[0]):
+            top = int(np.argmin(steps) if h % 2 else np.argmax(steps))
+            np.testing.assert_allclose(row, s.v[p[top], 0, o[top]], rtol=1e-6)
+    assert float(weight.sum()) == group
