@@ -21,6 +21,13 @@ NO_POSITION = -1
 PAIRINGS = {"adjacent": 0, "halves": 1}
 
 
+def _u32(name: str, value: int) -> int:
+    """The C-ABI's unsigned numbers, which ctypes would cut to their low 32 bits."""
+    if 0 <= value <= 0xFFFFFFFF:
+        return value
+    raise ValueError(f"{name}: {value} is not in 0..2^32 - 1")
+
+
 class PagedKV:
     """A layer's cache: k, v fp16 [n_pages][n_kv_heads][page_size][head_dim] and a
     block table, int32 [sequences][entries] or, for one sequence whose tokens the
@@ -31,6 +38,8 @@ class PagedKV:
             raise ValueError("k and v must be float16 [n_pages][n_kv_heads][page_size][head_dim] of one shape")
         if block_table.dim() not in (1, 2) or block_table.dtype != torch.int32 or block_table.shape[-1] == 0:
             raise ValueError("block_table must be int32 [sequences][entries] or [entries]")
+        if 0 in k.shape or block_table.shape[-1] * k.shape[2] > 1 << 24:
+            raise ValueError(f"{block_table.shape[-1]} entries of pages {tuple(k.shape)}: a sequence has 1..2^24 positions")
         if not (k.is_contiguous() and v.is_contiguous()) or block_table.stride(-1) != 1:
             raise ValueError("the cache and the rows of its block table must be contiguous")
         if not (k.is_cuda and k.device == v.device == block_table.device):
@@ -43,7 +52,8 @@ class PagedKV:
         stride = 0 if self.one_sequence else max(block_table.stride(0), block_table.shape[1])
         if not self.one_sequence and self.sequences > 1 and block_table.stride(0) < block_table.shape[1]:
             raise ValueError("the rows of the block table overlap")
-        self._struct = PagedKVStruct(k.data_ptr(), v.data_ptr(), block_table.data_ptr(), stride, self.n_pages,
+        self._struct = PagedKVStruct(k.data_ptr(), v.data_ptr(), block_table.data_ptr(),
+                                     _u32("the block table's row stride", stride), _u32("n_pages", self.n_pages),
                                      self.n_kv_heads, self.head_dim, self.page_size, self.capacity)
         self.ref = ctypes.addressof(self._struct)
 
@@ -128,8 +138,8 @@ def qk_norm_rope_append(cache: PagedKV, q: torch.Tensor, k: torch.Tensor, v: tor
     sw = None if slot_weight is None else cache._check("slot_weight", slot_weight, state)
     q_out = cache._output("q_out", q_out, q.shape, fill=0.0)
     cache._call("rtxllm_qk_norm_rope_append_f16", q.data_ptr(), qs, k.data_ptr(), ks, v.data_ptr(), vs, qw, kw,
-                q.shape[1], cache.head_dim if rotary_dim is None else rotary_dim, PAIRINGS[pairing], theta, eps, pp, lp,
-                count, q_out.data_ptr(), sp, sw)
+                q.shape[1], cache.head_dim if rotary_dim is None else _u32("rotary_dim", rotary_dim), PAIRINGS[pairing],
+                theta, eps, pp, lp, count, q_out.data_ptr(), sp, sw)
     return q_out
 
 
@@ -141,12 +151,13 @@ def page_bounds(cache: PagedKV, last: torch.Tensor, bounds: torch.Tensor, first:
     cache._rows(count)
     b = cache._check("bounds", bounds, (cache.n_pages, cache.n_kv_heads, 2, cache.head_dim), torch.float16)
     f = None if first is None else cache._check("first", first, (count,), torch.int32)
-    cache._call("rtxllm_kv_page_bounds_f16", f, cache._check("last", last, (count,), torch.int32), count, span, b)
+    cache._call("rtxllm_kv_page_bounds_f16", f, cache._check("last", last, (count,), torch.int32), count,
+                _u32("span", span), b)
     return bounds
 
 
 def select_workspace(cache: PagedKV, count: int) -> torch.Tensor:
-    return cache._space(None, int(lib().rtxllm_attn_select_workspace(cache.ref, count)))
+    return cache._space(None, int(lib().rtxllm_attn_select_workspace(cache.ref, _u32("count", count))))
 
 
 def select_pages(cache: PagedKV, bounds: torch.Tensor, q: torch.Tensor, pos: torch.Tensor, n_select: int,
@@ -161,15 +172,17 @@ def select_pages(cache: PagedKV, bounds: torch.Tensor, q: torch.Tensor, pos: tor
     b = cache._check("bounds", bounds, (cache.n_pages, cache.n_kv_heads, 2, cache.head_dim), torch.float16)
     qp = cache._check("q", q, (count, heads, cache.head_dim))
     pp = cache._check("pos", pos, (count,), torch.int32)
+    first, last, select = _u32("n_first", n_first), _u32("n_last", n_last), _u32("n_select", n_select)
     pages = cache._output("pages", pages, (count, cache.n_kv_heads, n_select), torch.int32, -1)
     ws = cache._space(workspace, int(lib().rtxllm_attn_select_workspace(cache.ref, count)))
-    cache._call("rtxllm_attn_select_pages", b, qp, heads, pp, count, n_first, n_last, n_select, pages.data_ptr(),
+    cache._call("rtxllm_attn_select_pages", b, qp, heads, pp, count, first, last, select, pages.data_ptr(),
                 ws.data_ptr(), ws.numel())
     return pages
 
 
 def attn_pages_workspace(cache: PagedKV, n_heads: int, n_select: int, count: int) -> torch.Tensor:
-    return cache._space(None, int(lib().rtxllm_attn_pages_workspace(cache.ref, n_heads, n_select, count)))
+    return cache._space(None, int(lib().rtxllm_attn_pages_workspace(cache.ref, _u32("n_heads", n_heads), _u32("n_select", n_select),
+                                                              _u32("count", count))))
 
 
 def attn_pages(cache: PagedKV, q: torch.Tensor, pages: torch.Tensor, pos: torch.Tensor,
@@ -191,7 +204,7 @@ def attn_pages(cache: PagedKV, q: torch.Tensor, pages: torch.Tensor, pos: torch.
 
 
 def attn_weights_workspace(cache: PagedKV, n_heads: int, count: int) -> torch.Tensor:
-    return cache._space(None, int(lib().rtxllm_attn_weights_workspace(cache.ref, n_heads, count)))
+    return cache._space(None, int(lib().rtxllm_attn_weights_workspace(cache.ref, _u32("n_heads", n_heads), _u32("count", count))))
 
 
 def attn_weights(cache: PagedKV, q: torch.Tensor, last: torch.Tensor, weight: torch.Tensor,
@@ -217,7 +230,7 @@ def attn_weights(cache: PagedKV, q: torch.Tensor, last: torch.Tensor, weight: to
 
 
 def evict_workspace(cache: PagedKV, keep: int, count: int) -> torch.Tensor:
-    return cache._space(None, int(lib().rtxllm_kv_evict_workspace(cache.ref, keep, count)))
+    return cache._space(None, int(lib().rtxllm_kv_evict_workspace(cache.ref, _u32("keep", keep), _u32("count", count))))
 
 
 def evict(cache: PagedKV, length: torch.Tensor, pos: torch.Tensor, keep: int, weight: torch.Tensor,
@@ -237,6 +250,7 @@ def evict(cache: PagedKV, length: torch.Tensor, pos: torch.Tensor, keep: int, we
     wo = wp if weight_out is None else cache._check("weight_out", weight_out, state)
     so = sp if slot_pos_out is None else cache._check("slot_pos_out", slot_pos_out, state, torch.int32)
     lo = lp if length_out is None else cache._check("length_out", length_out, (count,), torch.int32)
-    ws = cache._space(workspace, int(lib().rtxllm_kv_evict_workspace(cache.ref, keep, count)))
-    cache._call("rtxllm_kv_evict_f16", lp, pp, count, keep, n_first, n_recent, wp, sp, wo, so, lo, ws.data_ptr(),
+    first, recent = _u32("n_first", n_first), _u32("n_recent", n_recent)
+    ws = cache._space(workspace, int(lib().rtxllm_kv_evict_workspace(cache.ref, _u32("keep", keep), count)))
+    cache._call("rtxllm_kv_evict_f16", lp, pp, count, keep, first, recent, wp, sp, wo, so, lo, ws.data_ptr(),
                 ws.numel())

@@ -265,3 +265,47 @@ def test_attention_with_the_largest_queries(group, dim):
             top = int(np.argmin(steps) if h % 2 else np.argmax(steps))
             np.testing.assert_allclose(row, s.v[p[top], 0, o[top]], rtol=1e-6)
     assert float(weight.sum()) == group
+
+
+# ---- the wrapper's numbers --------------------------------------------------------------
+
+
+def test_numbers_are_not_cut_to_32_bits():
+    """What the C-ABI's unsigned arguments cannot hold is refused, not taken for its low bits."""
+    k = torch.zeros(1, 1, 65536, 64, dtype=torch.float16, device=DEV)
+    for entries in (65537, 257, 65536):  # 2^32 + 65536, just above 2^24 and 2^32 positions
+        with pytest.raises(ValueError):
+            paged.PagedKV(k, k, torch.zeros(entries, dtype=torch.int32, device=DEV))
+            pytest.fail(f"{entries} entries were not refused")
+    paged.PagedKV(k, k, torch.zeros(256, dtype=torch.int32, device=DEV))
+    for shape in ((0, 1, 8, 64), (1, 0, 8, 64), (1, 1, 0, 64), (1, 1, 8, 0)):
+        none = torch.zeros(shape, dtype=torch.float16, device=DEV)
+        with pytest.raises(ValueError):
+            paged.PagedKV(none, none, torch.zeros(4, dtype=torch.int32, device=DEV))
+            pytest.fail(f"{shape} was not refused")
+    s = Setup(1, [20, 20], 2, 64, 8)
+    c, pos = s.cache, u32([3, 4])
+    q, kn = torch.zeros(2, 4, 64, device=DEV), torch.zeros(2, 2, 64, device=DEV)
+    bounds = torch.zeros(s.n_pages, 2, 2, 64, dtype=torch.float16, device=DEV)
+    state = torch.zeros(2, 2, s.capacity, device=DEV)
+    over = 1 << 32
+    before = [t.clone() for t in (s.kd, s.vd, bounds, state)]
+    bad = [lambda: paged.qk_norm_rope_append(c, q, kn, kn, None, None, pos, theta=1e4, rotary_dim=over + 64),
+           lambda: paged.page_bounds(c, pos, bounds, span=over + 1),
+           lambda: paged.select_workspace(c, over + 1),
+           lambda: paged.select_pages(c, bounds, q, pos, over + 3),
+           lambda: paged.select_pages(c, bounds, q, pos, 3, n_first=over),
+           lambda: paged.select_pages(c, bounds, q, pos, 3, n_last=-over),
+           lambda: paged.attn_pages_workspace(c, over + 4, 3, 2),
+           lambda: paged.attn_pages_workspace(c, 4, over + 3, 2),
+           lambda: paged.attn_weights_workspace(c, 4, over + 2),
+           lambda: paged.evict_workspace(c, over + 4, 2),
+           lambda: paged.evict(c, pos, pos, over + 4, state, state.int()),
+           lambda: paged.evict(c, pos, pos, 4, state, state.int(), n_first=over),
+           lambda: paged.evict(c, pos, pos, 4, state, state.int(), n_recent=-1)]
+    for i, call in enumerate(bad):
+        with pytest.raises(ValueError):
+            call()
+            pytest.fail(f"call {i} was not refused")
+    for t, b in zip((s.kd, s.vd, bounds, state), before):
+        torch.testing.assert_close(t, b, rtol=0, atol=0, equal_nan=True)
