@@ -12,7 +12,8 @@
  * arguments (before any launch), or the launch's error. A workspace belongs to
  * one call until that call's work is done: calls that may overlap (two streams,
  * two graphs replayed at once) need one each. Results do not depend on it or on
- * timing: no call adds with atomics. */
+ * timing: no call adds with atomics. What a call writes (the workspace among it) shares
+ * memory with no other array of the call but where its description allows it. */
 #ifndef RTXLLM_PAGED_KV_H
 #define RTXLLM_PAGED_KV_H
 

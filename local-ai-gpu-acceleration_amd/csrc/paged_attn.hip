@@ -684,6 +684,10 @@ extern "C" hipError_t rtxllm_attn_decode_pages_gqa_f16(const rtxllm_paged_kv* ca
     return hipErrorInvalidValue;
   const AttnSpace s = attn_space(cache, n_heads, static_cast<std::uint64_t>(n_select) * cache->page_size, count, false);
   if (s.bytes == 0u || workspace_bytes < s.bytes) return hipErrorInvalidValue;
+  // a row of one split has its result while others read their lists and positions
+  const std::uint64_t rows = rows_bytes(cache, n_heads, count);
+  if (overlap(out, rows, pages, 4ull * count * cache->n_kv_heads * n_select) || overlap(out, rows, pos, 4u * count))
+    return hipErrorInvalidValue;
   AttnArgs a = attn_args(q, pos, out, workspace, s, paged_group(cache, n_heads));
   a.pages = pages;
   a.n_select = n_select;
@@ -709,7 +713,11 @@ extern "C" hipError_t rtxllm_attn_decode_weights_gqa_f16(const rtxllm_paged_kv* 
   const AttnSpace s = attn_space(cache, n_heads, cache->capacity, count, true);
   if (s.bytes == 0u || workspace_bytes < s.bytes) return hipErrorInvalidValue;
   const std::size_t n = 4u * static_cast<std::size_t>(count) * cache->n_kv_heads * cache->capacity;
-  if (weight_out != weight && overlap(weight_out, n, weight, n)) return hipErrorInvalidValue;
+  const std::uint64_t rows = rows_bytes(cache, n_heads, count);
+  // some workgroups of the merge write results while others read weights
+  if ((weight_out != weight && overlap(weight_out, n, weight, n)) || overlap(out, rows, weight, n) ||
+      overlap(out, rows, weight_out, n) || overlap(weight_out, n, last, 4u * count) || overlap(out, rows, last, 4u * count))
+    return hipErrorInvalidValue;
   const AttnArgs a = attn_args(q, last, out, workspace, s, paged_group(cache, n_heads));
   const PagedView view = paged_view(cache);
   return cache->head_dim == 64u    ? launch_weights<64>(a, view, count, weight, weight_out, stream)

@@ -733,7 +733,9 @@ extern "C" hipError_t rtxllm_kv_evict_f16(const rtxllm_paged_kv* cache, const ui
       overlap(weight_out, n, slot_pos_out, n) || (length_out != length && overlap(length_out, 4u * count, length, 4u * count)) ||
       overlap(length_out, 4u * count, pos, 4u * count) || overlap(length_out, 4u * count, weight, n) ||
       overlap(length_out, 4u * count, slot_pos, n) || overlap(length_out, 4u * count, weight_out, n) ||
-      overlap(length_out, 4u * count, slot_pos_out, n))
+      overlap(length_out, 4u * count, slot_pos_out, n) || overlap(weight_out, n, length, 4u * count) ||
+      overlap(weight_out, n, pos, 4u * count) || overlap(slot_pos_out, n, length, 4u * count) ||
+      overlap(slot_pos_out, n, pos, 4u * count))
     return hipErrorInvalidValue;
   const PagedView view = paged_view(cache);
   const std::uint32_t most = most_moves(cache, keep), per = kThreads / (cache->head_dim / 8u);
