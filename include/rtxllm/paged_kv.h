@@ -59,7 +59,8 @@ typedef struct {
  * q, k and v rows lie q_stride, k_stride and v_stride floats apart (one stacked
  * projection's output: the same stride three times); any 4-byte alignment.
  * rotary_dim % 8 == 0, 8..head_dim. pos[r] RTXLLM_NO_POSITION: a padded row. A slot >=
- * capacity (or in no page) stores nothing; q_out is written all the same.
+ * capacity stores nothing, one in no page its position and weight alone; q_out is written all the
+ * same.
  * slot_pos, slot_weight (each may be null): uint32 and fp32 [rows][n_kv_heads]
  * [capacity], one row per sequence (one in all with table_stride 0); the new slot
  * gets pos[r] and 0 for every head. Rows of one call must not share a slot.
@@ -153,7 +154,8 @@ hipError_t rtxllm_attn_decode_weights_gqa_f16(const rtxllm_paged_kv* cache, cons
  * length). A row with pos[r] RTXLLM_NO_POSITION is a padded row. A slot in no
  * page has nothing to move and no room: whatever its weight and position it stays where
  * it lies below keep and leaves where it lies behind, and the others fill what is left of keep.
- * Sequences of one call must not share pages. n_first + n_recent <= keep <=
+ * Page bounds do not follow: those of the kept slots' pages are to be computed anew (first 0, last
+ * keep - 1). Sequences of one call must not share pages. n_first + n_recent <= keep <=
  * capacity, keep >= 1, count <= 65535; table_stride 0 only with count 1. */
 size_t rtxllm_kv_evict_workspace(const rtxllm_paged_kv* cache, uint32_t keep, uint32_t count);
 hipError_t rtxllm_kv_evict_f16(const rtxllm_paged_kv* cache, const uint32_t* length, const uint32_t* pos,

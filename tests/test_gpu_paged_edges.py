@@ -12,7 +12,7 @@ import pytest
 torch = pytest.importorskip("torch")
 
 from rtxllm_amd import paged  # noqa: E402
-from test_gpu_paged import DEV, Setup, dev, u32  # noqa: E402
+from test_gpu_paged import DEV, Setup, check_attention, dev, u32  # noqa: E402
 
 pytestmark = pytest.mark.gpu
 
@@ -309,3 +309,35 @@ def test_numbers_are_not_cut_to_32_bits():
             pytest.fail(f"call {i} was not refused")
     for t, b in zip((s.kd, s.vd, bounds, state), before):
         torch.testing.assert_close(t, b, rtol=0, atol=0, equal_nan=True)
+
+
+# ---- eviction and selection of one cache --------------------------------------------------
+
+
+def test_selection_after_an_eviction():
+    """Rows move into other pages: with the bounds of the kept slots' pages computed anew the
+    selection and its attention are those of what the slots hold now."""
+    s = Setup(23, [200, 150], 2, 128, 16)
+    group, keep, select = 3, 100, 4
+    weight = s.rng.random((2, 2, s.capacity)).astype(np.float32)
+    slot_pos = np.broadcast_to(np.arange(s.capacity, dtype=np.uint32), weight.shape)
+    length, pos = u32(s.lens), u32(s.last())
+    bounds = torch.zeros(s.n_pages, 2, 2, 128, dtype=torch.float16, device=DEV)
+    zero = torch.zeros_like(pos)
+    paged.page_bounds(s.cache, pos, bounds, zero, s.entries)
+    paged.evict(s.cache, length, pos, keep, dev(weight), u32(slot_pos), 2, 10)
+    last = u32([keep - 1] * 2)
+    paged.page_bounds(s.cache, last, bounds, zero, s.entries)
+    q = s.rng.standard_normal((2, 2 * group, 128)).astype(np.float32)
+    pages = paged.select_pages(s.cache, bounds, dev(q), last, select, 1, 1)
+    out = paged.attn_pages(s.cache, dev(q), pages, last).cpu().numpy()
+    s.k, s.v = s.kd.cpu().numpy(), s.vd.cpu().numpy()
+    gb, gp = bounds.cpu().numpy(), pages.cpu().numpy()
+    for i in range(2):
+        for g in range(2):
+            for t in range(-(-keep // 16)):
+                p = s.table[i, t]
+                np.testing.assert_array_equal(gb[p, g], ref.bounds_of(s.k[p, g, :min(16, keep - 16 * t)]))
+            want = ref.select(q[i, g * group:(g + 1) * group], gb[:, g], s.table[i], s.n_pages, 7, 1, 1, select)
+            assert gp[i, g].tolist() == want
+            check_attention(s, out, q, i, g, group, [x for t in want for x in range(16 * t, min(keep, 16 * t + 16))])
