@@ -87,6 +87,52 @@ inline std::uint32_t paged_group(const rtxllm_paged_kv* c, std::uint32_t n_heads
   return g <= kMaxQueryGroup ? g : 0u;
 }
 
+// ---- which form of a kernel takes a call ----------------------------------------
+
+// Append: one workgroup a row saves the row's angles and the others' starts where rows alone
+// fill the chip (us of one / several a row: 32 + 2 x 8 heads of 128 at 512 rows 7.6 /
+// 6.8, 1024 11.7 / 11.9, 4001 32.5 / 34.2; 16 + 2 x 2 of 256 at 4001 27.8 / 30.7; rows that
+// one workgroup holds at once, 8 + 2 x 1 of 64 at 4001, 8.8 / 7.9). units: heads of a row, per: of a
+// workgroup.
+inline bool append_row_a_workgroup(std::uint32_t count, std::uint32_t units, std::uint32_t per) {
+  return count >= 1024u && units > per;
+}
+
+// Page bounds: three ways to share the pages out, by the units (a page of a head) and by the
+// rounds of 256 / L keys (L = head_dim / 8 lanes a key) that a wave reads one at a page of them.
+// Few units: a page's rounds go to the four waves of a workgroup (8 heads of 128, us of one wave / four:
+// 256 keys at 8000 positions 12.5 / 5.9 and at 24000 15.0 / 10.9, 128 at 16000 9.1 / 8.7
+// and at 32000 13.0 / 13.2, 64 at 4000 5.4 / 4.4 and at 8000 5.6 / 6.2, 32 at 2000 3.4 / 3.7; the newest page
+// alone of 256 keys 6.2 / 3.4, of 16, one round, 2.8 / 3.1). The keys stay in the
+// caches then: a newest page alone is attended next.
+// Pages of less than a round: L lanes take a page each (60000 positions of 8 heads, us of
+// a wave / L lanes: 8 keys of 128 38.2 / 29.0, 16 of 64 30.1 / 19.6, 16 of 128 26.6 / 27.3).
+// Everything else: a wave a page, streamed past the caches, which hold nothing of it for
+// long.
+enum class BoundsForm { kFourWaves, kLanes, kWave };
+inline BoundsForm bounds_form(std::uint64_t units, std::uint32_t rounds) {
+  if (rounds >= 2u && units <= 128u * rounds && units <= 1024u) return BoundsForm::kFourWaves;
+  return rounds == 0u ? BoundsForm::kLanes : BoundsForm::kWave;
+}
+
+// Page scores: four steps a wave from where single steps, whose sums grow with the heads, fill
+// the chip more than once (us of four / one: 504 waves of 4 heads 9.5 / 7.8, 4096 12.0 / 11.5, 8000
+// 12.0 / 12.0, 16384 15.5 / 16.4; the scores alone of 4980 waves of 12 heads 14.0 / 8.6).
+// waves: of single steps.
+inline bool score_four_steps(std::uint64_t waves, std::uint32_t group) {
+  return waves > 8192u * ((group + 3u) / 4u);
+}
+
+// Eviction: a workgroup of 16 waves, but of four where short sequences give each CU several
+// (us of four / 16: 1024 slots of 8 x 8 8.8 / 8.4, of 64 x 8 16.2 / 20.5, 2112 of 8 x 8
+// 14.9 / 9.4). pairs: of a sequence and a kv head.
+inline bool evict_four_waves(std::uint32_t capacity, std::uint64_t pairs) { return capacity <= 1024u && pairs > 256u; }
+
+// Moves that the choosing workgroup makes itself, at most (us of here / in a launch of
+// their own: 64 of 2112 slots 9.3 / 10.6, 96 of 4096 10.6 / 11.1, 256 of 2304 13.5 / 12.4, 512 of
+// 2560 18.3 / 14.4).
+constexpr std::uint32_t kEvictMovesHere = 128;
+
 inline bool aligned_to(const void* p, std::size_t bytes) { return reinterpret_cast<std::uintptr_t>(p) % bytes == 0u; }
 // Whether two ranges of bytes share memory.
 inline bool overlap(const void* a, std::size_t an, const void* b, std::size_t bn) {

@@ -323,11 +323,7 @@ extern "C" hipError_t rtxllm_qk_norm_rope_append_f16(const rtxllm_paged_kv* cach
     else
       hipLaunchKernelGGL((append_kernel<32, kRow>), grid, dim3(kThreads), 0, stream, a, view);
   };
-  // One workgroup a row saves the row's angles and the others' starts where rows alone
-  // fill the chip (us of one / several a row: 32 + 2 x 8 heads of 128 at 512 rows 7.6 /
-  // 6.8, 1024 11.7 / 11.9, 4001 32.5 / 34.2; 16 + 2 x 2 of 256 at 4001 27.8 / 30.7; rows that
-  // one workgroup holds at once, 8 + 2 x 1 of 64 at 4001, 8.8 / 7.9).
-  if (count >= 1024u && units > per)
+  if (append_row_a_workgroup(count, units, per))
     launch(std::true_type{});
   else
     launch(std::false_type{});
@@ -345,25 +341,15 @@ extern "C" hipError_t rtxllm_kv_page_bounds_f16(const rtxllm_paged_kv* cache, co
   const std::uint64_t waves = static_cast<std::uint64_t>(pages) * view.n_kv;
   if (waves > (1ull << 24)) return hipErrorInvalidValue;  // the launch's thread count
   const dim3 grid(static_cast<std::uint32_t>((waves + 3u) / 4u), count);
-  // Three ways to share the pages out, by the units (a page of a head) and by the rounds of
-  // 256 / L keys that a wave reads one at a page of them:
-  // Few units: a page's rounds go to the four waves of a workgroup (8 heads of 128, us of one wave / four:
-  // 256 keys at 8000 positions 12.5 / 5.9 and at 24000 15.0 / 10.9, 128 at 16000 9.1 / 8.7
-  // and at 32000 13.0 / 13.2, 64 at 4000 5.4 / 4.4 and at 8000 5.6 / 6.2, 32 at 2000 3.4 / 3.7; the newest page
-  // alone of 256 keys 6.2 / 3.4, of 16, one round, 2.8 / 3.1). The keys stay in the
-  // caches then: a newest page alone is attended next.
-  // Pages of less than a round: L lanes take a page each (60000 positions of 8 heads, us of
-  // a wave / L lanes: 8 keys of 128 38.2 / 29.0, 16 of 64 30.1 / 19.6, 16 of 128 26.6 / 27.3).
-  // Everything else: a wave a page, streamed past the caches, which hold nothing of it for
-  // long.
   auto launch = [&](auto lanes) {
     constexpr int L = decltype(lanes)::value;
     const std::uint32_t per = kThreads / L, rounds = view.page_size / (256u / L);
     const std::uint64_t units = waves * count;
-    if (rounds >= 2u && units <= 128u * rounds && units <= 1024u)
+    const BoundsForm form = bounds_form(units, rounds);
+    if (form == BoundsForm::kFourWaves)
       hipLaunchKernelGGL((page_bounds_kernel<L, 4>), dim3(static_cast<std::uint32_t>(waves), count), dim3(kThreads), 0,
                          stream, view, first, last, pages, bounds);
-    else if (rounds == 0u)
+    else if (form == BoundsForm::kLanes)
       hipLaunchKernelGGL(prompt_bounds_kernel<L>, dim3(static_cast<std::uint32_t>((waves + per - 1u) / per), count),
                          dim3(kThreads), 0, stream, view, first, last, pages, bounds);
     else

@@ -644,10 +644,7 @@ hipError_t launch_select(const PagedView& view, const std::uint16_t* bounds, con
                        dim3(kThreads), 0, stream, view, bounds, q, group, pos, n_first, n_last, keys);
   };
   const std::uint64_t waves = static_cast<std::uint64_t>(count) * view.n_kv * ((view.entries + 64u / L - 1u) / (64u / L));
-  // four steps a wave from where single steps, whose sums grow with the heads, fill the
-  // chip more than once (us of four / one: 504 waves of 4 heads 9.5 / 7.8, 4096 12.0 / 11.5, 8000
-  // 12.0 / 12.0, 16384 15.5 / 16.4; the scores alone of 4980 waves of 12 heads 14.0 / 8.6)
-  if (waves > 8192u * ((group + 3u) / 4u))
+  if (score_four_steps(waves, group))
     score(std::integral_constant<int, 4>{});
   else
     score(std::integral_constant<int, 1>{});
@@ -664,11 +661,6 @@ hipError_t launch_select(const PagedView& view, const std::uint16_t* bounds, con
     hipLaunchKernelGGL(page_choice_kernel<1024>, choices, dim3(1024), held, stream, view, pos, keys, room, n_select, pages);
   return hipGetLastError();
 }
-
-// Moves that the choosing workgroup makes itself, at most (us of here / in a launch of
-// their own: 64 of 2112 slots 9.3 / 10.6, 96 of 4096 10.6 / 11.1, 256 of 2304 13.5 / 12.4, 512 of
-// 2560 18.3 / 14.4).
-constexpr std::uint32_t kMoveHere = 128;
 
 std::uint32_t most_moves(const rtxllm_paged_kv* c, std::uint32_t keep) {
   const std::uint32_t behind = c->capacity - keep;
@@ -739,9 +731,7 @@ extern "C" hipError_t rtxllm_kv_evict_f16(const rtxllm_paged_kv* cache, const ui
     return hipErrorInvalidValue;
   const PagedView view = paged_view(cache);
   const std::uint32_t most = most_moves(cache, keep), per = kThreads / (cache->head_dim / 8u);
-  // 16 waves, but where short sequences give each CU several workgroups (us of four / 16
-  // waves: 1024 slots of 8 x 8 8.8 / 8.4, of 64 x 8 16.2 / 20.5, 2112 of 8 x 8 14.9 / 9.4)
-  const bool small = view.capacity <= 1024u && static_cast<std::uint64_t>(count) * view.n_kv > 256u;
+  const bool small = evict_four_waves(view.capacity, static_cast<std::uint64_t>(count) * view.n_kv);
   const std::size_t held = held_bytes(view.capacity, 4u, small ? 256u : 1024u);
   const EvictArgs a{length, pos, weight, slot_pos, weight_out, slot_pos_out, static_cast<std::uint32_t*>(workspace),
                     keep,   n_first, n_recent, most, static_cast<std::uint32_t>(held / 4u)};
@@ -753,7 +743,7 @@ extern "C" hipError_t rtxllm_kv_evict_f16(const rtxllm_paged_kv* cache, const ui
       hipLaunchKernelGGL((evict_choice_kernel<1024, L>), dim3(view.n_kv, count), dim3(1024), held, stream, view, a, length_out);
   };
   // In place, a kv head's workgroup may read the length after another has written it.
-  if (most <= kMoveHere && length_out != length) {
+  if (most <= kEvictMovesHere && length_out != length) {
     if (cache->head_dim == 64u)
       choose(std::integral_constant<int, 8>{});
     else if (cache->head_dim == 128u)
