@@ -116,9 +116,9 @@ inline BoundsForm bounds_form(std::uint64_t units, std::uint32_t rounds) {
 }
 
 // Page scores: four steps a wave from where single steps, whose sums grow with the heads, fill
-// the chip more than once (us of four / one: 504 waves of 4 heads 9.5 / 7.8, 4096 12.0 / 11.5, 8000
-// 12.0 / 12.0, 16384 15.5 / 16.4; the scores alone of 4980 waves of 12 heads 14.0 / 8.6).
-// waves: of single steps.
+// the chip more than once (us of the selection with four / one: 504 waves of 4 heads 9.7 / 8.1, 4096
+// 10.9 / 10.6, 8192 13.2 / 14.2, 12000 15.6 / 17.1; of 8 heads 8192 18.8 / 19.1, 12000 23.5 / 24.2; of 12
+// 4096 16.2 / 14.8, 12000 28.3 / 28.6; of 16 12000 33.3 / 33.1). waves: of single steps.
 inline bool score_four_steps(std::uint64_t waves, std::uint32_t group) {
   return waves > 8192u * ((group + 3u) / 4u);
 }

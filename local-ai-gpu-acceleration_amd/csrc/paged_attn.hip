@@ -64,7 +64,10 @@ RTXLLM_HD std::uint32_t attn_per(std::uint64_t items, std::uint64_t tiles, bool 
 // there is room for (a list that ends early, a cache that is not full) is split anew, into at
 // most as many parts (us without / with: 9997 positions of four, lists of 120 pages of 256
 // 37.9 / 22.1; one of 600, lists of 1024 pages of 16 15.8 / 10.3; 2000 slots of 32768 21.9 / 9.7, of
-// eight 51.3 / 26.8, contexts up to 16384 of eight in 16384 68 / 62).
+// eight 51.3 / 26.8, contexts up to 16384 of eight in 16384 68 / 62). A list's end is looked for
+// by every workgroup from the list's start, 64 entries at a time: full lists of 128 pages of 16
+// of 8 kv heads take 8.9 us and 0.2 less with the end known, 1024 19.7 and 2.2, 8192 122 and
+// 34, 65536, the most, 2230 and 1530.
 template <bool WEIGHTS>
 __device__ __forceinline__ std::uint32_t row_per(const AttnArgs& a, std::uint32_t items, std::uint32_t tiles, bool light) {
   if (a.splits == 1u || 2u * tiles > a.per * a.splits) return a.per;
@@ -97,9 +100,12 @@ __device__ __forceinline__ std::uint32_t row_per(const AttnArgs& a, std::uint32_
 // registers in flight, at half the waves, 31.4; with loads that stay in the caches, which a
 // step's other reads need more, 26.8. Workgroups next to each other take the
 // kv heads of one place, which lie next to each other in a page.
-// Waves a SIMD that the registers are held down for, where that pays: 9 to 16 heads (12
-// heads of 64 35.9 -> 33.1 us, of 128 62.9 -> 58.9, of 256 listed 51.0 -> 45.7; of 256 with
-// weights it spills, 67 -> 109, and up to 8 heads of 128 with weights lose, 68 -> 80).
+// Waves a SIMD that the registers are held down for, where that pays: 9 to 16 heads (with
+// weights, 12 heads a kv head, 8 kv heads, six contexts to 16000: of 64 35.9 -> 33.1 us, though
+// two registers spill, of 128 62.9 -> 58.9; 52 listed pages of 64 of seven to 4377, of 256: 51.0 ->
+// 45.7; of 256 with weights it spills more, six to 8000 67 -> 109, and up to 8 heads of 128 with
+// weights lose, eight to 16384 of 4 heads 68 -> 80). 12 heads over 64 listed pages of 64 of eight
+// take the time of their reads: of 128 (134 MB) 25.1 us, of 256 (268 MB) 49.1, 5.4 TB/s.
 template <int D, int T, bool WEIGHTS>
 constexpr int attn_waves() { return T < 4 || (D == 256 && WEIGHTS) ? 1 : D == 64 ? 3 : 2; }
 template <int D, int T, bool WEIGHTS>
@@ -464,7 +470,7 @@ __global__ __launch_bounds__(kThreads, (attn_waves<D, T, WEIGHTS>())) void paged
 // Maximum and sum of one head over its splits' records, by one wave.
 __device__ __forceinline__ float2 head_ml(const float2* __restrict__ ml, std::uint32_t splits, std::uint32_t lane) {
   float M = -INFINITY, l = 0.0f;
-  for (std::uint32_t c0 = 0; c0 < splits; c0 += 256u) {  // (one round up to 262144 positions)
+  for (std::uint32_t c0 = 0; c0 < splits; c0 += 256u) {  // (one round up to 32768 positions; 131072 of one pair: two)
     float2 x[4];
     float m = M;
 #pragma unroll
