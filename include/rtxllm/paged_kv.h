@@ -116,7 +116,7 @@ hipError_t rtxllm_attn_select_pages(const rtxllm_paged_kv* cache, const uint16_t
  * sums in fp32; out fp32 [count][n_heads][head_dim]; a row that attends nothing
  * is 0. What a position that is not attended holds, NaN and infinities included, has
  * no effect; a NaN or an infinity among the attended keys or values makes NaN of what
- * it enters. q and the softmax terms enter the products as pairs of fp16: a query off by
+ * it enters, a score beyond fp32 of its head's result. q and the softmax terms enter the products as pairs of fp16: a query off by
  * 2^-22 of itself or 2^-39 of its head's largest at most, a term by 2^-22 of itself or 2^-40
  * of the largest term. out may be q, and shares no memory with it otherwise. n_heads /
  * n_kv_heads 1..16; count <= 65535; n_select 1..65536, n_select * page_size <= 2^30.

@@ -34,9 +34,8 @@ __device__ __forceinline__ unsigned long long score_key(double s) {
 // Keys of the pages of one (row, kv head): a wave scores kSteps times 64 / L pages, L =
 // head_dim / 8 lanes a page, 8 dimensions a lane. max(q hi, q lo) is q times the larger
 // extreme where q >= 0, the smaller one where it is not: chosen by the sign, two dimensions
-// at a time as fp16 pairs, so that the other extreme enters nothing (an infinite q times a
-// zero of its page would be a NaN, and equal scores would differ by the roundings of what
-// cancels). Products of fp32 and fp16 values are exact in 64 bits; their sums take one
+// at a time as fp16 pairs, so that the other extreme enters nothing (with an infinite q it would
+// make a NaN, and equal scores would differ by the roundings of what cancels). Products of fp32 and fp16 values are exact in 64 bits; their sums take one
 // order for every page. Four heads at a time: two halving exchanges
 // leave each lane one head's part, so that four heads take one head's further steps.
 // What bounds it is the chain of reads (table and q, then bounds): the position is
