@@ -2,7 +2,8 @@
  * KV cache: the append of new keys and values with the norm of every head and
  * its rotation in the same pass; decode attention over pages that a cheap score
  * selects; decode attention that gathers each position's softmax weight, and the
- * eviction of the positions that gathered least. No counterpart in the reference
+ * eviction of the positions that gathered least; attention of new tokens, one or many a
+ * sequence, with a sliding window. No counterpart in the reference
  * (its KV is a flat fp32 arena of side-writes, decode_kernels.cu:1600-1606).
  *
  * All functions but the workspace sizes are asynchronous on `stream`, allocate
@@ -163,6 +164,38 @@ hipError_t rtxllm_kv_evict_f16(const rtxllm_paged_kv* cache, const uint32_t* len
                                const float* weight, const uint32_t* slot_pos, float* weight_out,
                                uint32_t* slot_pos_out, uint32_t* length_out, void* workspace,
                                size_t workspace_bytes, hipStream_t stream);
+
+/* Attention of new tokens with a sliding window: query row i at position p attends, of positions
+ * j <= p, those with p - j < window and those with j < sinks (the first tokens, which stay
+ * visible). window >= 1; one of capacity or more hides nothing.
+ *
+ * The rows of a call: sequence s (0 .. sequences - 1) reads block-table row s and has rows
+ * start[s] .. start[s + 1] - 1 of q and out, none where that is empty; start [sequences + 1] ascends, and
+ * rows behind its last entry, or beyond `rows`, are neither read nor written. start null: row s is sequence s's
+ * only one, rows == sequences. Row start[s] + i is at position pos[s] + i; pos[s]
+ * RTXLLM_NO_POSITION: none of the sequence's rows count. A position at or behind the
+ * capacity attends as the last one does. The cache holds the rows' keys and values already.
+ *
+ * q and out [rows][n_heads][head_dim] of `type`, any alignment to an element; out may be
+ * q and shares no memory with it otherwise. Scores q k / sqrt(head_dim), softmax with the maximum
+ * subtracted, sums in fp32; a row that attends nothing is 0. What a position that a query does not attend holds, NaN
+ * and infinities included, has no effect on it; a NaN in q or among the attended keys or
+ * values makes NaN of what it enters; an infinity makes an infinity or NaN of it, but a score of -infinity weighs
+ * nothing.
+ * RTXLLM_F32: q and the softmax terms enter the products as pairs of fp16, as in
+ * rtxllm_attn_decode_pages_gqa_f16. RTXLLM_F16: q as it is, and where many rows
+ * of a sequence share the reads of its cache, each softmax term as one fp16, off by
+ * 2^-11 of itself or 2^-40 of the largest, as the result is by its own rounding.
+ * n_heads / n_kv_heads 1..16; sequences 1..65535; rows 1..2^20; with table_stride 0 every
+ * sequence reads the one table row. workspace:
+ * rtxllm_attn_window_workspace() bytes for the same numbers, 256-byte aligned. */
+enum { RTXLLM_F32 = 0, RTXLLM_F16 = 1 };
+size_t rtxllm_attn_window_workspace(const rtxllm_paged_kv* cache, uint32_t n_heads, uint32_t sequences,
+                                    uint32_t rows, uint32_t window, uint32_t sinks);
+hipError_t rtxllm_attn_window_f16(const rtxllm_paged_kv* cache, const void* q, int type, uint32_t n_heads,
+                                  const uint32_t* start, const uint32_t* pos, uint32_t sequences, uint32_t rows,
+                                  uint32_t window, uint32_t sinks, void* out, void* workspace, size_t workspace_bytes,
+                                  hipStream_t stream);
 
 #ifdef __cplusplus
 }

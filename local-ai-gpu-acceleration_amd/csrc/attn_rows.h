@@ -1,0 +1,73 @@
+// What the kernels of attention over new rows (attn_rows.hip, attn_prompt.hip) share:
+// the call, and which positions a tile of query rows sees.
+#pragma once
+
+#include "rows.h"
+
+namespace rtxllm {
+
+constexpr std::uint32_t kRowTile = 32;  // positions of a tile
+
+struct AttnRows {
+  const void* q;
+  void* out;
+  float2* ml;   // [unit][kv head][column][split]: maximum (in log2), sum
+  float* part;  // [unit][kv head][column][split][head_dim], not divided by the sum
+  std::uint32_t f16, group, tq, window, sinks, splits, units;  // tq: query rows of a unit
+};
+
+// A unit: up to tq query rows of one sequence. The tiles of positions that one of them sees, in the
+// order they are taken: sink tiles before the window, the window's in the pages, the tail's.
+struct RowSpan {
+  std::uint32_t s, row, nq;      // sequence, first row, rows (0: none)
+  std::uint32_t p0, plast, pos;  // positions of the first and last row (below the capacity); of row i: row_pos
+  std::uint32_t code_end;        // positions below it are read from the pages,
+  std::uint32_t tail;            // those from here on (a block's start) from the tail
+  std::uint32_t ns, lo_tile, ncode, total;  // sink tiles, the window's first tile, tiles in the pages, all
+};
+
+RTXLLM_HD std::uint32_t row_pos(std::uint32_t pos, std::uint32_t i, std::uint32_t capacity) {
+  return pos >= capacity || i >= capacity - pos ? capacity - 1u : pos + i;
+}
+
+RTXLLM_HD RowSpan row_span(const CallRows& c, const RowsCache& kv, std::uint32_t w, std::uint32_t tq, std::uint32_t window,
+                           std::uint32_t sinks, std::uint32_t tile) {
+  RowSpan r{};
+  std::uint32_t base = w;
+  r.s = w;
+  if (c.start != nullptr) r.s = unit_sequence(c, w, tq, 1u, base);
+  const SeqRows q = seq_rows(c, r.s);
+  const std::uint32_t t = w - base;
+  if (w < base || t > q.n / tq || t * tq >= q.n) return r;
+  const std::uint32_t i0 = t * tq, cap = kv.p.capacity;
+  r.row = q.row + i0;
+  r.nq = q.n - i0 < tq ? q.n - i0 : tq;
+  r.pos = q.pos >= cap ? cap : q.pos + i0;
+  r.p0 = row_pos(r.pos, 0u, cap);
+  r.plast = row_pos(r.pos, r.nq - 1u, cap);
+  r.code_end = r.plast + 1u;
+  r.tail = r.plast + 1u;
+  if (kv.block_shift != 0u) {
+    const std::uint32_t whole = held_end(q.pos, q.n, cap) >> kv.block_shift << kv.block_shift;
+    if (whole < r.code_end) r.code_end = r.tail = whole;
+  }
+  r.lo_tile = (r.p0 + 1u > window ? r.p0 + 1u - window : 0u) / tile;
+  const std::uint32_t front = sinks < r.code_end ? sinks : r.code_end, nf = (front + tile - 1u) / tile;
+  const std::uint32_t end_tile = (r.code_end + tile - 1u) / tile;
+  r.ns = nf < r.lo_tile ? nf : r.lo_tile;
+  r.ncode = r.ns + (end_tile > r.lo_tile ? end_tile - r.lo_tile : 0u);
+  r.total = r.ncode + (r.plast + 1u - r.tail + tile - 1u) / tile;
+  return r;
+}
+
+// The first position of tile u of a unit that lies in the pages.
+RTXLLM_HD std::uint32_t span_position(const RowSpan& r, std::uint32_t u, std::uint32_t tile) {
+  return (u < r.ns ? u : u - r.ns + r.lo_tile) * tile;
+}
+
+// Tiles of a split when `splits` may share them, of whole rounds of the workgroup's waves.
+RTXLLM_HD std::uint32_t span_per(std::uint32_t total, std::uint32_t splits, std::uint32_t round) {
+  return ((total + splits - 1u) / splits + round - 1u) / round * round;
+}
+
+}  // namespace rtxllm

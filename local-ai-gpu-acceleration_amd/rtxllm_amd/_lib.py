@@ -75,6 +75,10 @@ _LAUNCH_SIGS: dict[str, list] = {
     "rtxllm_attn_decode_pages_gqa_f16": [_P, _P, _U, _P, _U, _P, _U, _P, _P, c_size_t, _S],
     "rtxllm_attn_decode_weights_gqa_f16": [_P, _P, _U, _P, _U, _P, _P, _P, _P, c_size_t, _S],
     "rtxllm_kv_evict_f16": [_P, _P, _P, _U, _U, _U, _U, _P, _P, _P, _P, _P, _P, c_size_t, _S],
+    "rtxllm_attn_window_f16": [_P, _P, c_int, _U, _P, _P, _U, _U, _U, _U, _P, _P, c_size_t, _S],
+    "rtxllm_kv8_append": [_P, _P, c_size_t, _P, c_size_t, c_int, _P, _P, _U, _U, _S],
+    "rtxllm_kv8_read": [_P, _P, _P, _P, _U, _U, c_int, _P, _P, _S],
+    "rtxllm_attn_kv8": [_P, _P, c_int, _U, _P, _P, _U, _U, _U, _U, _P, _P, c_size_t, _S],
     "rtxllm_iq2s_units_pack": [_P, _U, _U, _P, _S],
     "rtxllm_iq3s_units_pack": [_P, _U, _U, _P, _S],
 }
@@ -105,6 +109,13 @@ class PackOptions(ctypes.Structure):
                 ("names", ctypes.c_char_p), ("layer", c_int), ("limit", c_uint64)]
 
 
+class PagedKV8Struct(ctypes.Structure):
+    """rtxllm_paged_kv8 (include/rtxllm/kv8.h)."""
+    _fields_ = [(n, c_void_p) for n in ("k", "v", "k_scale", "v_scale", "k_tail", "v_tail", "block_table")] + [
+        (n, c_uint32) for n in ("table_stride", "n_pages", "n_kv_heads", "head_dim", "page_size", "capacity",
+                                "block")] + [("format", c_int)]
+
+
 class PagedKVStruct(ctypes.Structure):
     """rtxllm_paged_kv (include/rtxllm/paged_kv.h)."""
     _fields_ = [("k", c_void_p), ("v", c_void_p), ("block_table", c_void_p)] + [
@@ -130,6 +141,8 @@ _HOST_SIGS: dict[str, tuple] = {
     "rtxllm_attn_pages_workspace": (c_size_t, [_P, c_uint32, c_uint32, c_uint32]),
     "rtxllm_attn_weights_workspace": (c_size_t, [_P, c_uint32, c_uint32]),
     "rtxllm_kv_evict_workspace": (c_size_t, [_P, c_uint32, c_uint32]),
+    "rtxllm_attn_window_workspace": (c_size_t, [_P, c_uint32, c_uint32, c_uint32, c_uint32, c_uint32]),
+    "rtxllm_attn_kv8_workspace": (c_size_t, [_P, c_uint32, c_uint32, c_uint32, c_uint32, c_uint32]),
     "rtxllm_llama_destroy": (None, [_P]),
     "rtxllm_llama_weights_changed": (None, [_P]),
     "rtxllm_llama_region": (_P, [_P, ctypes.c_char_p, _U, _P]),
@@ -199,4 +212,4 @@ def check(name: str, code: int) -> None:
 
 
 __all__ = ["lib", "probe_lib", "check", "HipError", "exported_names", "LIB_PATH", "PROBE_LIB_PATH", "PackOptions",
-           "PagedKVStruct", "c_uint16"]
+           "PagedKVStruct", "PagedKV8Struct", "c_uint16"]

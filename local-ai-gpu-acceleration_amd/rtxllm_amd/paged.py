@@ -19,6 +19,7 @@ from ._lib import PagedKVStruct, check, lib
 
 NO_POSITION = -1
 PAIRINGS = {"adjacent": 0, "halves": 1}
+TYPES = {torch.float32: 0, torch.float16: 1}
 
 
 def _u32(name: str, value: int) -> int:
@@ -99,6 +100,22 @@ class PagedKV:
             with torch.cuda.device(index):
                 rc = call(self.ref, *args, stream)
         check(name, rc)
+
+
+def _type_of(name: str, x: torch.Tensor) -> int:
+    if x.dtype in TYPES:
+        return TYPES[x.dtype]
+    raise ValueError(f"{name}: expected float32 or float16, got {x.dtype}")
+
+
+def _call_rows(cache: PagedKV, rows: int, pos: torch.Tensor, start: torch.Tensor | None) -> tuple:
+    """(start, pos, sequences) of a call whose sequences have rows start[s] .. start[s + 1] - 1, or one each."""
+    sequences = pos.numel()
+    cache._rows(sequences)
+    if start is None and rows != sequences:
+        raise ValueError(f"{rows} rows for {sequences} sequences without their starts")
+    at = None if start is None else cache._check("start", start, (sequences + 1,), torch.int32)
+    return at, cache._check("pos", pos, (sequences,), torch.int32), sequences
 
 
 def _rows_of(name: str, cache: PagedKV, x: torch.Tensor, count: int, heads: int | None) -> int:
@@ -254,3 +271,36 @@ def evict(cache: PagedKV, length: torch.Tensor, pos: torch.Tensor, keep: int, we
     ws = cache._space(workspace, int(lib().rtxllm_kv_evict_workspace(cache.ref, _u32("keep", keep), count)))
     cache._call("rtxllm_kv_evict_f16", lp, pp, count, keep, first, recent, wp, sp, wo, so, lo, ws.data_ptr(),
                 ws.numel())
+
+
+def _attn_rows(cache: PagedKV, name: tuple, q: torch.Tensor, pos: torch.Tensor, start: torch.Tensor | None,
+               window: int | None, sinks: int, out: torch.Tensor | None, workspace: torch.Tensor | None) -> torch.Tensor:
+    if q.dim() != 3:
+        raise ValueError(f"q: expected [rows][n_heads][{cache.head_dim}], got {tuple(q.shape)}")
+    rows, heads = q.shape[0], q.shape[1]
+    cache._group(heads)
+    kind = _type_of("q", q)
+    qp = cache._check("q", q, (rows, heads, cache.head_dim), q.dtype)
+    sp, pp, sequences = _call_rows(cache, rows, pos, start)
+    near, first = cache.capacity if window is None else _u32("window", window), _u32("sinks", sinks)
+    out = cache._output("out", out, q.shape, q.dtype, fill=0.0)
+    ws = cache._space(workspace, int(getattr(lib(), name[0])(cache.ref, heads, sequences, rows, near, first)))
+    cache._call(name[1], qp, kind, heads, sp, pp, sequences, rows, near, first, out.data_ptr(), ws.data_ptr(), ws.numel())
+    return out
+
+
+def attn_window_workspace(cache: PagedKV, n_heads: int, sequences: int, rows: int, window: int | None = None,
+                          sinks: int = 0) -> torch.Tensor:
+    near = cache.capacity if window is None else _u32("window", window)
+    return cache._space(None, int(lib().rtxllm_attn_window_workspace(
+        cache.ref, _u32("n_heads", n_heads), _u32("sequences", sequences), _u32("rows", rows), near, _u32("sinks", sinks))))
+
+
+def attn_window(cache: PagedKV, q: torch.Tensor, pos: torch.Tensor, start: torch.Tensor | None = None, *,
+                window: int | None = None, sinks: int = 0, out: torch.Tensor | None = None,
+                workspace: torch.Tensor | None = None) -> torch.Tensor:
+    """Attention of new tokens, q [rows][n_heads][head_dim] of float32 or float16: sequence s has rows start[s] ..
+    start[s + 1] - 1 (start None: row s) at positions pos[s], pos[s] + 1, ... Each sees the positions up to
+    its own that are less than `window` (None: any number) behind it, and the first `sinks`."""
+    return _attn_rows(cache, ("rtxllm_attn_window_workspace", "rtxllm_attn_window_f16"), q, pos, start, window, sinks, out,
+                      workspace)
