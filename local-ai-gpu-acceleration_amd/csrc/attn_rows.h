@@ -6,7 +6,19 @@
 
 namespace rtxllm {
 
-constexpr std::uint32_t kRowTile = 32;  // positions of a tile
+constexpr std::uint32_t kRowTile = 32;     // positions of a tile of attn_rows.hip's form,
+constexpr std::uint32_t kPromptTile = 64;  // of attn_prompt.hip's
+
+// attn_prompt.hip: waves of a workgroup and blocks of 16 columns (query rows times query heads) of a wave.
+constexpr int kPromptWaves = 8;
+constexpr int prompt_blocks(int head_dim, bool f32) { return head_dim == 256 ? 1 : head_dim == 128 ? 2 : f32 ? 1 : 4; }
+inline std::uint32_t prompt_columns(std::uint32_t head_dim, bool f32) {
+  return 16u * kPromptWaves * static_cast<std::uint32_t>(prompt_blocks(static_cast<int>(head_dim), f32));
+}
+
+inline bool rows_prompt(std::uint32_t sequences, std::uint32_t rows, std::uint32_t group, std::uint32_t page_size) {
+  return static_cast<std::uint64_t>(rows) * group >= 64ull * sequences && page_size % 4u == 0u;
+}
 
 struct AttnRows {
   const void* q;
@@ -69,5 +81,10 @@ RTXLLM_HD std::uint32_t span_position(const RowSpan& r, std::uint32_t u, std::ui
 RTXLLM_HD std::uint32_t span_per(std::uint32_t total, std::uint32_t splits, std::uint32_t round) {
   return ((total + splits - 1u) / splits + round - 1u) / round * round;
 }
+
+#if defined(__HIPCC__)
+hipError_t attn_prompt(Cached kind, std::uint32_t head_dim, const AttnRows& a, const CallRows& rows, const RowsCache& kv,
+                       hipStream_t stream);
+#endif
 
 }  // namespace rtxllm

@@ -1,45 +1,12 @@
 // Attention of new rows over a paged cache of fp16 values or 8-bit codes, with a
 // sliding window and sinks: the form for few rows a sequence.
-#include "attn_rows.h"
-#include "common.h"
-#include "layer_common.cuh"
+#include "attn_rows.cuh"
 
 namespace rtxllm {
 namespace {
 
-typedef _Float16 half2 __attribute__((ext_vector_type(2)));
-typedef _Float16 half4 __attribute__((ext_vector_type(4)));
-typedef _Float16 half8 __attribute__((ext_vector_type(8)));
-typedef _Float16 half4_any __attribute__((ext_vector_type(4), aligned(2)));
-typedef _Float16 half8_any __attribute__((ext_vector_type(8), aligned(2)));
-typedef std::uint32_t u32x4 __attribute__((ext_vector_type(4)));
-typedef float f32x4 __attribute__((ext_vector_type(4)));
-
 constexpr std::uint32_t kThreads = 256, kWaves = kThreads / 64u, kCols = 16, kTile = kRowTile;
 constexpr int kLift = 15;  // queries and softmax terms are brought to 2^15, as in paged_attn.hip
-
-__device__ __forceinline__ std::uint32_t from_lane(std::uint32_t v, std::uint32_t lane) {
-  return static_cast<std::uint32_t>(__builtin_amdgcn_ds_bpermute(static_cast<int>(4u * lane), static_cast<int>(v)));
-}
-
-// Two values as fp16, each 1152 too large: 1024 + (code + 128) is 0x6400 | the code with its top bit turned.
-__device__ __forceinline__ std::uint32_t less_1152(std::uint32_t w) {
-  const half2 bias = {static_cast<_Float16>(1152.0f), static_cast<_Float16>(1152.0f)};
-  return __builtin_bit_cast(std::uint32_t, __builtin_bit_cast(half2, w) - bias);
-}
-
-// Four codes of a word as fp16, exactly.
-template <Cached F>
-__device__ __forceinline__ uint2 codes_to_half(std::uint32_t w) {
-  if constexpr (F == Cached::kInt8) {
-    w ^= 0x80808080u;
-    return make_uint2(less_1152(__builtin_amdgcn_perm(0x64646464u, w, 0x05010400u)),
-                      less_1152(__builtin_amdgcn_perm(0x64646464u, w, 0x07030602u)));
-  } else {
-    return make_uint2(__builtin_bit_cast(std::uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.0f, false)),
-                      __builtin_bit_cast(std::uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.0f, true)));
-  }
-}
 
 // A tile's keys and values in a lane's registers. Keys: position col of each half tile, the lane's
 // quarter of the dimensions in D / 32 steps of 8. Values: VPL dimensions from VPL * col on of the 8 positions
@@ -168,7 +135,7 @@ __global__ __launch_bounds__(kThreads) void attn_rows_kernel(AttnRows a, CallRow
     top = fmaxf(top, lane_xor<32>(top));
     int e = 0;
     if (top > 0.0f && top < INFINITY) frexpf(top, &e);
-    qscale = ldexpf(1.4426950408889634f / (D == 64 ? 8.0f : D == 128 ? 11.313708498984761f : 16.0f), e - kLift);
+    qscale = ldexpf(score_scale<D>(), e - kLift);
 #pragma unroll
     for (int j = 0; j < J; ++j)
 #pragma unroll
@@ -456,13 +423,7 @@ __global__ __launch_bounds__(kThreads) void attn_rows_kernel(AttnRows a, CallRow
       const float inv = L == 0.0f ? 0.0f : 1.0f / L;
       const std::uint32_t i = c / a.group;
       const std::size_t dst = (static_cast<std::size_t>(sp.row + i) * n_heads + g * a.group + (c - i * a.group)) * D + d;
-      v *= inv;
-      if (a.f16 != 0u) {
-        const half4 r = {static_cast<_Float16>(v[0]), static_cast<_Float16>(v[1]), static_cast<_Float16>(v[2]), static_cast<_Float16>(v[3])};
-        *reinterpret_cast<half4_any*>(static_cast<_Float16*>(a.out) + dst) = half4_any(r);
-      } else {
-        *reinterpret_cast<f32x4_any*>(static_cast<float*>(a.out) + dst) = f32x4_any(v);
-      }
+      store_row4(a, dst, v * inv);
     } else {
       const std::size_t dst = ((static_cast<std::size_t>(unit) * kv.p.n_kv + g) * ncol + c) * a.splits + split;
       *reinterpret_cast<f32x4*>(a.part + dst * D + d) = v;
@@ -512,34 +473,61 @@ __global__ __launch_bounds__(kThreads) void merge_rows_kernel(AttnRows a, CallRo
   v *= L == 0.0f ? 0.0f : 1.0f / L;
   const std::uint32_t i = c / a.group;
   const std::size_t dst = (static_cast<std::size_t>(sp.row + i) * a.group * kv.p.n_kv + g * a.group + (c - i * a.group)) * D + d;
-  if (a.f16 != 0u) {
-    const half4 r = {static_cast<_Float16>(v[0]), static_cast<_Float16>(v[1]), static_cast<_Float16>(v[2]), static_cast<_Float16>(v[3])};
-    *reinterpret_cast<half4_any*>(static_cast<_Float16*>(a.out) + dst) = half4_any(r);
-  } else {
-    *reinterpret_cast<f32x4_any*>(static_cast<float*>(a.out) + dst) = f32x4_any(v);
+  store_row4(a, dst, v);
+}
+
+// The same for many columns of few splits: D / 4 lanes a column, its records one after the other.
+template <int D>
+__global__ __launch_bounds__(kThreads) void merge_few_kernel(AttnRows a, CallRows rows, RowsCache kv, std::uint32_t tile,
+                                                             std::uint32_t round) {
+  constexpr std::uint32_t kLanes = D / 4u, kPer = kThreads / kLanes;
+  const std::uint32_t ncol = a.tq * a.group, blocks = (ncol + kPer - 1u) / kPer, ug = blockIdx.x / blocks, g = ug % kv.p.n_kv;
+  const std::uint32_t c = (blockIdx.x % blocks) * kPer + threadIdx.x / kLanes, d = 4u * (threadIdx.x % kLanes);
+  const RowSpan sp = row_span(rows, kv, ug / kv.p.n_kv, a.tq, a.window, a.sinks, tile);
+  if (c >= sp.nq * a.group) return;
+  const std::uint32_t per = span_per(sp.total, a.splits, round), used = (sp.total + per - 1u) / per;
+  if (used <= 1u) return;
+  const std::size_t at = (static_cast<std::size_t>(ug) * ncol + c) * a.splits;
+  f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
+  float M = -INFINITY, L = 0.0f;
+#pragma unroll 4
+  for (std::uint32_t x = 0; x < used; ++x) {
+    const float2 t = a.ml[at + x];
+    const f32x4 o = *reinterpret_cast<const f32x4*>(a.part + (at + x) * D + d);
+    const float mn = fmaxf(M, t.x), base = mn == -INFINITY ? 0.0f : mn;
+    const float f0 = __builtin_amdgcn_exp2f(M - base), f1 = __builtin_amdgcn_exp2f(t.x - base);
+    v = v * f0 + o * f1;
+    L = L * f0 + t.y * f1;
+    M = mn;
   }
+  const std::uint32_t i = c / a.group;
+  store_row4(a, (static_cast<std::size_t>(sp.row + i) * a.group * kv.p.n_kv + g * a.group + (c - i * a.group)) * D + d,
+             v * (L == 0.0f ? 0.0f : 1.0f / L));
 }
 
 struct RowsPlan {
+  bool prompt = false;
   std::uint32_t tq = 0, units = 0, splits = 0;
   std::size_t ml = 0, bytes = 0;  // bytes 0: refused
 };
 
-RowsPlan rows_plan(const rtxllm_paged_kv* c, std::uint32_t n_heads, bool one_each, std::uint32_t sequences, std::uint32_t rows,
-                   std::uint32_t window, std::uint32_t sinks) {
+RowsPlan rows_plan(const rtxllm_paged_kv* c, std::uint32_t n_heads, bool f16, bool one_each, std::uint32_t sequences,
+                   std::uint32_t rows, std::uint32_t window, std::uint32_t sinks) {
   RowsPlan p;
   const std::uint32_t group = paged_group(c, n_heads);
   if (group == 0u || window == 0u) return p;
-  p.tq = one_each ? 1u : kCols / group;
+  p.prompt = !one_each && rows_prompt(sequences, rows, group, c->page_size);
+  p.tq = one_each ? 1u : (p.prompt ? prompt_columns(c->head_dim, !f16) : kCols) / group;
   p.units = one_each ? sequences : units_of(sequences, rows, p.tq, 1u);
   const std::uint64_t items = static_cast<std::uint64_t>(p.units) * c->n_kv_heads;
   const std::uint64_t near = static_cast<std::uint64_t>(window) + p.tq + sinks;
-  const std::uint64_t tiles = (near < c->capacity ? near : c->capacity) / kTile + 3u;
-  std::uint64_t splits = (1024u + items - 1u) / items;
-  const std::uint64_t most = (tiles + 7u) / 8u;
+  const std::uint64_t tiles = (near < c->capacity ? near : c->capacity) / (p.prompt ? kPromptTile : kTile) + 3u;
+  std::uint64_t splits = p.prompt ? (items >= 192u ? 1u : (256u + items - 1u) / items) : (1024u + items - 1u) / items;
+  const std::uint64_t most = p.prompt ? (tiles + 3u) / 4u : (tiles + 7u) / 8u;
   if (splits > most) splits = most;
   p.splits = static_cast<std::uint32_t>(splits);
-  if (items * splits > (1u << 24) || items * p.tq * group > (1u << 24)) return p;  // the launches' thread counts
+  // the launches' thread counts
+  if (items * splits * (p.prompt ? 64u * kPromptWaves : kThreads) > 0xFFFFFFFFull || (splits > 1u && items * p.tq * group > (1u << 24))) return p;
   const std::uint64_t records = splits > 1u ? items * p.tq * group * splits : 0u;
   p.ml = round_256(8u * records);
   p.bytes = p.ml + round_256(4u * records * c->head_dim) + 256u;
@@ -547,9 +535,12 @@ RowsPlan rows_plan(const rtxllm_paged_kv* c, std::uint32_t n_heads, bool one_eac
 }
 
 template <int D>
-hipError_t launch_rows(Cached kind, const AttnRows& a, const CallRows& rows, const RowsCache& kv, hipStream_t stream) {
+hipError_t launch_rows(Cached kind, bool prompt, const AttnRows& a, const CallRows& rows, const RowsCache& kv, hipStream_t stream) {
   const dim3 grid(a.units * a.splits * kv.p.n_kv), block(kThreads);
-  if (kind == Cached::kInt8)
+  hipError_t rc = hipSuccess;
+  if (prompt)
+    rc = attn_prompt(kind, D, a, rows, kv, stream);
+  else if (kind == Cached::kInt8)
     hipLaunchKernelGGL((attn_rows_kernel<D, Cached::kInt8, true>), grid, block, 0, stream, a, rows, kv);
   else if (kind == Cached::kE4m3)
     hipLaunchKernelGGL((attn_rows_kernel<D, Cached::kE4m3, true>), grid, block, 0, stream, a, rows, kv);
@@ -557,9 +548,14 @@ hipError_t launch_rows(Cached kind, const AttnRows& a, const CallRows& rows, con
     hipLaunchKernelGGL((attn_rows_kernel<D, Cached::kF16, true>), grid, block, 0, stream, a, rows, kv);
   else
     hipLaunchKernelGGL((attn_rows_kernel<D, Cached::kF16, false>), grid, block, 0, stream, a, rows, kv);
-  const hipError_t rc = hipGetLastError();
+  if (rc == hipSuccess) rc = hipGetLastError();
   if (rc != hipSuccess || a.splits == 1u) return rc;
-  hipLaunchKernelGGL(merge_rows_kernel<D>, dim3(a.units * kv.p.n_kv * a.tq * a.group), block, 0, stream, a, rows, kv, kTile, kWaves);
+  const std::uint32_t cols = a.tq * a.group, per = kThreads / (D / 4u);
+  if (prompt)
+    hipLaunchKernelGGL(merge_few_kernel<D>, dim3(a.units * kv.p.n_kv * ((cols + per - 1u) / per)), block, 0, stream, a, rows, kv,
+                       kPromptTile, 1u);
+  else
+    hipLaunchKernelGGL(merge_rows_kernel<D>, dim3(a.units * kv.p.n_kv * cols), block, 0, stream, a, rows, kv, kTile, kWaves);
   return hipGetLastError();
 }
 
@@ -569,7 +565,7 @@ hipError_t attn_rows(Cached kind, const rtxllm_paged_kv* pages, const RowsCache&
   if (q == nullptr || out == nullptr || workspace == nullptr || !type_ok(type) || !aligned_to(q, type_bytes(type)) ||
       !aligned_to(out, type_bytes(type)) || !aligned_to(workspace, 256u))
     return hipErrorInvalidValue;
-  const RowsPlan p = rows_plan(pages, n_heads, rows.start == nullptr, rows.sequences, rows.rows, window, sinks);
+  const RowsPlan p = rows_plan(pages, n_heads, type == RTXLLM_F16, rows.start == nullptr, rows.sequences, rows.rows, window, sinks);
   if (p.bytes == 0u || workspace_bytes < p.bytes) return hipErrorInvalidValue;
   const std::uint64_t n = type_bytes(type) * static_cast<std::uint64_t>(rows.rows) * n_heads * pages->head_dim;
   const std::uint64_t table = 4ull * ((rows.sequences - 1ull) * pages->table_stride + pages->capacity / pages->page_size);
@@ -593,19 +589,24 @@ hipError_t attn_rows(Cached kind, const rtxllm_paged_kv* pages, const RowsCache&
   a.sinks = sinks < pages->capacity ? sinks : pages->capacity;
   a.splits = p.splits;
   a.units = p.units;
-  return pages->head_dim == 64u    ? launch_rows<64>(kind, a, rows, kv, stream)
-         : pages->head_dim == 128u ? launch_rows<128>(kind, a, rows, kv, stream)
-                                   : launch_rows<256>(kind, a, rows, kv, stream);
+  return pages->head_dim == 64u    ? launch_rows<64>(kind, p.prompt, a, rows, kv, stream)
+         : pages->head_dim == 128u ? launch_rows<128>(kind, p.prompt, a, rows, kv, stream)
+                                   : launch_rows<256>(kind, p.prompt, a, rows, kv, stream);
 }
 
-// A call's workspace serves both forms of its rows, one each or with starts.
+// A workspace serves every call of its numbers: of either type, with starts or one row each.
 std::size_t attn_rows_bytes(const rtxllm_paged_kv* c, std::uint32_t n_heads, std::uint32_t sequences, std::uint32_t rows,
                             std::uint32_t window, std::uint32_t sinks) {
   if (sequences == 0u || sequences > 65535u || rows == 0u || rows > (1u << 20)) return 0u;
-  const std::size_t many = rows_plan(c, n_heads, false, sequences, rows, window, sinks).bytes;
-  if (many == 0u || rows != sequences) return many;
-  const std::size_t one = rows_plan(c, n_heads, true, sequences, rows, window, sinks).bytes;
-  return one == 0u ? 0u : one > many ? one : many;
+  std::size_t most = 0u;
+  for (const bool f16 : {false, true})
+    for (const bool one_each : {false, true}) {
+      if (one_each && rows != sequences) continue;
+      const std::size_t n = rows_plan(c, n_heads, f16, one_each, sequences, rows, window, sinks).bytes;
+      if (n == 0u) return 0u;
+      most = n > most ? n : most;
+    }
+  return most;
 }
 
 }  // namespace
