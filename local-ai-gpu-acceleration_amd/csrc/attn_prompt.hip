@@ -193,17 +193,11 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_prompt_kernel(AttnRows a, Cal
       v[i] = make_uint2(__builtin_amdgcn_perm(w[1][i / 2], w[0][i / 2], sel), __builtin_amdgcn_perm(w[3][i / 2], w[2][i / 2], sel));
     }
   };
-  // Values that are not finite leave a tile that some row sees in part (0 times them would not be 0); rows that
-  // see them get their NaN at the end.
-  auto finite_only = [](u32x2& w) {
-    bool bad = false;
-#pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      const bool lo = (w[k] & 0x7C00u) == 0x7C00u, hi = (w[k] & 0x7C000000u) == 0x7C000000u;
-      if (lo || hi) w[k] &= (lo ? 0u : 0xFFFFu) | (hi ? 0u : 0xFFFF0000u);
-      bad |= lo || hi;
-    }
-    return bad;
+  auto drop = [](u32x2& w) {
+    std::uint32_t lo = w[0], hi = w[1];
+    const bool bad_lo = finite_only(lo), bad_hi = finite_only(hi);
+    w = u32x2{lo, hi};
+    return bad_lo || bad_hi;
   };
   // Whether some row of the unit does not see all of a tile that some row sees.
   auto is_edge = [&](std::uint32_t j0, unsigned long long s) {
@@ -271,7 +265,7 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_prompt_kernel(AttnRows a, Cal
           for (int e = 0; e < 4; ++e) w[e] = vraw[i][e];
           if (edge) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) bad |= finite_only(w[e]);
+            for (int e = 0; e < 4; ++e) bad |= drop(w[e]);
           }
           turn_halves(w, v);
         }
@@ -306,7 +300,7 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_prompt_kernel(AttnRows a, Cal
         for (int e = 0; e < 4; ++e) {
           const u32x2 t = *reinterpret_cast<const u32x2*>(kv.vt + place(4u * quad + e) + 4u * unit_dims(x));
           w[e] = (seen >> (4u * quad + e) & 1u) != 0u ? t : u32x2{0u, 0u};
-          bad |= finite_only(w[e]);
+          bad |= drop(w[e]);
         }
         uint2 v[4];
         turn_halves(w, v);
@@ -535,43 +529,7 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_prompt_kernel(AttnRows a, Cal
       if (qq == 0u) a.ml[at] = make_float2(sum != sum ? INFINITY : m[n], sum);
     }
   }
-  if (odd == 0u) return;
-  // Some value of a tile at an edge is not finite: NaN where a row sees it.
-  __syncthreads();
-#pragma unroll 1
-  for (std::uint32_t u = u0; u < u1; ++u) {
-#pragma unroll 1
-    for (std::uint32_t x = tid; x < 64u * D; x += T) {
-      const std::uint32_t j = first_of(u) + x / D, d = x % D;
-      if (j > sp.plast) continue;
-      bool bad = false;
-      if (u >= sp.ncode) {
-        const std::uint32_t block = 1u << kv.block_shift;
-        bad = CODES && (kv.vt[((static_cast<std::size_t>(sp.s) * kv.p.n_kv + g) * block + (j & (block - 1u))) * D + d] & 0x7C00u) == 0x7C00u;
-      } else if (j < sp.code_end) {
-        const std::uint32_t r = paged_slot_row(kv.p, table, g, j);
-        if (r != kNoRow)
-          bad = CODES ? !(fabsf(kv.vs[r >> kv.block_shift]) < INFINITY)
-                      : (reinterpret_cast<const std::uint16_t*>(kv.v)[static_cast<std::size_t>(r) * D + d] & 0x7C00u) == 0x7C00u;
-      }
-      if (!bad) continue;
-#pragma unroll 1
-      for (std::uint32_t i = 0; i < sp.nq; ++i) {
-        const std::uint32_t p = row_pos(sp.pos, i, cap);
-        if (j > p || !(p - j < a.window || j < a.sinks)) continue;
-#pragma unroll 1
-        for (std::uint32_t h = 0; h < a.group; ++h) {
-          const std::size_t at = (static_cast<std::size_t>(sp.row + i) * n_heads + g * a.group + h) * D + d;
-          if (per < sp.total)
-            a.part[(((static_cast<std::size_t>(unit) * kv.p.n_kv + g) * (a.tq * a.group) + i * a.group + h) * a.splits + split) * D + d] = NAN;
-          else if (a.f16 != 0u)
-            static_cast<_Float16*>(a.out)[at] = static_cast<_Float16>(NAN);
-          else
-            static_cast<float*>(a.out)[at] = NAN;
-        }
-      }
-    }
-  }
+  if (odd != 0u) not_finite_rows<D, CODES, !F32>(a, rows, kv, unit, g, split, kTile, 1u);
 }
 
 template <int D, Cached F, bool F32>

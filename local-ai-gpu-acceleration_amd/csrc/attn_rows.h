@@ -16,8 +16,25 @@ inline std::uint32_t prompt_columns(std::uint32_t head_dim, bool f32) {
   return 16u * kPromptWaves * static_cast<std::uint32_t>(prompt_blocks(static_cast<int>(head_dim), f32));
 }
 
+// Whether tiles of many rows (attn_prompt.hip) take a call, or attn_rows.hip's 16 columns.
 inline bool rows_prompt(std::uint32_t sequences, std::uint32_t rows, std::uint32_t group, std::uint32_t page_size) {
   return static_cast<std::uint64_t>(rows) * group >= 64ull * sequences && page_size % 4u == 0u;
+}
+
+// Splits of a unit's tiles (at most `tiles`) in attn_rows.hip: the largest of 64 to 4 tiles a workgroup that make as
+// many workgroups as run at once (512; 256 where registers leave room for two of fp16 heads of 128 or one of 256 a CU), not a
+// few more than those, and at most twice as many, which long contexts of different lengths need. us of 1024 / 512 / 256
+// workgroups: eight contexts to 65500 in 8 bits 113 / 140 / 223 (of 256 dimensions 220 / 211 / 317), one of 65000
+// 42 / 36 / 42, one of 16001 - / 15.7 / 16.3, of 4000 - / 12.3 / 10.5 (32 of 8 tiles or of 4), four of 4000 - / 13.4 /
+// 15.4; windows of 1024 over fp16 pages, eight 320 workgroups 17.0, 256 14.0, 32 sequences 41 / 35 / 27.
+inline std::uint32_t rows_splits(std::uint64_t items, std::uint64_t tiles, bool codes, std::uint32_t head_dim) {
+  const std::uint64_t slots = head_dim == 64u || (codes && head_dim == 128u) ? 512u : 256u;
+  std::uint64_t per = 64u;
+  while (per > 4u && items * ((tiles + per - 1u) / per) < slots) per /= 2u;
+  std::uint64_t splits = (tiles + per - 1u) / per;
+  if (items * splits > 2u * slots) splits = (2u * slots + items - 1u) / items;
+  if (items * splits > slots && 2u * items * splits < 3u * slots) splits = slots / items != 0u ? slots / items : 1u;
+  return static_cast<std::uint32_t>(splits);
 }
 
 struct AttnRows {

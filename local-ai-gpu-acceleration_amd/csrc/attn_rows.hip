@@ -6,6 +6,7 @@ namespace rtxllm {
 namespace {
 
 constexpr std::uint32_t kThreads = 256, kWaves = kThreads / 64u, kCols = 16, kTile = kRowTile;
+constexpr std::uint32_t kUnitsY = 32768;  // units of a launch's second dimension, at most
 constexpr int kLift = 15;  // queries and softmax terms are brought to 2^15, as in paged_attn.hip
 
 // A tile's keys and values in a lane's registers. Keys: position col of each half tile, the lane's
@@ -89,23 +90,44 @@ __device__ __forceinline__ std::uint32_t key_dim(int j, std::uint32_t qq) {
 //    values for those positions: rows of the cache in whole lines, bytes turned in registers.
 // Bound by the reads of the cache.
 template <int D, Cached F, bool QUAD>
-__global__ __launch_bounds__(kThreads) void attn_rows_kernel(AttnRows a, CallRows rows, RowsCache kv) {
+__global__ __launch_bounds__(kThreads, (D == 256 ? 1 : 2)) void attn_rows_kernel(AttnRows a, CallRows rows, RowsCache kv) {
   constexpr bool CODES = F != Cached::kF16;
   constexpr int J = D / 32, B = D / 16, VPL = D / 16;
   constexpr std::uint32_t kPad = D + 4u;
   __shared__ __align__(16) float rec[kWaves][kCols][kPad];
   __shared__ float2 rml[kWaves][kCols];
-  const std::uint32_t g = blockIdx.x % kv.p.n_kv, us = blockIdx.x / kv.p.n_kv, split = us % a.splits, unit = us / a.splits;
+  __shared__ std::uint32_t odd;
+  // kv heads first: workgroups next to each other read what lies next to each other in a page
+  const std::uint32_t split = blockIdx.x / kv.p.n_kv, g = blockIdx.x - split * kv.p.n_kv, unit = blockIdx.z * kUnitsY + blockIdx.y;
+  if (unit >= a.units) return;
+  const std::uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const std::uint32_t col = lane & 15u, qq = lane >> 4;
+  const std::uint32_t n_heads = a.group * kv.p.n_kv;
+  const bool f16 = a.f16 != 0u;
+  const std::uint32_t qi = rows.start == nullptr ? (col < a.group ? 0u : 1u) : col / a.group;  // the column's query row
+  const std::uint32_t h = col - qi * a.group;                                               // and head
+  // The column's q, as it lies there: read before anything is known of the sequence where row and unit are one.
+  // (16 bytes at a time; fp16: the second 16 are the first again and not used)
+  u32x4 raw[J][2];
+  auto load_q = [&](std::uint32_t row, bool there) {
+    const std::size_t at = (static_cast<std::size_t>(row) * n_heads + g * a.group + (there ? h : 0u)) * D;
+    const std::uint8_t* const base = static_cast<const std::uint8_t*>(a.q) + (f16 ? 2u : 4u) * at;
+#pragma unroll
+    for (int j = 0; j < J; ++j) {
+      const std::uint8_t* const x = base + (f16 ? 2u : 4u) * key_dim<CODES>(j, qq);
+      raw[j][0] = u32x4(*reinterpret_cast<const u32x4_any*>(x));
+      raw[j][1] = u32x4(*reinterpret_cast<const u32x4_any*>(x + (f16 ? 0u : 16u)));
+    }
+  };
+  if (rows.start == nullptr) load_q(unit, qi == 0u);
+  if (threadIdx.x == 0u) odd = 0u;
   const RowSpan sp = row_span(rows, kv, unit, a.tq, a.window, a.sinks, kTile);
   if (sp.nq == 0u) return;
   const std::uint32_t per = span_per(sp.total, a.splits, kWaves), u0 = split * per;
   if (u0 >= sp.total) return;  // (merge_rows_kernel counts the records alike)
   const std::uint32_t u1 = u0 + per < sp.total ? u0 + per : sp.total;
-  const std::uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const std::uint32_t col = lane & 15u, qq = lane >> 4;
-  const std::uint32_t n_heads = a.group * kv.p.n_kv;
-  const std::uint32_t qi = col / a.group, h = col - qi * a.group;  // the column's query row and head
   const bool mine = qi < sp.nq;
+  if (rows.start != nullptr) load_q(sp.row + (mine ? qi : 0u), mine);
   const std::uint32_t pc = row_pos(sp.pos, mine ? qi : 0u, kv.p.capacity);
   const std::int32_t* const table = kv.p.table + static_cast<std::size_t>(sp.s) * kv.p.table_stride;
 
@@ -113,24 +135,27 @@ __global__ __launch_bounds__(kThreads) void attn_rows_kernel(AttnRows a, CallRow
   half8 qh[J], ql[J];
   float qscale;
   {
-    const std::size_t at = (static_cast<std::size_t>(sp.row + (mine ? qi : 0u)) * n_heads + g * a.group + (mine ? h : 0u)) * D;
     float x[J][8], top = 0.0f;
+    if (f16) {
 #pragma unroll
-    for (int j = 0; j < J; ++j) {
-      const std::size_t d = at + key_dim<CODES>(j, qq);
-      if (a.f16 != 0u) {
-        const half8 t = half8(*reinterpret_cast<const half8_any*>(static_cast<const _Float16*>(a.q) + d));
+      for (int j = 0; j < J; ++j) {
+        const half8 t = __builtin_bit_cast(half8, raw[j][0]);
 #pragma unroll
         for (int i = 0; i < 8; ++i) x[j][i] = static_cast<float>(t[i]);
-      } else {
-        const float* f = static_cast<const float*>(a.q) + d;
-        const f32x4_any lo = *reinterpret_cast<const f32x4_any*>(f), hi = *reinterpret_cast<const f32x4_any*>(f + 4);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) x[j][i] = lo[i], x[j][i + 4] = hi[i];
       }
+    } else {
+#pragma unroll
+      for (int j = 0; j < J; ++j)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const std::uint32_t w = raw[j][i / 4][i & 3];
+          x[j][i] = __uint_as_float(w);
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < J; ++j)
 #pragma unroll
       for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(x[j][i]));
-    }
     top = fmaxf(top, lane_xor<16>(top));
     top = fmaxf(top, lane_xor<32>(top));
     int e = 0;
@@ -166,7 +191,7 @@ __global__ __launch_bounds__(kThreads) void attn_rows_kernel(AttnRows a, CallRow
       for (int j = 0; j < J; ++j) {
         const half8 kj = f.key(t, j);
         sc[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kj, qh[j], sc[t], 0, 0, 0);
-        if (a.f16 == 0u) sc[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kj, ql[j], sc[t], 0, 0, 0);
+        sc[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kj, ql[j], sc[t], 0, 0, 0);
       }
     }
     float ks[2] = {qscale, qscale}, vs[2] = {1.0f, 1.0f};
@@ -177,12 +202,16 @@ __global__ __launch_bounds__(kThreads) void attn_rows_kernel(AttnRows a, CallRow
                                                               (sp.plast - j0 < a.window || j0 + kTile <= a.sinks)));
     std::uint32_t sees = seen >> (4u * qq);  // bits 16 t + i: the lane's positions
     if (!plain && sp.nq > 1u) {
+      // of the lane's positions j0 + 4 qq + (16 t + i): up to `last`, behind `past` or before `first`
+      const auto base = static_cast<int>(j0 + 4u * qq);
+      const int last = static_cast<int>(pc) - base, past = last - static_cast<int>(a.window), first = static_cast<int>(a.sinks) - base;
 #pragma unroll
       for (int t = 0; t < 2; ++t)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const std::uint32_t j = j0 + 16u * t + 4u * qq + i;
-          if (!(j <= pc && (pc - j < a.window || j < a.sinks))) sees &= ~(1u << (16 * t + i));
+          const int x = 16 * t + i;
+          const bool yes = (x <= last) & ((x > past) | (x < first));
+          sees &= yes ? ~0u : ~(1u << x);
         }
     }
     float s[2][4], top = -INFINITY;
@@ -241,39 +270,22 @@ __global__ __launch_bounds__(kThreads) void attn_rows_kernel(AttnRows a, CallRow
         for (int w = 0; w < Fr::VW; ++w) f.v[e][w] = (seen >> (16u * (e / 4) + 4u * qq + (e & 3)) & 1u) != 0u ? f.v[e][w] : 0u;
     }
     if constexpr (!SCALED) {
-      // A value that is not finite and that only some of the rows see: each row's products with what it sees.
-      bool odd = false;
-      if (!plain && sp.nq > 1u) {
+      if (!plain && sp.nq > 1u) {  // values that are not finite and that only some of the rows see: at the end
+        u16x2 most = {0, 0};
 #pragma unroll
         for (int e = 0; e < 8; ++e)
 #pragma unroll
-          for (int w = 0; w < Fr::VW; ++w)
-            odd |= (f.v[e][w] & 0x7C00u) == 0x7C00u || (f.v[e][w] & 0x7C000000u) == 0x7C000000u;
-      }
-      if (__ballot(odd) != 0ull) {
-        for (std::uint32_t i = 0; i < sp.nq; ++i) {
-          const std::uint32_t pi = row_pos(sp.pos, i, kv.p.capacity);
-          std::uint32_t of = seen;
-          for (std::uint32_t j = 0; j < kTile; ++j)
-            if (!(j0 + j <= pi && (pi - (j0 + j) < a.window || j0 + j < a.sinks))) of &= ~(1u << j);
-          Fr c = f;
+          for (int w = 0; w < Fr::VW; ++w) {
+            const std::uint32_t m = f.v[e][w] & 0x7FFF7FFFu;
+            most = __builtin_elementwise_max(most, __builtin_bit_cast(u16x2, m));
+          }
+        if (__ballot(most[0] >= 0x7C00u || most[1] >= 0x7C00u) != 0ull) {
+          odd = 1u;
 #pragma unroll
           for (int e = 0; e < 8; ++e)
 #pragma unroll
-            for (int w = 0; w < Fr::VW; ++w) c.v[e][w] = (of >> (16u * (e / 4) + 4u * qq + (e & 3)) & 1u) != 0u ? f.v[e][w] : 0u;
-#pragma unroll
-          for (int w = 0; w < VPL / 4; ++w) {
-            half8 va[4];
-            c.values(w, va);
-#pragma unroll
-            for (int b = 0; b < 4; ++b) {
-              f32x4 x = __builtin_amdgcn_mfma_f32_16x16x32_f16(va[b], ph, f32x4{}, 0, 0, 0);
-              x = __builtin_amdgcn_mfma_f32_16x16x32_f16(va[b], pl, x, 0, 0, 0);
-              if (qi == i) o[4 * w + b] += x;
-            }
-          }
+            for (int w = 0; w < Fr::VW; ++w) finite_only(f.v[e][w]);
         }
-        return;
       }
     }
 #pragma unroll
@@ -430,6 +442,7 @@ __global__ __launch_bounds__(kThreads) void attn_rows_kernel(AttnRows a, CallRow
       if (d == 0u) a.ml[dst] = make_float2(M, L);
     }
   }
+  if (odd != 0u) not_finite_rows<D, CODES, false>(a, rows, kv, unit, g, split, kTile, kWaves);
 }
 
 // One workgroup a (unit, kv head, column): the splits' records merged, D / 4 lanes a record.
@@ -448,13 +461,26 @@ __global__ __launch_bounds__(kThreads) void merge_rows_kernel(AttnRows a, CallRo
   const std::size_t at = static_cast<std::size_t>(blockIdx.x) * a.splits;
   f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
   float M = -INFINITY, L = 0.0f;
-  for (std::uint32_t x = sub; x < used; x += kSub) {
-    const float2 t = a.ml[at + x];
-    const f32x4 o = *reinterpret_cast<const f32x4*>(a.part + (at + x) * D + d);
-    const float mn = fmaxf(M, t.x), base = mn == -INFINITY ? 0.0f : mn;
-    const float f0 = __builtin_amdgcn_exp2f(M - base), f1 = __builtin_amdgcn_exp2f(t.x - base);
-    v = v * f0 + o * f1;
-    L = L * f0 + t.y * f1;
+  for (std::uint32_t x0 = sub; x0 < used; x0 += 8u * kSub) {  // eight records of a lane in flight
+    f32x4 o[8];
+    float2 t[8];
+    float mn = M;
+#pragma unroll
+    for (std::uint32_t k = 0; k < 8u; ++k) {
+      const std::uint32_t x = x0 + kSub * k < used ? x0 + kSub * k : x0;  // past the last: read again, weighted 0
+      o[k] = *reinterpret_cast<const f32x4*>(a.part + (at + x) * D + d);
+      t[k] = a.ml[at + x];
+    }
+#pragma unroll
+    for (std::uint32_t k = 0; k < 8u; ++k) mn = fmaxf(mn, t[k].x);
+    const float base = mn == -INFINITY ? 0.0f : mn, f0 = __builtin_amdgcn_exp2f(M - base);
+    v *= f0;
+    L *= f0;
+#pragma unroll
+    for (std::uint32_t k = 0; k < 8u; ++k) {
+      const float f1 = x0 + kSub * k < used ? __builtin_amdgcn_exp2f(t[k].x - base) : 0.0f;
+      if (x0 + kSub * k < used) v += o[k] * f1, L += t[k].y * f1;
+    }
     M = mn;
   }
   *reinterpret_cast<f32x4*>(&sums[sub][d]) = v;
@@ -511,7 +537,7 @@ struct RowsPlan {
   std::size_t ml = 0, bytes = 0;  // bytes 0: refused
 };
 
-RowsPlan rows_plan(const rtxllm_paged_kv* c, std::uint32_t n_heads, bool f16, bool one_each, std::uint32_t sequences,
+RowsPlan rows_plan(Cached kind, const rtxllm_paged_kv* c, std::uint32_t n_heads, bool f16, bool one_each, std::uint32_t sequences,
                    std::uint32_t rows, std::uint32_t window, std::uint32_t sinks) {
   RowsPlan p;
   const std::uint32_t group = paged_group(c, n_heads);
@@ -522,9 +548,12 @@ RowsPlan rows_plan(const rtxllm_paged_kv* c, std::uint32_t n_heads, bool f16, bo
   const std::uint64_t items = static_cast<std::uint64_t>(p.units) * c->n_kv_heads;
   const std::uint64_t near = static_cast<std::uint64_t>(window) + p.tq + sinks;
   const std::uint64_t tiles = (near < c->capacity ? near : c->capacity) / (p.prompt ? kPromptTile : kTile) + 3u;
-  std::uint64_t splits = p.prompt ? (items >= 192u ? 1u : (256u + items - 1u) / items) : (1024u + items - 1u) / items;
-  const std::uint64_t most = p.prompt ? (tiles + 3u) / 4u : (tiles + 7u) / 8u;
-  if (splits > most) splits = most;
+  std::uint64_t splits = rows_splits(items, tiles, kind != Cached::kF16, c->head_dim);
+  if (p.prompt) {
+    const std::uint64_t most = (tiles + 3u) / 4u;
+    splits = items >= 192u ? 1u : (256u + items - 1u) / items;
+    if (splits > most) splits = most;
+  }
   p.splits = static_cast<std::uint32_t>(splits);
   // the launches' thread counts
   if (items * splits * (p.prompt ? 64u * kPromptWaves : kThreads) > 0xFFFFFFFFull || (splits > 1u && items * p.tq * group > (1u << 24))) return p;
@@ -536,7 +565,8 @@ RowsPlan rows_plan(const rtxllm_paged_kv* c, std::uint32_t n_heads, bool f16, bo
 
 template <int D>
 hipError_t launch_rows(Cached kind, bool prompt, const AttnRows& a, const CallRows& rows, const RowsCache& kv, hipStream_t stream) {
-  const dim3 grid(a.units * a.splits * kv.p.n_kv), block(kThreads);
+  const std::uint32_t y = a.units < kUnitsY ? a.units : kUnitsY;
+  const dim3 grid(a.splits * kv.p.n_kv, y, (a.units + y - 1u) / y), block(kThreads);
   hipError_t rc = hipSuccess;
   if (prompt)
     rc = attn_prompt(kind, D, a, rows, kv, stream);
@@ -565,7 +595,7 @@ hipError_t attn_rows(Cached kind, const rtxllm_paged_kv* pages, const RowsCache&
   if (q == nullptr || out == nullptr || workspace == nullptr || !type_ok(type) || !aligned_to(q, type_bytes(type)) ||
       !aligned_to(out, type_bytes(type)) || !aligned_to(workspace, 256u))
     return hipErrorInvalidValue;
-  const RowsPlan p = rows_plan(pages, n_heads, type == RTXLLM_F16, rows.start == nullptr, rows.sequences, rows.rows, window, sinks);
+  const RowsPlan p = rows_plan(kind, pages, n_heads, type == RTXLLM_F16, rows.start == nullptr, rows.sequences, rows.rows, window, sinks);
   if (p.bytes == 0u || workspace_bytes < p.bytes) return hipErrorInvalidValue;
   const std::uint64_t n = type_bytes(type) * static_cast<std::uint64_t>(rows.rows) * n_heads * pages->head_dim;
   const std::uint64_t table = 4ull * ((rows.sequences - 1ull) * pages->table_stride + pages->capacity / pages->page_size);
@@ -595,14 +625,14 @@ hipError_t attn_rows(Cached kind, const rtxllm_paged_kv* pages, const RowsCache&
 }
 
 // A workspace serves every call of its numbers: of either type, with starts or one row each.
-std::size_t attn_rows_bytes(const rtxllm_paged_kv* c, std::uint32_t n_heads, std::uint32_t sequences, std::uint32_t rows,
+std::size_t attn_rows_bytes(Cached kind, const rtxllm_paged_kv* c, std::uint32_t n_heads, std::uint32_t sequences, std::uint32_t rows,
                             std::uint32_t window, std::uint32_t sinks) {
   if (sequences == 0u || sequences > 65535u || rows == 0u || rows > (1u << 20)) return 0u;
   std::size_t most = 0u;
   for (const bool f16 : {false, true})
     for (const bool one_each : {false, true}) {
       if (one_each && rows != sequences) continue;
-      const std::size_t n = rows_plan(c, n_heads, f16, one_each, sequences, rows, window, sinks).bytes;
+      const std::size_t n = rows_plan(kind, c, n_heads, f16, one_each, sequences, rows, window, sinks).bytes;
       if (n == 0u) return 0u;
       most = n > most ? n : most;
     }
@@ -616,7 +646,7 @@ using namespace rtxllm;
 
 extern "C" size_t rtxllm_attn_window_workspace(const rtxllm_paged_kv* cache, uint32_t n_heads, uint32_t sequences,
                                                uint32_t rows, uint32_t window, uint32_t sinks) {
-  return paged_cache_ok(cache, sequences) ? attn_rows_bytes(cache, n_heads, sequences, rows, window, sinks) : 0u;
+  return paged_cache_ok(cache, sequences) ? attn_rows_bytes(Cached::kF16, cache, n_heads, sequences, rows, window, sinks) : 0u;
 }
 
 extern "C" hipError_t rtxllm_attn_window_f16(const rtxllm_paged_kv* cache, const void* q, int type, uint32_t n_heads,
@@ -636,7 +666,7 @@ extern "C" size_t rtxllm_attn_kv8_workspace(const rtxllm_paged_kv8* cache, uint3
                                             uint32_t rows, uint32_t window, uint32_t sinks) {
   if (!kv8_cache_ok(cache, sequences)) return 0u;
   const rtxllm_paged_kv pages = kv8_pages(cache);
-  return attn_rows_bytes(&pages, n_heads, sequences, rows, window, sinks);
+  return attn_rows_bytes(kv8_kind(cache), &pages, n_heads, sequences, rows, window, sinks);
 }
 
 extern "C" hipError_t rtxllm_attn_kv8(const rtxllm_paged_kv8* cache, const void* q, int type, uint32_t n_heads,
@@ -648,6 +678,6 @@ extern "C" hipError_t rtxllm_attn_kv8(const rtxllm_paged_kv8* cache, const void*
   const Kv8Ranges r = kv8_ranges(cache, sequences);
   if (!apart(r, out, o) || !apart(r, workspace, workspace_bytes)) return hipErrorInvalidValue;
   const rtxllm_paged_kv pages = kv8_pages(cache);
-  return attn_rows(cache->format == RTXLLM_KV8_E4M3 ? Cached::kE4m3 : Cached::kInt8, &pages, kv8_view(cache), q, type, n_heads,
+  return attn_rows(kv8_kind(cache), &pages, kv8_view(cache), q, type, n_heads,
                    CallRows{start, pos, sequences, rows}, window, sinks, out, workspace, workspace_bytes, stream);
 }

@@ -121,6 +121,8 @@ inline RowsCache kv8_view(const rtxllm_paged_kv8* c) {
   return RowsCache{paged_view(&pages), c->k, c->v, c->k_scale, c->v_scale, c->k_tail, c->v_tail, kv8_block_shift(c->block)};
 }
 
+inline Cached kv8_kind(const rtxllm_paged_kv8* c) { return c->format == RTXLLM_KV8_E4M3 ? Cached::kE4m3 : Cached::kInt8; }
+
 inline RowsCache f16_view(const rtxllm_paged_kv* c) {
   return RowsCache{paged_view(c), reinterpret_cast<const std::uint8_t*>(c->k), reinterpret_cast<const std::uint8_t*>(c->v),
                    nullptr,       nullptr, nullptr, nullptr, 0u};
