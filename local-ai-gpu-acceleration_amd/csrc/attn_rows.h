@@ -16,9 +16,15 @@ inline std::uint32_t prompt_columns(std::uint32_t head_dim, bool f32) {
   return 16u * kPromptWaves * static_cast<std::uint32_t>(prompt_blocks(static_cast<int>(head_dim), f32));
 }
 
-// Whether tiles of many rows (attn_prompt.hip) take a call, or attn_rows.hip's 16 columns.
-inline bool rows_prompt(std::uint32_t sequences, std::uint32_t rows, std::uint32_t group, std::uint32_t page_size) {
-  return static_cast<std::uint64_t>(rows) * group >= 64ull * sequences && page_size % 4u == 0u;
+// Whether tiles of many rows (attn_prompt.hip) take a call, or attn_rows.hip's 16 columns: by the columns (rows times
+// query heads) that a sequence has on average. us of 16 columns / tiles: heads of 128, 128 columns of one context of
+// 1000 17 / 29, of 16000 57 / 50, of eight of 16000 145 / 153; 256 of one of 1000 23 / 38, of 4000 41 / 44, of 16000
+// 100 / 98, windows of 1024 57 / 56; 512 of eight prompts of 128 19 / 32; heads of 64, 128 of 4000 19 / 22, 256 30 / 28;
+// of 256 over 16000, where 16 columns fill the registers: 20 30 / 34, 40 40 / 36, 80 62 / 45.
+inline bool rows_prompt(std::uint32_t sequences, std::uint32_t rows, std::uint32_t group, std::uint32_t head_dim,
+                        std::uint32_t page_size) {
+  const std::uint64_t enough = head_dim == 256u ? 40u : 192u;
+  return static_cast<std::uint64_t>(rows) * group >= enough * sequences && page_size % 4u == 0u;
 }
 
 // Splits of a unit's tiles (at most `tiles`) in attn_rows.hip: the largest of 64 to 4 tiles a workgroup that make as

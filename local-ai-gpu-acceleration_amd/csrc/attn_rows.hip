@@ -542,7 +542,7 @@ RowsPlan rows_plan(Cached kind, const rtxllm_paged_kv* c, std::uint32_t n_heads,
   RowsPlan p;
   const std::uint32_t group = paged_group(c, n_heads);
   if (group == 0u || window == 0u) return p;
-  p.prompt = !one_each && rows_prompt(sequences, rows, group, c->page_size);
+  p.prompt = !one_each && rows_prompt(sequences, rows, group, c->head_dim, c->page_size);
   p.tq = one_each ? 1u : (p.prompt ? prompt_columns(c->head_dim, !f16) : kCols) / group;
   p.units = one_each ? sequences : units_of(sequences, rows, p.tq, 1u);
   const std::uint64_t items = static_cast<std::uint64_t>(p.units) * c->n_kv_heads;
@@ -556,7 +556,9 @@ RowsPlan rows_plan(Cached kind, const rtxllm_paged_kv* c, std::uint32_t n_heads,
   }
   p.splits = static_cast<std::uint32_t>(splits);
   // the launches' thread counts
-  if (items * splits * (p.prompt ? 64u * kPromptWaves : kThreads) > 0xFFFFFFFFull || (splits > 1u && items * p.tq * group > (1u << 24))) return p;
+  if ((p.prompt ? items * splits * 64u * kPromptWaves : splits * c->n_kv_heads * kThreads) > 0xFFFFFFFFull ||
+      (splits > 1u && items * p.tq * group > (1u << 24)))
+    return p;
   const std::uint64_t records = splits > 1u ? items * p.tq * group * splits : 0u;
   p.ml = round_256(8u * records);
   p.bytes = p.ml + round_256(4u * records * c->head_dim) + 256u;

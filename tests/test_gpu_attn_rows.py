@@ -144,6 +144,28 @@ def test_drafts_and_prompts(shape, fmt, f16, window, sinks):
     s.check(got, window, sinks, sample=9, single=f16)
 
 
+@pytest.mark.parametrize("window,sinks", [(ALL, 0), (1, 0), (70, 5), (64, 64), (200, 130)])
+@pytest.mark.parametrize("f16", [False, True], ids=["f32", "half"])
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("shape", SHAPES, ids=str)
+def test_prompts(shape, fmt, f16, window, sinks):
+    """Prompts long enough for tiles that many rows share: from nothing, over a held context, beside a few rows."""
+    kv, group, dim, page, block = shape
+    s = Setup(dim + 3 * group, fmt, [330, 400, ref.NONE, 3], [330, 250, 2, 3], kv, group, dim, page, block, f16=f16)
+    got = s.call(window, sinks)
+    s.check(got, window, sinks, sample=41, single=f16)
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_prompts_over_long_contexts(fmt, dim):
+    """Few tiles of rows over a long context: its tiles of positions in splits."""
+    for f16 in (False, True):
+        s = Setup(18, fmt, [2900, 700], [70, 61], 1, 6, dim, 64, 32, f16=f16)
+        for window, sinks in ((ALL, 0), (900, 100)):
+            s.check(s.call(window, sinks), window, sinks, sample=35, single=f16)
+
+
 @pytest.mark.parametrize("page", [1, 5, 7, 30])
 def test_pages_of_any_size(page):
     s = Setup(page, "f16", [97, 60], [20, 1], 2, 3, 128, page)
@@ -165,11 +187,12 @@ def test_pages_that_are_not_there(fmt):
 
 
 @pytest.mark.parametrize("fmt", FORMATS)
-def test_late_rows_do_not_reach_earlier_ones(fmt):
+@pytest.mark.parametrize("dim", [64, 128])
+def test_late_rows_do_not_reach_earlier_ones(fmt, dim):
     """Infinities and NaN in a prompt's keys and values: rows before them, and rows whose window has passed them, are
     numbers (and right); rows that attend them are NaN where they enter."""
     for f16 in (False, True):
-        s = Setup(8, fmt, [140, 70], [90, 70], 2, 4, 128, 32, 8, f16=f16)
+        s = Setup(8, fmt, [140, 70], [90, 70], 2, 4 if dim == 128 else 3, dim, 32, 8, f16=f16)
         bad_v, bad_k = 77, 93  # of sequence 0
         for i, p, d, x in ((1, bad_v, 5, np.nan), (1, bad_v + 1, 6, np.inf), (0, bad_k, 3, np.nan), (1, 139, 7, np.nan)):
             s.x[i][0, p, 1, d] = x
@@ -183,15 +206,17 @@ def test_late_rows_do_not_reach_earlier_ones(fmt):
         for window, sinks in ((ALL, 0), (11, 3)):
             got = s.call(window, sinks)
             s.check(got, window, sinks, single=f16)
-            heads = got[:90, 4:].isnan()
-            assert not got[:90, :4].isnan().any() and not got[90:].isnan().any()
+            heads = got[:90, s.group:].isnan()
+            assert not got[:90, :s.group].isnan().any() and not got[90:].isnan().any()
             first = bad_v // 8 * 8 if fmt != "f16" else bad_v  # (of an 8-bit block, all of it)
             assert not heads[:first - 50].any() and heads[bad_v - 50:].any()
 
 
 @pytest.mark.parametrize("fmt", FORMATS)
-def test_queries_that_are_not_finite(fmt):
-    s = Setup(9, fmt, [80, 40], [30, 1], 2, 4, 128, 64, 16)
+@pytest.mark.parametrize("f16", [False, True], ids=["f32", "half"])
+@pytest.mark.parametrize("rows", [30, 130])
+def test_queries_that_are_not_finite(fmt, rows, f16):
+    s = Setup(9, fmt, [180, 40], [rows, 1], 2, 4, 128, 64, 16, f16=f16)
     s.q[3, 5, 7], s.q[20, 0, 0] = np.nan, np.inf
     got = s.call(50, 2)
     bad = got.isnan()
@@ -265,14 +290,15 @@ def test_rows_outside_every_sequence(fmt):
 
 @pytest.mark.parametrize("fmt", FORMATS)
 @pytest.mark.parametrize("f16", [False, True], ids=["f32", "half"])
-def test_unaligned_and_in_place(fmt, f16):
-    s = Setup(15, fmt, [90, 33], [40, 1], 2, 4, 128, 64, 8, f16=f16)
+@pytest.mark.parametrize("rows", [40, 150])
+def test_unaligned_and_in_place(fmt, f16, rows):
+    s = Setup(15, fmt, [190, 33], [rows, 1], 2, 4, 128, 64, 8, f16=f16)
     want = s.call(50, 3)
     flat = torch.zeros(s.q.size + 1, dtype=want.dtype, device=DEV)
     q = flat[1:].view(want.shape)
     q.copy_(dev(s.q))
     run = paged.attn_window if fmt == "f16" else kv8.attn
-    got = run(s.cache, q, u32(s.pos), u32([0, 40, 41]), window=50, sinks=3, out=q)
+    got = run(s.cache, q, u32(s.pos), u32([0, rows, rows + 1]), window=50, sinks=3, out=q)
     assert got.data_ptr() == q.data_ptr() and torch.equal(got, want) and flat[0] == 0.0
 
 
