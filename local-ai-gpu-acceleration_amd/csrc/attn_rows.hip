@@ -445,41 +445,48 @@ __global__ __launch_bounds__(kThreads, (D == 256 ? 1 : 2)) void attn_rows_kernel
   if (odd != 0u) not_finite_rows<D, CODES, false>(a, rows, kv, unit, g, split, kTile, kWaves);
 }
 
-// One workgroup a (unit, kv head, column): the splits' records merged, D / 4 lanes a record.
+// One workgroup a (unit, kv head, column): the splits' records merged, D / 4 lanes a record, eight records of a lane in
+// flight; the first eight are read before it is known how many there are.
 template <int D>
 __global__ __launch_bounds__(kThreads) void merge_rows_kernel(AttnRows a, CallRows rows, RowsCache kv, std::uint32_t tile,
                                                               std::uint32_t round) {
   constexpr std::uint32_t kLanes = D / 4u, kSub = kThreads / kLanes;
   __shared__ __align__(16) float sums[kSub][D];
   __shared__ float2 tops[kSub];
-  const std::uint32_t ncol = a.tq * a.group, c = blockIdx.x % ncol, ug = blockIdx.x / ncol, g = ug % kv.p.n_kv;
+  const std::uint32_t ncol = a.tq * a.group, ug = blockIdx.x / ncol, c = blockIdx.x - ug * ncol, g = ug % kv.p.n_kv;
+  const std::uint32_t d = 4u * (threadIdx.x % kLanes), sub = threadIdx.x / kLanes;
+  const std::size_t at = static_cast<std::size_t>(blockIdx.x) * a.splits;
+  f32x4 o[8];
+  float2 t[8];
+  auto load = [&](std::uint32_t x0, std::uint32_t end) {
+#pragma unroll
+    for (std::uint32_t k = 0; k < 8u; ++k) {
+      const std::uint32_t x = x0 + kSub * k < end ? x0 + kSub * k : 0u;  // past the last: not counted
+      o[k] = *reinterpret_cast<const f32x4*>(a.part + (at + x) * D + d);
+      t[k] = a.ml[at + x];
+    }
+  };
+  load(sub, a.splits);
   const RowSpan sp = row_span(rows, kv, ug / kv.p.n_kv, a.tq, a.window, a.sinks, tile);
   if (c >= sp.nq * a.group) return;
   const std::uint32_t per = span_per(sp.total, a.splits, round), used = (sp.total + per - 1u) / per;
   if (used <= 1u) return;
-  const std::uint32_t d = 4u * (threadIdx.x % kLanes), sub = threadIdx.x / kLanes;
-  const std::size_t at = static_cast<std::size_t>(blockIdx.x) * a.splits;
   f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
   float M = -INFINITY, L = 0.0f;
-  for (std::uint32_t x0 = sub; x0 < used; x0 += 8u * kSub) {  // eight records of a lane in flight
-    f32x4 o[8];
-    float2 t[8];
+  for (std::uint32_t x0 = sub; x0 < used; x0 += 8u * kSub) {
+    if (x0 != sub) load(x0, used);
     float mn = M;
 #pragma unroll
-    for (std::uint32_t k = 0; k < 8u; ++k) {
-      const std::uint32_t x = x0 + kSub * k < used ? x0 + kSub * k : x0;  // past the last: read again, weighted 0
-      o[k] = *reinterpret_cast<const f32x4*>(a.part + (at + x) * D + d);
-      t[k] = a.ml[at + x];
-    }
-#pragma unroll
-    for (std::uint32_t k = 0; k < 8u; ++k) mn = fmaxf(mn, t[k].x);
+    for (std::uint32_t k = 0; k < 8u; ++k) mn = x0 + kSub * k < used ? fmaxf(mn, t[k].x) : mn;
     const float base = mn == -INFINITY ? 0.0f : mn, f0 = __builtin_amdgcn_exp2f(M - base);
     v *= f0;
     L *= f0;
 #pragma unroll
     for (std::uint32_t k = 0; k < 8u; ++k) {
-      const float f1 = x0 + kSub * k < used ? __builtin_amdgcn_exp2f(t[k].x - base) : 0.0f;
-      if (x0 + kSub * k < used) v += o[k] * f1, L += t[k].y * f1;
+      if (x0 + kSub * k < used) {
+        const float f1 = __builtin_amdgcn_exp2f(t[k].x - base);
+        v += o[k] * f1, L += t[k].y * f1;
+      }
     }
     M = mn;
   }
