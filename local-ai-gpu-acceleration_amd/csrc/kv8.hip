@@ -30,8 +30,8 @@ __device__ __forceinline__ half8 load8(const void* x, std::size_t at) {
     h = half8(__builtin_nontemporal_load(reinterpret_cast<const half8_any*>(static_cast<const _Float16*>(x) + at)));
   } else {
     const float* f = static_cast<const float*>(x) + at;
-    const f32x4_any a = __builtin_nontemporal_load(reinterpret_cast<const f32x4_any*>(f));
-    const f32x4_any b = __builtin_nontemporal_load(reinterpret_cast<const f32x4_any*>(f + 4));
+    // (through the caches: a line's halves are two reads; past them a prompt's 17.1 us are 22.2)
+    const f32x4_any a = *reinterpret_cast<const f32x4_any*>(f), b = *reinterpret_cast<const f32x4_any*>(f + 4);
 #pragma unroll
     for (int i = 0; i < 4; ++i) h[i] = static_cast<_Float16>(a[i]), h[i + 4] = static_cast<_Float16>(b[i]);
   }
@@ -165,12 +165,14 @@ struct Kv8Read {
 };
 
 // L lanes a position of a head, 8 values each; the heads of a row lie next to each other in the result. A lane takes
-// kUnits positions of heads a workgroup's width apart, whose reads, each behind two others (the table's and the
-// sequence's), are in flight together. Bound by bytes.
-constexpr int kUnits = 4;
+// read_units positions of heads a workgroup's width apart, whose reads, each behind two others (the table's and the
+// sequence's), are in flight together. Bound by bytes: 65530 positions of 8 heads of 128 (134 MB of codes) as fp16 85.9 us, as
+// fp32 133 (2 / 4 / 8 positions a lane: 102 / 86 / 96, 155 / 146 / 133; through the caches 89, 164).
+constexpr int read_units(bool f16) { return f16 ? 4 : 8; }
 template <int L, bool E4M3, bool F16>
 __global__ __launch_bounds__(kThreads) void kv8_read_kernel(Kv8Read a, CallRows rows, RowsCache kv) {
   constexpr std::uint32_t D = 8u * L, kPer = kThreads / L;
+  constexpr int kUnits = read_units(F16);
   const std::uint32_t part = threadIdx.x % L, which = blockIdx.y, block = 1u << kv.block_shift;
   const std::uint32_t units = rows.rows * kv.p.n_kv;
   const std::uint8_t* const codes = which == 0u ? kv.k : kv.v;
@@ -268,7 +270,7 @@ void launch_append_block(std::uint32_t block, bool e4m3, bool f16, const Kv8Appe
 
 template <int L>
 void launch_read(bool e4m3, bool f16, const Kv8Read& a, const CallRows& rows, const RowsCache& kv, hipStream_t stream) {
-  const std::uint64_t units = static_cast<std::uint64_t>(rows.rows) * kv.p.n_kv, per = kUnits * kThreads / L;
+  const std::uint64_t units = static_cast<std::uint64_t>(rows.rows) * kv.p.n_kv, per = read_units(f16) * kThreads / L;
   // both, or k (y 0), or v alone (moved to y 0 by the caller)
   const dim3 grid(static_cast<std::uint32_t>((units + per - 1u) / per), a.out[1] != nullptr ? 2u : 1u);
   auto run = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(kThreads), 0, stream, a, rows, kv); };

@@ -76,9 +76,9 @@ inline bool rows_ok(const std::uint32_t* start, const std::uint32_t* pos, std::u
 }
 
 // Append: a block of 8 rounds (16 bytes a lane of fp16) or more is four waves', which keeps all of them from waiting for
-// their last read and then computing at once (us of one wave / four, 64 positions of 8 heads: 8192 of 128 in fp32 22.4 /
-// 22.3, in e4m3 19.1 / 21.0, from fp16 14.1 / 11.7, 1024 of 128 11.6 / 7.2, 4096 of 256 31.9 / 21.3; of 4 rounds, 16
-// positions of 128, 19.7 / 21.4).
+// their last read and then computing at once (us of one wave / four, 64 positions of 8 heads: 8192 of 128 in fp32 20.0 /
+// 17.2, in e4m3 17.1 / 16.9, from fp16 14.2 / 11.9, 1024 of 128 10.4 / 7.0, 4096 of 256 26.7 / 19.4; of 4 rounds, 16
+// positions of 128, 17.1 / 17.3).
 constexpr bool append_shared(int rounds) { return rounds >= 8; }
 
 inline bool type_ok(int type) { return type == RTXLLM_F32 || type == RTXLLM_F16; }
