@@ -165,14 +165,13 @@ struct Kv8Read {
 };
 
 // L lanes a position of a head, 8 values each; the heads of a row lie next to each other in the result. A lane takes
-// read_units positions of heads a workgroup's width apart, whose reads, each behind two others (the table's and the
+// kUnits positions of heads a workgroup's width apart, whose reads, each behind two others (the table's and the
 // sequence's), are in flight together. Bound by bytes: 65530 positions of 8 heads of 128 (134 MB of codes) as fp16 85.9 us, as
 // fp32 133 (2 / 4 / 8 positions a lane: 102 / 86 / 96, 155 / 146 / 133; through the caches 89, 164).
-constexpr int read_units(bool f16) { return f16 ? 4 : 8; }
-template <int L, bool E4M3, bool F16>
+template <int L, bool E4M3, bool F16, bool MANY>
 __global__ __launch_bounds__(kThreads) void kv8_read_kernel(Kv8Read a, CallRows rows, RowsCache kv) {
   constexpr std::uint32_t D = 8u * L, kPer = kThreads / L;
-  constexpr int kUnits = read_units(F16);
+  constexpr int kUnits = MANY ? read_units(F16) : 1;
   const std::uint32_t part = threadIdx.x % L, which = blockIdx.y, block = 1u << kv.block_shift;
   const std::uint32_t units = rows.rows * kv.p.n_kv;
   const std::uint8_t* const codes = which == 0u ? kv.k : kv.v;
@@ -270,14 +269,18 @@ void launch_append_block(std::uint32_t block, bool e4m3, bool f16, const Kv8Appe
 
 template <int L>
 void launch_read(bool e4m3, bool f16, const Kv8Read& a, const CallRows& rows, const RowsCache& kv, hipStream_t stream) {
-  const std::uint64_t units = static_cast<std::uint64_t>(rows.rows) * kv.p.n_kv, per = read_units(f16) * kThreads / L;
+  const std::uint64_t units = static_cast<std::uint64_t>(rows.rows) * kv.p.n_kv;
+  const bool many = read_many(units, L, f16);
+  const std::uint64_t per = (many ? read_units(f16) : 1) * kThreads / L;
   // both, or k (y 0), or v alone (moved to y 0 by the caller)
   const dim3 grid(static_cast<std::uint32_t>((units + per - 1u) / per), a.out[1] != nullptr ? 2u : 1u);
-  auto run = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(kThreads), 0, stream, a, rows, kv); };
+  auto run = [&](auto one, auto more) { hipLaunchKernelGGL(many ? more : one, grid, dim3(kThreads), 0, stream, a, rows, kv); };
   if (e4m3) {
-    f16 ? run(kv8_read_kernel<L, true, true>) : run(kv8_read_kernel<L, true, false>);
+    f16 ? run(kv8_read_kernel<L, true, true, false>, kv8_read_kernel<L, true, true, true>)
+        : run(kv8_read_kernel<L, true, false, false>, kv8_read_kernel<L, true, false, true>);
   } else {
-    f16 ? run(kv8_read_kernel<L, false, true>) : run(kv8_read_kernel<L, false, false>);
+    f16 ? run(kv8_read_kernel<L, false, true, false>, kv8_read_kernel<L, false, true, true>)
+        : run(kv8_read_kernel<L, false, false, false>, kv8_read_kernel<L, false, false, true>);
   }
 }
 

@@ -81,6 +81,12 @@ inline bool rows_ok(const std::uint32_t* start, const std::uint32_t* pos, std::u
 // positions of 128, 17.1 / 17.3).
 constexpr bool append_shared(int rounds) { return rounds >= 8; }
 
+// Read: positions of a head that a lane takes where there are many (units: positions times heads), one where there are
+// few. us of one / many, 8 heads of 128: 2000 positions as fp16 4.9 / 5.3, as fp32 7.6 / 8.8; 4000 9.0 / 8.4, 12.7 / 12.1;
+// 32000 65.6 / 45.0, 88.7 / 69.5.
+constexpr int read_units(bool f16) { return f16 ? 4 : 8; }
+inline bool read_many(std::uint64_t units, std::uint32_t lanes, bool f16) { return units * lanes >= 393216u; }
+
 inline bool type_ok(int type) { return type == RTXLLM_F32 || type == RTXLLM_F16; }
 inline std::size_t type_bytes(int type) { return type == RTXLLM_F32 ? 4u : 2u; }
 
