@@ -244,6 +244,42 @@ def test_read(shape, fmt, dtype):
         assert not single[2].any()
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16], ids=["f32", "f16"])
+@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_long_reads(dim, fmt, dtype):
+    """Reads of many positions, which a lane takes several of, are those of few: ragged, a hole, open blocks, rows behind."""
+    kv, page = 8 if dim == 64 else 4, 96
+    lens, held = [5001, 3, 0, 4099], [5000, 77, 40, 4096]
+    n_pages = 200
+    rng = np.random.default_rng(dim)
+    table = rng.integers(0, n_pages, (4, 53)).astype(np.int32)
+    table[0, 7] = -1
+    cache = kv8.PagedKV8.empty(n_pages, kv, page, dim, 32, dev(table), DTYPE[fmt])
+    g = torch.Generator(device=DEV)
+    g.manual_seed(dim)
+    for x in (cache.k, cache.v):
+        x.copy_(torch.randint(-100, 100, x.shape, device=DEV, generator=g).to(torch.float32).to(x.dtype))
+    for x in (cache.k_scale, cache.v_scale, cache.k_tail, cache.v_tail):
+        x.copy_(torch.rand(x.shape, device=DEV, generator=g))
+    start = np.cumsum([0] + lens)
+    pos = [0, 70, 5, 0]
+    rows = int(start[-1]) + 5
+    many = [torch.full((rows, kv, dim), 7.0, dtype=dtype, device=DEV) for _ in range(2)]
+    kv8.read(cache, u32(pos), u32(held), u32(start), k_out=many[0], v_out=many[1])
+    few = [torch.full((rows, kv, dim), 7.0, dtype=dtype, device=DEV) for _ in range(2)]
+    for i, n in enumerate(lens):
+        for a in range(0, n, 300):
+            b = min(n, a + 300)
+            part = [x[start[i] + a:start[i] + b] for x in few]
+            at = [ref.NONE] * 4
+            at[i] = pos[i] + a
+            kv8.read(cache, u32(at), u32(held), u32([0] * (i + 1) + [b - a] * (4 - i)), k_out=part[0], v_out=part[1])
+    assert torch.equal(many[0], few[0]) and torch.equal(many[1], few[1])
+    assert bool((many[0][-5:] == 7.0).all()) and bool((many[0][5000] == 7.0).all()) and bool((many[0][7 * 96:8 * 96] == 7.0).all())
+    assert rows * kv * (dim // 8) >= 393216
+
+
 def test_v_alone_and_both():
     s = Setup(9, 1, 2, 2, 64, 32, 8, "int8")
     s.append([40], [0], s.tokens(40))
