@@ -18,6 +18,7 @@ from ._lib import PagedKV8Struct, lib
 from .paged import PagedKV, _attn_rows, _call_rows, _type_of, _u32
 
 FORMATS = {torch.int8: 0, torch.float8_e4m3fn: 1}
+CALLS = frozenset(("rtxllm_kv8_append", "rtxllm_kv8_read", "rtxllm_attn_kv8"))
 
 
 class PagedKV8(PagedKV):
@@ -69,6 +70,16 @@ class PagedKV8(PagedKV):
         tails = [torch.zeros(block_table.shape[0], n_kv_heads, block, head_dim, dtype=torch.float16, device=dev) for _ in range(2)]
         return cls(*codes, *scales, *tails, block_table)
 
+    def _call(self, name: str, *args) -> None:
+        if name not in CALLS:  # (of the functions of rtxllm_amd.paged, which take another struct)
+            raise ValueError(f"{name}: takes fp16 pages, not a cache in 8 bits")
+        super()._call(name, *args)
+
+
+def _in_8_bits(cache: PagedKV) -> None:
+    if not isinstance(cache, PagedKV8):
+        raise ValueError(f"expected a PagedKV8, got a {type(cache).__name__}")
+
 
 def _stride_of(name: str, cache: PagedKV8, x: torch.Tensor, rows: int, dtype: torch.dtype) -> int:
     """Stride in elements between the rows of x [rows][n_kv_heads][head_dim], which may lie apart."""
@@ -83,6 +94,7 @@ def _stride_of(name: str, cache: PagedKV8, x: torch.Tensor, rows: int, dtype: to
 def append(cache: PagedKV8, k: torch.Tensor, v: torch.Tensor, pos: torch.Tensor, start: torch.Tensor | None = None) -> None:
     """New tokens enter the cache, k and v [rows][n_kv_heads][head_dim] of float32 or float16: sequence s has rows
     start[s] .. start[s + 1] - 1 (start None: row s), its positions pos[s], pos[s] + 1, ..."""
+    _in_8_bits(cache)
     rows, kind = k.shape[0], _type_of("k", k)
     ks, vs = _stride_of("k", cache, k, rows, k.dtype), _stride_of("v", cache, v, rows, k.dtype)
     sp, pp, sequences = _call_rows(cache, rows, pos, start)
@@ -94,6 +106,7 @@ def read(cache: PagedKV8, pos: torch.Tensor, held: torch.Tensor, start: torch.Te
          v_out: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
     """Positions pos[s], pos[s] + 1, ... of each sequence, which holds held[s], as rows of k and v
     [rows][n_kv_heads][head_dim] (rows as in append). Outputs that are not passed are of `rows` rows of dtype."""
+    _in_8_bits(cache)
     given = k_out if k_out is not None else v_out
     if given is not None:
         rows, dtype = given.shape[0], given.dtype
@@ -114,6 +127,7 @@ def read(cache: PagedKV8, pos: torch.Tensor, held: torch.Tensor, start: torch.Te
 
 def attn_workspace(cache: PagedKV8, n_heads: int, sequences: int, rows: int, window: int | None = None,
                    sinks: int = 0) -> torch.Tensor:
+    _in_8_bits(cache)
     near = cache.capacity if window is None else _u32("window", window)
     return cache._space(None, int(lib().rtxllm_attn_kv8_workspace(
         cache.ref, _u32("n_heads", n_heads), _u32("sequences", sequences), _u32("rows", rows), near, _u32("sinks", sinks))))
@@ -123,4 +137,5 @@ def attn(cache: PagedKV8, q: torch.Tensor, pos: torch.Tensor, start: torch.Tenso
          window: int | None = None, sinks: int = 0, out: torch.Tensor | None = None,
          workspace: torch.Tensor | None = None) -> torch.Tensor:
     """rtxllm_amd.paged.attn_window over this cache, which holds the call's rows already."""
+    _in_8_bits(cache)
     return _attn_rows(cache, ("rtxllm_attn_kv8_workspace", "rtxllm_attn_kv8"), q, pos, start, window, sinks, out, workspace)

@@ -5,6 +5,7 @@ rows out to units of work as documented; rows.h and attn_rows.h on the CPU."""
 from __future__ import annotations
 
 import ctypes
+import re
 import shutil
 import subprocess
 from pathlib import Path
@@ -12,7 +13,9 @@ from pathlib import Path
 import numpy as np
 import pytest
 import rows_ref as ref
+import torch
 
+from rtxllm_amd import kv8, paged
 from rtxllm_amd._lib import PagedKV8Struct, PagedKVStruct
 
 REPO = Path(__file__).resolve().parent.parent
@@ -184,3 +187,18 @@ def test_tiles_cover_what_rows_see(tmp_path, tile):
                 covered += here
             assert len(covered) == len(set(covered)) and seen <= set(covered), (pos, n, window, sinks, shift, unit)
         assert rows == n
+
+
+def test_a_cache_of_the_other_kind_is_refused():
+    """fp16 pages and a cache in 8 bits are different structs: neither reaches the other's functions."""
+    pages, codes = object.__new__(paged.PagedKV), object.__new__(kv8.PagedKV8)
+    x, pos = torch.zeros(1, 2, 128), torch.zeros(1, dtype=torch.int32)
+    for call in (lambda: kv8.append(pages, x, x, pos), lambda: kv8.read(pages, pos, pos), lambda: kv8.attn(pages, x, pos),
+                 lambda: kv8.attn_workspace(pages, 2, 1, 1)):
+        with pytest.raises(ValueError, match="expected a PagedKV8"):
+            call()
+    names = set(re.findall(r'_call\("(rtxllm_\w+)"', Path(paged.__file__).read_text())) | {"rtxllm_attn_window_f16"}
+    assert len(names) >= 6
+    for name in names:
+        with pytest.raises(ValueError, match="not a cache in 8 bits"):
+            codes._call(name)
