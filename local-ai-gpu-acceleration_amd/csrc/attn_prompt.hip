@@ -39,9 +39,9 @@ __device__ __forceinline__ void lds_barrier() {
 //  * o += V^T p, values turned when they are stored ([dimension][position], the positions in the order in which the
 //    scores' layout holds their terms), so that both products read 16 bytes a lane.
 // Bound by the latencies of a wave's own chain (reads, 32 products, softmax, 32 products a half tile) at two waves a
-// SIMD: 8192 rows over int8 codes, 32 heads over 8 kv heads of 128, 718 us (766 TFLOP/s; an 8192^3 fp16
-// product of the library 1193), over fp16 pages 645 for 8000 rows. Without the next tile's reads and stores 495;
-// columns a wave: 16 1190, 32 720, 48 850 (spills), 64 at one wave a SIMD 1430 us; matrix and
+// SIMD: 8192 rows over int8 codes, 32 heads over 8 kv heads of 128, 722 us (761 TFLOP/s; an 8192^3 fp16
+// product of the library 1162), over fp16 pages 637 for 8000 rows. Without the next tile's reads and stores 550 and 495;
+// columns a wave, when 32 took 777: 16 1190, 48 850 (spills), 64 at one wave a SIMD 1430 us; matrix and
 // vector work of the two waves kept apart by barriers 1000; two halves' scores at once, to mix both in one wave, spills.
 template <int D, Cached F, bool F32, int NB, int NW>
 __global__ __launch_bounds__(64 * NW, 2) void attn_prompt_kernel(AttnRows a, CallRows rows, RowsCache kv) {
