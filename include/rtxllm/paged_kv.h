@@ -182,10 +182,9 @@ hipError_t rtxllm_kv_evict_f16(const rtxllm_paged_kv* cache, const uint32_t* len
  * and infinities included, has no effect on it; a NaN in q or among the attended keys or
  * values makes NaN of what it enters; an infinity makes an infinity or NaN of it, but a score of -infinity weighs
  * nothing.
- * RTXLLM_F32: q and the softmax terms enter the products as pairs of fp16, as in
- * rtxllm_attn_decode_pages_gqa_f16. RTXLLM_F16: q as it is, and where many rows
- * of a sequence share the reads of its cache, each softmax term as one fp16, off by
- * 2^-11 of itself or 2^-40 of the largest, as the result is by its own rounding.
+ * The softmax terms enter the products as pairs of fp16, off by 2^-22 of themselves or
+ * 2^-32 of the largest; q as such a pair too (RTXLLM_F32, as in
+ * rtxllm_attn_decode_pages_gqa_f16) or as it is (RTXLLM_F16).
  * n_heads / n_kv_heads 1..16; sequences 1..65535; rows 1..2^20; with table_stride 0 every
  * sequence reads the one table row. workspace:
  * rtxllm_attn_window_workspace() bytes for the same numbers, 256-byte aligned. */

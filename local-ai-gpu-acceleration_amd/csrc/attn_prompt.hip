@@ -6,7 +6,7 @@ namespace rtxllm {
 namespace {
 
 constexpr std::uint32_t kTile = kPromptTile;  // 64 positions
-constexpr int kLift = 7;           // F16: softmax terms are at most 2^7 times that of the maximum they count from,
+constexpr int kLift = 7;           // F16: softmax terms are 2^7 times what they are to the maximum they count from,
 constexpr float kSlack = 8.0f;     // which may lag 2^8 behind: 2^15 at most
 constexpr int kPairLift = 15;      // F32: exact maxima, as in attn_rows.hip
 
@@ -33,16 +33,15 @@ __device__ __forceinline__ void lds_barrier() {
 // computed the next one's codes are on their way into registers, and become fp16 once it is done.
 //  * scores: S = K q^T by v_mfma_f32_16x16x32_f16, keys' rows from the LDS, q in registers (F32: an fp16 pair, lifted as
 //    in attn_rows.hip); an 8-bit key enters as its code, its scale multiplies the scores of four positions at a time;
-//  * terms: F32 as in attn_rows.hip. F16: p = 2^(s - m + 7) as one fp16, where the m counted from may lag up to 2^8
+//  * terms: as fp16 pairs. F32 as in attn_rows.hip. F16: p = 2^(s - m + 7), where the m counted from may lag up to 2^8
 //    behind the maximum, so that it hardly ever moves; an 8-bit value's scale over 2^E is added to the exponent as its
-//    logarithm (off by 2^-19 of the term) and taken out of the sum;
+//    logarithm (off by 2^-19 of the term) and taken out of the sum. (Terms as one fp16 were 717 and 357 us where pairs are
+//    842 and 425, but off by as much as the result's own rounding is, and only in the calls that take this form.)
 //  * o += V^T p, values turned when they are stored ([dimension][position], the positions in the order in which the
 //    scores' layout holds their terms), so that both products read 16 bytes a lane.
-// Bound by the latencies of a wave's own chain (reads, 32 products, softmax, 32 products a half tile) at two waves a
-// SIMD: 8192 rows over int8 codes, 32 heads over 8 kv heads of 128, 722 us (761 TFLOP/s; an 8192^3 fp16
-// product of the library 1162), over fp16 pages 637 for 8000 rows. Without the next tile's reads and stores 550 and 495;
-// columns a wave, when 32 took 777: 16 1190, 48 850 (spills), 64 at one wave a SIMD 1430 us; matrix and
-// vector work of the two waves kept apart by barriers 1000; two halves' scores at once, to mix both in one wave, spills.
+// Bound by what a wave issues, vector instructions beside matrix ones, at two waves a SIMD: 8192 rows over int8 codes, 32
+// heads over 8 kv heads of 128, 842 us, over fp16 pages 425 for 8000 rows with a window of 2048. Columns a wave: heads of
+// 128 32, which fill the registers; heads of 64 64 (spills of up to 25 registers; 48 without spills 687 us instead of 580, 32 704).
 template <int D, Cached F, bool F32, int NB, int NW>
 __global__ __launch_bounds__(64 * NW, 2) void attn_prompt_kernel(AttnRows a, CallRows rows, RowsCache kv) {
   constexpr bool CODES = F != Cached::kF16;
@@ -336,8 +335,8 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_prompt_kernel(AttnRows a, Cal
     }
     const std::uint8_t* const kt = keys[buf];
     const std::uint8_t* const vt = vals[buf];
-    // AHEAD: fragments are read ahead of the products that use them, a half tile's values before its softmax, the next
-    // one's keys before this one's products.
+    // AHEAD: a half tile's values are read ahead of its softmax. (Its keys as well, ahead of the products before: spills,
+    // 904 us instead of 842.)
     half8 kf[2][J];
     auto load_keys = [&](int x) {
 #pragma unroll
@@ -346,12 +345,10 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_prompt_kernel(AttnRows a, Cal
         for (int j = 0; j < J; ++j)
           kf[t][j] = *reinterpret_cast<const half8*>(kt + kat[j % kKeyAts] + ((2 * x + t) * 32 * D + (j / kKeyAts) * 64 * kKeyAts));
     };
-    if (AHEAD) load_keys(0);
 #pragma unroll
     for (int x = 0; x < 2; ++x) {
       f32x4 s[NB][2];
-      if (AHEAD) __builtin_amdgcn_sched_barrier(0);
-      if (!AHEAD) load_keys(x);
+      load_keys(x);
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
 #pragma unroll
@@ -426,7 +423,7 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_prompt_kernel(AttnRows a, Cal
           for (int b = 0; b < B; ++b) o[n][b] *= alpha;
         }
       }
-      half8 ph[NB], pl[F32 ? NB : 1];
+      half8 ph[NB], pl[NB];
 #pragma unroll
       for (int n = 0; n < NB; ++n) {
         const float base = (m[n] == -INFINITY ? 0.0f : m[n]) - static_cast<float>(F32 ? kPairLift : kLift);
@@ -437,41 +434,26 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_prompt_kernel(AttnRows a, Cal
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             p[i] = __builtin_amdgcn_exp2f(fmaf(s[n][t][i], c[n][t], from));
-            if constexpr (F32) {
-              l[n] += p[i];
-              if constexpr (CODES) p[i] = (vis[n] >> (4 * t + i) & 1u) != 0u ? p[i] * sc[t][1] : 0.0f;
-              asm("" : "+v"(p[i]));
-              const _Float16 hi = static_cast<_Float16>(p[i]);
-              ph[n][4 * t + i] = hi;
-              pl[n][4 * t + i] = static_cast<_Float16>(p[i] - static_cast<float>(hi));
-            } else {
-              ph[n][4 * t + i] = static_cast<_Float16>(p[i]);
-            }
+            if constexpr (F32 || !CODES) l[n] += p[i];
+            if constexpr (F32 && CODES) p[i] = (vis[n] >> (4 * t + i) & 1u) != 0u ? p[i] * sc[t][1] : 0.0f;
+            asm("" : "+v"(p[i]));
+            const _Float16 hi = static_cast<_Float16>(p[i]);
+            ph[n][4 * t + i] = hi;
+            pl[n][4 * t + i] = static_cast<_Float16>(p[i] - static_cast<float>(hi));
           }
           if constexpr (CODES && !F32) l[n] = fmaf((p[0] + p[1]) + (p[2] + p[3]), sc[t][2], l[n]);
         }
-        if constexpr (!CODES && !F32) {  // the sum of the terms as they enter the products
-          const half2 one = {static_cast<_Float16>(1.0f), static_cast<_Float16>(1.0f)};
-          const u32x4 w = __builtin_bit_cast(u32x4, ph[n]);
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            const std::uint32_t wk = w[k];
-            l[n] = __builtin_amdgcn_fdot2(__builtin_bit_cast(half2, wk), one, l[n], false);
-          }
-        }
       }
-      if (AHEAD) {
-        if (x == 0) load_keys(1);
+      if (AHEAD)
         __builtin_amdgcn_sched_barrier(0);
-      } else {
+      else
         load_values();
-      }
 #pragma unroll
       for (int b = 0; b < B; ++b)
 #pragma unroll
         for (int n = 0; n < NB; ++n) {
           o[n][b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf[b], ph[n], o[n][b], 0, 0, 0);
-          if constexpr (F32) o[n][b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf[b], pl[n], o[n][b], 0, 0, 0);
+          o[n][b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf[b], pl[n], o[n][b], 0, 0, 0);
         }
     }
   };

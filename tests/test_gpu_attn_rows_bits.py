@@ -1,0 +1,60 @@
+"""What the attention of new rows (rtxllm_attn_window_f16, rtxllm_attn_kv8) keeps of its terms and of its rows, against
+float64 (rows_ref.py) with bounds of each row's own attended values."""
+
+from __future__ import annotations
+
+import numpy as np
+import pytest
+import rows_ref as ref
+
+torch = pytest.importorskip("torch")
+
+from test_gpu_attn_rows import ALL, FORMATS, Setup  # noqa: E402
+
+pytestmark = pytest.mark.gpu
+
+
+def bound(q, keys, values, f16, codes, lift):
+    """(the result, a bound of its error): that of rows_ref.attend, with terms as pairs of which the smaller half ends at
+    2^-25 where the largest term is at least 2^(lift - 2): 2^(-23 - lift) of the largest attended value, n times. codes: a
+    scale may enter a term and the sum as its logarithm, off by 2^-19 each. f16: rounded once (2^-11)."""
+    out, _ = ref.attend(q, keys, values)
+    n, d = keys.shape
+    q, keys, values = (np.asarray(x, np.float64) for x in (q, keys, values))
+    s = keys @ q / np.sqrt(d)
+    p = np.exp(s - s.max())
+    p /= p.sum()
+    size = np.abs(keys) @ np.abs(q) / np.sqrt(d)
+    delta = (2.0 ** -22 + (d + 16) * 2.0 ** -24) * size.max() + 2.0 ** -21 * (1.0 + np.abs(s).max())
+    tol = (2.0 * delta + (n + 64) * 2.0 ** -24 + 2.0 ** -22 + (2.0 ** -18 if codes else 0.0)) * (p @ np.abs(values))
+    tol = tol + 2.0 ** (-23 - lift) * n * np.abs(values).max() + 1e-37
+    if f16:
+        tol = tol + 2.0 ** -11 * (np.abs(out) + tol) + 2.0 ** -25
+    return out, tol
+
+
+def rows_within(s, got, window, sinks, lift, sample=1):
+    """Every sample-th row of a Setup's call within `bound`."""
+    got, row = got.cpu().numpy().astype(np.float64), 0
+    for i, n in enumerate(s.lens):
+        for r in range(n):
+            here, row = row, row + 1
+            if r % sample and r != n - 1:
+                continue
+            p = s.pos[i] + r
+            j = ref.visible(p, window, sinks)
+            for g in range(s.kv):
+                k, v = (np.stack([s.value(c, i, g, int(t)) for t in j]) for c in range(2))
+                for h in range(g * s.group, (g + 1) * s.group):
+                    want, tol = bound(s.q[here, h], k, v, s.f16, s.fmt != "f16", lift)
+                    assert bool((np.abs(got[here, h] - want) <= tol).all()), (i, r, p, h, float((np.abs(got[here, h] - want) / tol).max()))
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("dim,kv,group", [(64, 2, 4), (128, 2, 4), (256, 1, 3)])
+def test_terms_of_fp16_prompts_keep_their_bits(dim, kv, group, fmt):
+    """fp16 queries of many rows: softmax terms are held as finely as in the form for few rows, so that the result's own
+    rounding is what an element of any size is off by."""
+    s = Setup(21, fmt, [330, 250], [330, 240], kv, group, dim, 64, 16, f16=True)
+    for window, sinks in ((12, 2), (ALL, 0)):
+        rows_within(s, s.call(window, sinks), window, sinks, 7, sample=11)
