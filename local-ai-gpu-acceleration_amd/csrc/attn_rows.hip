@@ -100,7 +100,7 @@ __global__ __launch_bounds__(kThreads, (D == 256 ? 1 : 2)) void attn_rows_kernel
   constexpr std::uint32_t kPad = D + 4u;
   __shared__ __align__(16) float rec[kWaves][kCols][kPad];
   __shared__ float2 rml[kWaves][kCols];
-  __shared__ std::uint32_t odd;
+  __shared__ std::uint32_t odd[kWaves];  // whether a wave left out values that are not finite: not_finite_rows
   // kv heads first: workgroups next to each other read what lies next to each other in a page
   const std::uint32_t split = blockIdx.x / kv.p.n_kv, g = blockIdx.x - split * kv.p.n_kv, unit = blockIdx.z * kUnitsY + blockIdx.y;
   if (unit >= a.units) return;
@@ -124,7 +124,6 @@ __global__ __launch_bounds__(kThreads, (D == 256 ? 1 : 2)) void attn_rows_kernel
     }
   };
   if (rows.start == nullptr) load_q(unit, qi == 0u);
-  if (threadIdx.x == 0u) odd = 0u;
   const RowSpan sp = row_span(rows, kv, unit, a.tq, a.window, a.sinks, kTile);
   if (sp.nq == 0u) return;
   const std::uint32_t per = span_per(sp.total, a.splits, kWaves), u0 = split * per;
@@ -178,6 +177,7 @@ __global__ __launch_bounds__(kThreads, (D == 256 ? 1 : 2)) void attn_rows_kernel
 
   float m = -INFINITY, l = 0.0f;
   int E = -126;  // of the values' scales so far
+  std::uint32_t left_out = 0u;  // the wave's own mark, in LDS only behind all tiles: nothing clears another wave's
   f32x4 o[B];
 #pragma unroll
   for (int b = 0; b < B; ++b) o[b] = f32x4{};
@@ -284,7 +284,7 @@ __global__ __launch_bounds__(kThreads, (D == 256 ? 1 : 2)) void attn_rows_kernel
             most = __builtin_elementwise_max(most, __builtin_bit_cast(u16x2, m));
           }
         if (__ballot(most[0] >= 0x7C00u || most[1] >= 0x7C00u) != 0ull) {
-          odd = 1u;
+          left_out = 1u;
 #pragma unroll
           for (int e = 0; e < 8; ++e)
 #pragma unroll
@@ -412,6 +412,7 @@ __global__ __launch_bounds__(kThreads, (D == 256 ? 1 : 2)) void attn_rows_kernel
   l += lane_xor<32>(l);
   // a NaN among the scores makes the row NaN, also where no number gave a maximum
   if (qq == 0u) rml[wave][col] = make_float2(l != l ? INFINITY : m, l);
+  if (lane == 0u) odd[wave] = left_out;
   const float lift = CODES ? ldexpf(1.0f, E) : 1.0f;
 #pragma unroll
   for (int i = 0; i < 4; ++i)
@@ -446,7 +447,7 @@ __global__ __launch_bounds__(kThreads, (D == 256 ? 1 : 2)) void attn_rows_kernel
       if (d == 0u) a.ml[dst] = make_float2(M, L);
     }
   }
-  if (odd != 0u) not_finite_rows<D, CODES, false>(a, rows, kv, unit, g, split, kTile, kWaves);
+  if ((odd[0] | odd[1] | odd[2] | odd[3]) != 0u) not_finite_rows<D, CODES, false>(a, rows, kv, unit, g, split, kTile, kWaves);
 }
 
 // One workgroup a (unit, kv head, column): the splits' records merged, D / 4 lanes a record, eight records of a lane in

@@ -58,3 +58,24 @@ def test_terms_of_fp16_prompts_keep_their_bits(dim, kv, group, fmt):
     s = Setup(21, fmt, [330, 250], [330, 240], kv, group, dim, 64, 16, f16=True)
     for window, sinks in ((12, 2), (ALL, 0)):
         rows_within(s, s.call(window, sinks), window, sinks, 7, sample=11)
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("wave", range(4))
+def test_every_wave_hands_on_what_it_left_out(wave, fmt):
+    """A value that is not finite in a tile that rows see in part is left out of the products and given to its rows at the
+    end, whichever of a workgroup's waves met it: tile `wave` of the sinks, and the newest positions."""
+    s = Setup(22, fmt, [420], [4], 1, 4, 128, 32, 8)
+    at = 32 * wave + 3
+    if fmt == "f16":
+        s.cache.v[int(s.real[0, at // 32]), 0, at % 32, 9] = float("inf")
+    else:
+        s.cache.v_scale[int(s.real[0, at // 32]), 0, at % 32 // 8] = float("nan")
+    bad = s.call(5, 32 * wave + 5).isfinite().logical_not()
+    assert bad[..., 9].all() and (bad.all() if fmt != "f16" else int(bad.sum()) == 16)
+    assert s.call(5, 32 * wave).isfinite().all()
+    if fmt != "f16":  # the tail's two tiles are the last
+        s = Setup(23, fmt, [380 + 32 * wave], [4], 1, 4, 128, 64, 64)
+        s.cache.v_tail[0, 0, (s.held[0] - 2) % 64, 9] = float("inf")
+        bad = s.call(ALL, 0).isfinite().logical_not()
+        assert bad[2:, :, 9].all() and int(bad.sum()) == 8
