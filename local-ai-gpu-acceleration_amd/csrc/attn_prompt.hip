@@ -213,8 +213,11 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_prompt_kernel(AttnRows a, Cal
     if constexpr (F32) {
       x[1] = ldexpf(vs1, -e_tile);
     } else if (vs1 > 0.0f || !number) {  // (values of scale 0 are 0: their terms enter as they are)
-      x[1] = __builtin_amdgcn_logf(vs1) - static_cast<float>(e_tile);
-      x[2] = ldexpf(1.0f / vs1, e_tile);
+      // Below 2^-64 of the largest a term is 0 whatever it is; both numbers stay finite, also those of a scale that no row
+      // sees (what lies behind the positions held, or in row 0, which those without a page read).
+      const float v = number ? fmaxf(vs1, ldexpf(1.0f, e_tile - 64 > -126 ? e_tile - 64 : -126)) : vs1;
+      x[1] = __builtin_amdgcn_logf(v) - static_cast<float>(e_tile);
+      x[2] = ldexpf(1.0f / v, e_tile);
       if (edge && !number) {
         if (counts) odd = 1u;
         x[1] = 0.0f, x[2] = 1.0f;

@@ -9,7 +9,7 @@ import rows_ref as ref
 
 torch = pytest.importorskip("torch")
 
-from test_gpu_attn_rows import ALL, FORMATS, Setup  # noqa: E402
+from test_gpu_attn_rows import ALL, FORMATS, Setup, dev  # noqa: E402
 
 pytestmark = pytest.mark.gpu
 
@@ -79,3 +79,24 @@ def test_every_wave_hands_on_what_it_left_out(wave, fmt):
         s.cache.v_tail[0, 0, (s.held[0] - 2) % 64, 9] = float("inf")
         bad = s.call(ALL, 0).isfinite().logical_not()
         assert bad[2:, :, 9].all() and int(bad.sum()) == 8
+
+
+@pytest.mark.parametrize("bad", [1e-44, 1e-38, 1e-30, 3e38, -1.0, float("inf")])
+@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
+@pytest.mark.parametrize("dim,rows,f16", [(128, 130, True), (128, 130, False), (64, 200, True), (256, 60, True), (128, 3, True), (128, 1, False)])
+def test_scales_that_no_row_sees(dim, rows, f16, fmt, bad):
+    """Scales of blocks that are not held, of pages in no table (page 0 among them, whose first row stands in for what is not
+    there) and of positions that every window has passed: any number, and the results are the same bits."""
+    seed = next(i for i in range(99) if 0 not in np.random.default_rng(i).permutation(23)[:20])  # (the table's draw)
+    s = Setup(seed, fmt, [310, 290], [rows, min(rows, 60)], 1, 4, dim, 32, 8, f16=f16)
+    assert s.n_pages == 23 and 0 not in s.table
+    held, passed = np.zeros((s.n_pages, 4), bool), np.zeros((s.n_pages, 4), bool)
+    for i, h in enumerate(s.held):
+        for b in range(h // 8):
+            held[s.table[i, b // 4], b % 4] = True
+            passed[s.table[i, b // 4], b % 4] = 8 <= 8 * b and 8 * b + 8 <= s.pos[i] - 40
+    want = s.call(40, 3)
+    assert bool(want.isfinite().all())
+    for x in (s.cache.k_scale, s.cache.v_scale):
+        x[dev(~held | passed)[:, None]] = bad
+    assert torch.equal(s.call(40, 3), want)
