@@ -237,7 +237,8 @@ __global__ __launch_bounds__(kThreads, (D == 256 ? 1 : 2)) void attn_rows_kernel
     if constexpr (CODES) {
       float big = 0.0f;
 #pragma unroll
-      for (int t = 0; t < 2; ++t) big = fmaxf(big, (seen >> (16u * t + 4u * qq) & 15u) != 0u ? vs[t] : 0.0f);
+      for (int t = 0; t < 2; ++t)  // (one that is not a number, which only some rows may see, scales nothing)
+        big = fmaxf(big, (seen >> (16u * t + 4u * qq) & 15u) != 0u && vs[t] < INFINITY ? vs[t] : 0.0f);
       big = fmaxf(big, lane_xor<16>(big));
       big = fmaxf(big, lane_xor<32>(big));
       const int e = big > 0.0f && big < INFINITY ? __builtin_amdgcn_frexp_expf(big) : E;

@@ -100,3 +100,28 @@ def test_scales_that_no_row_sees(dim, rows, f16, fmt, bad):
     for x in (s.cache.k_scale, s.cache.v_scale):
         x[dev(~held | passed)[:, None]] = bad
     assert torch.equal(s.call(40, 3), want)
+
+
+@pytest.mark.parametrize("bad", [float("inf"), float("nan")])
+@pytest.mark.parametrize("which", ["k_scale", "v_scale"])
+@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
+@pytest.mark.parametrize("dim,rows,f16", [(64, 4, False), (128, 4, True), (256, 4, False), (128, 130, False), (128, 130, True)])
+def test_scales_that_some_rows_see(dim, rows, f16, fmt, which, bad):
+    """A scale that is not finite, of a block that the window of the first row reaches and no other's, of a prompt the first
+    half's: those rows are not finite, the others the same bits."""
+    s = Setup(24, fmt, [160], [rows], 1, 4, dim, 32, 8, f16=f16)
+    first = s.pos[0] if rows == 4 else 87
+    window = 9 if rows == 4 else 20
+    block = (first + 1 - window) // 8  # its last position is the row's first
+    window += first + 1 - window - (8 * block + 7)
+    sees = [s.pos[0] + i - window < 8 * block + 7 and s.pos[0] + i >= 8 * block for i in range(rows)]
+    want = s.call(window, 0)
+    assert bool(want.isfinite().all()) and 0 < sum(sees) < rows and (rows > 4 or sees == [True, False, False, False])
+    getattr(s.cache, which)[int(s.table[0, block // 4]), 0, block % 4] = bad
+    got = s.call(window, 0)
+    hit = torch.tensor(sees, device=got.device)
+    assert torch.equal(got[~hit], want[~hit])
+    if which == "v_scale":
+        assert not got[hit].isfinite().any()
+    else:  # (an infinite score of -infinity weighs nothing, every other row has NaN)
+        assert bad == float("inf") or got[hit].isnan().all()
