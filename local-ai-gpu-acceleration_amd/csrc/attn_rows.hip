@@ -83,8 +83,9 @@ __device__ __forceinline__ std::uint32_t key_dim(int j, std::uint32_t qq) {
 //  * scores: S = K q^T by v_mfma_f32_16x16x32_f16, q as an fp16 pair lifted by a power of two
 //    (F16 queries: hi alone); int8 and e4m3 codes are fp16 numbers, so a product is exact and the key's
 //    scale multiplies the score;
-//  * p = 2^(s - m + 15) times the value's scale over 2^E, the largest scale's power of two so far, so that
-//    it fits fp16 whatever the scales' size; split into an fp16 pair;
+//  * p = 2^(s - m + 15) enters the sum; times the value's scale over 2^E it is split into an fp16 pair. 2^E is the column's
+//    own: the largest 2^(s - m) times scale that it has seen, so that what it does not see, or what hardly weighs, takes
+//    no bits from the rest, whatever the scales' size;
 //  * o += V^T p by the same instruction. The scores' layout (4 positions of each half tile a lane) is
 //    taken as the order of the products' 32 positions, so p needs no exchange, and a lane loads its
 //    values for those positions: rows of the cache in whole lines, bytes turned in registers.
@@ -176,7 +177,8 @@ __global__ __launch_bounds__(kThreads, (D == 256 ? 1 : 2)) void attn_rows_kernel
   }
 
   float m = -INFINITY, l = 0.0f;
-  int E = -126;  // of the values' scales so far
+  float lead = -INFINITY;  // codes: the largest log2 of a position's term times its value's scale,
+  int E = 0;               // lead - m in whole powers of two, over which o is held
   std::uint32_t left_out = 0u;  // the wave's own mark, in LDS only behind all tiles: nothing clears another wave's
   f32x4 o[B];
 #pragma unroll
@@ -186,7 +188,7 @@ __global__ __launch_bounds__(kThreads, (D == 256 ? 1 : 2)) void attn_rows_kernel
   // `next` runs once the keys are used.
   auto step = [&](auto& f, std::uint32_t j0, std::uint32_t seen, auto next) {
     using Fr = std::remove_reference_t<decltype(f)>;
-    constexpr bool SCALED = Fr::kind != Cached::kF16;
+    constexpr bool SCALED = Fr::kind != Cached::kF16, TAIL = CODES && !SCALED;
     f32x4 sc[2];
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
@@ -218,38 +220,44 @@ __global__ __launch_bounds__(kThreads, (D == 256 ? 1 : 2)) void attn_rows_kernel
           sees &= yes ? ~0u : ~(1u << x);
         }
     }
-    float s[2][4], top = -INFINITY;
+    float s[2][4], top = -INFINITY, most = -INFINITY;
 #pragma unroll
-    for (int t = 0; t < 2; ++t)
+    for (int t = 0; t < 2; ++t) {
+      float quad = -INFINITY;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const float x = sc[t][i] * ks[t];
         s[t][i] = (sees >> (16 * t + i) & 1u) != 0u ? x : -INFINITY;
-        top = fmaxf(top, s[t][i]);
+        quad = fmaxf(quad, s[t][i]);
       }
+      top = fmaxf(top, quad);
+      if constexpr (CODES)  // (a scale that is 0 or no number has no size)
+        most = fmaxf(most, vs[t] > 0.0f && vs[t] < INFINITY ? quad + static_cast<float>(__builtin_amdgcn_frexp_expf(vs[t])) : -INFINITY);
+    }
     top = fmaxf(top, lane_xor<16>(top));
     top = fmaxf(top, lane_xor<32>(top));
     const float mn = fmaxf(m, top), base = mn == -INFINITY ? 0.0f : mn;
     float alpha = __builtin_amdgcn_exp2f(m - base);
-    bool moved = mn != m;
-    m = mn;
     l *= alpha;
+    bool moved = mn != m;
     if constexpr (CODES) {
-      float big = 0.0f;
+      most = fmaxf(most, lane_xor<16>(most));
+      most = fmaxf(most, lane_xor<32>(most));
+      // The tail's values are as they are, of scale 1 whatever their size, and come last: their terms alone say where
+      // they are held (2^60 and o has room).
+      lead = TAIL ? most : fmaxf(lead, most);
+      int e = lead - base > -126.0f ? static_cast<int>(ceilf(lead - base)) : E;
+      if (TAIL && e < E - 60) e = E - 60;
+      alpha = __builtin_amdgcn_exp2f((m - base) + static_cast<float>(E - e));
+      moved |= e != E;
+      E = e;
 #pragma unroll
-      for (int t = 0; t < 2; ++t)  // (one that is not a number, which only some rows may see, scales nothing)
-        big = fmaxf(big, (seen >> (16u * t + 4u * qq) & 15u) != 0u && vs[t] < INFINITY ? vs[t] : 0.0f);
-      big = fmaxf(big, lane_xor<16>(big));
-      big = fmaxf(big, lane_xor<32>(big));
-      const int e = big > 0.0f && big < INFINITY ? __builtin_amdgcn_frexp_expf(big) : E;
-      if (__builtin_amdgcn_readfirstlane(e) > E) {
-        alpha = ldexpf(alpha, E - e);
-        E = __builtin_amdgcn_readfirstlane(e);
-        moved = true;
+      for (int t = 0; t < 2; ++t) {  // (a finite scale stays finite)
+        const int room = 127 - __builtin_amdgcn_frexp_expf(vs[t]);
+        vs[t] = ldexpf(vs[t], -E < room ? -E : room);
       }
-      vs[0] = ldexpf(vs[0], -E);
-      vs[1] = ldexpf(vs[1], -E);
     }
+    m = mn;
     half8 ph, pl;
     float sum = 0.0f;
 #pragma unroll
@@ -408,18 +416,19 @@ __global__ __launch_bounds__(kThreads, (D == 256 ? 1 : 2)) void attn_rows_kernel
     }
   }
 
-  // the waves' records, merged: o = sum 2^(m_w - M) 2^E_w o_w, the sums alike
+  // the waves' records, merged: o = sum 2^(m_w - M + E_w) o_w, the sums without E_w
   l += lane_xor<16>(l);
   l += lane_xor<32>(l);
   // a NaN among the scores makes the row NaN, also where no number gave a maximum
   if (qq == 0u) rml[wave][col] = make_float2(l != l ? INFINITY : m, l);
   if (lane == 0u) odd[wave] = left_out;
-  const float lift = CODES ? ldexpf(1.0f, E) : 1.0f;
 #pragma unroll
   for (int i = 0; i < 4; ++i)
 #pragma unroll
     for (int b = 0; b < B; b += 4)
-      *reinterpret_cast<f32x4*>(&rec[wave][col][VPL * (4u * qq + i) + b]) = f32x4{o[b][i], o[b + 1][i], o[b + 2][i], o[b + 3][i]} * lift;
+      *reinterpret_cast<f32x4*>(&rec[wave][col][VPL * (4u * qq + i) + b]) =
+          CODES ? f32x4{ldexpf(o[b][i], E), ldexpf(o[b + 1][i], E), ldexpf(o[b + 2][i], E), ldexpf(o[b + 3][i], E)}
+                : f32x4{o[b][i], o[b + 1][i], o[b + 2][i], o[b + 3][i]};
   __syncthreads();
   const bool whole = per >= sp.total;
   const std::uint32_t ncol = a.tq * a.group;

@@ -9,15 +9,20 @@ import rows_ref as ref
 
 torch = pytest.importorskip("torch")
 
-from test_gpu_attn_rows import ALL, FORMATS, Setup, dev  # noqa: E402
+from test_gpu_attn_rows import ALL, FORMATS, Setup, dev, u32  # noqa: E402
+
+from rtxllm_amd import kv8  # noqa: E402
 
 pytestmark = pytest.mark.gpu
 
 
-def bound(q, keys, values, f16, codes, lift):
+def bound(q, keys, values, f16, codes, lift, tops=None):
     """(the result, a bound of its error): that of rows_ref.attend, with terms as pairs of which the smaller half ends at
     2^-25 where the largest term is at least 2^(lift - 2): 2^(-23 - lift) of the largest attended value, n times. codes: a
-    scale may enter a term and the sum as its logarithm, off by 2^-19 each. f16: rounded once (2^-11)."""
+    scale may enter a term and the sum as its logarithm, off by 2^-19 each. f16: rounded once (2^-11).
+    tops: over codes, the largest |value| of each position's block. A term times the scale is what enters as a pair, to the
+    largest such: 2^(-23 - lift) of the largest weight times scale, n codes; a scale times the format's largest code
+    is at most twice the block's largest value (e4m3: 224 / scale or more). And no logarithms."""
     out, _ = ref.attend(q, keys, values)
     n, d = keys.shape
     q, keys, values = (np.asarray(x, np.float64) for x in (q, keys, values))
@@ -26,8 +31,8 @@ def bound(q, keys, values, f16, codes, lift):
     p /= p.sum()
     size = np.abs(keys) @ np.abs(q) / np.sqrt(d)
     delta = (2.0 ** -22 + (d + 16) * 2.0 ** -24) * size.max() + 2.0 ** -21 * (1.0 + np.abs(s).max())
-    tol = (2.0 * delta + (n + 64) * 2.0 ** -24 + 2.0 ** -22 + (2.0 ** -18 if codes else 0.0)) * (p @ np.abs(values))
-    tol = tol + 2.0 ** (-23 - lift) * n * np.abs(values).max() + 1e-37
+    tol = (2.0 * delta + (n + 64) * 2.0 ** -24 + 2.0 ** -22 + (2.0 ** -18 if codes and tops is None else 0.0)) * (p @ np.abs(values))
+    tol = tol + 2.0 ** (-23 - lift) * n * (np.abs(values).max() if tops is None else 2.0 * (p * tops).max()) + 1e-37
     if f16:
         tol = tol + 2.0 ** -11 * (np.abs(out) + tol) + 2.0 ** -25
     return out, tol
@@ -125,3 +130,52 @@ def test_scales_that_some_rows_see(dim, rows, f16, fmt, which, bad):
         assert not got[hit].isfinite().any()
     else:  # (an infinite score of -infinity weighs nothing, every other row has NaN)
         assert bad == float("inf") or got[hit].isnan().all()
+
+
+def tops_of(s, i, g, j):
+    """The largest |value| of the blocks of positions j; of those in the tail, the largest of them that is attended."""
+    x, block = np.abs(s.x[1][i, :, g].astype(np.float64)).max(-1), s.m.block
+    whole = s.held[i] // block * block
+    tops = np.array([x[t // block * block:t // block * block + block].max() for t in j])
+    tops[j >= whole] = x[j[j >= whole]].max(initial=0.0)
+    return tops
+
+
+# where the large values are, for 4 rows and for many: (positions held, the first, the one behind the last)
+LARGE = dict(passed=((235, 40, 48), (235, 112, 120)), little=((235, 96, 104), (235, 96, 104)),
+             later=((233, 230, 232), (235, 168, 176)), tail=((235, 234, 235), (235, 234, 235)))
+
+
+@pytest.mark.parametrize("where", sorted(LARGE))
+@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_large_values_that_do_not_count_few_rows(dim, fmt, where):
+    large_values(dim, fmt, where, 4, False)
+
+
+def large_values(dim, fmt, where, rows, f16):
+    """Values of one size, but 6e4 in a few positions: those that the windows of a unit's later rows have passed, that weigh
+    nothing by their scores, that only later rows see, in whole blocks and in the tail. Each row is as exact as its own
+    attended and weighted values are large."""
+    held, lo, hi = LARGE[where][rows > 4]
+    s = Setup(25, fmt, [held], [rows], 1, 4, dim, 32, 8, f16=f16)
+    size = 1e-3 if f16 else 1e-5
+    s.x[1][0] = (size * s.rng.standard_normal(s.x[1][0].shape)).astype(np.float16)
+    s.x[1][0, lo:hi] = (6e4 * np.sign(s.rng.standard_normal(s.x[1][0, lo:hi].shape))).astype(np.float16)
+    s.q = (s.q * 0.1 + 1.0).astype(s.q.dtype)
+    if where == "little":
+        s.x[0][0, lo:hi] = -6.0
+    kv8.append(s.cache, dev(s.x[0][0, :held]), dev(s.x[1][0, :held]), u32([0]), u32([0, held]))
+    s.m.append(0, 0, [s.x[i][0, :held] for i in range(2)])
+    window = ALL if where != "passed" else s.pos[0] - 44 if rows == 4 else 21
+    got, seen = s.call(window, 0).cpu().numpy().astype(np.float64), []
+    for r in range(0, rows, 1 if rows == 4 else 3):
+        p = s.pos[0] + r
+        j = ref.visible(p, window, 0)
+        seen.append(bool(((j >= lo) & (j < hi)).any()))
+        k, v = (np.stack([s.value(c, 0, 0, int(t)) for t in j]) for c in range(2))
+        for h in range(4):
+            want, tol = bound(s.q[r, h], k, v, f16, True, 15 if rows == 4 or not f16 else 7, tops_of(s, 0, 0, j))
+            off = np.abs(got[r, h] - want) / tol
+            assert bool((off <= 1.0).all()), (r, p, h, float(off.max()), float(np.abs(want).max()))
+    assert all(seen) if where == "little" else not all(seen)
