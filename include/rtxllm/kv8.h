@@ -79,7 +79,8 @@ hipError_t rtxllm_kv8_read(const rtxllm_paged_kv8* cache, const uint32_t* held, 
 /* rtxllm_attn_window_f16 (rtxllm/paged_kv.h) over this cache, which holds the call's
  * rows already: sequence s holds pos[s] + its rows positions. A query sees the positions as the cache holds them, those
  * of its own call too. Codes enter the products as they are, a key's scale multiplies its scores and a value's its
- * softmax term. Scales that are not finite and tails behind what is held have no effect where they are not
+ * softmax term, which enters as a pair then: off by 2^-22 of itself or 2^-34 of the largest term times scale that
+ * the query attends, whatever lies where it does not. Scales that are not finite and tails behind what is held have no effect where they are not
  * attended. (e4m3 codes of NaN, which the append never writes, make NaN of the queries whose call reads
  * them, attended or not.) */
 size_t rtxllm_attn_kv8_workspace(const rtxllm_paged_kv8* cache, uint32_t n_heads, uint32_t sequences, uint32_t rows,

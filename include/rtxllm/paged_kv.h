@@ -183,7 +183,7 @@ hipError_t rtxllm_kv_evict_f16(const rtxllm_paged_kv* cache, const uint32_t* len
  * values makes NaN of what it enters; an infinity makes an infinity or NaN of it, but a score of -infinity weighs
  * nothing.
  * The softmax terms enter the products as pairs of fp16, off by 2^-22 of themselves or
- * 2^-32 of the largest; q as such a pair too (RTXLLM_F32, as in
+ * 2^-36 of the largest; q as such a pair too (RTXLLM_F32, as in
  * rtxllm_attn_decode_pages_gqa_f16) or as it is (RTXLLM_F16).
  * n_heads / n_kv_heads 1..16; sequences 1..65535; rows 1..2^20; with table_stride 0 every
  * sequence reads the one table row. workspace:

@@ -6,8 +6,8 @@ namespace rtxllm {
 namespace {
 
 constexpr std::uint32_t kTile = kPromptTile;  // 64 positions
-constexpr int kLift = 7;           // F16: softmax terms are 2^7 times what they are to the maximum they count from,
-constexpr float kSlack = 8.0f;     // which may lag 2^8 behind: 2^15 at most
+constexpr int kLift = 11;          // F16: softmax terms are 2^11 times what they are to the maximum they count from,
+constexpr float kSlack = 4.0f;     // which may lag 2^4 behind: 2^15 at most
 constexpr int kPairLift = 15;      // F32: exact maxima, as in attn_rows.hip
 
 // Where a row's 16-byte slots lie, so that what the lanes of one phase of an LDS access touch (16 of them for a
@@ -33,30 +33,30 @@ __device__ __forceinline__ void lds_barrier() {
 // computed the next one's codes are on their way into registers, and become fp16 once it is done.
 //  * scores: S = K q^T by v_mfma_f32_16x16x32_f16, keys' rows from the LDS, q in registers (F32: an fp16 pair, lifted as
 //    in attn_rows.hip); an 8-bit key enters as its code, its scale multiplies the scores of four positions at a time;
-//  * terms: as fp16 pairs. F32 as in attn_rows.hip. F16: p = 2^(s - m + 7), where the m counted from may lag up to 2^8
-//    behind the maximum, so that it hardly ever moves; an 8-bit value's scale over 2^E is added to the exponent as its
-//    logarithm (off by 2^-19 of the term) and taken out of the sum. (Terms as one fp16 were 717 and 357 us where pairs are
-//    842 and 425, but off by as much as the result's own rounding is, and only in the calls that take this form.)
+//  * terms: as fp16 pairs. F32 as in attn_rows.hip. F16: p = 2^(s - m + 11), where the m counted from may lag up to 2^4
+//    behind the maximum, so that it hardly ever moves. An 8-bit value's scale over 2^E multiplies its term before it is
+//    split, E the column's own as in attn_rows.hip, so that what a row does not see takes no bits from it. (8192 rows
+//    over int8 codes, us: terms as one fp16 717, but off by as much as the result's own rounding, and only in calls that
+//    take this form; pairs relative to the largest scale that any row of the unit had seen 842; the column's own 867.)
 //  * o += V^T p, values turned when they are stored ([dimension][position], the positions in the order in which the
 //    scores' layout holds their terms), so that both products read 16 bytes a lane.
 // Bound by what a wave issues, vector instructions beside matrix ones, at two waves a SIMD: 8192 rows over int8 codes, 32
-// heads over 8 kv heads of 128, 842 us, over fp16 pages 425 for 8000 rows with a window of 2048. Columns a wave: heads of
-// 128 32, which fill the registers; heads of 64 64 (spills of up to 25 registers; 48 without spills 687 us instead of 580, 32 704).
+// heads over 8 kv heads of 128, 867 us, over fp16 pages 428 for 8000 rows with a window of 2048. Columns a wave: heads of
+// 128 32, which fill the registers; heads of 64 64 (spills of up to 25 registers; 48 without spills 747 us instead of 645).
 template <int D, Cached F, bool F32, int NB, int NW>
-__global__ __launch_bounds__(64 * NW, 2) void attn_prompt_kernel(AttnRows a, CallRows rows, RowsCache kv) {
+__global__ __launch_bounds__(64 * NW, F32 && D == 64 ? 4 : 2) void attn_prompt_kernel(AttnRows a, CallRows rows, RowsCache kv) {
   constexpr bool CODES = F != Cached::kF16;
   constexpr int BYTES = CODES ? 1 : 2, T = 64 * NW, J = D / 32, B = D / 16;
   constexpr int KC = (64 * D * BYTES / 16 + T - 1) / T;  // 16-byte pieces of keys a thread
   constexpr int VU = (4 * D + T - 1) / T;                // units of values a thread: 4 positions of 4 dimensions
   constexpr int KL = D * BYTES / 16;                     // pieces of a row
-  constexpr bool AHEAD = !F32 && D <= 128;
+  constexpr bool AHEAD = !F32 && (D == 128 || (D == 64 && !CODES));
   typedef std::uint32_t vword __attribute__((ext_vector_type(BYTES)));
   __shared__ __align__(16) std::uint8_t keys[2][64 * D * 2];
   __shared__ __align__(16) std::uint8_t vals[2][64 * D * 2];  // [dimension][position], positions as the products take them
-  // of each position: its key's scale, and its value's over 2^E as a factor (F32), or in log2 with what undoes it
+  // of each position: its key's scale, its value's, log2 of that in whole powers of two (-infinity: none)
   __shared__ __align__(16) float scales[2][CODES ? 64 : 1][4];
   __shared__ std::uint32_t odd;
-  __shared__ int exponent[2];
 
   const std::uint32_t g = blockIdx.x % kv.p.n_kv, us = blockIdx.x / kv.p.n_kv, split = us % a.splits;
   const std::uint32_t unit = a.units - 1u - us / a.splits;  // the last rows, which see most, first
@@ -122,11 +122,12 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_prompt_kernel(AttnRows a, Cal
   const std::uint32_t pa = row_pos(sp.pos, idle ? 0u : c0 / a.group, cap), pb = row_pos(sp.pos, idle ? 0u : (c1 - 1u) / a.group, cap);
 
   float m[NB], l[NB];
-  int E = -126, e_tile = -126;  // of the values' scales: in o, and (wave 0) up to the tile that was stored last
+  float lead[NB];  // codes: the largest log2 of a position's term times its value's scale (it may lag as m does),
+  int E[NB];       // lead - m in whole powers of two, over which o is held
   f32x4 o[NB][B];
 #pragma unroll
   for (int n = 0; n < NB; ++n) {
-    m[n] = -INFINITY, l[n] = 0.0f;
+    m[n] = -INFINITY, l[n] = 0.0f, lead[n] = -INFINITY, E[n] = 0;
 #pragma unroll
     for (int b = 0; b < B; ++b) o[n][b] = f32x4{};
   }
@@ -202,32 +203,17 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_prompt_kernel(AttnRows a, Cal
   auto is_edge = [&](std::uint32_t j0, unsigned long long s) {
     return s != ~0ull || j0 + kTile - 1u > sp.p0 || !(sp.plast - j0 < a.window || j0 + kTile <= a.sinks);
   };
-  auto put_scales = [&](int buf, bool edge) {
+  auto put_scales = [&](int buf) {
     if (wave != 0u) return;
-    const bool counts = (seen >> lane & 1ull) != 0ull, number = vs1 < INFINITY;
-    const float big = wave_max(counts && number ? vs1 : 0.0f);
-    const int e = __builtin_amdgcn_readfirstlane(big > 0.0f ? __builtin_amdgcn_frexp_expf(big) : e_tile);
-    e_tile = e > e_tile ? e : e_tile;
-    if (lane == 0u) exponent[buf] = e_tile;
-    f32x4 x = {ks1, 0.0f, 1.0f, 0.0f};
-    if constexpr (F32) {
-      x[1] = ldexpf(vs1, -e_tile);
-    } else if (vs1 > 0.0f || !number) {  // (values of scale 0 are 0: their terms enter as they are)
-      // Below 2^-64 of the largest a term is 0 whatever it is; both numbers stay finite, also those of a scale that no row
-      // sees (what lies behind the positions held, or in row 0, which those without a page read).
-      const float v = number ? fmaxf(vs1, ldexpf(1.0f, e_tile - 64 > -126 ? e_tile - 64 : -126)) : vs1;
-      x[1] = __builtin_amdgcn_logf(v) - static_cast<float>(e_tile);
-      x[2] = ldexpf(1.0f / v, e_tile);
-      if (edge && !number) {
-        if (counts) odd = 1u;
-        x[1] = 0.0f, x[2] = 1.0f;
-      }
-    }
+    const bool number = vs1 < INFINITY && vs1 > -INFINITY;
+    if (!number && (seen >> lane & 1ull) != 0ull) odd = 1u;  // (0 times what a row does not see must stay 0)
+    const float v = number ? vs1 : 0.0f;
+    const f32x4 x = {ks1, v, v > 0.0f ? static_cast<float>(__builtin_amdgcn_frexp_expf(v)) : -INFINITY, 0.0f};
     *reinterpret_cast<f32x4*>(scales[buf][lane]) = x;
   };
   auto store_tile = [&](int buf, std::uint32_t j0) {
     bool bad = false;
-    const bool edge = is_edge(j0, seen);
+    const bool edge = !CODES && is_edge(j0, seen);
 #pragma unroll
     for (int i = 0; i < KC; ++i) {
       const std::uint32_t piece = tid + T * i, r = piece / KL, c = piece % KL;
@@ -274,7 +260,7 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_prompt_kernel(AttnRows a, Cal
         put_values(buf, x, v);
       }
     }
-    if constexpr (CODES) put_scales(buf, edge);
+    if constexpr (CODES) put_scales(buf);
     if (bad) odd = 1u;
   };
   // The newest block, fp16, at once.
@@ -309,7 +295,7 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_prompt_kernel(AttnRows a, Cal
         put_values(buf, x, v);
       }
       ks1 = vs1 = 1.0f;
-      put_scales(buf, false);
+      put_scales(buf);
       if (bad) odd = 1u;
     }
   };
@@ -322,24 +308,17 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_prompt_kernel(AttnRows a, Cal
   for (int j = 0; j < kKeyAts; ++j) kat[j] = col * (D * 2u) + 16u * key_slot<D>(col, 4u * j + qq);
 #pragma unroll
   for (int y = 0; y < 4; ++y) vat[y] = col * 128u + 16u * (value_slot(col, qq) ^ (y & 1) ^ (4u * (y >> 1)));  // odd b, x 1
-  auto compute = [&](int buf, std::uint32_t j0, unsigned long long sees_any) {
+  auto compute = [&](int buf, std::uint32_t j0, unsigned long long sees_any, bool tail) {
     // every column of the wave sees every position
     const bool plain = sees_any == ~0ull && j0 + kTile - 1u <= pa && (pb - j0 < a.window || j0 + kTile <= a.sinks);
-    if constexpr (CODES) {
-      const int e_now = __builtin_amdgcn_readfirstlane(exponent[buf]);
-      if (e_now > E) {
-        const float f = ldexpf(1.0f, E - e_now);
+    if (CODES && tail) {  // values of scale 1, whatever their size, and last: their terms alone say where they are held
 #pragma unroll
-        for (int n = 0; n < NB; ++n)
-#pragma unroll
-          for (int b = 0; b < B; ++b) o[n][b] *= f;
-        E = e_now;
-      }
+      for (int n = 0; n < NB; ++n) lead[n] = -INFINITY;
     }
     const std::uint8_t* const kt = keys[buf];
     const std::uint8_t* const vt = vals[buf];
     // AHEAD: a half tile's values are read ahead of its softmax. (Its keys as well, ahead of the products before: spills,
-    // 904 us instead of 842.)
+    // 904 us where this was 842. Heads of 64 over codes: spills too, 670 instead of 644.)
     half8 kf[2][J];
     auto load_keys = [&](int x) {
 #pragma unroll
@@ -377,16 +356,14 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_prompt_kernel(AttnRows a, Cal
       f32x4 sc[2];
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
-        sc[t] = f32x4{1.0f, 0.0f, 1.0f, 0.0f};
+        sc[t] = f32x4{1.0f, 1.0f, 0.0f, 0.0f};
         if constexpr (CODES) sc[t] = *reinterpret_cast<const f32x4*>(scales[buf][32 * x + 16 * t + 4u * qq]);
       }
-      float c[NB][2], top[NB];
-      std::uint32_t vis[NB];
+      float c[NB][2], top[NB], most[NB];
       bool moves = false;
 #pragma unroll
       for (int n = 0; n < NB; ++n) {
         c[n][0] = sc[0][0] * qscale[n], c[n][1] = sc[1][0] * qscale[n];
-        vis[n] = 0xFFu;
         if (!plain) {
           // of the lane's positions j0 + 32 x + 4 qq + (16 t + i): up to `last`, behind `past` or before `first`
           std::uint32_t quad = qq;
@@ -394,7 +371,6 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_prompt_kernel(AttnRows a, Cal
           const auto base = static_cast<int>(j0 + 32u * x + 4u * quad);
           const int last = static_cast<int>(pc[n]) - base, past = last - static_cast<int>(a.window), first = static_cast<int>(a.sinks) - base;
           const std::uint32_t bits = static_cast<std::uint32_t>(sees_any >> (32 * x)) >> (4u * quad);
-          vis[n] = 0u;
 #pragma unroll
           for (int t = 0; t < 2; ++t)
 #pragma unroll
@@ -402,26 +378,38 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_prompt_kernel(AttnRows a, Cal
               const int at = 16 * t + i;
               const bool yes = (at <= last) & ((at > past) | (at < first)) & ((bits >> at & 1u) != 0u);
               s[n][t][i] = yes ? s[n][t][i] * c[n][t] : -INFINITY;
-              vis[n] |= yes ? 1u << (4 * t + i) : 0u;
             }
           c[n][0] = c[n][1] = 1.0f;
         }
-        top[n] = -INFINITY;
+        top[n] = most[n] = -INFINITY;
 #pragma unroll
-        for (int t = 0; t < 2; ++t)
-          top[n] = fmaxf(top[n], fmaxf(fmaxf(s[n][t][0], s[n][t][1]), fmaxf(s[n][t][2], s[n][t][3])) * c[n][t]);
-        moves |= F32 ? top[n] > m[n] : top[n] > m[n] + kSlack;  // (from no maximum: anything)
+        for (int t = 0; t < 2; ++t) {
+          const float quad = fmaxf(fmaxf(s[n][t][0], s[n][t][1]), fmaxf(s[n][t][2], s[n][t][3])) * c[n][t];
+          top[n] = fmaxf(top[n], quad);
+          if constexpr (CODES) most[n] = fmaxf(most[n], quad + sc[t][2]);
+        }
+        constexpr float kLag = F32 ? 0.0f : kSlack;
+        moves |= top[n] > m[n] + kLag;  // (from no maximum: anything)
+        if constexpr (CODES) moves |= most[n] > lead[n] + kLag;
       }
-      // F16: the maximum counted from moves once a score is 2^8 above it
+      // F16: the maxima counted from move once they are 2^4 behind
       if (__ballot(moves) != 0ull) {
 #pragma unroll
         for (int n = 0; n < NB; ++n) {
           float t = fmaxf(top[n], lane_xor<16>(top[n]));
           t = fmaxf(t, lane_xor<32>(t));
           const float mn = fmaxf(m[n], t), base = mn == -INFINITY ? 0.0f : mn;
-          const float alpha = __builtin_amdgcn_exp2f(m[n] - base);
-          m[n] = mn;
+          float alpha = __builtin_amdgcn_exp2f(m[n] - base);
           l[n] *= alpha;
+          if constexpr (CODES) {
+            t = fmaxf(most[n], lane_xor<16>(most[n]));
+            lead[n] = fmaxf(lead[n], fmaxf(t, lane_xor<32>(t)));
+            int e = lead[n] - base > -126.0f ? static_cast<int>(ceilf(lead[n] - base)) : E[n];
+            if (tail && e < E[n] - 60) e = E[n] - 60;  // (o has room for that)
+            alpha = __builtin_amdgcn_exp2f((m[n] - base) + static_cast<float>(E[n] - e));
+            E[n] = e;
+          }
+          m[n] = mn;
 #pragma unroll
           for (int b = 0; b < B; ++b) o[n][b] *= alpha;
         }
@@ -432,19 +420,17 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_prompt_kernel(AttnRows a, Cal
         const float base = (m[n] == -INFINITY ? 0.0f : m[n]) - static_cast<float>(F32 ? kPairLift : kLift);
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
-          const float from = (CODES && !F32 ? sc[t][1] : 0.0f) - base;
-          float p[4];
+          float scale = 1.0f;
+          if constexpr (CODES) scale = fminf(ldexpf(sc[t][1], -E[n]), 3e38f);  // (finite also where the row does not see)
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            p[i] = __builtin_amdgcn_exp2f(fmaf(s[n][t][i], c[n][t], from));
-            if constexpr (F32 || !CODES) l[n] += p[i];
-            if constexpr (F32 && CODES) p[i] = (vis[n] >> (4 * t + i) & 1u) != 0u ? p[i] * sc[t][1] : 0.0f;
-            asm("" : "+v"(p[i]));
-            const _Float16 hi = static_cast<_Float16>(p[i]);
-            ph[n][4 * t + i] = hi;
-            pl[n][4 * t + i] = static_cast<_Float16>(p[i] - static_cast<float>(hi));
+            float p = __builtin_amdgcn_exp2f(fmaf(s[n][t][i], c[n][t], -base));
+            l[n] += p;
+            if constexpr (CODES) p *= scale;
+            asm("" : "+v"(p));  // one rounded value for hi and lo
+            ph[n][4 * t + i] = static_cast<_Float16>(p);
+            pl[n][4 * t + i] = static_cast<_Float16>(p - static_cast<float>(ph[n][4 * t + i]));
           }
-          if constexpr (CODES && !F32) l[n] = fmaf((p[0] + p[1]) + (p[2] + p[3]), sc[t][2], l[n]);
         }
       }
       if (AHEAD)
@@ -482,7 +468,7 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_prompt_kernel(AttnRows a, Cal
     }
     // (a wave whose rows see none of the tile: before it, or with their windows past it)
     if (!idle && j0 <= pb && (j0 + kTile - 1u + a.window > pa || j0 < a.sinks))
-      compute(buf, j0, now);
+      compute(buf, j0, now, u >= sp.ncode);
     if (u + 1u < u1) {
       if (u + 1u < code1)
         store_tile(buf ^ 1, first_of(u + 1u));
@@ -501,20 +487,21 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_prompt_kernel(AttnRows a, Cal
     sum += lane_xor<32>(sum);
     const std::uint32_t c = (wave * NB + n) * 16u + col, ci = c / a.group;
     if (ci >= sp.nq) continue;
-    const float lift = CODES ? ldexpf(1.0f, E) : 1.0f;
     if (per >= sp.total) {
-      const float inv = sum == 0.0f ? 0.0f : lift / sum;
+      const float inv = sum == 0.0f ? 0.0f : ldexpf(1.0f / sum, E[n]);
       const std::size_t at = (static_cast<std::size_t>(sp.row + ci) * n_heads + g * a.group + (c - ci * a.group)) * D + 4u * qq;
 #pragma unroll
       for (int b = 0; b < B; ++b) store_row4(a, at + 16 * b, o[n][b] * inv);
     } else {
       const std::size_t at = ((static_cast<std::size_t>(unit) * kv.p.n_kv + g) * (a.tq * a.group) + c) * a.splits + split;
 #pragma unroll
-      for (int b = 0; b < B; ++b) *reinterpret_cast<f32x4*>(a.part + at * D + 16 * b + 4u * qq) = o[n][b] * lift;
+      for (int b = 0; b < B; ++b)
+        *reinterpret_cast<f32x4*>(a.part + at * D + 16 * b + 4u * qq) =
+            f32x4{ldexpf(o[n][b][0], E[n]), ldexpf(o[n][b][1], E[n]), ldexpf(o[n][b][2], E[n]), ldexpf(o[n][b][3], E[n])};
       if (qq == 0u) a.ml[at] = make_float2(sum != sum ? INFINITY : m[n], sum);
     }
   }
-  if (odd != 0u) not_finite_rows<D, CODES, !F32>(a, rows, kv, unit, g, split, kTile, 1u);
+  if (odd != 0u) not_finite_rows<D, CODES, true>(a, rows, kv, unit, g, split, kTile, 1u);
 }
 
 template <int D, Cached F, bool F32>
