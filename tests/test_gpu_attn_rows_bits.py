@@ -187,3 +187,36 @@ def large_values(dim, fmt, where, rows, f16):
             off = np.abs(got[r, h] - want) / tol
             assert bool((off <= 1.0).all()), (r, p, h, float(off.max()), float(np.abs(want).max()))
     assert all(seen) if where == "little" else not all(seen)
+
+
+@pytest.mark.parametrize("bad", [float("inf"), float("nan")])
+@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
+@pytest.mark.parametrize("rows,f16", [(1, False), (4, True), (130, False), (130, True)])
+def test_scales_that_every_row_sees(rows, f16, fmt, bad):
+    """A value scale that is not finite, of a block in a tile that all rows see whole: none of its head's rows is a number,
+    the other head's are the same bits."""
+    s = Setup(27, fmt, [330], [rows], 2, 4, 128, 32, 8, f16=f16)
+    want = s.call(ALL, 0)
+    s.cache.v_scale[int(s.table[0, 1]), 1, 2] = bad
+    got = s.call(ALL, 0)
+    assert not got[:, 4:].isfinite().any() and torch.equal(got[:, :4], want[:, :4]) and bool(want.isfinite().all())
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_terms_of_few_fp16_rows_keep_their_bits(fmt):
+    """fp16 queries of one row and of drafts: terms as pairs, so that nothing but the result's rounding is fp16's."""
+    for lens in ([1, 1], [4, 3]):
+        s = Setup(28, fmt, [330, 250], lens, 2, 4, 128, 64, 16, f16=True)
+        for window, sinks in ((12, 2), (ALL, 0)):
+            rows_within(s, s.call(window, sinks), window, sinks, 15)
+
+
+@pytest.mark.parametrize("f16", [False, True], ids=["f32", "half"])
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("lens", [[300, 1], [1, 300, 1, 1], [40, 1, 5]], ids=str)
+def test_prompts_beside_tokens(lens, fmt, f16):
+    """One call of a prompt and of single tokens, and drafts, of far longer contexts, in either form."""
+    held = [n if n > 5 else 3000 + 500 * n for n in lens]
+    s = Setup(29, fmt, held, lens, 1, 4, 128, 64, 16, f16=f16)
+    for window, sinks in ((ALL, 0), (900, 70)):
+        rows_within(s, s.call(window, sinks), window, sinks, 11 if f16 else 15, sample=60)
