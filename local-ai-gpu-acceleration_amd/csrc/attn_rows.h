@@ -16,15 +16,30 @@ inline std::uint32_t prompt_columns(std::uint32_t head_dim, bool f32) {
   return 16u * kPromptWaves * static_cast<std::uint32_t>(prompt_blocks(static_cast<int>(head_dim), f32));
 }
 
-// Whether tiles of many rows (attn_prompt.hip) take a call, or attn_rows.hip's 16 columns: by the columns (rows times
-// query heads) that a sequence has on average. us of 16 columns / tiles: heads of 128, 128 columns of one context of
-// 1000 17 / 29, of 16000 57 / 50, of eight of 16000 145 / 153; 256 of one of 1000 23 / 38, of 4000 41 / 44, of 16000
-// 100 / 98, windows of 1024 57 / 56; 512 of eight prompts of 128 19 / 32; heads of 64, 128 of 4000 19 / 22, 256 30 / 28;
-// of 256 over 16000, where 16 columns fill the registers: 20 30 / 34, 40 40 / 36, 80 62 / 45.
+// Whether tiles of many rows (attn_prompt.hip) take a call, or attn_rows.hip's 16 columns (rows times query heads): by the
+// columns that a sequence has on average, and by the work, the call's columns times the positions that a row can see
+// (`near`), of which tiles need many before their fewer workgroups fill the card. us of 16 columns / tiles over int8 codes,
+// 8 kv heads of 128, fp32 and fp16 rows:
+//   128 columns over one context of 1000      18 /  28    17 /  22
+//   128 over one of 16000                     60 /  52    57 /  40   (16 columns all the same)
+//   112 over each of eight of up to 16000    202 / 389   204 / 279
+//   256 over one of 1000                      23 /  38    22 /  30
+//   256 over one of 4000                      38 /  43    38 /  36
+//   256 over one of 16000                     90 /  96    90 /  72   tiles
+//   1024 over one of 1000                     25 /  46    25 /  38
+//   1024 over one of 4000                     81 /  70    82 /  56   tiles
+//   4000, a prompt of 1000                    55 /  69    53 /  54   tiles
+//   288 each, eight prompts of up to 128      20 /  32    19 /  28
+//   675 each, eight prompts of up to 300      40 /  43    37 /  31   tiles
+//   4000 over one of 16000                   905 / 574   905 / 415   tiles
+// Over 258 such calls (heads of 64, 128 and 256, fp16 pages too) the choice is 3 % behind the faster form on average; by the
+// columns alone it was 14 %. Heads of 256, where 16 columns fill the registers: 64 columns over 16000 61 / 53, 61 / 44 and
+// 2048, 512 rows over 1000, 85 / 72, 83 / 61 are tiles', 512 over 1000 27 / 45, 27 / 38 are not. The averages are the
+// call's: a long prompt beside many single tokens is better off in a call of its own.
 inline bool rows_prompt(std::uint32_t sequences, std::uint32_t rows, std::uint32_t group, std::uint32_t head_dim,
-                        std::uint32_t page_size) {
-  const std::uint64_t enough = head_dim == 256u ? 40u : 192u;
-  return static_cast<std::uint64_t>(rows) * group >= enough * sequences && page_size % 4u == 0u;
+                        std::uint32_t page_size, bool f32, std::uint64_t near) {
+  const std::uint64_t columns = static_cast<std::uint64_t>(rows) * group, enough = head_dim == 256u ? 40u : 192u;
+  return columns >= enough * sequences && columns * near >= 6144ull * prompt_columns(head_dim, f32) && page_size % 4u == 0u;
 }
 
 // Splits of a unit's tiles (at most `tiles`) in attn_rows.hip: the largest of 64 to 4 tiles a workgroup that make as

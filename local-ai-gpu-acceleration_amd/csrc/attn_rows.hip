@@ -564,11 +564,12 @@ RowsPlan rows_plan(Cached kind, const rtxllm_paged_kv* c, std::uint32_t n_heads,
   RowsPlan p;
   const std::uint32_t group = paged_group(c, n_heads);
   if (group == 0u || window == 0u) return p;
-  p.prompt = !one_each && rows_prompt(sequences, rows, group, c->head_dim, c->page_size);
+  const std::uint64_t sees = static_cast<std::uint64_t>(window) + sinks;  // positions that a row can see
+  p.prompt = !one_each && rows_prompt(sequences, rows, group, c->head_dim, c->page_size, !f16, sees < c->capacity ? sees : c->capacity);
   p.tq = one_each ? 1u : (p.prompt ? prompt_columns(c->head_dim, !f16) : kCols) / group;
   p.units = one_each ? sequences : units_of(sequences, rows, p.tq, 1u);
   const std::uint64_t items = static_cast<std::uint64_t>(p.units) * c->n_kv_heads;
-  const std::uint64_t near = static_cast<std::uint64_t>(window) + p.tq + sinks;
+  const std::uint64_t near = sees + p.tq;
   const std::uint64_t tiles = (near < c->capacity ? near : c->capacity) / (p.prompt ? kPromptTile : kTile) + 3u;
   std::uint64_t splits = rows_splits(items, tiles, kind != Cached::kF16, c->head_dim);
   if (p.prompt) {
