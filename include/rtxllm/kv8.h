@@ -62,7 +62,11 @@ typedef struct {
  * behind the other, rows k_stride and v_stride elements apart, any alignment to an
  * element. The cache has to hold the positions before pos[s]; of those the newest block's
  * are read from the tail where the new tokens make it whole. To write a sequence anew from an earlier
- * position, go back to a block's start or within the newest block. Rows at or behind the capacity store
+ * position, go back to a block's start or within the newest block. Rows that make a block whole leave codes alone, and
+ * the rows behind them go over its tail, so a program that may drop rows it has appended (drafts) has to keep the
+ * keys and values of the newest block itself, up to block - 1 positions before the first such row: if the dropped rows
+ * had made that block whole, append again from its start. Nothing marks a sequence that was cut shorter without that;
+ * its next calls read what the dropped rows left. Rows at or behind the capacity store
  * nothing; those of a whole block in no page are dropped. Sequences of one call must not share pages that they
  * write. rows <= 2^20, sequences <= 65535. */
 hipError_t rtxllm_kv8_append(const rtxllm_paged_kv8* cache, const void* k, size_t k_stride, const void* v,

@@ -47,7 +47,9 @@ inline bool rows_prompt(std::uint32_t sequences, std::uint32_t rows, std::uint32
 // few more than those, and at most twice as many, which long contexts of different lengths need. us of 1024 / 512 / 256
 // workgroups: eight contexts to 65500 in 8 bits 113 / 140 / 223 (of 256 dimensions 220 / 211 / 317), one of 65000
 // 42 / 36 / 42, one of 16001 - / 15.7 / 16.3, of 4000 - / 12.3 / 10.5 (32 of 8 tiles or of 4), four of 4000 - / 13.4 /
-// 15.4; windows of 1024 over fp16 pages, eight 320 workgroups 17.0, 256 14.0, 32 sequences 41 / 35 / 27.
+// 15.4; windows of 1024 over fp16 pages, eight 320 workgroups 17.0, 256 14.0, 32 sequences 41 / 35 / 27. A split's tiles
+// are whole rounds of its four waves (span_per), so some splits may get none: of those 256, with 33 tiles in 4 splits of 12,
+// 192 have work.
 inline std::uint32_t rows_splits(std::uint64_t items, std::uint64_t tiles, bool codes, std::uint32_t head_dim) {
   const std::uint64_t slots = head_dim == 64u || (codes && head_dim == 128u) ? 512u : 256u;
   std::uint64_t per = 64u;

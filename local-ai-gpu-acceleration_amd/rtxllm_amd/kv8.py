@@ -93,7 +93,9 @@ def _stride_of(name: str, cache: PagedKV8, x: torch.Tensor, rows: int, dtype: to
 
 def append(cache: PagedKV8, k: torch.Tensor, v: torch.Tensor, pos: torch.Tensor, start: torch.Tensor | None = None) -> None:
     """New tokens enter the cache, k and v [rows][n_kv_heads][head_dim] of float32 or float16: sequence s has rows
-    start[s] .. start[s + 1] - 1 (start None: row s), its positions pos[s], pos[s] + 1, ..."""
+    start[s] .. start[s + 1] - 1 (start None: row s), its positions pos[s], pos[s] + 1, ... Rows that are dropped again
+    (drafts) are written over from within the newest block; if they had made a block whole, from its start, with the keys
+    and values that the program has kept."""
     _in_8_bits(cache)
     rows, kind = k.shape[0], _type_of("k", k)
     ks, vs = _stride_of("k", cache, k, rows, k.dtype), _stride_of("v", cache, v, rows, k.dtype)
