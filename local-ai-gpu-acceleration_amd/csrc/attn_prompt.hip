@@ -41,9 +41,10 @@ __device__ __forceinline__ void lds_barrier() {
 //  * o += V^T p, values turned when they are stored ([dimension][position], the positions in the order in which the
 //    scores' layout holds their terms), so that both products read 16 bytes a lane.
 // Bound by what a wave issues: at two waves a SIMD vector instructions take 67 % of the cycles and matrix ones 40 %, with
-// hardly any overlap: 8192 rows over int8 codes, 32
-// heads over 8 kv heads of 128, 867 us, over fp16 pages 435 for 8000 rows with a window of 2048. Columns a wave: heads of
-// 128 32, which fill the registers; heads of 64 64 (spills of up to 25 registers; 48 without spills 747 us instead of 645).
+// hardly any overlap: 8192 rows over int8 codes, 32 heads over 8 kv heads of 128, 867 us, over fp16 pages 435 for 8000 rows
+// with a window of 2048. Columns a wave: heads of 128 32, which fill the registers; heads of 64 64 (spills of up to 25
+// registers; 48 without spills 747 us instead of 645), in fp32 16, at four waves a SIMD (765 us; five registers more, and so
+// two waves, were 1126).
 template <int D, Cached F, bool F32, int NB, int NW>
 __global__ __launch_bounds__(64 * NW, F32 && D == 64 ? 4 : 2) void attn_prompt_kernel(AttnRows a, CallRows rows, RowsCache kv) {
   constexpr bool CODES = F != Cached::kF16;
